@@ -510,6 +510,51 @@ int64_t ti8_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t seq);
 int ti8_attention_bwd(const ti8_attention_args* a, ti8_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
+ * A key / value cache in 4 bits, for serving (no counterpart in the reference).
+ *   pool     uint8 [pages][kv_heads][page_size * (head_dim + head_dim / 16)], dense, 16-byte aligned; head_dim 64 or 128, page_size
+ *            16, 32, 64, 128 or 256.  A page of a head holds page_size entries: codes of the keys [page_size][head_dim / 2], codes of the values
+ *            likewise, scales of the keys [page_size][head_dim / 32], scales of the values likewise.
+ *   A code is a 4-bit float (bit 3 the sign, magnitudes 0 .5 1 1.5 2 3 4 6), the even element in the low half of its byte; a scale is
+ *   the exponent byte e (1 .. 252) of 2^(e - 127), which 32 neighbouring elements share: the smallest power of two by which the largest of
+ *   them is at most 6 in magnitude.  An element is rounded to the nearest code, of two the even one.  Everything stored is finite: a NaN counts as
+ *   zero, what is beyond 1.5 * 2^127 as that.
+ *   table    int32 [batch][table_pages] (rows table_stride apart): page of entry j of a sequence = table[b][j / page_size], its row there j % page_size
+ *   weights  float [pages][kv_heads][page_size] or NULL: what entries were attended to so far
+ * Lengths, starts and counts are int32 [batch] on the device and are not looked at on the host, so a recorded graph may change them.  A page number that the
+ * pool does not have, and entries that the table has no room for, are not touched: such entries are neither written nor seen. */
+typedef struct {
+    void* pool;
+    const int32_t* table;
+    float* weights;
+    int64_t pages, kv_heads, page_size, head_dim;
+    int64_t batch, table_pages, table_stride;
+} ti8_cache4;
+/* Keys and values of new tokens, bf16 [batch][tokens][kv_heads][head_dim] with element strides (multiples of 8; the last dim dense; 16-byte
+ * aligned), become entries starts[b] .. starts[b] + counts[b] - 1 (counts NULL: `tokens` of every sequence), their weights zero. */
+int ti8_cache4_append(const ti8_cache4* c, const int32_t* starts, const int32_t* counts, int64_t tokens,
+                      const void* k, int64_t k_stride_b, int64_t k_stride_t, int64_t k_stride_h,
+                      const void* v, int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, ti8_stream_t stream);
+/* The values that entries starts[b] .. of each sequence stand for, bf16 [batch][tokens][kv_heads][head_dim] (dense; exact).  Rows from counts[b] on, and of entries that are not there, are zeros. */
+int ti8_cache4_read(const ti8_cache4* c, const int32_t* starts, const int32_t* counts, int64_t tokens, void* k, void* v, ti8_stream_t stream);
+/* Attention over the cache: q bf16 [batch][tokens][heads][head_dim] (strides as above; heads a multiple of kv_heads, neighbouring heads share
+ * a kv head), the last counts[b] of lengths[b] entries being those of the queries' own tokens: query i of sequence b sees entries
+ * j <= lengths[b] - counts[b] + i.
+ *   out bf16 and lse float, dense [batch][tokens][heads][head_dim] and [batch][tokens][heads]: out = sum_j p_j v_j, p_j = exp(scale q k_j - lse),
+ *   lse = log sum_j exp(scale q k_j).  Rows that see nothing and rows from counts[b] on: out 0, lse -inf.
+ *   accumulate != 0: weights of every entry j += the sum of its p_j over the queries and the heads that share its kv head.
+ *   workspace: ti8_cache4_attention_workspace bytes (-1 for sizes it does not take), 16-byte aligned, contents undefined before and after. */
+int64_t ti8_cache4_attention_workspace(const ti8_cache4* c, int64_t tokens, int64_t heads);
+int ti8_cache4_attention(const ti8_cache4* c, const int32_t* lengths, const int32_t* counts, int64_t tokens, int64_t heads,
+                         const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h, float scale, int accumulate,
+                         void* out, float* lse, void* workspace, int64_t workspace_bytes, ti8_stream_t stream);
+/* Every sequence and kv head cut down to `keep` entries: the `recent` newest (0 <= recent <= keep) and the heaviest of the others by `weights`
+ * (among equals the older one; NaN counts as heavier than any number), which become entries 0 .. in their old order, in the pages of new_table
+ * int32 [batch][new_pages] (rows new_stride apart; new_pages * page_size >= keep; other pages than those of `table`).  Their weights go with them.
+ * new_lengths[b] = min(lengths[b], keep); kept int32 [batch][kv_heads][keep]: which entry each of them was, -1 behind the last. */
+int ti8_cache4_evict(const ti8_cache4* c, const int32_t* lengths, const int32_t* new_table, int64_t new_pages, int64_t new_stride,
+                     int64_t keep, int64_t recent, int32_t* kept, int32_t* new_lengths, ti8_stream_t stream);
+
+/* ---------------------------------------------------------------------------------
  * Measurement aid (no counterpart in the reference; used by bench.py --probe mfma): a loop of nothing
  * but v_mfma_i32_32x32x32_i8 on `workgroups` workgroups of 8 waves, `iters` x 16 MFMAs per wave,
  * operands all zero or pseudo-random, optionally with the block-channel promotion's vector work

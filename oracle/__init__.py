@@ -21,6 +21,7 @@ oracle module                  reference file followed
 ``tilelang_block_channel_bwd`` tilelang/block_channel_bwd.py
 ``hadamard``                   external fast_hadamard_transform (closed form)
 ``linear``                     linear-layer wiring + modes (no reference file)
+``cache4``                     the 4-bit key/value cache (no reference file)
 =============================  ==============================================
 
 Pinning status (what fixes each function besides its own formula):

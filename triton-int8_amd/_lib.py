@@ -49,6 +49,12 @@ class AttentionArgs(ctypes.Structure):
         ("lse", _vp), ("workspace", _vp), ("batch", _i64), ("heads", _i64), ("seq", _i64), ("head_dim", _i64), ("scale", _f32)]
 
 
+class Cache4(ctypes.Structure):
+    """ti8_cache4 of include/ti8.h."""
+    _fields_ = [("pool", _vp), ("table", _vp), ("weights", _vp), ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64),
+                ("batch", _i64), ("table_pages", _i64), ("table_stride", _i64)]
+
+
 # name -> argument types, in the order of include/ti8.h
 PROTOTYPES = {
     "ti8_quant_block": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
@@ -80,10 +86,14 @@ PROTOTYPES = {
     "ti8_swiglu": [_vp, _vp, _vp, _i64, _vp],
     "ti8_swiglu_bwd": [_vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "ti8_attention_bwd": [ctypes.POINTER(AttentionArgs), _vp],
+    "ti8_cache4_append": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp],
+    "ti8_cache4_read": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _vp, _vp, _vp],
+    "ti8_cache4_attention": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _i64, _vp],
+    "ti8_cache4_evict": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
     "ti8_probe_mfma": [_vp, _i64, _vp, _int, _int, _int, _int, _vp],
 }
 EXPORTS = ["ti8_version", "ti8_last_error", "ti8_arch", "ti8_init", "ti8_last_gemm_kernel", "ti8_linear_fwd_bwd_workspace", "ti8_linear_workspace", "ti8_linear_group_workspace",
-           "ti8_rmsnorm_bwd_workspace", "ti8_column_sum_workspace", "ti8_attention_bwd_workspace"] + list(PROTOTYPES)
+           "ti8_rmsnorm_bwd_workspace", "ti8_column_sum_workspace", "ti8_attention_bwd_workspace", "ti8_cache4_attention_workspace"] + list(PROTOTYPES)
 
 # enums of include/ti8.h
 Q_CLAMP, Q_EPS_ADD, Q_SCALE_BF16, Q_HAD128, Q_WS_PINGPONG, Q_WS_SECOND, Q_TORCH_ROUND, Q_TORCH_BF16, Q_WS_IS_ZERO, Q_SCALE_T = 1, 2, 4, 8, 16, 32, 64, 128, 256, 512
@@ -137,6 +147,8 @@ def lib():
         l.ti8_attention_bwd_workspace.argtypes = [_i64, _i64, _i64]
         l.ti8_column_sum_workspace.restype = _i64
         l.ti8_column_sum_workspace.argtypes = [_i64, _i64]
+        l.ti8_cache4_attention_workspace.restype = _i64
+        l.ti8_cache4_attention_workspace.argtypes = [ctypes.POINTER(Cache4), _i64, _i64]
         for name, args in PROTOTYPES.items():
             fn = getattr(l, name)
             fn.argtypes = args

@@ -458,6 +458,13 @@ TI8_HD bool attention_stride_ok(int64_t stride, int64_t seq, int64_t head_dim) {
     return stride >= head_dim && stride <= 0x3fffffff / (seq + 512);
 }
 
+// ---- cache in 4 bits (cache4.hip, cache4_attention.hip) -------------------------------------------
+// byte offsets within a page of a head: of a row's codes and scales, of keys or values
+TI8_HD int cache4_block_bytes(int page, int dim) { return page * (dim + dim / 16); }
+TI8_HD int cache4_codes(int page, int dim, int values, int row) { return values * page * (dim / 2) + row * (dim / 2); }
+TI8_HD int cache4_scales(int page, int dim, int values, int row) { return page * dim + values * page * (dim / 32) + row * (dim / 32); }
+TI8_HD int log2_of(int page) { return page <= 16 ? 4 : page <= 32 ? 5 : page <= 64 ? 6 : page <= 128 ? 7 : 8; }
+
 // ---- which kernel an entry point launches (decided on the host) ------------------------------
 
 // per-row quantiser: NLOAD 16-byte chunks per thread, one wave (4 rows per workgroup) or one
