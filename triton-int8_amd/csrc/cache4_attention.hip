@@ -1,4 +1,11 @@
 // Attention over a cache in 4 bits.
+//
+// out = sum_j p_j v_j, p_j = exp(s_j - lse), s_j = scale q k_j, in one pass over the entries with a running maximum m and sum l of exp(s_j - m).  Keys and
+// values go from codes to bf16 in registers (exact: a code has two significant bits and a scale is a power of two) and into
+// v_mfma_f32_16x16x32_bf16 with fp32 sums; scores, m and l are fp32, probabilities are rounded to bf16 as operands of the product with the values, as
+// in any attention on bf16 tensors (that rounding, 2^-9 of each, averages out over the entries; the result is rounded to bf16 anyway).
+//
+// step_kernel: up to 64 rows per kv head (rows = new tokens x heads that share it).  Bound by the cache's bytes.  See below.
 #include "cache4.h"
 
 namespace ti8 {
@@ -6,8 +13,15 @@ namespace cache4 {
 
 namespace {
 
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef const __attribute__((address_space(4))) int32_t* constant_ints;        // read through the scalar cache
+
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int KEYS = 128;       // keys at a time, and threads of a workgroup
+constexpr int KEYS = 128;       // weights_kernel: entries per workgroup
 
 struct Args {
     Cache c;
@@ -16,9 +30,376 @@ struct Args {
     int64_t q_sb, q_st, q_sh;
     uint16_t* out;
     float* lse;
+    float* parts;               // step_kernel: two per workgroup, see Part
     int tokens, heads, group;       // group = query heads per kv head
     float scale;
+    int groups;                 // workgroups of step_kernel
 };
+
+// entries of a sequence that any of its queries sees
+__device__ __forceinline__ int seen_of(const Args& a, int b) { return count_of(a.counts, b, a.tokens) ? length_of(a.c, a.lengths, b) : 0; }
+
+// ---- sharing out ---------------------------------------------------------------------------------------------
+
+struct Share {
+    int64_t units;      // of all sequences and heads
+    int before, b;      // units in front of sequence b
+};
+__device__ __forceinline__ int wave_prefix(int v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(v, d, 64);
+        if (lane >= d) v += x;
+    }
+    return v;
+}
+// all units, by every wave
+__device__ __forceinline__ int64_t all_units(const Args& a, int lane) {
+    int sum = 0;
+    for (int b = lane; b < a.c.batch; b += 64) sum += idx::cache4_units(seen_of(a, b));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    return (int64_t)__builtin_amdgcn_readfirstlane(sum) * a.c.heads;
+}
+// units of the sequences in front of b
+__device__ __forceinline__ int units_before(const Args& a, int b, int lane) {
+    int sum = 0;
+    for (int i = lane; i < b; i += 64) sum += idx::cache4_units(seen_of(a, i));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    return __builtin_amdgcn_readfirstlane(sum) * a.c.heads;
+}
+// the sequence that a unit belongs to, and the units in front of that sequence
+__device__ __forceinline__ int sequence_of(const Args& a, int unit, int lane, int& before) {
+    before = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
+        const int own = b0 + lane < a.c.batch ? idx::cache4_units(seen_of(a, b0 + lane)) * a.c.heads : 0;
+        const int upto = wave_prefix(own, lane);
+        const int here = __popcll(__ballot(before + upto <= unit));        // sequences of these that end in front of the unit
+        if (here < 64) {
+            before += __builtin_amdgcn_readfirstlane(here ? __shfl(upto, max(here - 1, 0), 64) : 0);
+            return b0 + here;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return a.c.batch;
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ v4f mfma16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v8bf operand(uint4 x) { return __builtin_bit_cast(v8bf, x); }
+// of the four lanes that have the same place in a row of 16, in each of them
+template <bool SUM>
+__device__ __forceinline__ float over_rows(float x) {
+    v2u y = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = SUM ? __uint_as_float(y[0]) + __uint_as_float(y[1]) : fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    y = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return SUM ? __uint_as_float(y[0]) + __uint_as_float(y[1]) : fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+#endif
+
+// ---- few rows: a pass over the cache ---------------------------------------------------------------------------
+//
+// The rows of a kv head are the columns of 16 x 16 products: S^T = K Q^T with 16 entries as rows, O^T = V^T P^T with 16 elements of a head as
+// rows.  So a lane has one row of queries (lane % 16) throughout, its maximum, its sum and a quarter of its result, and the probabilities
+// that come out of the first product (entries 4 (lane / 16) .. + 3 of each 16) are the second one's operand as they are.
+//
+// A wave takes 32 entries at a time, on its own: their keys go from memory to registers in the order of the operand (a lane has 32 or 16 neighbouring
+// elements of a key, which share a scale; the order of the elements in the sum is the same on both sides), their values in the same way, as
+// bf16 through 32 rows of LDS that are the wave's own and out again transposed (ds_read_b64_tr_b16).  The next 32 entries' loads are in flight
+// meanwhile.  Four waves of a workgroup take turns and add up at the end, with their workgroups' neighbours through memory.
+
+template <int D>
+struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 16 rows' writes of a chunk and 4 x 4 rows' transposing reads spread over the banks
+    static constexpr int ROW = 2 * D, BYTES = 32 * ROW;
+    __device__ static __forceinline__ int swizzle(int row) {
+        return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    }
+};
+
+template <int D>
+struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e)) and sums of its rows
+    static constexpr int ROW = D + 2;
+};
+
+constexpr int WAVES = 4, ENTRIES = 32;      // waves of a workgroup; entries of a wave's turn
+static_assert(idx::CACHE4_UNIT == WAVES * ENTRIES, "a unit is a turn of every wave");
+
+template <int D, int TILES>     // TILES * 16 rows
+__global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) void step_kernel(const Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    using V = Values<D>;
+    constexpr int STEPS = D / 32;       // words of codes of an entry that a lane has; products over D
+    constexpr int BLOCKS = D / 16;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * V::BYTES];
+    __shared__ float stats[WAVES][2][16];
+    const Cache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quarter = lane >> 4;
+    const int64_t units = all_units(a, lane);
+    const int groups = (int)min((int64_t)a.groups, units);
+    if ((int)blockIdx.x >= groups) return;
+    const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
+    int before;
+    int b = sequence_of(a, begin, lane, before);
+    int length = seen_of(a, b), per_head = idx::cache4_units(length);
+    int h = (begin - before) / per_head, unit = (begin - before) % per_head;
+    uint8_t* const mine = smem + wave * V::BYTES;
+    // (a negative scale: the queries' signs are changed, which is exact.  Above zero, so that what is masked stays at -inf)
+    const float factor = fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+
+    for (int left = end - begin; left > 0;) {
+        const int n = min(left, per_head - unit), first = unit * WAVES + wave, last = (unit + n) * WAVES;       // this wave's turns
+        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group;
+        const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
+        // this wave's queries as operands, and up to where each row sees
+        v8bf q[TILES][STEPS];
+        int sees[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int row = t * 16 + r16, token = row / a.group, head = h * a.group + row % a.group;
+            sees[t] = row < rows ? length - count + token + 1 : 0;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + token * a.q_st + head * a.q_sh + quarter * (D / 4) + s * 8);
+                q[t][s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
+            }
+        }
+        const int all_see = length - count + 1;         // entries that every row sees
+
+        struct Turn {
+            uint32_t k[2][STEPS], v[2][STEPS], ks[2], vs[2];
+            int absent;     // a bit for each 16 whose page the pool does not have
+        };
+        const auto pages_of = [&](int turn, int (&page)[2]) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) page[u] = table[min(turn * ENTRIES + u * 16, c.capacity() - 1) >> c.log2_page];
+        };
+        const auto load = [&](int turn, const int (&page)[2], Turn& x) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int j = turn * ENTRIES + u * 16;
+                const bool there = j < length && (unsigned)page[u] < (unsigned)c.pages;
+                const uint8_t* const block = block_of(c, there ? page[u] : 0, h);
+                const int row = (j & (c.page - 1)) + r16;
+                const uint8_t *const kc = block + idx::cache4_codes(c.page, D, 0, row) + quarter * (D / 8), *const vc = block + idx::cache4_codes(c.page, D, 1, row) + quarter * (D / 8);
+                if constexpr (D == 128) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(kc), z = *reinterpret_cast<const uint4*>(vc);
+                    x.k[u][0] = y.x; x.k[u][1] = y.y; x.k[u][2] = y.z; x.k[u][3] = y.w;
+                    x.v[u][0] = z.x; x.v[u][1] = z.y; x.v[u][2] = z.z; x.v[u][3] = z.w;
+                } else {
+                    const uint2 y = *reinterpret_cast<const uint2*>(kc), z = *reinterpret_cast<const uint2*>(vc);
+                    x.k[u][0] = y.x; x.k[u][1] = y.y;
+                    x.v[u][0] = z.x; x.v[u][1] = z.y;
+                }
+                x.ks[u] = block[idx::cache4_scales(c.page, D, 0, row) + quarter * (D / 4) / GROUP];
+                x.vs[u] = block[idx::cache4_scales(c.page, D, 1, row) + quarter * (D / 4) / GROUP];
+                // (entries that are not there: whatever lies in their place must not be multiplied by a probability of zero)
+                if (!there || j + r16 >= length) x.vs[u] = 0;
+            }
+            const int j = turn * ENTRIES;
+            const bool one = (unsigned)page[0] < (unsigned)c.pages, two = (unsigned)page[1] < (unsigned)c.pages;
+            x.absent = (one || j >= length ? 0 : 1) | (two || j + 16 >= length ? 0 : 2);
+        };
+
+        v4f o[TILES][BLOCKS];
+        float top[TILES], shift[TILES], sum[TILES];      // maximum, the same times factor (0 while there is none), sum of this lane's entries
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            top[t] = -INFINITY;
+            shift[t] = sum[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) o[t][d] = v4f{0, 0, 0, 0};
+        }
+
+        const auto compute = [&](int turn, const Turn& x) {
+            v4f s[TILES][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float scale = scale_of(x.ks[u]);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) s[t][u] = v4f{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const v8bf k = operand(decode8(x.k[u][i], scale));
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) s[t][u] = mfma16(k, q[t][i], s[t][u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float scale = scale_of(x.vs[u]);
+                const int row = u * 16 + r16;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i)
+                    *reinterpret_cast<uint4*>(mine + row * V::ROW + (((quarter * STEPS + i) ^ V::swizzle(row)) << 4)) = decode8(x.v[u][i], scale);
+            }
+            const int j0 = turn * ENTRIES;
+            if (j0 + ENTRIES > all_see || x.absent)
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (j0 + u * 16 + quarter * 4 + i >= sees[t] || (x.absent >> u & 1)) s[t][u][i] = -INFINITY;
+            v8bf p[TILES];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                const v4f z = s[t][0], y = s[t][1];
+                const float largest = over_rows<false>(fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
+                // sums go on under the old maximum until a score is 2^8 above it: the same result, as everything is divided by the sum in the end
+                if (__any((largest - top[t]) * factor > 8.0f)) {
+                    const float higher = fmaxf(top[t], largest), shrink = higher == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[t] - higher) * factor);
+                    top[t] = higher;
+                    shift[t] = higher == -INFINITY ? 0.0f : higher * factor;
+                    sum[t] *= shrink;
+#pragma unroll
+                    for (int d = 0; d < BLOCKS; ++d) o[t][d] *= shrink;
+                }
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], factor, -shift[t]));
+                sum[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                p[t] = operand(make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]), pack_bf16x2(e[6], e[7])));
+            }
+            // (LDS is read back by the wave that wrote it, which its LDS instructions' order is enough for)
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) {
+                const int row = quarter * 4 + (r16 >> 2), chunk = d * 2 + ((r16 >> 1) & 1);
+                const uint8_t* const at = mine + row * V::ROW + ((chunk ^ V::swizzle(row)) << 4) + (r16 & 1) * 8;
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 16 * V::ROW));
+                const v8bf v = __builtin_bit_cast(v8bf, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) o[t][d] = mfma16(v, p[t], o[t][d]);
+            }
+            asm volatile("" ::: "memory");
+        };
+
+        if (first < last) {
+            Turn now, next;
+            int page[2];
+            pages_of(first, page);
+            load(first, page, now);
+            pages_of(min(first + WAVES, last - 1), page);
+            for (int turn = first; turn < last; turn += WAVES) {
+                if (turn + WAVES < last) load(turn + WAVES, page, next);
+                pages_of(min(turn + 2 * WAVES, last - 1), page);
+                compute(turn, now);
+                now = next;
+            }
+        }
+
+        // the waves' results meet in LDS, 16 rows at a time
+        const bool whole = n == per_head;
+        float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (unit == 0)) * (TILES * 16) * Part<D>::ROW;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const float total = over_rows<true>(sum[t]);
+            __syncthreads();
+            if (quarter == 0) {
+                stats[wave][0][r16] = top[t];
+                stats[wave][1][r16] = total;
+            }
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d)
+                *reinterpret_cast<v4f*>(mine + r16 * (4 * D) + (((d * 4 + quarter) ^ r16) << 4)) = o[t][d];
+            __syncthreads();
+            const int row = threadIdx.x >> 4;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w][0][row]);
+            float f[WAVES];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                f[w] = stats[w][0][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((stats[w][0][row] - m) * factor);
+                // (a NaN in the sum passes a maximum of -inf)
+                l += stats[w][0][row] == -INFINITY ? stats[w][1][row] : stats[w][1][row] * f[w];
+            }
+            const int at = t * 16 + row, token = at / a.group;
+            if (at >= rows) l = 0.0f;       // (no query: zeros were multiplied)
+            const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + h * a.group + at % a.group;
+            const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const int chunk = i * 16 + (threadIdx.x & 15);
+                v4f x{0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) x += *reinterpret_cast<const v4f*>(smem + w * V::BYTES + row * (4 * D) + ((chunk ^ row) << 4)) * f[w];
+                if (!whole) *reinterpret_cast<v4f*>(part + at * Part<D>::ROW + chunk * 4) = x;
+                else if (at < a.tokens * a.group)
+                    *reinterpret_cast<uint2*>(a.out + to * D + chunk * 4) = make_uint2(pack_bf16x2(x[0] * norm, x[1] * norm), pack_bf16x2(x[2] * norm, x[3] * norm));
+            }
+            if ((threadIdx.x & 15) == 0) {
+                if (!whole) {
+                    part[at * Part<D>::ROW + D] = m * factor;
+                    part[at * Part<D>::ROW + D + 1] = l;
+                } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor + __builtin_amdgcn_logf(l)) * LN2;
+            }
+        }
+        left -= n;
+        unit = 0;
+        if (++h == c.heads && left > 0) {
+            h = 0;
+            length = seen_of(a, ++b);
+            per_head = idx::cache4_units(length);
+        }
+        __syncthreads();        // nobody writes values while somebody still adds up
+    }
+#endif
+}
+
+// Rows whose (sequence, head) several workgroups had: one workgroup each
+template <int D, int TILES>
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LANES = D / 4, PARTS = 256 / LANES;       // lanes of a row; parts that are read at a time
+    __shared__ v4f shared[PARTS][LANES];
+    __shared__ float shared_m[PARTS], shared_l[PARTS];
+    const Cache& c = a.c;
+    const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
+    const int lane = threadIdx.x & 63, per_head = idx::cache4_units(seen_of(a, b));
+    const int64_t units = all_units(a, lane);
+    const int begin = units_before(a, b, lane) + h * per_head;
+    const int groups = (int)min((int64_t)a.groups, units);
+    const int first = idx::share_of(begin, groups, units), last = idx::share_of(begin + per_head - 1, groups, units);
+    if (first == last) return;
+    const int own = threadIdx.x / LANES, at = threadIdx.x % LANES;
+    float m = -INFINITY, l = 0.0f;
+    v4f o{0, 0, 0, 0};
+    for (int w = first + own; w <= last; w += PARTS) {
+        // a workgroup's second part is the one that starts with the head's first unit
+        const float* const part = a.parts + (((int64_t)w * 2 + (idx::share_begin(w, groups, units) <= begin)) * (TILES * 16) + row) * Part<D>::ROW;
+        const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
+        const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
+        const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - higher);
+        o = o * fa + x * fb;
+        l = l * fa + (pm == -INFINITY ? pl : pl * fb);
+        m = higher;
+    }
+    shared[own][at] = o;
+    if (at == 0) {
+        shared_m[own] = m;
+        shared_l[own] = l;
+    }
+    __syncthreads();
+    if (own) return;
+    for (int i = 1; i < PARTS; ++i) {
+        const float pm = shared_m[i], higher = fmaxf(m, pm);
+        const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - higher);
+        o = o * fa + shared[i][at] * fb;
+        l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? shared_l[i] : shared_l[i] * fb);
+        m = higher;
+    }
+    const int64_t to = ((int64_t)b * a.tokens + row / a.group) * a.heads + h * a.group + row % a.group;
+    if (row / a.group >= count_of(a.counts, b, a.tokens)) l = 0.0f;
+    const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(a.out + to * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
+    if (at == 0) a.lse[to] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+#endif
+}
 
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ float dot(const uint8_t* block, const Cache& c, int row, const float* q) {
@@ -104,6 +485,22 @@ __global__ __launch_bounds__(KEYS) void weights_kernel(const Args a) {
 #endif
 }
 
+// Workgroups of step_kernel: as many as run at a time (four per CU with 16 rows, which the registers allow, two otherwise), and no more than there are units
+int step_groups(const Cache& c, int tiles) {
+    const int64_t units = (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity()), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
+    return (int)(units < most ? units : most);
+}
+// Row tiles of step_kernel that hold all rows of a kv head (1, 2 or 4), or 0
+int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0; }
+
+template <int D, int TILES>
+int launch_step(const char* fn, const Args& a, hipStream_t st) {
+    hipLaunchKernelGGL((step_kernel<D, TILES>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
+    if (int e = check_launch(fn)) return e;
+    hipLaunchKernelGGL((join_kernel<D, TILES>), dim3((unsigned)(a.c.batch * a.c.heads * a.tokens * a.group)), dim3(256), 0, st, a);
+    return check_launch(fn);
+}
+
 }  // namespace
 
 }  // namespace cache4
@@ -116,9 +513,10 @@ extern "C" int64_t ti8_cache4_attention_workspace(const ti8_cache4* p, int64_t t
     Cache c;
     if (check("ti8_cache4_attention_workspace", p, c)) return -1;
     if (tokens <= 0 || tokens > (1 << 24) || heads <= 0 || heads % c.heads || heads / c.heads > 4096 || c.batch * tokens * heads > 0x7fffffff ||
-        (int64_t)c.batch * c.heads * ((c.capacity() + 127) / 128) > 0x7fffffff)
+        (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity()) > 0x3fffffff)
         return -1;
-    return 0;
+    const int tiles = step_tiles(tokens * (heads / c.heads));
+    return tiles ? (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths, const int32_t* counts, int64_t tokens, int64_t heads,
@@ -135,11 +533,18 @@ extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths,
     if (need > workspace_bytes) return fail(TI8_ERR_SHAPE, "%s: %lld bytes of workspace are needed, got %lld", fn, (long long)need, (long long)workspace_bytes);
     if (!aligned16(q) || !aligned16(out) || (reinterpret_cast<uintptr_t>(lse) & 3) || !aligned16(workspace) || q_stride_b % 8 || q_stride_t % 8 || q_stride_h % 8)
         return fail(TI8_ERR_ALIGN, "%s: q, out and the workspace must be 16-byte aligned, q's strides multiples of 8 elements", fn);
-    const Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse,
-                 (int)tokens, (int)heads, (int)(heads / c.heads), scale};
+    const int tiles = step_tiles(tokens * (heads / c.heads));
+    const Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace),
+                 (int)tokens, (int)heads, (int)(heads / c.heads), scale, tiles ? step_groups(c, tiles) : 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(row_kernel, dim3((unsigned)(c.batch * tokens * heads)), dim3(KEYS), 0, st, a);
-    if (int e = check_launch(fn)) return e;
+    if (tiles) {
+        const int e = c.dim == 128 ? (tiles == 1 ? launch_step<128, 1>(fn, a, st) : tiles == 2 ? launch_step<128, 2>(fn, a, st) : launch_step<128, 4>(fn, a, st))
+                                   : (tiles == 1 ? launch_step<64, 1>(fn, a, st) : tiles == 2 ? launch_step<64, 2>(fn, a, st) : launch_step<64, 4>(fn, a, st));
+        if (e) return e;
+    } else {
+        hipLaunchKernelGGL(row_kernel, dim3((unsigned)(c.batch * tokens * heads)), dim3(KEYS), 0, st, a);
+        if (int e = check_launch(fn)) return e;
+    }
     if (accumulate) hipLaunchKernelGGL(weights_kernel, dim3((unsigned)((int64_t)c.batch * c.heads * ((c.capacity() + KEYS - 1) / KEYS))), dim3(KEYS), 0, st, a);
     return check_launch(fn);
 }
