@@ -5,7 +5,7 @@
 // v_mfma_f32_16x16x32_bf16 with fp32 sums; scores, m and l are fp32, probabilities are rounded to bf16 as operands of the product with the values, as
 // in any attention on bf16 tensors (that rounding, 2^-9 of each, averages out over the entries; the result is rounded to bf16 anyway).
 //
-// step_kernel: up to 64 rows per kv head (rows = new tokens x heads that share it).  Bound by the cache's bytes.  See below.
+// step_kernel: up to 64 rows per kv head (rows = new tokens x heads that share it).  prompt_kernel: more.  weights_kernel: what every entry got.
 #include "cache4.h"
 
 namespace ti8 {
@@ -21,7 +21,9 @@ typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef const __attribute__((address_space(4))) int32_t* constant_ints;        // read through the scalar cache
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int KEYS = 128;       // weights_kernel: entries per workgroup
+// Exponentials are carried times 2^UP, which their common divisor takes away again: those of scores far below the maximum stay above 2^-126, below which
+// v_exp_f32 gives zero, for 2^UP further (where sums are put under another maximum exp2f goes on below it).  Up to 2^(8 + UP) each (see step_kernel), their sums stay far below 2^127
+constexpr float UP = 24.0f;
 
 struct Args {
     Cache c;
@@ -33,7 +35,8 @@ struct Args {
     float* parts;               // step_kernel: two per workgroup, see Part
     int tokens, heads, group;       // group = query heads per kv head
     float scale;
-    int groups;                 // workgroups of step_kernel
+    int groups;                 // workgroups that share the units
+    int blocks, splits;         // prompt_kernel: row blocks of a kv head, workgroups that share the entries of each
 };
 
 // entries of a sequence that any of its queries sees
@@ -118,7 +121,7 @@ struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 
 };
 
 template <int D>
-struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e)) and sums of its rows
+struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e), less UP) and sums of its rows
     static constexpr int ROW = D + 2;
 };
 
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
         };
 
         v4f o[TILES][BLOCKS];
-        float top[TILES], shift[TILES], sum[TILES];      // maximum, the same times factor (0 while there is none), sum of this lane's entries
+        float top[TILES], shift[TILES], sum[TILES];      // maximum, what is taken from a score times factor, sum of this lane's entries
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             top[t] = -INFINITY;
@@ -251,9 +254,9 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
                 const float largest = over_rows<false>(fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))));
                 // sums go on under the old maximum until a score is 2^8 above it: the same result, as everything is divided by the sum in the end
                 if (__any((largest - top[t]) * factor > 8.0f)) {
-                    const float higher = fmaxf(top[t], largest), shrink = higher == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[t] - higher) * factor);
+                    const float higher = fmaxf(top[t], largest), shrink = higher == -INFINITY ? 1.0f : exp2f((top[t] - higher) * factor);
                     top[t] = higher;
-                    shift[t] = higher == -INFINITY ? 0.0f : higher * factor;
+                    shift[t] = higher == -INFINITY ? 0.0f : higher * factor - UP;
                     sum[t] *= shrink;
 #pragma unroll
                     for (int d = 0; d < BLOCKS; ++d) o[t][d] *= shrink;
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
             float f[WAVES];
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                f[w] = stats[w][0][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((stats[w][0][row] - m) * factor);
+                f[w] = stats[w][0][row] == -INFINITY ? 0.0f : exp2f((stats[w][0][row] - m) * factor);
                 // (a NaN in the sum passes a maximum of -inf)
                 l += stats[w][0][row] == -INFINITY ? stats[w][1][row] : stats[w][1][row] * f[w];
             }
@@ -334,9 +337,9 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
             }
             if ((threadIdx.x & 15) == 0) {
                 if (!whole) {
-                    part[at * Part<D>::ROW + D] = m * factor;
+                    part[at * Part<D>::ROW + D] = m * factor - UP;
                     part[at * Part<D>::ROW + D + 1] = l;
-                } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor + __builtin_amdgcn_logf(l)) * LN2;
+                } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor - UP + __builtin_amdgcn_logf(l)) * LN2;
             }
         }
         left -= n;
@@ -374,7 +377,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
         const float* const part = a.parts + (((int64_t)w * 2 + (idx::share_begin(w, groups, units) <= begin)) * (TILES * 16) + row) * Part<D>::ROW;
         const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
         const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
-        const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - higher);
+        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
         o = o * fa + x * fb;
         l = l * fa + (pm == -INFINITY ? pl : pl * fb);
         m = higher;
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     if (own) return;
     for (int i = 1; i < PARTS; ++i) {
         const float pm = shared_m[i], higher = fmaxf(m, pm);
-        const float fa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(pm - higher);
+        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
         o = o * fa + shared[i][at] * fb;
         l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? shared_l[i] : shared_l[i] * fb);
         m = higher;
@@ -401,87 +404,321 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 #endif
 }
 
-#if defined(__HIP_DEVICE_COMPILE__)
-__device__ __forceinline__ float dot(const uint8_t* block, const Cache& c, int row, const float* q) {
-    float s = 0.0f;
-    for (int w = 0; w < c.dim / 8; ++w) {
-        const uint4 x = decode8(*reinterpret_cast<const uint32_t*>(block + idx::cache4_codes(c.page, c.dim, 0, row) + w * 4),
-                                scale_of(block[idx::cache4_scales(c.page, c.dim, 0, row) + w / 4]));
-        const float* p = q + w * 8;
-        s = fmaf(bf16_lo(x.x), p[0], s); s = fmaf(bf16_hi(x.x), p[1], s); s = fmaf(bf16_lo(x.y), p[2], s); s = fmaf(bf16_hi(x.y), p[3], s);
-        s = fmaf(bf16_lo(x.z), p[4], s); s = fmaf(bf16_hi(x.z), p[5], s); s = fmaf(bf16_lo(x.w), p[6], s); s = fmaf(bf16_hi(x.w), p[7], s);
+// ---- many rows: prompts ------------------------------------------------------------------------------------------
+//
+// A wave has 32 rows of queries as the columns of 32 x 32 products (S^T = K Q^T, O^T = V^T P^T: a lane has one row of queries, as above); the waves
+// of a workgroup go through the entries together, 64 at a time, which they turn into bf16 in LDS once for all: while one tile is multiplied,
+// the next one's codes, loaded in front of it, are converted into the other half, and the one's after that are on their way.
+// A head's row blocks lie on one XCD, whose L2 then serves the entries; where there are too few row blocks for the chip, several workgroups share the
+// entries of one and join_rows_kernel adds them up.
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int TILE = 64;        // entries of a tile
+
+template <int D>
+struct Tile32 {     // rows of D bf16 in LDS, 16-byte chunks permuted as in Values
+    static constexpr int ROW = 2 * D, BYTES = TILE * ROW;
+    // this lane's chunk of an operand whose rows are the tile's: XOR with step << 5 (plus 32 rows)
+    __device__ static __forceinline__ int rows_at(int lane) { return (lane & 31) * ROW + (((lane >> 5) ^ Values<D>::swizzle(lane & 31)) << 4); }
+    // the same of an operand over the rows (transposing read): XOR with column tile << 6 and u << 5, plus (16 t + 8 u) ROW
+    __device__ static __forceinline__ int columns_at(int lane) {
+        const int i = lane & 15, h = lane >> 5, chunk = ((lane >> 4) & 1) * 2 + ((i >> 1) & 1), r = 4 * h + (i >> 2);
+        return r * ROW + ((chunk ^ Values<D>::swizzle(r)) << 4) + (i & 1) * 8;
     }
-    return s;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ v16f mfma32(v8bf a, v8bf b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <bool SUM>
+__device__ __forceinline__ float over_halves(float x) {
+    const v2u y = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return SUM ? __uint_as_float(y[0]) + __uint_as_float(y[1]) : fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
+// 16 or 8 bytes of codes of an entry and the scale of their elements
+template <int D>
+struct Codes {
+    static constexpr int WORDS = D / 32;
+    uint32_t w[WORDS], scale;
+    __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales) {
+        if constexpr (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(codes);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(codes);
+            w[0] = x.x; w[1] = x.y;
+        }
+        scale = *scales;
+    }
+};
 #endif
 
-// one row of queries per workgroup
-__global__ __launch_bounds__(KEYS) void row_kernel(const Args a) {
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float q[128], p[KEYS], part[2];
+    using T = Tile32<D>;
+    constexpr int STEPS = D / 16, BLOCKS = D / 32, PARTS = 8 / NW;      // PARTS: of a tile (keys and values in quarters) that a wave converts
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];        // [2][keys, values]
+    __shared__ int absent[2][4];        // whether the pool does not have the page of 16 entries of a tile
     const Cache& c = a.c;
-    const int head = blockIdx.x % a.heads, t = (int)(blockIdx.x / a.heads) % a.tokens, b = (int)(blockIdx.x / a.heads) / a.tokens;
-    const int h = head / a.group, tid = threadIdx.x, count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b);
-    const int sees = t < count ? max(length - count + t + 1, 0) : 0;
-    if (tid < c.dim) q[tid] = bf16_lo(a.q[b * a.q_sb + t * a.q_st + head * a.q_sh + tid]);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    const auto all = [&](float x, bool largest) {
-        for (int d = 32; d; d >>= 1) { const float y = __shfl_xor(x, d, 64); x = largest ? fmaxf(x, y) : x + y; }
-        __syncthreads();
-        if ((tid & 63) == 0) part[tid >> 6] = x;
-        __syncthreads();
-        return largest ? fmaxf(part[0], part[1]) : part[0] + part[1];
+    const idx::AttentionPlace place = idx::attention_place(blockIdx.x, a.blocks * a.splits);
+    if (place.pair >= c.batch * c.heads) return;
+    const int b = place.pair / c.heads, h = place.pair % c.heads;
+    const int block = a.blocks - 1 - place.block / a.splits, split = place.block % a.splits;     // the longest first
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5, r16 = lane & 15, quarter = lane >> 4;
+    const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), rows = count * a.group;
+    const int row0 = block * (NW * 32), row = row0 + wave * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
+    // entries that this lane's row, any row of the workgroup, any and every row of the wave sees
+    const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
+    const int sees = row < rows ? sees_of(row) : 0, most = row0 < rows ? sees_of(min(row0 + NW * 32, rows) - 1) : 0;
+    const int wave0 = row0 + wave * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0, wave_all = wave0 + 32 <= rows ? sees_of(wave0) : 0;
+    const int tiles = (most + TILE - 1) / TILE, begin = (int)((int64_t)split * tiles / a.splits), end = (int)((int64_t)(split + 1) * tiles / a.splits);
+    const float factor = fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
+
+    v8bf q[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + token * a.q_st + head * a.q_sh + s * 16 + half * 8);
+        q[s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
+    }
+    v16f o[BLOCKS];
+#pragma unroll
+    for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float top = -INFINITY, shift = 0.0f, sum = 0.0f;
+
+    Codes<D> raw[PARTS];
+    int there[PARTS];
+    // the wave's part p of a tile: keys (p < 4) or values of 16 entries; a lane has a quarter of an entry's elements
+    const auto load = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int p = wave + i * NW, j = tile * TILE + (p & 3) * 16;
+            const int page = table[min(j, c.capacity() - 1) >> c.log2_page];
+            there[i] = j < length && (unsigned)page < (unsigned)c.pages;
+            const uint8_t* const from = block_of(c, there[i] ? page : 0, h);
+            const int at = (j & (c.page - 1)) + r16;
+            raw[i].load(from + idx::cache4_codes(c.page, D, p >> 2, at) + quarter * (D / 8), from + idx::cache4_scales(c.page, D, p >> 2, at) + quarter * (D / 4) / GROUP);
+            if (!there[i] || j + r16 >= length) raw[i].scale = 0;       // (nothing that is no number)
+        }
     };
-    for (int j0 = 0; j0 < sees; j0 += KEYS) {
-        __syncthreads();
-        const int j = j0 + tid, page = j < sees ? page_of(c, b, j) : -1;
-        float s = -INFINITY;
-        if (page >= 0) s = dot(block_of(c, page, h), c, j & (c.page - 1), q) * (a.scale * LOG2E);
-        const float top = fmaxf(m, all(s, true)), from = top == -INFINITY ? 0.0f : top;
-        const float e = exp2f(s - from);
-        p[tid] = e;
-        const float shrink = exp2f(m - from);
-        l = l * shrink + all(e, false);
-        m = top;
-        if (tid < c.dim) {
-            o *= shrink;
-            for (int i = 0; i < min(KEYS, sees - j0); ++i) {
-                const int page_i = page_of(c, b, j0 + i);
-                if (page_i < 0) continue;
-                const uint8_t* block = block_of(c, page_i, h);
-                const int row = (j0 + i) & (c.page - 1);
-                const uint32_t code = block[idx::cache4_codes(c.page, c.dim, 1, row) + tid / 2];
-                const uint32_t x = decode<0>(code, scale_of(block[idx::cache4_scales(c.page, c.dim, 1, row) + tid / GROUP]));
-                o = fmaf(p[i], tid & 1 ? bf16_hi(x) : bf16_lo(x), o);
+    const auto convert = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int p = wave + i * NW, at = (p & 3) * 16 + r16;
+            uint8_t* const to = smem + ((tile & 1) * 2 + (p >> 2)) * T::BYTES + at * T::ROW;
+            const float scale = scale_of(raw[i].scale);
+#pragma unroll
+            for (int w = 0; w < Codes<D>::WORDS; ++w)
+                *reinterpret_cast<uint4*>(to + (((quarter * Codes<D>::WORDS + w) ^ Values<D>::swizzle(at)) << 4)) = decode8(raw[i].w[w], scale);
+            if (p < 4 && lane == 0) absent[tile & 1][p] = !there[i] && tile * TILE + p * 16 < length;
+        }
+    };
+    const int rows_at = T::rows_at(lane), columns_at = T::columns_at(lane);
+    const auto compute = [&](int tile) {
+        const uint8_t* const kt = smem + (tile & 1) * 2 * T::BYTES;
+        const uint8_t* const vt = kt + T::BYTES;
+        const int j0 = tile * TILE;
+        v16f s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < STEPS; ++x) s[u] = mfma32(*reinterpret_cast<const v8bf*>(kt + u * 32 * T::ROW + (rows_at ^ (x << 5))), q[x], s[u]);
+        }
+        int gone = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) gone |= absent[tile & 1][i] << i;
+        gone = __builtin_amdgcn_readfirstlane(gone);
+        if (j0 + TILE > wave_all || gone)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+                    if (j0 + j >= sees || (gone >> (2 * u + (i >> 3)) & 1)) s[u][i] = -INFINITY;
+                }
+        float largest = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fmaxf(s[0][i], s[1][i]));
+        largest = over_halves<false>(largest);
+        if (__any((largest - top) * factor > 8.0f)) {       // see step_kernel
+            const float higher = fmaxf(top, largest), shrink = higher == -INFINITY ? 1.0f : exp2f((top - higher) * factor);
+            top = higher;
+            shift = higher == -INFINITY ? 0.0f : higher * factor - UP;
+            sum *= shrink;
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) o[d] *= shrink;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], factor, -shift));
+                part += s[u][i];
+            }
+            sum += part;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const v8bf p = operand(make_uint4(pack_bf16x2(s[u][8 * x], s[u][8 * x + 1]), pack_bf16x2(s[u][8 * x + 2], s[u][8 * x + 3]),
+                                                  pack_bf16x2(s[u][8 * x + 4], s[u][8 * x + 5]), pack_bf16x2(s[u][8 * x + 6], s[u][8 * x + 7])));
+#pragma unroll
+                for (int d = 0; d < BLOCKS; ++d) {
+                    const uint8_t* const at = vt + (u * 32 + x * 16) * T::ROW;
+                    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + (columns_at ^ (d << 6))));
+                    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * T::ROW + (columns_at ^ (d << 6) ^ 32)));
+                    o[d] = mfma32(__builtin_bit_cast(v8bf, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p, o[d]);
+                }
+            }
+        }
+    };
+
+    if (begin < end) {
+        load(begin);
+        convert(begin);
+        if (begin + 1 < end) load(begin + 1);
+        for (int tile = begin; tile < end; ++tile) {
+            __syncthreads();        // the tile is there, and nobody reads the one before
+            if (tile + 1 < end) convert(tile + 1);
+            if (tile + 2 < end) load(tile + 2);
+            if (tile * TILE < wave_most) compute(tile);
+        }
+    }
+    sum = over_halves<true>(sum);
+    if (token >= a.tokens) return;
+    const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + head;
+    if (a.splits > 1) {
+        float* const part = a.parts + (to * a.splits + split) * Part<D>::ROW;
+#pragma unroll
+        for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float2*>(part + d * 32 + 2 * i + 4 * half) = make_float2(o[d][i], o[d][i + 1]),
+                *reinterpret_cast<float2*>(part + d * 32 + 2 * i + 4 * half + 2) = make_float2(o[d][i + 2], o[d][i + 3]);
+        if (half == 0) {
+            part[D] = top * factor - UP;
+            part[D + 1] = row < rows ? sum : 0.0f;
+        }
+        return;
+    }
+    if (row >= rows) sum = 0.0f;
+    const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint2*>(a.out + to * D + d * 32 + 2 * i + 4 * half) = make_uint2(pack_bf16x2(o[d][i] * norm, o[d][i + 1] * norm), pack_bf16x2(o[d][i + 2] * norm, o[d][i + 3] * norm));
+    if (half == 0) a.lse[to] = sum == 0.0f ? -INFINITY : (shift + __builtin_amdgcn_logf(sum)) * LN2;
+#endif
+}
+
+// Rows whose entries several workgroups shared: D / 4 lanes each
+template <int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t rows) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LANES = D / 4;
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= rows) return;
+    const int at = threadIdx.x % LANES;
+    float m = -INFINITY, l = 0.0f;
+    v4f o{0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* const part = a.parts + (row * a.splits + s) * Part<D>::ROW;
+        const float2 x = *reinterpret_cast<const float2*>(part + at * 4), y = *reinterpret_cast<const float2*>(part + at * 4 + 2);
+        const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
+        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
+        o = o * fa + v4f{x.x, x.y, y.x, y.y} * fb;
+        l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? pl : pl * fb);
+        m = higher;
+    }
+    const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(a.out + row * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
+    if (at == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+#endif
+}
+
+// ---- what the entries got ------------------------------------------------------------------------------------------
+//
+// weights of entry j += sum over rows of exp(s_j - lse): the scores once more, with the entries as columns of 32 x 32 products, so that a lane adds up the
+// rows of one entry.  The units of step_kernel are shared out in the same way; a wave has 32 entries' keys in registers and goes through the rows
+// that see them, 32 at a time.  Every entry has one owner: no atomics, sums in a fixed order.
+
+template <int D>
+__global__ __launch_bounds__(WAVES * 64) void weights_kernel(const Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int STEPS = D / 16;
+    const Cache& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5;
+    const int64_t units = all_units(a, lane);
+    const int groups = (int)min((int64_t)a.groups, units);
+    if ((int)blockIdx.x >= groups) return;
+    const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
+    int before;
+    int b = sequence_of(a, begin, lane, before);
+    int length = seen_of(a, b), per_head = idx::cache4_units(length);
+    int h = (begin - before) / per_head, unit = (begin - before) % per_head;
+    const float factor = fabsf(a.scale) * LOG2E;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    for (int left = end - begin; left > 0; --left) {
+        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, j0 = unit * idx::CACHE4_UNIT + wave * ENTRIES, j = j0 + r32;
+        if (j0 < length) {
+            const int page = page_of(c, b, min(j, length - 1));
+            const bool there = j < length && page >= 0;
+            // this lane's half of its entry's elements: two groups of 32, or one; the order of the elements is the same for the queries
+            const uint8_t* const block = block_of(c, max(page, 0), h);
+            v8bf k[STEPS];
+#pragma unroll
+            for (int g = 0; g < D / 64; ++g) {
+                const uint4 x = *reinterpret_cast<const uint4*>(block + idx::cache4_codes(c.page, D, 0, j & (c.page - 1)) + half * (D / 4) + g * 16);
+                const float scale = scale_of(there ? block[idx::cache4_scales(c.page, D, 0, j & (c.page - 1)) + half * (D / 64) + g] : 0);
+                k[g * 4] = operand(decode8(x.x, scale));
+                k[g * 4 + 1] = operand(decode8(x.y, scale));
+                k[g * 4 + 2] = operand(decode8(x.z, scale));
+                k[g * 4 + 3] = operand(decode8(x.w, scale));
+            }
+            // the first token that sees the wave's first entry, and the first one that sees all of them
+            const int some = max(j0 - (length - count), 0), all = max(j0 + ENTRIES - 1 - (length - count), 0);
+            float sum = 0.0f;
+            for (int row0 = some * a.group / 32 * 32; row0 < rows; row0 += 32) {
+                const int row = row0 + r32, token = row / a.group;
+                v16f s;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+                const uint16_t* const from = a.q + b * a.q_sb + token * a.q_st + (h * a.group + row % a.group) * a.q_sh + half * (D / 2);
+                float lse = INFINITY;       // rows that are none: exp(s - inf) = 0
+                if (row < rows) lse = a.lse[((int64_t)b * a.tokens + token) * a.heads + h * a.group + row % a.group] * LOG2E;
+#pragma unroll
+                for (int x = 0; x < STEPS; ++x) {
+                    uint4 y = make_uint4(0, 0, 0, 0);
+                    if (row < rows) y = *reinterpret_cast<const uint4*>(from + x * 8);
+                    s = mfma32(operand(make_uint4(y.x ^ flip, y.y ^ flip, y.z ^ flip, y.w ^ flip)), k[x], s);
+                }
+                const bool edge = row0 < all * a.group;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = 8 * (i >> 2) + 4 * half + (i & 3);
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -__shfl(lse, at, 64)));
+                    if (!edge || j <= length - count + (row0 + at) / a.group) sum += p;
+                }
+            }
+            sum = over_halves<true>(sum);
+            if (there && half == 0) c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))] += sum;
+        }
+        if (++unit == per_head) {
+            unit = 0;
+            if (++h == c.heads && left > 1) {
+                h = 0;
+                length = seen_of(a, ++b);
+                per_head = idx::cache4_units(length);
             }
         }
     }
-    const int64_t row = ((int64_t)b * a.tokens + t) * a.heads + head;
-    if (tid < c.dim) a.out[row * c.dim + tid] = (uint16_t)f32_to_bf16_bits(l > 0.0f ? o / l : l);
-    if (tid == 0) a.lse[row] = l > 0.0f ? (m + log2f(l)) * LN2 : l == 0.0f ? -INFINITY : l;
-#endif
-}
-
-// one key per thread
-__global__ __launch_bounds__(KEYS) void weights_kernel(const Args a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float q[128];
-    const Cache& c = a.c;
-    const int blocks = (c.capacity() + KEYS - 1) / KEYS;
-    const int j = (int)(blockIdx.x % blocks) * KEYS + threadIdx.x, h = (int)(blockIdx.x / blocks) % c.heads, b = (int)(blockIdx.x / blocks) / c.heads;
-    const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), page = j < length ? page_of(c, b, j) : -1;
-    float sum = 0.0f;
-    for (int t = 0; t < count; ++t)
-        for (int g = 0; g < a.group; ++g) {
-            const int head = h * a.group + g;
-            __syncthreads();
-            if (threadIdx.x < c.dim) q[threadIdx.x] = bf16_lo(a.q[b * a.q_sb + t * a.q_st + head * a.q_sh + threadIdx.x]);
-            __syncthreads();
-            if (page < 0 || j > length - count + t) continue;
-            const float lse = a.lse[((int64_t)b * a.tokens + t) * a.heads + head] * LOG2E;
-            sum += exp2f(dot(block_of(c, page, h), c, j & (c.page - 1), q) * (a.scale * LOG2E) - lse);
-        }
-    if (page >= 0) c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))] += sum;
 #endif
 }
 
@@ -493,6 +730,28 @@ int step_groups(const Cache& c, int tiles) {
 // Row tiles of step_kernel that hold all rows of a kv head (1, 2 or 4), or 0
 int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0; }
 
+// prompt_kernel: waves of a workgroup, and how many workgroups share the entries of its rows.  Eight waves convert every entry for 256 rows; four are taken
+// where there are too few rows to give every CU eight.  Parts are worth it from 4 tiles of entries on.
+struct PromptPlan {
+    int waves, blocks, splits;
+};
+PromptPlan prompt_plan(const Cache& c, int64_t rows) {
+    const int64_t pairs = (int64_t)c.batch * c.heads, cus = device_cu_count();
+    PromptPlan p;
+    p.waves = pairs * ((rows + 255) / 256) >= cus ? 8 : 4;
+    p.blocks = (int)((rows + p.waves * 32 - 1) / (p.waves * 32));
+    const int64_t groups = pairs * p.blocks, room = cus * (8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
+    const int64_t splits = room / groups;
+    p.splits = (int)(splits < 1 ? 1 : splits < most ? splits : most);
+    return p;
+}
+int64_t workspace_bytes_of(const Cache& c, int64_t tokens, int64_t heads) {
+    const int64_t rows = tokens * (heads / c.heads);
+    if (const int tiles = step_tiles(rows)) return (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 2) * (int64_t)sizeof(float);
+    const PromptPlan p = prompt_plan(c, rows);
+    return p.splits > 1 ? c.batch * tokens * heads * p.splits * (c.dim + 2) * (int64_t)sizeof(float) : 0;
+}
+
 template <int D, int TILES>
 int launch_step(const char* fn, const Args& a, hipStream_t st) {
     hipLaunchKernelGGL((step_kernel<D, TILES>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
@@ -501,7 +760,55 @@ int launch_step(const char* fn, const Args& a, hipStream_t st) {
     return check_launch(fn);
 }
 
+template <int D, int NW>
+int prepare_prompt(const char* fn) {
+    static OncePerDevice once;
+    const hipError_t e = raise_lds_limit(once, reinterpret_cast<const void*>(prompt_kernel<D, NW>), 4 * Tile32<D>::BYTES);
+    return e == hipSuccess ? TI8_OK : fail(TI8_ERR_HIP, "%s: cannot raise the LDS limit: %s", fn, hipGetErrorString(e));
+}
+
+template <int D, int NW>
+int launch_prompt(const char* fn, const Args& a, hipStream_t st) {
+    if (int e = prepare_prompt<D, NW>(fn)) return e;
+    const int64_t grid = idx::round8((int64_t)a.c.batch * a.c.heads) * a.blocks * a.splits;
+    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)grid), dim3(NW * 64), 4 * Tile32<D>::BYTES, st, a);
+    if (int e = check_launch(fn)) return e;
+    if (a.splits == 1) return TI8_OK;
+    const int64_t rows = (int64_t)a.c.batch * a.tokens * a.heads, per = 256 / (D / 4);
+    hipLaunchKernelGGL((join_rows_kernel<D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a, rows);
+    return check_launch(fn);
+}
+
+template <int D>
+int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
+    const int64_t rows = (int64_t)a.tokens * a.group;
+    const int tiles = step_tiles(rows);
+    int e;
+    if (tiles) {
+        a.groups = step_groups(a.c, tiles);
+        e = tiles == 1 ? launch_step<D, 1>(fn, a, st) : tiles == 2 ? launch_step<D, 2>(fn, a, st) : launch_step<D, 4>(fn, a, st);
+    } else {
+        const PromptPlan p = prompt_plan(a.c, rows);
+        a.blocks = p.blocks;
+        a.splits = p.splits;
+        e = p.waves == 8 ? launch_prompt<D, 8>(fn, a, st) : launch_prompt<D, 4>(fn, a, st);
+    }
+    if (e || !accumulate) return e;
+    const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity()), most = device_cu_count() * 4;
+    a.groups = (int)(units < most ? units : most);
+    hipLaunchKernelGGL((weights_kernel<D>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
+    return check_launch(fn);
+}
+
 }  // namespace
+
+int init_attention() {
+    const char* fn = "ti8_init";
+    int e = prepare_prompt<128, 8>(fn);
+    if (!e) e = prepare_prompt<128, 4>(fn);
+    if (!e) e = prepare_prompt<64, 8>(fn);
+    return e ? e : prepare_prompt<64, 4>(fn);
+}
 
 }  // namespace cache4
 }  // namespace ti8
@@ -512,11 +819,11 @@ using namespace ti8::cache4;
 extern "C" int64_t ti8_cache4_attention_workspace(const ti8_cache4* p, int64_t tokens, int64_t heads) {
     Cache c;
     if (check("ti8_cache4_attention_workspace", p, c)) return -1;
-    if (tokens <= 0 || tokens > (1 << 24) || heads <= 0 || heads % c.heads || heads / c.heads > 4096 || c.batch * tokens * heads > 0x7fffffff ||
+    if (tokens <= 0 || tokens > (1 << 24) || heads <= 0 || heads % c.heads || heads / c.heads > 4096 || c.batch * tokens * heads > 0x3fffffff ||
         (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity()) > 0x3fffffff)
         return -1;
-    const int tiles = step_tiles(tokens * (heads / c.heads));
-    return tiles ? (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 2) * (int64_t)sizeof(float) : 0;
+    if (idx::round8((int64_t)c.batch * c.heads) * ((tokens * (heads / c.heads) + 127) / 128) > 0x3fffffff) return -1;
+    return workspace_bytes_of(c, tokens, heads);
 }
 
 extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths, const int32_t* counts, int64_t tokens, int64_t heads,
@@ -533,18 +840,8 @@ extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths,
     if (need > workspace_bytes) return fail(TI8_ERR_SHAPE, "%s: %lld bytes of workspace are needed, got %lld", fn, (long long)need, (long long)workspace_bytes);
     if (!aligned16(q) || !aligned16(out) || (reinterpret_cast<uintptr_t>(lse) & 3) || !aligned16(workspace) || q_stride_b % 8 || q_stride_t % 8 || q_stride_h % 8)
         return fail(TI8_ERR_ALIGN, "%s: q, out and the workspace must be 16-byte aligned, q's strides multiples of 8 elements", fn);
-    const int tiles = step_tiles(tokens * (heads / c.heads));
-    const Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace),
-                 (int)tokens, (int)heads, (int)(heads / c.heads), scale, tiles ? step_groups(c, tiles) : 0};
+    Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace),
+           (int)tokens, (int)heads, (int)(heads / c.heads), scale, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (tiles) {
-        const int e = c.dim == 128 ? (tiles == 1 ? launch_step<128, 1>(fn, a, st) : tiles == 2 ? launch_step<128, 2>(fn, a, st) : launch_step<128, 4>(fn, a, st))
-                                   : (tiles == 1 ? launch_step<64, 1>(fn, a, st) : tiles == 2 ? launch_step<64, 2>(fn, a, st) : launch_step<64, 4>(fn, a, st));
-        if (e) return e;
-    } else {
-        hipLaunchKernelGGL(row_kernel, dim3((unsigned)(c.batch * tokens * heads)), dim3(KEYS), 0, st, a);
-        if (int e = check_launch(fn)) return e;
-    }
-    if (accumulate) hipLaunchKernelGGL(weights_kernel, dim3((unsigned)((int64_t)c.batch * c.heads * ((c.capacity() + KEYS - 1) / KEYS))), dim3(KEYS), 0, st, a);
-    return check_launch(fn);
+    return c.dim == 128 ? launch<128>(fn, a, accumulate != 0, st) : launch<64>(fn, a, accumulate != 0, st);
 }

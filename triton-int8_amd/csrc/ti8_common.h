@@ -62,6 +62,9 @@ int init_mid_kernels();
 int init_fwht_kernels();
 int init_attention_kernels();
 int init_quant_scratch();
+namespace cache4 {
+int init_attention();
+}
 
 // ---- pieces of quant.hip and fwht.hip that the layer calls (step.hip) use ----------
 // `valid_rows` (of R, the rest counts as zeros and is not read): an activation whose token count is no multiple of the tile
