@@ -62,6 +62,16 @@ __device__ __forceinline__ int length_of(const Cache& c, const int32_t* lengths,
 __device__ __forceinline__ int start_of(const int32_t* starts, int b) { return min(max(starts[b], -(1 << 30)), 1 << 30); }
 __device__ __forceinline__ int count_of(const int32_t* counts, int b, int tokens) { return counts ? min(max(counts[b], 0), tokens) : tokens; }
 
+// sums over the lanes up to this one
+__device__ __forceinline__ int wave_prefix(int v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(v, d, 64);
+        if (lane >= d) v += x;
+    }
+    return v;
+}
+
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 #if defined(__HIP_DEVICE_COMPILE__)
 // the two bf16 that byte I of a word of codes stands for (v_cvt_scalef32_pk_bf16_fp4)

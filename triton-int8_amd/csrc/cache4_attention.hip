@@ -44,39 +44,30 @@ __device__ __forceinline__ int seen_of(const Args& a, int b) { return count_of(a
 
 // ---- sharing out ---------------------------------------------------------------------------------------------
 
-struct Share {
-    int64_t units;      // of all sequences and heads
-    int before, b;      // units in front of sequence b
-};
-__device__ __forceinline__ int wave_prefix(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(v, d, 64);
-        if (lane >= d) v += x;
-    }
-    return v;
-}
 // all units, by every wave
+template <int UNIT>
 __device__ __forceinline__ int64_t all_units(const Args& a, int lane) {
     int sum = 0;
-    for (int b = lane; b < a.c.batch; b += 64) sum += idx::cache4_units(seen_of(a, b));
+    for (int b = lane; b < a.c.batch; b += 64) sum += idx::cache4_units(seen_of(a, b), UNIT);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
     return (int64_t)__builtin_amdgcn_readfirstlane(sum) * a.c.heads;
 }
 // units of the sequences in front of b
+template <int UNIT>
 __device__ __forceinline__ int units_before(const Args& a, int b, int lane) {
     int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += idx::cache4_units(seen_of(a, i));
+    for (int i = lane; i < b; i += 64) sum += idx::cache4_units(seen_of(a, i), UNIT);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
     return __builtin_amdgcn_readfirstlane(sum) * a.c.heads;
 }
 // the sequence that a unit belongs to, and the units in front of that sequence
+template <int UNIT>
 __device__ __forceinline__ int sequence_of(const Args& a, int unit, int lane, int& before) {
     before = 0;
     for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
-        const int own = b0 + lane < a.c.batch ? idx::cache4_units(seen_of(a, b0 + lane)) * a.c.heads : 0;
+        const int own = b0 + lane < a.c.batch ? idx::cache4_units(seen_of(a, b0 + lane), UNIT) * a.c.heads : 0;
         const int upto = wave_prefix(own, lane);
         const int here = __popcll(__ballot(before + upto <= unit));        // sequences of these that end in front of the unit
         if (here < 64) {
@@ -138,13 +129,13 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
     __shared__ float stats[WAVES][2][16];
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quarter = lane >> 4;
-    const int64_t units = all_units(a, lane);
+    const int64_t units = all_units<idx::CACHE4_UNIT>(a, lane);
     const int groups = (int)min((int64_t)a.groups, units);
     if ((int)blockIdx.x >= groups) return;
     const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
     int before;
-    int b = sequence_of(a, begin, lane, before);
-    int length = seen_of(a, b), per_head = idx::cache4_units(length);
+    int b = sequence_of<idx::CACHE4_UNIT>(a, begin, lane, before);
+    int length = seen_of(a, b), per_head = idx::cache4_units(length, idx::CACHE4_UNIT);
     int h = (begin - before) / per_head, unit = (begin - before) % per_head;
     uint8_t* const mine = smem + wave * V::BYTES;
     // (a negative scale: the queries' signs are changed, which is exact.  Above zero, so that what is masked stays at -inf)
@@ -347,7 +338,7 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
         if (++h == c.heads && left > 0) {
             h = 0;
             length = seen_of(a, ++b);
-            per_head = idx::cache4_units(length);
+            per_head = idx::cache4_units(length, idx::CACHE4_UNIT);
         }
         __syncthreads();        // nobody writes values while somebody still adds up
     }
@@ -363,9 +354,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     __shared__ float shared_m[PARTS], shared_l[PARTS];
     const Cache& c = a.c;
     const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
-    const int lane = threadIdx.x & 63, per_head = idx::cache4_units(seen_of(a, b));
-    const int64_t units = all_units(a, lane);
-    const int begin = units_before(a, b, lane) + h * per_head;
+    const int lane = threadIdx.x & 63, per_head = idx::cache4_units(seen_of(a, b), idx::CACHE4_UNIT);
+    const int64_t units = all_units<idx::CACHE4_UNIT>(a, lane);
+    const int begin = units_before<idx::CACHE4_UNIT>(a, b, lane) + h * per_head;
     const int groups = (int)min((int64_t)a.groups, units);
     const int first = idx::share_of(begin, groups, units), last = idx::share_of(begin + per_head - 1, groups, units);
     if (first == last) return;
@@ -646,76 +637,139 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 // ---- what the entries got ------------------------------------------------------------------------------------------
 //
 // weights of entry j += sum over rows of exp(s_j - lse): the scores once more, with the entries as columns of 32 x 32 products, so that a lane adds up the
-// rows of one entry.  The units of step_kernel are shared out in the same way; a wave has 32 entries' keys in registers and goes through the rows
-// that see them, 32 at a time.  Every entry has one owner: no atomics, sums in a fixed order.
+// rows of one entry.  Units of 256 entries are shared out as for step_kernel; each of four waves has the keys of 64 in registers and goes through the rows
+// that see them, 32 at a time, which the workgroup brings into LDS.  Every entry has one owner: no atomics, sums in a fixed order.
+
+constexpr int COLUMNS = 64, WEIGHTS_UNIT = WAVES * COLUMNS;
 
 template <int D>
-__global__ __launch_bounds__(WAVES * 64) void weights_kernel(const Args a) {
+__global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int STEPS = D / 16;
+    constexpr int UNIT = WEIGHTS_UNIT, STEPS = D / 16, ROW = 2 * D, CHUNKS = D / 8, PASSES = 32 * CHUNKS / (WAVES * 64);
+    __shared__ __attribute__((aligned(1024))) uint8_t queries[2][32 * ROW];
+    __shared__ __attribute__((aligned(16))) float lses[2][32];
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5;
-    const int64_t units = all_units(a, lane);
+    const int64_t units = all_units<UNIT>(a, lane);
     const int groups = (int)min((int64_t)a.groups, units);
     if ((int)blockIdx.x >= groups) return;
     const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
     int before;
-    int b = sequence_of(a, begin, lane, before);
-    int length = seen_of(a, b), per_head = idx::cache4_units(length);
+    int b = sequence_of<UNIT>(a, begin, lane, before);
+    int length = seen_of(a, b), per_head = idx::cache4_units(length, UNIT);
     int h = (begin - before) / per_head, unit = (begin - before) % per_head;
     const float factor = fabsf(a.scale) * LOG2E;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    const int step_token = 32 / a.group, step_head = 32 % a.group;
     for (int left = end - begin; left > 0; --left) {
-        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, j0 = unit * idx::CACHE4_UNIT + wave * ENTRIES, j = j0 + r32;
-        if (j0 < length) {
-            const int page = page_of(c, b, min(j, length - 1));
-            const bool there = j < length && page >= 0;
-            // this lane's half of its entry's elements: two groups of 32, or one; the order of the elements is the same for the queries
-            const uint8_t* const block = block_of(c, max(page, 0), h);
-            v8bf k[STEPS];
+        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, older = length - count;      // entry older + t is token t's own
+        const int unit0 = unit * UNIT, j0 = unit0 + wave * COLUMNS;
+        // keys: a lane has half of an entry's elements, whole groups of 32 or one; the queries' elements are taken in the same order
+        v8bf k[2][STEPS];
+        int page[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int j = j0 + u * 32 + r32;
+            page[u] = j < length ? page_of(c, b, j) : -1;
+            const uint8_t* const block = block_of(c, max(page[u], 0), h);
+            const int row = j & (c.page - 1);
 #pragma unroll
             for (int g = 0; g < D / 64; ++g) {
-                const uint4 x = *reinterpret_cast<const uint4*>(block + idx::cache4_codes(c.page, D, 0, j & (c.page - 1)) + half * (D / 4) + g * 16);
-                const float scale = scale_of(there ? block[idx::cache4_scales(c.page, D, 0, j & (c.page - 1)) + half * (D / 64) + g] : 0);
-                k[g * 4] = operand(decode8(x.x, scale));
-                k[g * 4 + 1] = operand(decode8(x.y, scale));
-                k[g * 4 + 2] = operand(decode8(x.z, scale));
-                k[g * 4 + 3] = operand(decode8(x.w, scale));
+                const uint4 x = *reinterpret_cast<const uint4*>(block + idx::cache4_codes(c.page, D, 0, row) + half * (D / 4) + g * 16);
+                const uint32_t byte = block[idx::cache4_scales(c.page, D, 0, row) + half * (D / 64) + g];
+                const float scale = scale_of(page[u] >= 0 ? byte : 0);
+                k[u][g * 4] = operand(decode8(x.x, scale));
+                k[u][g * 4 + 1] = operand(decode8(x.y, scale));
+                k[u][g * 4 + 2] = operand(decode8(x.z, scale));
+                k[u][g * 4 + 3] = operand(decode8(x.w, scale));
             }
-            // the first token that sees the wave's first entry, and the first one that sees all of them
-            const int some = max(j0 - (length - count), 0), all = max(j0 + ENTRIES - 1 - (length - count), 0);
-            float sum = 0.0f;
-            for (int row0 = some * a.group / 32 * 32; row0 < rows; row0 += 32) {
-                const int row = row0 + r32, token = row / a.group;
+        }
+        // rows: from the first token that sees the unit's first entry.  A thread's rows are 32 apart from one load to the next: their tokens and heads are
+        // counted on, a division each would take as long as the scores
+        const int first = max(unit0 - older, 0) * a.group / 32 * 32;
+        struct Place {
+            int row, token, head;
+        };
+        const auto place_of = [&](int row) { return Place{row, row / a.group, row % a.group}; };
+        const auto go_on = [&](Place& p) {
+            p.row += 32;
+            p.token += step_token;
+            p.head += step_head;
+            if (p.head >= a.group) {
+                p.head -= a.group;
+                ++p.token;
+            }
+        };
+        Place at[PASSES], at_lse = place_of(first + r32);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) at[i] = place_of(first + (i * WAVES * 64 + threadIdx.x) / CHUNKS);
+        uint4 next[PASSES];
+        float next_lse;
+        const auto load = [&]() {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                next[i] = make_uint4(0, 0, 0, 0);
+                if (at[i].row < rows)
+                    next[i] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + at[i].token * a.q_st + (h * a.group + at[i].head) * a.q_sh + (threadIdx.x % CHUNKS) * 8);
+                go_on(at[i]);
+            }
+            next_lse = INFINITY;        // rows that are none: exp(s - inf) = 0
+            if (at_lse.row < rows) next_lse = a.lse[((int64_t)b * a.tokens + at_lse.token) * a.heads + h * a.group + at_lse.head] * LOG2E;
+            go_on(at_lse);
+        };
+        const auto store = [&](int buffer) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int row = (i * WAVES * 64 + threadIdx.x) / CHUNKS, chunk = threadIdx.x % CHUNKS;
+                const uint4 x = make_uint4(next[i].x ^ flip, next[i].y ^ flip, next[i].z ^ flip, next[i].w ^ flip);
+                *reinterpret_cast<uint4*>(queries[buffer] + row * ROW + ((chunk ^ Values<D>::swizzle(row)) << 4)) = x;
+            }
+            if (threadIdx.x < 32) lses[buffer][threadIdx.x] = next_lse;
+        };
+        float sum[2] = {0.0f, 0.0f};
+        if (first < rows) load();
+        __syncthreads();        // (nobody reads the last unit's queries any more)
+        if (first < rows) store(0);
+        for (int row0 = first, buffer = 0; row0 < rows; row0 += 32, buffer ^= 1) {
+            if (row0 + 32 < rows) load();
+            __syncthreads();
+            const uint8_t* const from = queries[buffer] + r32 * ROW;
+            const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int ju = j0 + u * 32;
+                // somebody of these rows sees one of the 32 entries
+                if (ju >= length || (row0 + 32) <= (ju - older) * a.group) continue;
                 v16f s;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-                const uint16_t* const from = a.q + b * a.q_sb + token * a.q_st + (h * a.group + row % a.group) * a.q_sh + half * (D / 2);
-                float lse = INFINITY;       // rows that are none: exp(s - inf) = 0
-                if (row < rows) lse = a.lse[((int64_t)b * a.tokens + token) * a.heads + h * a.group + row % a.group] * LOG2E;
 #pragma unroll
-                for (int x = 0; x < STEPS; ++x) {
-                    uint4 y = make_uint4(0, 0, 0, 0);
-                    if (row < rows) y = *reinterpret_cast<const uint4*>(from + x * 8);
-                    s = mfma32(operand(make_uint4(y.x ^ flip, y.y ^ flip, y.z ^ flip, y.w ^ flip)), k[x], s);
-                }
-                const bool edge = row0 < all * a.group;
+                for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(from + ((chunk ^ x) << 4)), k[u][x], s);
+                const bool edge = row0 < (ju + 31 - older) * a.group;       // not every row sees every entry
+                const int sees = (ju + r32 - older) * a.group;              // the first row that sees this lane's
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = 8 * (i >> 2) + 4 * half + (i & 3);
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -__shfl(lse, at, 64)));
-                    if (!edge || j <= length - count + (row0 + at) / a.group) sum += p;
+                for (int g = 0; g < 4; ++g) {
+                    const v4f lse = *reinterpret_cast<const v4f*>(lses[buffer] + 8 * g + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -lse[i]));
+                        if (!edge || row0 + 8 * g + 4 * half + i >= sees) sum[u] += p;
+                    }
                 }
             }
-            sum = over_halves<true>(sum);
-            if (there && half == 0) c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))] += sum;
+            if (row0 + 32 < rows) store(buffer ^ 1);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float total = over_halves<true>(sum[u]);
+            if (page[u] >= 0 && half == 0) c.weights[((int64_t)page[u] * c.heads + h) * c.page + ((j0 + u * 32 + r32) & (c.page - 1))] += total;
         }
         if (++unit == per_head) {
             unit = 0;
             if (++h == c.heads && left > 1) {
                 h = 0;
                 length = seen_of(a, ++b);
-                per_head = idx::cache4_units(length);
+                per_head = idx::cache4_units(length, UNIT);
             }
         }
     }
@@ -724,7 +778,7 @@ __global__ __launch_bounds__(WAVES * 64) void weights_kernel(const Args a) {
 
 // Workgroups of step_kernel: as many as run at a time (four per CU with 16 rows, which the registers allow, two otherwise), and no more than there are units
 int step_groups(const Cache& c, int tiles) {
-    const int64_t units = (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity()), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
+    const int64_t units = (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity(), idx::CACHE4_UNIT), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
     return (int)(units < most ? units : most);
 }
 // Row tiles of step_kernel that hold all rows of a kv head (1, 2 or 4), or 0
@@ -794,7 +848,7 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
         e = p.waves == 8 ? launch_prompt<D, 8>(fn, a, st) : launch_prompt<D, 4>(fn, a, st);
     }
     if (e || !accumulate) return e;
-    const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity()), most = device_cu_count() * 4;
+    const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity(), WEIGHTS_UNIT), most = device_cu_count() * 6;
     a.groups = (int)(units < most ? units : most);
     hipLaunchKernelGGL((weights_kernel<D>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
     return check_launch(fn);
@@ -820,7 +874,7 @@ extern "C" int64_t ti8_cache4_attention_workspace(const ti8_cache4* p, int64_t t
     Cache c;
     if (check("ti8_cache4_attention_workspace", p, c)) return -1;
     if (tokens <= 0 || tokens > (1 << 24) || heads <= 0 || heads % c.heads || heads / c.heads > 4096 || c.batch * tokens * heads > 0x3fffffff ||
-        (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity()) > 0x3fffffff)
+        (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) > 0x3fffffff)
         return -1;
     if (idx::round8((int64_t)c.batch * c.heads) * ((tokens * (heads / c.heads) + 127) / 128) > 0x3fffffff) return -1;
     return workspace_bytes_of(c, tokens, heads);

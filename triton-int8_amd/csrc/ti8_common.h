@@ -63,6 +63,7 @@ int init_fwht_kernels();
 int init_attention_kernels();
 int init_quant_scratch();
 namespace cache4 {
+int init();
 int init_attention();
 }
 
