@@ -199,7 +199,7 @@ _native = None  # the extension module, False where there is none
 
 
 def native():
-    """The layer call's host side in C++ (``csrc/native.cpp``) on the entry points of :func:`lib`, or None: while calls are being timed
+    """The layer call's and the cache calls' host side in C++ (``csrc/native.cpp``) on the entry points of :func:`lib`, or None: while calls are being timed
     one by one, and where there is none or it was built for another torch, Python or argument block (the same launches are then made
     from Python)."""
     global _native
@@ -211,12 +211,13 @@ def native():
         try:
             spec = importlib.util.spec_from_file_location("_native", NATIVE_PATH)
             module = importlib.util.module_from_spec(spec)
-            here = (str(torch.__version__), sys.version_info[:2], ctypes.sizeof(LinearArgs), ctypes.sizeof(GemmProblem))
+            here = (str(torch.__version__), sys.version_info[:2], ctypes.sizeof(LinearArgs), ctypes.sizeof(GemmProblem), ctypes.sizeof(Cache4))
             built_for = getattr(module, "built_for", None)
             if built_for != here:
                 raise ImportError(f"{NATIVE_PATH} was built for {built_for}, this is {here}")
             address = lambda name: ctypes.cast(getattr(lib(), name), _vp).value
             module.set_up(address("ti8_linear"), address("ti8_linear_quantise"), address("ti8_gemm_i8_nt_multi"), torch.nn.Parameter)
+            module.set_up_cache4(*(address("ti8_cache4_" + name) for name in ("append", "read", "attention", "attention_workspace", "evict")))
             _native = module
         except ImportError:
             lib()

@@ -68,9 +68,22 @@ def _rows(x, name):
     return x, (sb, ss, sh)
 
 
+def _natively(name, *args):
+    """A call with its checks, allocations and launches made from C++, or None where it takes the Python way, which says what is wrong."""
+    native = _lib.native()
+    if native is None:
+        return None
+    out = getattr(native, name)(*args, _stream())
+    if type(out) is tuple:
+        raise _lib.failed(*out)
+    return out
+
+
 def append(pool, table, starts, k, v, counts=None, weights=None):
     """Keys and values of new tokens, bf16 [batch, tokens, kv_heads, head_dim], become entries ``starts[b]``, ``starts[b] + 1``, .. of each sequence;
     of sequence b the first ``counts[b]`` tokens (all of them without ``counts``).  The new entries' ``weights``, if given, become zero."""
+    if _natively("cache4_append", pool, table, starts, k, v, counts, weights):
+        return
     k, at_k = _rows(k, "k")
     v, at_v = _rows(v, "v")
     B, S, H, D = k.shape
@@ -83,6 +96,9 @@ def append(pool, table, starts, k, v, counts=None, weights=None):
 def read(pool, table, starts, tokens, head_dim, counts=None):
     """The values that entries ``starts[b]`` .. of each sequence stand for: (keys, values), bf16 [batch, tokens, kv_heads, head_dim], zeros from the
     ``counts[b]``-th on and where the sequence's pages end."""
+    made = _natively("cache4_read", pool, table, starts, counts, tokens, head_dim)
+    if made is not None:
+        return tuple(made)
     _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[0] > 0, "table must be an int32 tensor [batch, pages]")
     _need(isinstance(tokens, int) and tokens > 0, f"tokens must be a positive number, got {tokens}")
     B = table.shape[0]
@@ -99,6 +115,9 @@ def attention(pool, table, lengths, q, counts=None, scale=None, weights=None):
 
     Returns (out bf16 like q, lse float32 [batch, tokens, heads], the logarithms of the sums of the exponentials); rows that see nothing and rows that
     are no queries are zeros with an lse of -inf.  With ``weights``, every entry's probabilities over queries and heads are added to its weight."""
+    made = _natively("cache4_attention", pool, table, lengths, q, counts, weights, scale)
+    if made is not None:
+        return tuple(made)
     q, at_q = _rows(q, "q")
     B, S, H, D = q.shape
     c = _cache(pool, table, weights, D, B)
@@ -121,6 +140,9 @@ def evict(pool, table, lengths, weights, new_table, *, keep, recent):
     others than the sequences' present ones, which are only read.  Sequences of up to ``keep`` entries move as they are.
 
     Returns (kept int32 [batch, kv_heads, keep], which entry each of them was, -1 behind the last; the new lengths int32 [batch])."""
+    made = _natively("cache4_evict", pool, table, lengths, weights, new_table, keep, recent)
+    if made is not None:
+        return tuple(made)
     _need(isinstance(table, torch.Tensor) and table.dim() == 2 and table.shape[0] > 0, "table must be an int32 tensor [batch, pages]")
     _need(isinstance(weights, torch.Tensor) and weights.dim() == 3 and isinstance(pool, torch.Tensor) and pool.dim() == 3 and weights.shape[2] > 0,
           "weights must be a float32 tensor [pages, kv_heads, page_size]")
