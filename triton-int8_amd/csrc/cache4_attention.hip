@@ -44,40 +44,52 @@ __device__ __forceinline__ int seen_of(const Args& a, int b) { return count_of(a
 
 // ---- sharing out ---------------------------------------------------------------------------------------------
 
-// all units, by every wave
-template <int UNIT>
-__device__ __forceinline__ int64_t all_units(const Args& a, int lane) {
-    int sum = 0;
-    for (int b = lane; b < a.c.batch; b += 64) sum += idx::cache4_units(seen_of(a, b), UNIT);
+// What a workgroup has of the units, or a (sequence, head): found by every wave from the lengths, the first 64 of which are read once
+template <int UNIT, int EXTRA>     // EXTRA units of every head stand for what beginning and ending it takes
+struct Lengths {
+    const Args& a;
+    const int lane;
+    const int first;        // units of a head of sequence `lane`
+    __device__ __forceinline__ Lengths(const Args& a_, int lane_) : a(a_), lane(lane_), first(of(lane_)) {}
+    __device__ __forceinline__ int of(int b) const { return b < a.c.batch ? idx::cache4_units(seen_of(a, b), UNIT) + EXTRA : 0; }
+    __device__ __forceinline__ int chunk(int b0) const { return b0 ? of(b0 + lane) : first; }
+    __device__ __forceinline__ static int sum(int v) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    return (int64_t)__builtin_amdgcn_readfirstlane(sum) * a.c.heads;
-}
-// units of the sequences in front of b
-template <int UNIT>
-__device__ __forceinline__ int units_before(const Args& a, int b, int lane) {
-    int sum = 0;
-    for (int i = lane; i < b; i += 64) sum += idx::cache4_units(seen_of(a, i), UNIT);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    return __builtin_amdgcn_readfirstlane(sum) * a.c.heads;
-}
-// the sequence that a unit belongs to, and the units in front of that sequence
-template <int UNIT>
-__device__ __forceinline__ int sequence_of(const Args& a, int unit, int lane, int& before) {
-    before = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
-        const int own = b0 + lane < a.c.batch ? idx::cache4_units(seen_of(a, b0 + lane), UNIT) * a.c.heads : 0;
-        const int upto = wave_prefix(own, lane);
-        const int here = __popcll(__ballot(before + upto <= unit));        // sequences of these that end in front of the unit
-        if (here < 64) {
-            before += __builtin_amdgcn_readfirstlane(here ? __shfl(upto, max(here - 1, 0), 64) : 0);
-            return b0 + here;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+        return __builtin_amdgcn_readfirstlane(v);
     }
-    return a.c.batch;
-}
+    __device__ __forceinline__ int all() const {
+        int n = first;
+        for (int b0 = 64; b0 < a.c.batch; b0 += 64) n += chunk(b0);
+        return sum(n) * a.c.heads;
+    }
+    // units in front of sequence b; `own`: those of one of its heads
+    __device__ __forceinline__ int before(int b, int& own) const {
+        int n = 0;
+        for (int b0 = 0; b0 <= b; b0 += 64) {
+            const int x = chunk(b0);
+            n += b0 + lane < b ? x : 0;
+            if (b - b0 < 64) own = __builtin_amdgcn_readlane(x, b - b0);
+        }
+        return sum(n) * a.c.heads;
+    }
+    // the sequence that a unit belongs to, the units in front of that sequence and those of one of its heads
+    __device__ __forceinline__ int find(int unit, int& before, int& own) const {
+        before = 0;
+        for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
+            const int x = chunk(b0), upto = wave_prefix(x, lane) * a.c.heads;
+            const int here = __popcll(__ballot(before + upto <= unit));        // sequences of these that end in front of the unit
+            if (here < 64 && b0 + here < a.c.batch) {
+                before += here ? __builtin_amdgcn_readlane(upto, here - 1) : 0;
+                own = __builtin_amdgcn_readlane(x, here);
+                return b0 + here;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+        own = 1;
+        return a.c.batch;
+    }
+};
 
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ v4f mfma16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -113,10 +125,12 @@ struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 
 
 template <int D>
 struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e), less UP) and sums of its rows
-    static constexpr int ROW = D + 2;
+    static constexpr int ROW = D + 4;       // (16-byte aligned)
 };
 
 constexpr int WAVES = 4, ENTRIES = 32;      // waves of a workgroup; entries of a wave's turn
+// Units that beginning and ending a head count for when the units are shared out.  TUNE
+constexpr int EXTRA = 2;
 static_assert(idx::CACHE4_UNIT == WAVES * ENTRIES, "a unit is a turn of every wave");
 
 template <int D, int TILES>     // TILES * 16 rows
@@ -129,39 +143,24 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
     __shared__ float stats[WAVES][2][16];
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quarter = lane >> 4;
-    const int64_t units = all_units<idx::CACHE4_UNIT>(a, lane);
-    const int groups = (int)min((int64_t)a.groups, units);
-    if ((int)blockIdx.x >= groups) return;
-    const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
-    int before;
-    int b = sequence_of<idx::CACHE4_UNIT>(a, begin, lane, before);
-    int length = seen_of(a, b), per_head = idx::cache4_units(length, idx::CACHE4_UNIT);
-    int h = (begin - before) / per_head, unit = (begin - before) % per_head;
+    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, lane);
+    const idx::Share share = idx::share_out(lengths.all(), a.groups);
+    if ((int)blockIdx.x >= share.groups) return;
+    const int begin = idx::share_begin(share, blockIdx.x), end = idx::share_begin(share, blockIdx.x + 1);
+    int before, per_head, b = lengths.find(begin, before, per_head);
+    int length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
+    const int at_begin = (begin - before) % per_head;
+    int h = (begin - before) / per_head, unit = max(at_begin - EXTRA, 0);
+    per_head -= EXTRA;
     uint8_t* const mine = smem + wave * V::BYTES;
     // (a negative scale: the queries' signs are changed, which is exact.  Above zero, so that what is masked stays at -inf)
     const float factor = fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 
-    for (int left = end - begin; left > 0;) {
+    for (int left = end - begin - max(EXTRA - at_begin, 0); left > 0;) {
         const int n = min(left, per_head - unit), first = unit * WAVES + wave, last = (unit + n) * WAVES;       // this wave's turns
         const int count = count_of(a.counts, b, a.tokens), rows = count * a.group;
         const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
-        // this wave's queries as operands, and up to where each row sees
-        v8bf q[TILES][STEPS];
-        int sees[TILES];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const int row = t * 16 + r16, token = row / a.group, head = h * a.group + row % a.group;
-            sees[t] = row < rows ? length - count + token + 1 : 0;
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + token * a.q_st + head * a.q_sh + quarter * (D / 4) + s * 8);
-                q[t][s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
-            }
-        }
-        const int all_see = length - count + 1;         // entries that every row sees
-
         struct Turn {
             uint32_t k[2][STEPS], v[2][STEPS], ks[2], vs[2];
             int absent;     // a bit for each 16 whose page the pool does not have
@@ -196,6 +195,28 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
             const bool one = (unsigned)page[0] < (unsigned)c.pages, two = (unsigned)page[1] < (unsigned)c.pages;
             x.absent = (one || j >= length ? 0 : 1) | (two || j + 16 >= length ? 0 : 2);
         };
+
+        Turn now;
+        int page[2];
+        pages_of(first, page);
+        if (first < last) load(first, page, now);
+        pages_of(min(first + WAVES, last - 1), page);
+
+        // this wave's queries as operands, and up to where each row sees
+        v8bf q[TILES][STEPS];
+        int sees[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int row = t * 16 + r16, token = row / a.group, head = h * a.group + row % a.group;
+            sees[t] = row < rows ? length - count + token + 1 : 0;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + token * a.q_st + head * a.q_sh + quarter * (D / 4) + s * 8);
+                q[t][s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
+            }
+        }
+        const int all_see = length - count + 1;         // entries that every row sees
 
         v4f o[TILES][BLOCKS];
         float top[TILES], shift[TILES], sum[TILES];      // maximum, what is taken from a score times factor, sum of this lane's entries
@@ -272,18 +293,12 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
             asm volatile("" ::: "memory");
         };
 
-        if (first < last) {
-            Turn now, next;
-            int page[2];
-            pages_of(first, page);
-            load(first, page, now);
-            pages_of(min(first + WAVES, last - 1), page);
-            for (int turn = first; turn < last; turn += WAVES) {
-                if (turn + WAVES < last) load(turn + WAVES, page, next);
-                pages_of(min(turn + 2 * WAVES, last - 1), page);
-                compute(turn, now);
-                now = next;
-            }
+        for (int turn = first; turn < last; turn += WAVES) {
+            Turn next;
+            if (turn + WAVES < last) load(turn + WAVES, page, next);
+            pages_of(min(turn + 2 * WAVES, last - 1), page);
+            compute(turn, now);
+            now = next;
         }
 
         // the waves' results meet in LDS, 16 rows at a time
@@ -322,22 +337,22 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
                 v4f x{0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) x += *reinterpret_cast<const v4f*>(smem + w * V::BYTES + row * (4 * D) + ((chunk ^ row) << 4)) * f[w];
-                if (!whole) *reinterpret_cast<v4f*>(part + at * Part<D>::ROW + chunk * 4) = x;
-                else if (at < a.tokens * a.group)
+                if (!whole) {
+                    if (at < rows) *reinterpret_cast<v4f*>(part + at * Part<D>::ROW + chunk * 4) = x;
+                } else if (at < a.tokens * a.group)
                     *reinterpret_cast<uint2*>(a.out + to * D + chunk * 4) = make_uint2(pack_bf16x2(x[0] * norm, x[1] * norm), pack_bf16x2(x[2] * norm, x[3] * norm));
             }
             if ((threadIdx.x & 15) == 0) {
                 if (!whole) {
-                    part[at * Part<D>::ROW + D] = m * factor - UP;
-                    part[at * Part<D>::ROW + D + 1] = l;
+                    if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor - UP, l);
                 } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor - UP + __builtin_amdgcn_logf(l)) * LN2;
             }
         }
-        left -= n;
+        left -= n + EXTRA;
         unit = 0;
         if (++h == c.heads && left > 0) {
             h = 0;
-            length = seen_of(a, ++b);
+            length = __builtin_amdgcn_readfirstlane(seen_of(a, ++b));
             per_head = idx::cache4_units(length, idx::CACHE4_UNIT);
         }
         __syncthreads();        // nobody writes values while somebody still adds up
@@ -354,18 +369,20 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     __shared__ float shared_m[PARTS], shared_l[PARTS];
     const Cache& c = a.c;
     const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
-    const int lane = threadIdx.x & 63, per_head = idx::cache4_units(seen_of(a, b), idx::CACHE4_UNIT);
-    const int64_t units = all_units<idx::CACHE4_UNIT>(a, lane);
-    const int begin = units_before<idx::CACHE4_UNIT>(a, b, lane) + h * per_head;
-    const int groups = (int)min((int64_t)a.groups, units);
-    const int first = idx::share_of(begin, groups, units), last = idx::share_of(begin + per_head - 1, groups, units);
+    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, threadIdx.x & 63);
+    const idx::Share share = idx::share_out(lengths.all(), a.groups);
+    int per_head;
+    int begin = lengths.before(b, per_head);
+    begin += h * per_head + EXTRA;
+    per_head -= EXTRA;
+    const int first = idx::share_of(share, begin), last = idx::share_of(share, begin + per_head - 1);
     if (first == last) return;
     const int own = threadIdx.x / LANES, at = threadIdx.x % LANES;
     float m = -INFINITY, l = 0.0f;
     v4f o{0, 0, 0, 0};
     for (int w = first + own; w <= last; w += PARTS) {
         // a workgroup's second part is the one that starts with the head's first unit
-        const float* const part = a.parts + (((int64_t)w * 2 + (idx::share_begin(w, groups, units) <= begin)) * (TILES * 16) + row) * Part<D>::ROW;
+        const float* const part = a.parts + (((int64_t)w * 2 + (idx::share_begin(share, w) <= begin)) * (TILES * 16) + row) * Part<D>::ROW;
         const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
         const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
         const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
@@ -388,7 +405,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
         m = higher;
     }
     const int64_t to = ((int64_t)b * a.tokens + row / a.group) * a.heads + h * a.group + row % a.group;
-    if (row / a.group >= count_of(a.counts, b, a.tokens)) l = 0.0f;
+    if (row / a.group >= count_of(a.counts, b, a.tokens)) {       // no query, and no parts
+        l = 0.0f;
+        o = v4f{0, 0, 0, 0};
+    }
     const float norm = l == 0.0f ? 0.0f : 1.0f / l;
     *reinterpret_cast<uint2*>(a.out + to * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
     if (at == 0) a.lse[to] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
@@ -590,8 +610,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float2*>(part + d * 32 + 2 * i + 4 * half) = make_float2(o[d][i], o[d][i + 1]),
-                *reinterpret_cast<float2*>(part + d * 32 + 2 * i + 4 * half + 2) = make_float2(o[d][i + 2], o[d][i + 3]);
+                *reinterpret_cast<v4f*>(part + d * 32 + 2 * i + 4 * half) = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
         if (half == 0) {
             part[D] = top * factor - UP;
             part[D + 1] = row < rows ? sum : 0.0f;
@@ -621,10 +640,10 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
     v4f o{0, 0, 0, 0};
     for (int s = 0; s < a.splits; ++s) {
         const float* const part = a.parts + (row * a.splits + s) * Part<D>::ROW;
-        const float2 x = *reinterpret_cast<const float2*>(part + at * 4), y = *reinterpret_cast<const float2*>(part + at * 4 + 2);
+        const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
         const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
         const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
-        o = o * fa + v4f{x.x, x.y, y.x, y.y} * fb;
+        o = o * fa + x * fb;
         l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? pl : pl * fb);
         m = higher;
     }
@@ -650,13 +669,12 @@ __global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
     __shared__ __attribute__((aligned(16))) float lses[2][32];
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5;
-    const int64_t units = all_units<UNIT>(a, lane);
-    const int groups = (int)min((int64_t)a.groups, units);
-    if ((int)blockIdx.x >= groups) return;
-    const int begin = idx::share_begin(blockIdx.x, groups, units), end = idx::share_begin(blockIdx.x + 1, groups, units);
-    int before;
-    int b = sequence_of<UNIT>(a, begin, lane, before);
-    int length = seen_of(a, b), per_head = idx::cache4_units(length, UNIT);
+    const Lengths<UNIT, 0> lengths(a, lane);
+    const idx::Share share = idx::share_out(lengths.all(), a.groups);
+    if ((int)blockIdx.x >= share.groups) return;
+    const int begin = idx::share_begin(share, blockIdx.x), end = idx::share_begin(share, blockIdx.x + 1);
+    int before, per_head, b = lengths.find(begin, before, per_head);
+    int length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
     int h = (begin - before) / per_head, unit = (begin - before) % per_head;
     const float factor = fabsf(a.scale) * LOG2E;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -768,7 +786,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
             unit = 0;
             if (++h == c.heads && left > 1) {
                 h = 0;
-                length = seen_of(a, ++b);
+                length = __builtin_amdgcn_readfirstlane(seen_of(a, ++b));
                 per_head = idx::cache4_units(length, UNIT);
             }
         }
@@ -778,7 +796,7 @@ __global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
 
 // Workgroups of step_kernel: as many as run at a time (four per CU with 16 rows, which the registers allow, two otherwise), and no more than there are units
 int step_groups(const Cache& c, int tiles) {
-    const int64_t units = (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity(), idx::CACHE4_UNIT), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
+    const int64_t units = (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
     return (int)(units < most ? units : most);
 }
 // Row tiles of step_kernel that hold all rows of a kv head (1, 2 or 4), or 0
@@ -801,9 +819,9 @@ PromptPlan prompt_plan(const Cache& c, int64_t rows) {
 }
 int64_t workspace_bytes_of(const Cache& c, int64_t tokens, int64_t heads) {
     const int64_t rows = tokens * (heads / c.heads);
-    if (const int tiles = step_tiles(rows)) return (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 2) * (int64_t)sizeof(float);
+    if (const int tiles = step_tiles(rows)) return (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 4) * (int64_t)sizeof(float);
     const PromptPlan p = prompt_plan(c, rows);
-    return p.splits > 1 ? c.batch * tokens * heads * p.splits * (c.dim + 2) * (int64_t)sizeof(float) : 0;
+    return p.splits > 1 ? c.batch * tokens * heads * p.splits * (c.dim + 4) * (int64_t)sizeof(float) : 0;
 }
 
 template <int D, int TILES>
@@ -874,7 +892,7 @@ extern "C" int64_t ti8_cache4_attention_workspace(const ti8_cache4* p, int64_t t
     Cache c;
     if (check("ti8_cache4_attention_workspace", p, c)) return -1;
     if (tokens <= 0 || tokens > (1 << 24) || heads <= 0 || heads % c.heads || heads / c.heads > 4096 || c.batch * tokens * heads > 0x3fffffff ||
-        (int64_t)c.batch * c.heads * idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) > 0x3fffffff)
+        (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA) > 0x3fffffff)
         return -1;
     if (idx::round8((int64_t)c.batch * c.heads) * ((tokens * (heads / c.heads) + 127) / 128) > 0x3fffffff) return -1;
     return workspace_bytes_of(c, tokens, heads);

@@ -464,14 +464,24 @@ TI8_HD int cache4_block_bytes(int page, int dim) { return page * (dim + dim / 16
 TI8_HD int cache4_codes(int page, int dim, int values, int row) { return values * page * (dim / 2) + row * (dim / 2); }
 TI8_HD int cache4_scales(int page, int dim, int values, int row) { return page * dim + values * page * (dim / 32) + row * (dim / 32); }
 TI8_HD int log2_of(int page) { return page <= 16 ? 4 : page <= 32 ? 5 : page <= 64 ? 6 : page <= 128 ? 7 : 8; }
-// Attention of few rows: the entries of every (sequence, kv head) in units (of 128 for the attention, 256 for the weights), one behind the other (sequence, head, unit), are shared out evenly
-// among the workgroups, whatever the lengths: workgroup w of `groups` has units [share_begin(w), share_begin(w + 1)).  Products stay below 2^63: `units`
-// and `groups` are below 2^31.
+// Attention of few rows: the entries of every (sequence, kv head) in units (of 128 for the attention, 256 for the weights), one behind the other
+// (sequence, head, unit), are shared out evenly among the workgroups, whatever the lengths: the first `more` of `groups` workgroups have each + 1 units,
+// the others `each` (groups <= units, so nobody has none).
 constexpr int CACHE4_UNIT = 128;
 TI8_HD int cache4_units(int length, int unit) { return length <= unit ? 1 : (length + unit - 1) / unit; }     // a sequence without entries has one, too
-TI8_HD int share_begin(int w, int groups, int64_t units) { return (int)((int64_t)w * units / groups); }
+struct Share {
+    int groups, each, more;
+};
+TI8_HD Share share_out(int units, int groups) {
+    const int n = imin(groups, units), each = units / n;
+    return Share{n, each, units - each * n};
+}
+TI8_HD int share_begin(const Share& s, int w) { return w * s.each + imin(w, s.more); }
 // the workgroup that has a unit
-TI8_HD int share_of(int unit, int groups, int64_t units) { return (int)(((int64_t)(unit + 1) * groups - 1) / units); }
+TI8_HD int share_of(const Share& s, int unit) {
+    const int longer = s.more * (s.each + 1);
+    return unit < longer ? unit / (s.each + 1) : s.more + (unit - longer) / s.each;
+}
 
 // ---- which kernel an entry point launches (decided on the host) ------------------------------
 
