@@ -145,7 +145,7 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
         __syncthreads();
         // from the largest bin on: a thread has two neighbours
         const int top = BINS - 1 - 2 * tid, x = bins[top], y = bins[top - 1];
-        int upto = wave_prefix(x + y, lane);
+        int upto = wave_prefix(x + y);
         if (lane == 63) sums[0][wave] = upto;
         __syncthreads();
         for (int w = 0; w < wave; ++w) upto += sums[0][w];

@@ -49,45 +49,39 @@ template <int UNIT, int EXTRA>     // EXTRA units of every head stand for what b
 struct Lengths {
     const Args& a;
     const int lane;
-    const int first;        // units of a head of sequence `lane`
-    __device__ __forceinline__ Lengths(const Args& a_, int lane_) : a(a_), lane(lane_), first(of(lane_)) {}
+    const int first, upto;      // units of a head of sequence `lane`, and of those up to it
+    __device__ __forceinline__ Lengths(const Args& a_, int lane_) : a(a_), lane(lane_), first(of(lane_)), upto(wave_prefix(first)) {}
     __device__ __forceinline__ int of(int b) const { return b < a.c.batch ? idx::cache4_units(seen_of(a, b), UNIT) + EXTRA : 0; }
-    __device__ __forceinline__ int chunk(int b0) const { return b0 ? of(b0 + lane) : first; }
-    __device__ __forceinline__ static int sum(int v) {
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-        return __builtin_amdgcn_readfirstlane(v);
-    }
+    __device__ __forceinline__ static int last(int v) { return __builtin_amdgcn_readlane(v, 63); }
     __device__ __forceinline__ int all() const {
-        int n = first;
-        for (int b0 = 64; b0 < a.c.batch; b0 += 64) n += chunk(b0);
-        return sum(n) * a.c.heads;
+        int n = last(upto);
+        for (int b0 = 64; b0 < a.c.batch; b0 += 64) n += last(wave_prefix(of(b0 + lane)));
+        return n * a.c.heads;
     }
     // units in front of sequence b; `own`: those of one of its heads
     __device__ __forceinline__ int before(int b, int& own) const {
-        int n = 0;
-        for (int b0 = 0; b0 <= b; b0 += 64) {
-            const int x = chunk(b0);
-            n += b0 + lane < b ? x : 0;
-            if (b - b0 < 64) own = __builtin_amdgcn_readlane(x, b - b0);
+        int n = 0, b0 = 0, x = first, up = upto;
+        for (; b - b0 >= 64; b0 += 64) {
+            n += last(up);
+            x = of(b0 + 64 + lane);
+            up = wave_prefix(x);
         }
-        return sum(n) * a.c.heads;
+        own = __builtin_amdgcn_readlane(x, b - b0);
+        return (n + __builtin_amdgcn_readlane(up, b - b0) - own) * a.c.heads;
     }
     // the sequence that a unit belongs to, the units in front of that sequence and those of one of its heads
     __device__ __forceinline__ int find(int unit, int& before, int& own) const {
-        before = 0;
-        for (int b0 = 0; b0 < a.c.batch; b0 += 64) {
-            const int x = chunk(b0), upto = wave_prefix(x, lane) * a.c.heads;
-            const int here = __popcll(__ballot(before + upto <= unit));        // sequences of these that end in front of the unit
-            if (here < 64 && b0 + here < a.c.batch) {
-                before += here ? __builtin_amdgcn_readlane(upto, here - 1) : 0;
-                own = __builtin_amdgcn_readlane(x, here);
-                return b0 + here;
-            }
-            before += __builtin_amdgcn_readlane(upto, 63);
+        int n = 0, b0 = 0, x = first, up = upto;
+        while ((n + last(up)) * a.c.heads <= unit) {       // (a unit is below all(), so the walk ends with the sequences)
+            n += last(up);
+            b0 += 64;
+            x = of(b0 + lane);
+            up = wave_prefix(x);
         }
-        own = 1;
-        return a.c.batch;
+        const int here = __popcll(__ballot((n + up) * a.c.heads <= unit));        // sequences of these that end in front of the unit
+        own = __builtin_amdgcn_readlane(x, here);
+        before = (n + __builtin_amdgcn_readlane(up, here) - own) * a.c.heads;
+        return b0 + here;
     }
 };
 
@@ -656,17 +650,31 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 // ---- what the entries got ------------------------------------------------------------------------------------------
 //
 // weights of entry j += sum over rows of exp(s_j - lse): the scores once more, with the entries as columns of 32 x 32 products, so that a lane adds up the
-// rows of one entry.  Units of 256 entries are shared out as for step_kernel; each of four waves has the keys of 64 in registers and goes through the rows
-// that see them, 32 at a time, which the workgroup brings into LDS.  Every entry has one owner: no atomics, sums in a fixed order.
+// rows of one entry.  Units of 256 entries are shared out as for step_kernel; each of eight waves has the keys of 32 in registers and goes through the rows
+// that see them, which the workgroup brings into LDS 64 at a time, two tiles ahead, without a trip through registers.  Every entry has one owner: no
+// atomics, sums in a fixed order.  Bound by latency where there are few rows or few workgroups: a wave's products and exponentials take turns, so there are
+// many waves.
 
-constexpr int COLUMNS = 64, WEIGHTS_UNIT = WAVES * COLUMNS;
+constexpr int COLUMNS = 32, WEIGHT_WAVES = 8, WEIGHTS_UNIT = WEIGHT_WAVES * COLUMNS, ROWS = 64, RING = 3;
+
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef __attribute__((address_space(3))) void lds_void;
+// all but this wave's last N loads have landed, its LDS reads have returned, and the same holds for the other waves
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 0xf) | ((N >> 4) << 14) | 0x0070);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+#endif
 
 template <int D>
-__global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
+__global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int UNIT = WEIGHTS_UNIT, STEPS = D / 16, ROW = 2 * D, CHUNKS = D / 8, PASSES = 32 * CHUNKS / (WAVES * 64);
-    __shared__ __attribute__((aligned(1024))) uint8_t queries[2][32 * ROW];
-    __shared__ __attribute__((aligned(16))) float lses[2][32];
+    constexpr int UNIT = WEIGHTS_UNIT, STEPS = D / 16, ROW = 2 * D, CHUNKS = D / 8, PASSES = ROWS * CHUNKS / (WEIGHT_WAVES * 64), LOADS = PASSES + 1;
+    __shared__ __attribute__((aligned(1024))) uint8_t queries[RING][ROWS * ROW];
+    __shared__ __attribute__((aligned(1024))) float lses[RING][WEIGHT_WAVES][ROWS];       // every wave has its own
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5;
     const Lengths<UNIT, 0> lengths(a, lane);
@@ -678,110 +686,127 @@ __global__ __launch_bounds__(WAVES * 64, 3) void weights_kernel(const Args a) {
     int h = (begin - before) / per_head, unit = (begin - before) % per_head;
     const float factor = fabsf(a.scale) * LOG2E;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-    const int step_token = 32 / a.group, step_head = 32 % a.group;
+    const int step_token = ROWS / a.group, step_head = ROWS % a.group;
     for (int left = end - begin; left > 0; --left) {
         const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, older = length - count;      // entry older + t is token t's own
         const int unit0 = unit * UNIT, j0 = unit0 + wave * COLUMNS;
-        // keys: a lane has half of an entry's elements, whole groups of 32 or one; the queries' elements are taken in the same order
-        v8bf k[2][STEPS];
-        int page[2];
+        // from the first token that sees the unit's first entry
+        const int first = max(unit0 - older, 0) * a.group / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
+
+        // A thread's rows are 64 apart from one tile to the next: their heads and offsets are counted on, a division each would take as long as the scores.
+        // Offsets are those from the tile's first token (ti8_cache4_attention checks the strides); behind the last row's end zeros are loaded, and
+        // a row that is none but lies in front of it is some part of q.
+        struct Place {
+            int head;
+            uint32_t offset;        // in bytes
+        };
+        int token0 = __builtin_amdgcn_readfirstlane(first / a.group), head0 = __builtin_amdgcn_readfirstlane(first % a.group);
+        const auto place_of = [&](int row, int64_t st, int64_t sh) {
+            return Place{(first + row) % a.group, (uint32_t)((first + row) / a.group - token0) * (uint32_t)st + (uint32_t)((first + row) % a.group) * (uint32_t)sh};
+        };
+        // 64 rows on, seen from a first token that is `moved` on
+        const auto go_on = [&](Place& p, uint32_t st, uint32_t sh, uint32_t moved) {
+            p.head += step_head;
+            const bool over = p.head >= a.group;
+            p.head -= over ? a.group : 0;
+            p.offset += step_token * st + step_head * sh - moved * st + (over ? st - (uint32_t)a.group * sh : 0u);
+        };
+        const uint32_t q_st = (uint32_t)a.q_st * 2, q_sh = (uint32_t)a.q_sh * 2, lse_st = (uint32_t)a.heads * 4, lse_sh = 4;
+        Place at[PASSES], at_lse = place_of(lane, lse_st, lse_sh);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int j = j0 + u * 32 + r32;
-            page[u] = j < length ? page_of(c, b, j) : -1;
-            const uint8_t* const block = block_of(c, max(page[u], 0), h);
+        for (int i = 0; i < PASSES; ++i) {
+            const int row = ((i * WEIGHT_WAVES + wave) * 64 + lane) / CHUNKS;
+            at[i] = place_of(row, q_st, q_sh);
+            at[i].offset += ((lane % CHUNKS) ^ Values<D>::swizzle(row)) * 16;
+        }
+        const auto issue = [&](int stage) {
+            const int tokens = max(count - token0, 0);      // none are left for the tiles that are asked for behind the last
+            const auto rows_of = [&](const void* base, int64_t st, int64_t sh, int64_t bytes) {
+                const int64_t all = tokens ? (tokens - 1) * st + (a.group - 1) * sh + bytes : 0;
+                return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)min(all, (int64_t)0x7fffffff), 0x00027000);
+            };
+            const __amdgpu_buffer_rsrc_t rq = rows_of(a.q + b * a.q_sb + token0 * a.q_st + h * a.group * a.q_sh, a.q_st * 2, a.q_sh * 2, 2 * D);
+            const __amdgpu_buffer_rsrc_t rl = rows_of(a.lse + ((int64_t)b * a.tokens + token0) * a.heads + h * a.group, a.heads * 4, 4, 4);
+            int more = head0 + step_head >= a.group;
+            head0 += step_head - (more ? a.group : 0);
+            more += step_token;
+            token0 += more;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_void*)(queries[stage] + (i * WEIGHT_WAVES + wave) * 1024), 16, at[i].offset, 0, 0, 0);
+                go_on(at[i], q_st, q_sh, more);
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds_void*)lses[stage][wave], 4, at_lse.offset, 0, 0, 0);
+            go_on(at_lse, lse_st, lse_sh, more);
+        };
+
+        // keys: a lane has half of an entry's elements, whole groups of 32 or one; the queries' elements are taken in the same order
+        v8bf k[STEPS];
+        const int j = j0 + r32, page = j < length ? page_of(c, b, j) : -1;
+        {
+            const uint8_t* const block = block_of(c, max(page, 0), h);
             const int row = j & (c.page - 1);
 #pragma unroll
             for (int g = 0; g < D / 64; ++g) {
                 const uint4 x = *reinterpret_cast<const uint4*>(block + idx::cache4_codes(c.page, D, 0, row) + half * (D / 4) + g * 16);
                 const uint32_t byte = block[idx::cache4_scales(c.page, D, 0, row) + half * (D / 64) + g];
-                const float scale = scale_of(page[u] >= 0 ? byte : 0);
-                k[u][g * 4] = operand(decode8(x.x, scale));
-                k[u][g * 4 + 1] = operand(decode8(x.y, scale));
-                k[u][g * 4 + 2] = operand(decode8(x.z, scale));
-                k[u][g * 4 + 3] = operand(decode8(x.w, scale));
+                const float scale = scale_of(page >= 0 ? byte : 0);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 y = decode8(w[i], scale);
+                    k[g * 4 + i] = operand(make_uint4(y.x ^ flip, y.y ^ flip, y.z ^ flip, y.w ^ flip));
+                }
             }
         }
-        // rows: from the first token that sees the unit's first entry.  A thread's rows are 32 apart from one load to the next: their tokens and heads are
-        // counted on, a division each would take as long as the scores
-        const int first = max(unit0 - older, 0) * a.group / 32 * 32;
-        struct Place {
-            int row, token, head;
-        };
-        const auto place_of = [&](int row) { return Place{row, row / a.group, row % a.group}; };
-        const auto go_on = [&](Place& p) {
-            p.row += 32;
-            p.token += step_token;
-            p.head += step_head;
-            if (p.head >= a.group) {
-                p.head -= a.group;
-                ++p.token;
-            }
-        };
-        Place at[PASSES], at_lse = place_of(first + r32);
+        __builtin_amdgcn_s_waitcnt(0);      // from here on nothing but the tiles' loads is in flight: the loop counts them
+        float sum = 0.0f;
+        const auto add_up = [&](int row0, int stage) {
+            // somebody of these rows sees one of the wave's entries
+            if (j0 >= length || row0 + ROWS <= (j0 - older) * a.group) return;
+            const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32), sees = (j - older) * a.group - row0;        // sees: the first row that sees this lane's entry
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) at[i] = place_of(first + (i * WAVES * 64 + threadIdx.x) / CHUNKS);
-        uint4 next[PASSES];
-        float next_lse;
-        const auto load = [&]() {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                next[i] = make_uint4(0, 0, 0, 0);
-                if (at[i].row < rows)
-                    next[i] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + at[i].token * a.q_st + (h * a.group + at[i].head) * a.q_sh + (threadIdx.x % CHUNKS) * 8);
-                go_on(at[i]);
-            }
-            next_lse = INFINITY;        // rows that are none: exp(s - inf) = 0
-            if (at_lse.row < rows) next_lse = a.lse[((int64_t)b * a.tokens + at_lse.token) * a.heads + h * a.group + at_lse.head] * LOG2E;
-            go_on(at_lse);
-        };
-        const auto store = [&](int buffer) {
-#pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                const int row = (i * WAVES * 64 + threadIdx.x) / CHUNKS, chunk = threadIdx.x % CHUNKS;
-                const uint4 x = make_uint4(next[i].x ^ flip, next[i].y ^ flip, next[i].z ^ flip, next[i].w ^ flip);
-                *reinterpret_cast<uint4*>(queries[buffer] + row * ROW + ((chunk ^ Values<D>::swizzle(row)) << 4)) = x;
-            }
-            if (threadIdx.x < 32) lses[buffer][threadIdx.x] = next_lse;
-        };
-        float sum[2] = {0.0f, 0.0f};
-        if (first < rows) load();
-        __syncthreads();        // (nobody reads the last unit's queries any more)
-        if (first < rows) store(0);
-        for (int row0 = first, buffer = 0; row0 < rows; row0 += 32, buffer ^= 1) {
-            if (row0 + 32 < rows) load();
-            __syncthreads();
-            const uint8_t* const from = queries[buffer] + r32 * ROW;
-            const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int ju = j0 + u * 32;
-                // somebody of these rows sees one of the 32 entries
-                if (ju >= length || (row0 + 32) <= (ju - older) * a.group) continue;
+            for (int u = 0; u < ROWS / 32; ++u) {
+                if (row0 + u * 32 >= rows) break;
+                const uint8_t* const from = queries[stage] + (u * 32 + r32) * ROW;
                 v16f s;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-                for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(from + ((chunk ^ x) << 4)), k[u][x], s);
-                const bool edge = row0 < (ju + 31 - older) * a.group;       // not every row sees every entry
-                const int sees = (ju + r32 - older) * a.group;              // the first row that sees this lane's
+                for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(from + ((chunk ^ x) << 4)), k[x], s);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const v4f lse = *reinterpret_cast<const v4f*>(lses[buffer] + 8 * g + 4 * half);
+                    const v4f shift = *reinterpret_cast<const v4f*>(lses[stage][wave] + u * 32 + 8 * g + 4 * half) * LOG2E;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -lse[i]));
-                        if (!edge || row0 + 8 * g + 4 * half + i >= sees) sum[u] += p;
-                    }
+                    for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -shift[i]));
                 }
-            }
-            if (row0 + 32 < rows) store(buffer ^ 1);
-        }
+                if (row0 + u * 32 < (j0 + COLUMNS - 1 - older) * a.group || row0 + u * 32 + 32 > rows)        // not every row is one and sees every entry
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float total = over_halves<true>(sum[u]);
-            if (page[u] >= 0 && half == 0) c.weights[((int64_t)page[u] * c.heads + h) * c.page + ((j0 + u * 32 + r32) & (c.page - 1))] += total;
+                    for (int i = 0; i < 16; ++i) {
+                        const int row = u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+                        s[i] = row >= sees && row0 + row < rows ? s[i] : 0.0f;
+                    }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += s[i];
+            }
+        };
+        if (tiles == 1) {
+            issue(0);
+            wait_and_meet<0>();
+            add_up(first, 0);
+        } else if (tiles > 1) {
+            issue(0);
+            issue(1);
+            for (int t = 0, stage = 0; t < tiles; ++t) {
+                wait_and_meet<LOADS>();       // tile t is there, and nobody reads tile t - 1, whose place is the next one's
+                issue(stage == 0 ? RING - 1 : stage - 1);
+                add_up(first + t * ROWS, stage);
+                stage = stage == RING - 1 ? 0 : stage + 1;
+            }
         }
+        wait_and_meet<0>();
+        sum = over_halves<true>(sum);
+        if (page >= 0 && half == 0) c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))] += sum;
         if (++unit == per_head) {
             unit = 0;
             if (++h == c.heads && left > 1) {
@@ -866,9 +891,9 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
         e = p.waves == 8 ? launch_prompt<D, 8>(fn, a, st) : launch_prompt<D, 4>(fn, a, st);
     }
     if (e || !accumulate) return e;
-    const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity(), WEIGHTS_UNIT), most = device_cu_count() * 6;
+    const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity(), WEIGHTS_UNIT), most = device_cu_count() * 2;
     a.groups = (int)(units < most ? units : most);
-    hipLaunchKernelGGL((weights_kernel<D>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
+    hipLaunchKernelGGL((weights_kernel<D>), dim3((unsigned)a.groups), dim3(WEIGHT_WAVES * 64), 0, st, a);
     return check_launch(fn);
 }
 
