@@ -681,17 +681,80 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
     const idx::Share share = idx::share_out(lengths.all(), a.groups);
     if ((int)blockIdx.x >= share.groups) return;
     const int begin = idx::share_begin(share, blockIdx.x), end = idx::share_begin(share, blockIdx.x + 1);
-    int before, per_head, b = lengths.find(begin, before, per_head);
-    int length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
-    int h = (begin - before) / per_head, unit = (begin - before) % per_head;
     const float factor = fabsf(a.scale) * LOG2E;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     const int step_token = ROWS / a.group, step_head = ROWS % a.group;
-    for (int left = end - begin; left > 0; --left) {
-        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, older = length - count;      // entry older + t is token t's own
-        const int unit0 = unit * UNIT, j0 = unit0 + wave * COLUMNS;
-        // from the first token that sees the unit's first entry
-        const int first = max(unit0 - older, 0) * a.group / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
+    struct Unit {
+        int b, h, unit, length, count, per_head;
+        __device__ __forceinline__ void sequence(const Args& a, int b_) {
+            b = b_;
+            count = a.counts ? min(max(((constant_ints)a.counts)[b], 0), a.tokens) : a.tokens;
+            length = count ? min(max(((constant_ints)a.lengths)[b], 0), a.c.capacity()) : 0;
+            per_head = idx::cache4_units(length, UNIT);
+        }
+    };
+    int before, per_head, left = end - begin;
+    Unit now;
+    now.sequence(a, lengths.find(begin, before, per_head));
+    now.h = (begin - before) / per_head;
+    now.unit = (begin - before) % per_head;
+    // the keys, and what the entries have: a lane has half of an entry's elements, whole groups of 32 or one.  The next unit's are on their way
+    // while one is worked on
+    uint4 codes[D / 64];
+    uint32_t bytes[D / 64];
+    float* weight;
+    float has;
+    const auto fetch = [&](const Unit& u) {
+        const int j0 = u.unit * UNIT + wave * COLUMNS, j = j0 + r32;
+        const constant_ints table = (constant_ints)(c.table + u.b * c.table_stride);
+        int page = -1;
+        if (j0 < u.length) {
+            const int low = table[j0 >> c.log2_page], high = table[min(j0 + 16, c.capacity() - 1) >> c.log2_page];
+            page = r32 < 16 ? low : high;
+        }
+        const bool there = j < u.length && (unsigned)page < (unsigned)c.pages;
+        const int64_t block = (int64_t)(there ? page : 0) * c.heads + u.h;
+        const uint8_t* const from = c.pool + block * c.block_bytes;
+        const int row = j & (c.page - 1);
+#pragma unroll
+        for (int g = 0; g < D / 64; ++g) {
+            codes[g] = *reinterpret_cast<const uint4*>(from + idx::cache4_codes(c.page, D, 0, row) + half * (D / 4) + g * 16);
+            bytes[g] = from[idx::cache4_scales(c.page, D, 0, row) + half * (D / 64) + g];
+            if (!there) bytes[g] = 0;
+        }
+        weight = there ? c.weights + block * c.page + row : nullptr;
+        has = c.weights[block * c.page + row];
+    };
+    fetch(now);
+    int staged_b = -1, staged_h = -1;       // the head whose queries lie in LDS, all of them
+    while (true) {
+        const int b = now.b, h = now.h, length = now.length, count = now.count, rows = count * a.group, older = length - count;      // entry older + t is token t's own
+        const int unit0 = now.unit * UNIT, j0 = unit0 + wave * COLUMNS, j = j0 + r32;
+        v8bf k[STEPS];      // the queries' elements are taken in the same order
+#pragma unroll
+        for (int g = 0; g < D / 64; ++g) {
+            const float scale = scale_of(bytes[g]);
+            const uint32_t w[4] = {codes[g].x, codes[g].y, codes[g].z, codes[g].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 y = decode8(w[i], scale);
+                k[g * 4 + i] = operand(make_uint4(y.x ^ flip, y.y ^ flip, y.z ^ flip, y.w ^ flip));
+            }
+        }
+        float* const this_weight = weight;
+        const float had = has;
+        if (--left > 0) {
+            if (++now.unit == now.per_head) {
+                now.unit = 0;
+                if (++now.h == c.heads) {
+                    now.h = 0;
+                    now.sequence(a, b + 1);
+                }
+            }
+            fetch(now);
+        }
+        // from the first token that sees the unit's first entry, where the rows do not all fit into a tile
+        const int first = rows <= ROWS ? 0 : max(unit0 - older, 0) * a.group / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
 
         // A thread's rows are 64 apart from one tile to the next: their heads and offsets are counted on, a division each would take as long as the scores.
         // Offsets are those from the tile's first token (ti8_cache4_attention checks the strides); behind the last row's end zeros are loaded, and
@@ -740,26 +803,6 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             go_on(at_lse, lse_st, lse_sh, more);
         };
 
-        // keys: a lane has half of an entry's elements, whole groups of 32 or one; the queries' elements are taken in the same order
-        v8bf k[STEPS];
-        const int j = j0 + r32, page = j < length ? page_of(c, b, j) : -1;
-        {
-            const uint8_t* const block = block_of(c, max(page, 0), h);
-            const int row = j & (c.page - 1);
-#pragma unroll
-            for (int g = 0; g < D / 64; ++g) {
-                const uint4 x = *reinterpret_cast<const uint4*>(block + idx::cache4_codes(c.page, D, 0, row) + half * (D / 4) + g * 16);
-                const uint32_t byte = block[idx::cache4_scales(c.page, D, 0, row) + half * (D / 64) + g];
-                const float scale = scale_of(page >= 0 ? byte : 0);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 y = decode8(w[i], scale);
-                    k[g * 4 + i] = operand(make_uint4(y.x ^ flip, y.y ^ flip, y.z ^ flip, y.w ^ flip));
-                }
-            }
-        }
-        __builtin_amdgcn_s_waitcnt(0);      // from here on nothing but the tiles' loads is in flight: the loop counts them
         float sum = 0.0f;
         const auto add_up = [&](int row0, int stage) {
             // somebody of these rows sees one of the wave's entries
@@ -774,27 +817,36 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
                 for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(from + ((chunk ^ x) << 4)), k[x], s);
+                const bool edge = row0 + u * 32 < (j0 + COLUMNS - 1 - older) * a.group || row0 + u * 32 + 32 > rows;       // not every row is one and sees every entry
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
+                    if (row0 + u * 32 + 8 * g >= rows) break;       // (a step's few rows: no exponentials of rows that are none)
                     const v4f shift = *reinterpret_cast<const v4f*>(lses[stage][wave] + u * 32 + 8 * g + 4 * half) * LOG2E;
+                    float p[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[4 * g + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -shift[i]));
+                    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -shift[i]));
+                    if (edge)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int row = u * 32 + 8 * g + 4 * half + i;
+                            p[i] = row >= sees && row0 + row < rows ? p[i] : 0.0f;
+                        }
+                    sum += (p[0] + p[1]) + (p[2] + p[3]);
                 }
-                if (row0 + u * 32 < (j0 + COLUMNS - 1 - older) * a.group || row0 + u * 32 + 32 > rows)        // not every row is one and sees every entry
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int row = u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-                        s[i] = row >= sees && row0 + row < rows ? s[i] : 0.0f;
-                    }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sum += s[i];
             }
         };
-        if (tiles == 1) {
-            issue(0);
-            wait_and_meet<0>();
-            add_up(first, 0);
-        } else if (tiles > 1) {
+        if (rows <= ROWS) {
+            if (rows > 0 && (b != staged_b || h != staged_h)) {
+                wait_and_meet<0>();
+                issue(0);
+                wait_and_meet<0>();
+                staged_b = b;
+                staged_h = h;
+            }
+            if (rows > 0) add_up(0, 0);
+        } else {
+            staged_b = -1;
+            wait_and_meet<0>();     // from here on nothing but the tiles' loads is in flight: the loop counts them
             issue(0);
             issue(1);
             for (int t = 0, stage = 0; t < tiles; ++t) {
@@ -803,18 +855,11 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
                 add_up(first + t * ROWS, stage);
                 stage = stage == RING - 1 ? 0 : stage + 1;
             }
+            __builtin_amdgcn_s_waitcnt(0);      // the loads behind the last tile: LDS may be another workgroup's once the wave has ended
         }
-        wait_and_meet<0>();
         sum = over_halves<true>(sum);
-        if (page >= 0 && half == 0) c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))] += sum;
-        if (++unit == per_head) {
-            unit = 0;
-            if (++h == c.heads && left > 1) {
-                h = 0;
-                length = __builtin_amdgcn_readfirstlane(seen_of(a, ++b));
-                per_head = idx::cache4_units(length, UNIT);
-            }
-        }
+        if (this_weight && half == 0) *this_weight = had + sum;
+        if (left <= 0) break;
     }
 #endif
 }
