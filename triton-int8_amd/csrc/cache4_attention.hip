@@ -6,6 +6,7 @@
 // in any attention on bf16 tensors (that rounding, 2^-9 of each, averages out over the entries; the result is rounded to bf16 anyway).
 //
 // step_kernel: up to 64 rows per kv head (rows = new tokens x heads that share it).  prompt_kernel: more.  weights_kernel: what every entry got.
+#include <type_traits>
 #include "cache4.h"
 
 namespace ti8 {
@@ -412,8 +413,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // ---- many rows: prompts ------------------------------------------------------------------------------------------
 //
 // A wave has 32 rows of queries as the columns of 32 x 32 products (S^T = K Q^T, O^T = V^T P^T: a lane has one row of queries, as above); the waves
-// of a workgroup go through the entries together, 64 at a time, which they turn into bf16 in LDS once for all: while one tile is multiplied,
-// the next one's codes, loaded in front of it, are converted into the other half, and the one's after that are on their way.
+// of a workgroup go through the entries together, 64 at a time, which they turn into bf16 in LDS once for all, two tiles ahead (one, where four waves share
+// a CU with another four); the codes of the tile behind that are on their way meanwhile.
+// A wave's scores of 32 entries are multiplied while it takes the exponentials of the 32 before, and the maxima of the one's are found while the other's
+// values are multiplied: products and vector instructions of a wave alternate, or they would take turns on all waves, which the tiles keep in step.
 // A head's row blocks lie on one XCD, whose L2 then serves the entries; where there are too few row blocks for the chip, several workgroups share the
 // entries of one and join_rows_kernel adds them up.
 
@@ -422,14 +425,14 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int TILE = 64;        // entries of a tile
 
 template <int D>
-struct Tile32 {     // rows of D bf16 in LDS, 16-byte chunks permuted as in Values
-    static constexpr int ROW = 2 * D, BYTES = TILE * ROW;
-    // this lane's chunk of an operand whose rows are the tile's: XOR with step << 5 (plus 32 rows)
-    __device__ static __forceinline__ int rows_at(int lane) { return (lane & 31) * ROW + (((lane >> 5) ^ Values<D>::swizzle(lane & 31)) << 4); }
-    // the same of an operand over the rows (transposing read): XOR with column tile << 6 and u << 5, plus (16 t + 8 u) ROW
+struct Tile32 {     // rows of D bf16 in LDS, 32 bytes apart: neighbouring rows' chunks fall into other banks, and addresses are sums, most of them constants
+    static constexpr int ROW = 2 * D + 32, BYTES = TILE * ROW;
+    // this lane's chunk of an operand whose rows are the tile's: plus 32 per step, 32 ROW per 32 rows
+    __device__ static __forceinline__ int rows_at(int lane) { return (lane & 31) * ROW + (lane >> 5) * 16; }
+    // the same of an operand over the rows (transposing read): plus 64 per column tile, 8 ROW per 8 rows
     __device__ static __forceinline__ int columns_at(int lane) {
-        const int i = lane & 15, h = lane >> 5, chunk = ((lane >> 4) & 1) * 2 + ((i >> 1) & 1), r = 4 * h + (i >> 2);
-        return r * ROW + ((chunk ^ Values<D>::swizzle(r)) << 4) + (i & 1) * 8;
+        const int i = lane & 15;
+        return (4 * (lane >> 5) + (i >> 2)) * ROW + ((lane >> 4) & 1) * 32 + (i & 3) * 8;
     }
 };
 
@@ -458,13 +461,17 @@ struct Codes {
 };
 #endif
 
+// tiles in LDS: three with eight waves, which have a CU to themselves
+template <int NW> constexpr int PROMPT_STAGES = NW == 8 ? 3 : 2;
+
 template <int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = Tile32<D>;
     constexpr int STEPS = D / 16, BLOCKS = D / 32, PARTS = 8 / NW;      // PARTS: of a tile (keys and values in quarters) that a wave converts
-    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];        // [2][keys, values]
-    __shared__ int absent[2][4];        // whether the pool does not have the page of 16 entries of a tile
+    constexpr int STAGES = PROMPT_STAGES<NW>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];        // [STAGES][keys, values]
+    __shared__ __attribute__((aligned(16))) int absent[STAGES][4];        // whether the pool does not have the page of 16 entries of a tile
     const Cache& c = a.c;
     const idx::AttentionPlace place = idx::attention_place(blockIdx.x, a.blocks * a.splits);
     if (place.pair >= c.batch * c.heads) return;
@@ -473,11 +480,16 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5, r16 = lane & 15, quarter = lane >> 4;
     const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), rows = count * a.group;
     const int row0 = block * (NW * 32), row = row0 + wave * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
-    // entries that this lane's row, any row of the workgroup, any and every row of the wave sees
+    // entries that this lane's row, any row of the workgroup and any row of the wave sees
     const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
     const int sees = row < rows ? sees_of(row) : 0, most = row0 < rows ? sees_of(min(row0 + NW * 32, rows) - 1) : 0;
-    const int wave0 = row0 + wave * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0, wave_all = wave0 + 32 <= rows ? sees_of(wave0) : 0;
+    const int wave0 = row0 + wave * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
     const int tiles = (most + TILE - 1) / TILE, begin = (int)((int64_t)split * tiles / a.splits), end = (int)((int64_t)(split + 1) * tiles / a.splits);
+    // entries that every row of the workgroup sees: none where the pool does not have all the pages
+    bool gaps = false;
+    for (int i = (begin * TILE >> c.log2_page) + threadIdx.x; i < (min(end * TILE, length) + c.page - 1) >> c.log2_page; i += NW * 64)
+        gaps |= (unsigned)c.table[b * c.table_stride + i] >= (unsigned)c.pages;
+    const int all = !__syncthreads_or(gaps) && row0 < rows ? sees_of(row0) : 0;
     const float factor = fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
@@ -511,47 +523,48 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
             if (!there[i] || j + r16 >= length) raw[i].scale = 0;       // (nothing that is no number)
         }
     };
-    const auto convert = [&](int tile) {
+    const auto convert = [&](int tile, int stage) {
 #pragma unroll
         for (int i = 0; i < PARTS; ++i) {
             const int p = wave + i * NW, at = (p & 3) * 16 + r16;
-            uint8_t* const to = smem + ((tile & 1) * 2 + (p >> 2)) * T::BYTES + at * T::ROW;
+            uint8_t* const to = smem + (stage * 2 + (p >> 2)) * T::BYTES + at * T::ROW;
             const float scale = scale_of(raw[i].scale);
 #pragma unroll
             for (int w = 0; w < Codes<D>::WORDS; ++w)
-                *reinterpret_cast<uint4*>(to + (((quarter * Codes<D>::WORDS + w) ^ Values<D>::swizzle(at)) << 4)) = decode8(raw[i].w[w], scale);
-            if (p < 4 && lane == 0) absent[tile & 1][p] = !there[i] && tile * TILE + p * 16 < length;
+                *reinterpret_cast<uint4*>(to + (quarter * Codes<D>::WORDS + w) * 16) = decode8(raw[i].w[w], scale);
+            if (p < 4 && lane == 0) absent[stage][p] = !there[i] && tile * TILE + p * 16 < length;
         }
     };
     const int rows_at = T::rows_at(lane), columns_at = T::columns_at(lane);
-    const auto compute = [&](int tile) {
-        const uint8_t* const kt = smem + (tile & 1) * 2 * T::BYTES;
-        const uint8_t* const vt = kt + T::BYTES;
-        const int j0 = tile * TILE;
-        v16f s[2];
+    // scores of half `u` of a tile
+    const auto scores = [&](int stage, int u) {
+        const uint8_t* const kt = smem + rows_at + stage * 2 * T::BYTES;
+        v16f s;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+        for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(kt + u * 32 * T::ROW + x * 32), q[x], s);
+        return s;
+    };
+    const auto gone_of = [&](int stage) {       // a bit for each 16 entries whose page the pool does not have
+        const v4i x = *reinterpret_cast<const v4i*>(absent[stage]);
+        return __builtin_amdgcn_readfirstlane(x[0] | x[1] << 1 | x[2] << 2 | x[3] << 3);
+    };
+    // -inf for entries that the row does not see
+    const auto mask = [&](v16f& s, int tile, int u, int gone) {
+        const int up_to = sees - (tile * TILE + u * 32) - 4 * half;
 #pragma unroll
-            for (int x = 0; x < STEPS; ++x) s[u] = mfma32(*reinterpret_cast<const v8bf*>(kt + u * 32 * T::ROW + (rows_at ^ (x << 5))), q[x], s[u]);
-        }
-        int gone = 0;
+        for (int i = 0; i < 16; ++i)
+            if (8 * (i >> 2) + (i & 3) >= up_to || (gone >> (2 * u + (i >> 3)) & 1)) s[i] = -INFINITY;
+    };
+    const auto largest_of = [&](const v16f& s) {
+        // (v_med3_f32 with infinity is a maximum that does not ask whether its operands are quiet)
+        float m = s[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gone |= absent[tile & 1][i] << i;
-        gone = __builtin_amdgcn_readfirstlane(gone);
-        if (j0 + TILE > wave_all || gone)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = u * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-                    if (j0 + j >= sees || (gone >> (2 * u + (i >> 3)) & 1)) s[u][i] = -INFINITY;
-                }
-        float largest = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fmaxf(s[0][i], s[1][i]));
-        largest = over_halves<false>(largest);
+        for (int i = 1; i < 16; ++i) m = __builtin_amdgcn_fmed3f(m, s[i], INFINITY);
+        return over_halves<false>(m);
+    };
+    const auto raise = [&](float largest) {
         if (__any((largest - top) * factor > 8.0f)) {       // see step_kernel
             const float higher = fmaxf(top, largest), shrink = higher == -INFINITY ? 1.0f : exp2f((top - higher) * factor);
             top = higher;
@@ -560,40 +573,84 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d) o[d] *= shrink;
         }
+    };
+    const auto exponentials = [&](v16f& s, v8bf (&p)[2]) {
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float part = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], factor, -shift));
-                part += s[u][i];
-            }
-            sum += part;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const v8bf p = operand(make_uint4(pack_bf16x2(s[u][8 * x], s[u][8 * x + 1]), pack_bf16x2(s[u][8 * x + 2], s[u][8 * x + 3]),
-                                                  pack_bf16x2(s[u][8 * x + 4], s[u][8 * x + 5]), pack_bf16x2(s[u][8 * x + 6], s[u][8 * x + 7])));
-#pragma unroll
-                for (int d = 0; d < BLOCKS; ++d) {
-                    const uint8_t* const at = vt + (u * 32 + x * 16) * T::ROW;
-                    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + (columns_at ^ (d << 6))));
-                    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * T::ROW + (columns_at ^ (d << 6) ^ 32)));
-                    o[d] = mfma32(__builtin_bit_cast(v8bf, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p, o[d]);
-                }
-            }
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, -shift));
+            part[i & 3] += s[i];
         }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            p[x] = operand(make_uint4(pack_bf16x2(s[8 * x], s[8 * x + 1]), pack_bf16x2(s[8 * x + 2], s[8 * x + 3]),
+                                      pack_bf16x2(s[8 * x + 4], s[8 * x + 5]), pack_bf16x2(s[8 * x + 6], s[8 * x + 7])));
+    };
+    const auto add_values = [&](int stage, int u, const v8bf (&p)[2]) {
+        const uint8_t* const vt = smem + columns_at + (stage * 2 + 1) * T::BYTES;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) {
+                const uint8_t* const at = vt + (u * 32 + x * 16) * T::ROW + d * 64;
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * T::ROW));
+                o[d] = mfma32(__builtin_bit_cast(v8bf, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p[x], o[d]);
+            }
+    };
+    // from the scores of a half tile (s) to the next one's, of half u of a tile in `ahead`; the values are half 1 - u of `stage`
+    v16f s;
+    const auto step = [&](int stage, int ahead, int tile, int gone, auto u, auto masked) {
+        v8bf p[2];
+        v16f other = scores(ahead, u);
+        exponentials(s, p);
+        if (masked) mask(other, tile, u, gone);
+        const float largest = largest_of(other);
+        add_values(stage, 1 - u, p);
+        s = other;
+        raise(largest);
     };
 
     if (begin < end) {
+        const int mine = min(end, (wave_most + TILE - 1) / TILE);       // this wave's tiles end here
         load(begin);
-        convert(begin);
+        convert(begin, 0);
         if (begin + 1 < end) load(begin + 1);
-        for (int tile = begin; tile < end; ++tile) {
-            __syncthreads();        // the tile is there, and nobody reads the one before
-            if (tile + 1 < end) convert(tile + 1);
-            if (tile + 2 < end) load(tile + 2);
-            if (tile * TILE < wave_most) compute(tile);
+        if (STAGES == 3) {
+            if (begin + 1 < end) convert(begin + 1, 1);
+            if (begin + 2 < end) load(begin + 2);
         }
+        __syncthreads();
+        if (begin < mine) {
+            s = scores(0, 0);
+            mask(s, begin, 0, gone_of(0));
+            raise(largest_of(s));
+        }
+        using Half0 = std::integral_constant<int, 0>;
+        using Half1 = std::integral_constant<int, 1>;
+        int stage = 0;
+        const auto walk = [&](int from, int to, auto masked) {
+            for (int tile = from; tile < to; ++tile) {
+                const int next = stage + 1 == STAGES ? 0 : stage + 1;
+                if (tile > begin) __syncthreads();      // nobody reads the tile before; with three stages the next one is there
+                const int into = STAGES == 3 ? (next + 1 == STAGES ? 0 : next + 1) : next, ready = tile + STAGES - 1;
+                if (ready < end) convert(ready, into);
+                if (ready + 1 < end) load(ready + 1);
+                if (tile < mine) step(stage, stage, tile, masked ? gone_of(stage) : 0, Half1{}, masked);
+                if (STAGES == 2) __syncthreads();       // the next tile is there
+                if (tile + 1 < mine) step(stage, next, tile + 1, masked ? gone_of(next) : 0, Half0{}, masked);
+                else if (tile < mine) {
+                    v8bf p[2];
+                    exponentials(s, p);
+                    add_values(stage, 1, p);
+                }
+                stage = next;
+            }
+        };
+        // up to here every row sees every entry of a tile and of the next one
+        const int clear = min(max(all / TILE - 1, begin), end);
+        walk(begin, clear, std::false_type{});
+        walk(clear, end, std::true_type{});
     }
     sum = over_halves<true>(sum);
     if (token >= a.tokens) return;
@@ -905,7 +962,7 @@ int launch_step(const char* fn, const Args& a, hipStream_t st) {
 template <int D, int NW>
 int prepare_prompt(const char* fn) {
     static OncePerDevice once;
-    const hipError_t e = raise_lds_limit(once, reinterpret_cast<const void*>(prompt_kernel<D, NW>), 4 * Tile32<D>::BYTES);
+    const hipError_t e = raise_lds_limit(once, reinterpret_cast<const void*>(prompt_kernel<D, NW>), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES);
     return e == hipSuccess ? TI8_OK : fail(TI8_ERR_HIP, "%s: cannot raise the LDS limit: %s", fn, hipGetErrorString(e));
 }
 
@@ -913,7 +970,7 @@ template <int D, int NW>
 int launch_prompt(const char* fn, const Args& a, hipStream_t st) {
     if (int e = prepare_prompt<D, NW>(fn)) return e;
     const int64_t grid = idx::round8((int64_t)a.c.batch * a.c.heads) * a.blocks * a.splits;
-    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)grid), dim3(NW * 64), 4 * Tile32<D>::BYTES, st, a);
+    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)grid), dim3(NW * 64), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES, st, a);
     if (int e = check_launch(fn)) return e;
     if (a.splits == 1) return TI8_OK;
     const int64_t rows = (int64_t)a.c.batch * a.tokens * a.heads, per = 256 / (D / 4);
