@@ -5,7 +5,7 @@
 // v_mfma_f32_16x16x32_bf16 with fp32 sums; scores, m and l are fp32, probabilities are rounded to bf16 as operands of the product with the values, as
 // in any attention on bf16 tensors (that rounding, 2^-9 of each, averages out over the entries; the result is rounded to bf16 anyway).
 //
-// step_kernel: up to 64 rows per kv head (rows = new tokens x heads that share it).  prompt_kernel: more.  weights_kernel: what every entry got.
+// step_kernel: up to 32 rows per kv head (rows = new tokens x heads that share it).  prompt_kernel: more.  weights_kernel: what every entry got.
 #include <type_traits>
 #include "cache4.h"
 
@@ -129,7 +129,7 @@ constexpr int EXTRA = 2;
 static_assert(idx::CACHE4_UNIT == WAVES * ENTRIES, "a unit is a turn of every wave");
 
 template <int D, int TILES>     // TILES * 16 rows
-__global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) void step_kernel(const Args a) {
+__global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using V = Values<D>;
     constexpr int STEPS = D / 32;       // words of codes of an entry that a lane has; products over D
@@ -355,58 +355,76 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : TILES == 2 ? 2 : 1) vo
 #endif
 }
 
-// Rows whose (sequence, head) several workgroups had: one workgroup each
-template <int D, int TILES>
-__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+// A row from its `n` parts: the first one, and the others behind `rest` at a distance.  GROUPS times D / 4 lanes share it (with 256 threads of a workgroup in
+// all); the largest maximum comes first, so that the parts themselves are independent loads.
+template <int D, int GROUPS>
+__device__ __forceinline__ void join(const Args& a, const float* one, const float* rest, int64_t distance, int n, int64_t row, bool is) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LANES = D / 4, PARTS = 256 / LANES;       // lanes of a row; parts that are read at a time
-    __shared__ v4f shared[PARTS][LANES];
-    __shared__ float shared_m[PARTS], shared_l[PARTS];
-    const Cache& c = a.c;
-    const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
-    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, threadIdx.x & 63);
-    const idx::Share share = idx::share_out(lengths.all(), a.groups);
-    int per_head;
-    int begin = lengths.before(b, per_head);
-    begin += h * per_head + EXTRA;
-    per_head -= EXTRA;
-    const int first = idx::share_of(share, begin), last = idx::share_of(share, begin + per_head - 1);
-    if (first == last) return;
-    const int own = threadIdx.x / LANES, at = threadIdx.x % LANES;
+    constexpr int LANES = D / 4, THREADS = GROUPS * LANES;
+    __shared__ v4f shared[GROUPS][LANES];
+    __shared__ float shared_m[GROUPS], shared_l[GROUPS];
+    const int tid = threadIdx.x % THREADS, group = tid / LANES, at = tid % LANES;
+    const auto part = [&](int i) { return i ? rest + i * distance : one; };
     float m = -INFINITY, l = 0.0f;
+    for (int i = tid; i < n; i += THREADS) m = fmaxf(m, part(i)[D]);
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (GROUPS > 1) {
+        if (at == 0) shared_m[group] = m;
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, shared_m[g]);
+    }
+    // (a NaN in a sum passes a maximum of -inf)
+    const auto weight = [&](float pm) { return pm == -INFINITY ? 0.0f : exp2f(pm - m); };
+    for (int i = tid; i < n; i += THREADS) {
+        const float pm = part(i)[D], pl = part(i)[D + 1];
+        l += pm == -INFINITY ? pl : pl * weight(pm);
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) l += __shfl_xor(l, d, 64);
     v4f o{0, 0, 0, 0};
-    for (int w = first + own; w <= last; w += PARTS) {
-        // a workgroup's second part is the one that starts with the head's first unit
-        const float* const part = a.parts + (((int64_t)w * 2 + (idx::share_begin(share, w) <= begin)) * (TILES * 16) + row) * Part<D>::ROW;
-        const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
-        const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
-        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
-        o = o * fa + x * fb;
-        l = l * fa + (pm == -INFINITY ? pl : pl * fb);
-        m = higher;
+#pragma unroll 4
+    for (int i = group; i < n; i += GROUPS) o += *reinterpret_cast<const v4f*>(part(i) + at * 4) * weight(part(i)[D]);
+    if (GROUPS > 1) {
+        shared[group][at] = o;
+        if (at == 0) shared_l[group] = l;
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) {
+            o += shared[g][at];
+            l += shared_l[g];
+        }
     }
-    shared[own][at] = o;
-    if (at == 0) {
-        shared_m[own] = m;
-        shared_l[own] = l;
-    }
-    __syncthreads();
-    if (own) return;
-    for (int i = 1; i < PARTS; ++i) {
-        const float pm = shared_m[i], higher = fmaxf(m, pm);
-        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
-        o = o * fa + shared[i][at] * fb;
-        l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? shared_l[i] : shared_l[i] * fb);
-        m = higher;
-    }
-    const int64_t to = ((int64_t)b * a.tokens + row / a.group) * a.heads + h * a.group + row % a.group;
-    if (row / a.group >= count_of(a.counts, b, a.tokens)) {       // no query, and no parts
+    if (!is) {      // no query, and no parts
         l = 0.0f;
         o = v4f{0, 0, 0, 0};
     }
     const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2*>(a.out + to * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
-    if (at == 0) a.lse[to] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    *reinterpret_cast<uint2*>(a.out + row * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
+    if (at == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+#endif
+}
+
+// Rows whose (sequence, head) several workgroups had: one workgroup each
+template <int D, int TILES>
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const Cache& c = a.c;
+    const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
+    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, threadIdx.x & 63);
+    const idx::Share share = idx::share_out(lengths.all(), a.groups);
+    int per_head, begin = lengths.before(b, per_head);
+    begin += h * per_head + EXTRA;
+    per_head -= EXTRA;
+    const int first = idx::share_of(share, begin), last = idx::share_of(share, begin + per_head - 1);
+    if (first == last) return;
+    // a workgroup's second part is the one that starts with a head's first unit: here that of the first workgroup
+    constexpr int64_t PART = TILES * 16 * Part<D>::ROW;
+    const float* const from = a.parts + first * 2 * PART + row * Part<D>::ROW;
+    join<D, 1024 / D>(a, from + PART, from, 2 * PART, last - first + 1, ((int64_t)b * a.tokens + row / a.group) * a.heads + h * a.group + row % a.group,
+                      row / a.group < count_of(a.counts, b, a.tokens));
 #endif
 }
 
@@ -464,7 +482,8 @@ struct Codes {
 // tiles in LDS: three with eight waves, which have a CU to themselves
 template <int NW> constexpr int PROMPT_STAGES = NW == 8 ? 3 : 2;
 
-template <int D, int NW>
+// NW waves, of which SHARES at a time have the same 32 rows: with two, each takes its own half of every tile, and they add up at the end
+template <int D, int NW, int SHARES>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using T = Tile32<D>;
@@ -473,17 +492,19 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];        // [STAGES][keys, values]
     __shared__ __attribute__((aligned(16))) int absent[STAGES][4];        // whether the pool does not have the page of 16 entries of a tile
     const Cache& c = a.c;
-    const idx::AttentionPlace place = idx::attention_place(blockIdx.x, a.blocks * a.splits);
+    const idx::AttentionPlace place = idx::cache4_place(blockIdx.x, c.batch * c.heads, a.blocks * a.splits);
     if (place.pair >= c.batch * c.heads) return;
     const int b = place.pair / c.heads, h = place.pair % c.heads;
-    const int block = a.blocks - 1 - place.block / a.splits, split = place.block % a.splits;     // the longest first
+    const int block = place.block / a.splits, split = place.block % a.splits;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5, r16 = lane & 15, quarter = lane >> 4;
+    constexpr int ROWS_OF = NW / SHARES * 32;
+    const int mine_of = wave / (NW / SHARES);      // which half of a tile, with two shares
     const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), rows = count * a.group;
-    const int row0 = block * (NW * 32), row = row0 + wave * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
+    const int row0 = block * ROWS_OF, row = row0 + wave % (NW / SHARES) * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
     // entries that this lane's row, any row of the workgroup and any row of the wave sees
     const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
-    const int sees = row < rows ? sees_of(row) : 0, most = row0 < rows ? sees_of(min(row0 + NW * 32, rows) - 1) : 0;
-    const int wave0 = row0 + wave * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
+    const int sees = row < rows ? sees_of(row) : 0, most = row0 < rows ? sees_of(min(row0 + ROWS_OF, rows) - 1) : 0;
+    const int wave0 = row0 + wave % (NW / SHARES) * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
     const int tiles = (most + TILE - 1) / TILE, begin = (int)((int64_t)split * tiles / a.splits), end = (int)((int64_t)(split + 1) * tiles / a.splits);
     // entries that every row of the workgroup sees: none where the pool does not have all the pages
     bool gaps = false;
@@ -598,15 +619,15 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
                 o[d] = mfma32(__builtin_bit_cast(v8bf, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p[x], o[d]);
             }
     };
-    // from the scores of a half tile (s) to the next one's, of half u of a tile in `ahead`; the values are half 1 - u of `stage`
+    // from the scores of a half tile (s) to the next one's, of half u of a tile in `ahead`; the values are half `of` of `stage`
     v16f s;
-    const auto step = [&](int stage, int ahead, int tile, int gone, auto u, auto masked) {
+    const auto step = [&](int stage, int of, int ahead, int u, int tile, int gone, auto masked) {
         v8bf p[2];
         v16f other = scores(ahead, u);
         exponentials(s, p);
         if (masked) mask(other, tile, u, gone);
         const float largest = largest_of(other);
-        add_values(stage, 1 - u, p);
+        add_values(stage, of, p);
         s = other;
         raise(largest);
     };
@@ -622,12 +643,10 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         }
         __syncthreads();
         if (begin < mine) {
-            s = scores(0, 0);
-            mask(s, begin, 0, gone_of(0));
+            s = scores(0, SHARES == 2 ? mine_of : 0);
+            mask(s, begin, SHARES == 2 ? mine_of : 0, gone_of(0));
             raise(largest_of(s));
         }
-        using Half0 = std::integral_constant<int, 0>;
-        using Half1 = std::integral_constant<int, 1>;
         int stage = 0;
         const auto walk = [&](int from, int to, auto masked) {
             for (int tile = from; tile < to; ++tile) {
@@ -636,13 +655,14 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
                 const int into = STAGES == 3 ? (next + 1 == STAGES ? 0 : next + 1) : next, ready = tile + STAGES - 1;
                 if (ready < end) convert(ready, into);
                 if (ready + 1 < end) load(ready + 1);
-                if (tile < mine) step(stage, stage, tile, masked ? gone_of(stage) : 0, Half1{}, masked);
+                if (SHARES == 1 && tile < mine) step(stage, 0, stage, 1, tile, masked ? gone_of(stage) : 0, masked);
                 if (STAGES == 2) __syncthreads();       // the next tile is there
-                if (tile + 1 < mine) step(stage, next, tile + 1, masked ? gone_of(next) : 0, Half0{}, masked);
+                const int of = SHARES == 2 ? mine_of : 1, u = SHARES == 2 ? mine_of : 0;
+                if (tile + 1 < mine) step(stage, of, next, u, tile + 1, masked ? gone_of(next) : 0, masked);
                 else if (tile < mine) {
                     v8bf p[2];
                     exponentials(s, p);
-                    add_values(stage, 1, p);
+                    add_values(stage, of, p);
                 }
                 stage = next;
             }
@@ -653,6 +673,29 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         walk(clear, end, std::true_type{});
     }
     sum = over_halves<true>(sum);
+    if constexpr (SHARES == 2) {
+        __syncthreads();
+        float* const meet = reinterpret_cast<float*>(smem) + (wave % (NW / 2)) * (BLOCKS * 16 + 2) * 64 + lane;
+        if (mine_of == 1) {
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) meet[(d * 16 + i) * 64] = o[d][i];
+            meet[BLOCKS * 16 * 64] = top;
+            meet[(BLOCKS * 16 + 1) * 64] = sum;
+        }
+        __syncthreads();
+        if (mine_of == 1) return;
+        const float other = meet[BLOCKS * 16 * 64], more = meet[(BLOCKS * 16 + 1) * 64], higher = fmaxf(top, other);
+        const float fa = top == -INFINITY ? 0.0f : exp2f((top - higher) * factor), fb = other == -INFINITY ? 0.0f : exp2f((other - higher) * factor);
+        sum = (top == -INFINITY ? sum : sum * fa) + (other == -INFINITY ? more : more * fb);        // (a NaN in a sum passes a maximum of -inf)
+#pragma unroll
+        for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * fa + meet[(d * 16 + i) * 64] * fb;
+        top = higher;
+        shift = higher == -INFINITY ? 0.0f : higher * factor - UP;
+    }
     if (token >= a.tokens) return;
     const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + head;
     if (a.splits > 1) {
@@ -679,29 +722,13 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #endif
 }
 
-// Rows whose entries several workgroups shared: D / 4 lanes each
-template <int D>
+// Rows whose entries several workgroups shared
+template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t rows) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LANES = D / 4;
-    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t row = (int64_t)blockIdx.x * (1024 / D / GROUPS) + threadIdx.x / (GROUPS * D / 4);
     if (row >= rows) return;
-    const int at = threadIdx.x % LANES;
-    float m = -INFINITY, l = 0.0f;
-    v4f o{0, 0, 0, 0};
-    for (int s = 0; s < a.splits; ++s) {
-        const float* const part = a.parts + (row * a.splits + s) * Part<D>::ROW;
-        const v4f x = *reinterpret_cast<const v4f*>(part + at * 4);
-        const float pm = part[D], pl = part[D + 1], higher = fmaxf(m, pm);
-        const float fa = m == -INFINITY ? 0.0f : exp2f(m - higher), fb = pm == -INFINITY ? 0.0f : exp2f(pm - higher);
-        o = o * fa + x * fb;
-        l = (m == -INFINITY ? l : l * fa) + (pm == -INFINITY ? pl : pl * fb);
-        m = higher;
-    }
-    const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2*>(a.out + row * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
-    if (at == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
-#endif
+    const float* const from = a.parts + row * a.splits * Part<D>::ROW;
+    join<D, GROUPS>(a, from, from, Part<D>::ROW, a.splits, row, true);
 }
 
 // ---- what the entries got ------------------------------------------------------------------------------------------
@@ -923,22 +950,25 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
 
 // Workgroups of step_kernel: as many as run at a time (four per CU with 16 rows, which the registers allow, two otherwise), and no more than there are units
 int step_groups(const Cache& c, int tiles) {
-    const int64_t units = (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA), most = device_cu_count() * (tiles == 1 ? 3 : tiles == 2 ? 2 : 1);
+    const int64_t units = (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA), most = device_cu_count() * (tiles == 1 ? 3 : 2);
     return (int)(units < most ? units : most);
 }
-// Row tiles of step_kernel that hold all rows of a kv head (1, 2 or 4), or 0
-int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 0; }
+// Row tiles of step_kernel that hold all rows of a kv head (1 or 2), or 0: prompt_kernel.  Four of them take longer than it, 4 streams of 16384 entries and
+// 64 rows 62 us to 54; two less, 16 streams of 8192 and 32 rows 57 to 76
+int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 0; }
 
-// prompt_kernel: waves of a workgroup, and how many workgroups share the entries of its rows.  Eight waves convert every entry for 256 rows; four are taken
-// where there are too few rows to give every CU eight.  Parts are worth it from 4 tiles of entries on.
+// prompt_kernel: waves of a workgroup, how many of them have the same rows, and how many workgroups share the entries of a row block.  Eight waves convert every
+// entry for 256 rows; four are taken where the eight would hold more rows that are none and the CUs have not all got one.  Up to 64 rows two and two of
+// them share the rows (4 streams of 16384 entries, 64 rows: PAIRED).  Parts are worth it from 4 tiles of entries on.
 struct PromptPlan {
-    int waves, blocks, splits;
+    int waves, shares, blocks, splits;
 };
 PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     const int64_t pairs = (int64_t)c.batch * c.heads, cus = device_cu_count();
     PromptPlan p;
-    p.waves = pairs * ((rows + 255) / 256) >= cus ? 8 : 4;
-    p.blocks = (int)((rows + p.waves * 32 - 1) / (p.waves * 32));
+    p.waves = rows > 128 && (pairs * ((rows + 255) / 256) >= cus || (rows + 255) / 256 * 2 == (rows + 127) / 128) ? 8 : 4;
+    p.shares = rows <= 64 ? 2 : 1;
+    p.blocks = (int)((rows * p.shares + p.waves * 32 - 1) / (p.waves * 32));
     const int64_t groups = pairs * p.blocks, room = cus * (8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
     const int64_t splits = room / groups;
     p.splits = (int)(splits < 1 ? 1 : splits < most ? splits : most);
@@ -959,22 +989,24 @@ int launch_step(const char* fn, const Args& a, hipStream_t st) {
     return check_launch(fn);
 }
 
-template <int D, int NW>
+template <int D, int NW, int SHARES>
 int prepare_prompt(const char* fn) {
     static OncePerDevice once;
-    const hipError_t e = raise_lds_limit(once, reinterpret_cast<const void*>(prompt_kernel<D, NW>), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES);
+    const hipError_t e = raise_lds_limit(once, reinterpret_cast<const void*>(prompt_kernel<D, NW, SHARES>), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES);
     return e == hipSuccess ? TI8_OK : fail(TI8_ERR_HIP, "%s: cannot raise the LDS limit: %s", fn, hipGetErrorString(e));
 }
 
-template <int D, int NW>
+template <int D, int NW, int SHARES>
 int launch_prompt(const char* fn, const Args& a, hipStream_t st) {
-    if (int e = prepare_prompt<D, NW>(fn)) return e;
+    if (int e = prepare_prompt<D, NW, SHARES>(fn)) return e;
     const int64_t grid = idx::round8((int64_t)a.c.batch * a.c.heads) * a.blocks * a.splits;
-    hipLaunchKernelGGL((prompt_kernel<D, NW>), dim3((unsigned)grid), dim3(NW * 64), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES, st, a);
+    hipLaunchKernelGGL((prompt_kernel<D, NW, SHARES>), dim3((unsigned)grid), dim3(NW * 64), PROMPT_STAGES<NW> * 2 * Tile32<D>::BYTES, st, a);
     if (int e = check_launch(fn)) return e;
     if (a.splits == 1) return TI8_OK;
-    const int64_t rows = (int64_t)a.c.batch * a.tokens * a.heads, per = 256 / (D / 4);
-    hipLaunchKernelGGL((join_rows_kernel<D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a, rows);
+    // a whole workgroup for a row of many parts (64 of them: 3 us; 30 where their loads follow each other)
+    const int64_t rows = (int64_t)a.c.batch * a.tokens * a.heads, per = 1024 / D;
+    if (a.splits > 8) hipLaunchKernelGGL((join_rows_kernel<D, 1024 / D>), dim3((unsigned)rows), dim3(256), 0, st, a, rows);
+    else hipLaunchKernelGGL((join_rows_kernel<D, 1>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a, rows);
     return check_launch(fn);
 }
 
@@ -985,12 +1017,12 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
     int e;
     if (tiles) {
         a.groups = step_groups(a.c, tiles);
-        e = tiles == 1 ? launch_step<D, 1>(fn, a, st) : tiles == 2 ? launch_step<D, 2>(fn, a, st) : launch_step<D, 4>(fn, a, st);
+        e = tiles == 1 ? launch_step<D, 1>(fn, a, st) : launch_step<D, 2>(fn, a, st);
     } else {
         const PromptPlan p = prompt_plan(a.c, rows);
         a.blocks = p.blocks;
         a.splits = p.splits;
-        e = p.waves == 8 ? launch_prompt<D, 8>(fn, a, st) : launch_prompt<D, 4>(fn, a, st);
+        e = p.waves == 8 ? launch_prompt<D, 8, 1>(fn, a, st) : p.shares == 2 ? launch_prompt<D, 4, 2>(fn, a, st) : launch_prompt<D, 4, 1>(fn, a, st);
     }
     if (e || !accumulate) return e;
     const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity(), WEIGHTS_UNIT), most = device_cu_count() * 2;
@@ -1003,10 +1035,12 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
 
 int init_attention() {
     const char* fn = "ti8_init";
-    int e = prepare_prompt<128, 8>(fn);
-    if (!e) e = prepare_prompt<128, 4>(fn);
-    if (!e) e = prepare_prompt<64, 8>(fn);
-    return e ? e : prepare_prompt<64, 4>(fn);
+    int e = prepare_prompt<128, 8, 1>(fn);
+    if (!e) e = prepare_prompt<128, 4, 1>(fn);
+    if (!e) e = prepare_prompt<128, 4, 2>(fn);
+    if (!e) e = prepare_prompt<64, 8, 1>(fn);
+    if (!e) e = prepare_prompt<64, 4, 1>(fn);
+    return e ? e : prepare_prompt<64, 4, 2>(fn);
 }
 
 }  // namespace cache4

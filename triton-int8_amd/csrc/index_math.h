@@ -483,6 +483,14 @@ TI8_HD int share_of(const Share& s, int unit) {
     return unit < longer ? unit / (s.each + 1) : s.more + (unit - longer) / s.each;
 }
 
+// Attention of many rows: workgroup -> (sequence, kv head) pair and its block (and part).  A pair's blocks lie on one XCD, whose L2 then serves the entries; an
+// XCD has the last block of all its pairs first, which sees the most entries (one prompt of 4096 tokens and 32 heads 248 us with a pair's blocks behind each
+// other).  The grid has round8(pairs) * blocks workgroups; those of a pair beyond the last do nothing.
+TI8_HD AttentionPlace cache4_place(uint32_t workgroup, int pairs, int blocks) {
+    const int each = (pairs + 7) >> 3, at = (int)(workgroup >> 3);
+    return AttentionPlace{at % each * 8 + (int)(workgroup & 7), blocks - 1 - at / each};
+}
+
 // ---- which kernel an entry point launches (decided on the host) ------------------------------
 
 // per-row quantiser: NLOAD 16-byte chunks per thread, one wave (4 rows per workgroup) or one
