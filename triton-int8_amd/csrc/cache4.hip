@@ -129,7 +129,20 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
         const int page = page_of(c, b, j);
         return page < 0 ? 0u : order_of(c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))]);
     };
-    for (int j = tid; j < min(old, HELD); j += SELECT) orders[j] = fetch(j);
+    // eight entries of a thread at a time: their pages, then their weights
+    const int held = min(old, HELD);
+    for (int j0 = tid; j0 < held; j0 += 8 * SELECT) {
+        int page[8];
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) page[i] = c.table[b * c.table_stride + (min(j0 + i * SELECT, held - 1) >> c.log2_page)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = c.weights[((int64_t)((unsigned)page[i] < (unsigned)c.pages ? page[i] : 0) * c.heads + h) * c.page + ((j0 + i * SELECT) & (c.page - 1))];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j0 + i * SELECT < held) orders[j0 + i * SELECT] = (unsigned)page[i] < (unsigned)c.pages ? order_of(w[i]) : 0u;
+    }
     const auto order = [&](int j) { return j < HELD ? orders[j] : fetch(j); };
     uint32_t limit = 0;         // the heavy-th largest, as far as it is known
     int left = heavy;           // how many of those that agree with it so far are to stay
