@@ -176,19 +176,24 @@ class Cache4:
         self.weights = None if budget is None else torch.zeros((pages, kv_heads, page_size), dtype=torch.float32, device=device)
         self.table = torch.arange(batch * mine, dtype=torch.int32, device=device).view(batch, mine)
         self.spare = torch.arange(batch * mine, pages, dtype=torch.int32, device=device).view(batch, spare) if spare else None
-        self.lengths = torch.zeros((batch,), dtype=torch.int32, device=device)
-        self.positions = torch.zeros((batch,), dtype=torch.int32, device=device)
-        self.filled = 0         # entries of the longest sequence, as far as the host knows (all tokens of a call counted)
+        self._counts = torch.zeros((2, batch), dtype=torch.int32, device=device)
+        self.lengths, self.positions = self._counts
+        # entries and tokens of the longest sequence, as far as the host knows (all tokens of a call counted, replays of a graph not)
+        self.filled = self.seen = 0
 
     def append(self, k, v, counts=None):
         """New tokens, bf16 [batch, tokens, kv_heads, head_dim], behind the entries of each sequence (of sequence b the first ``counts[b]``)."""
         tokens = k.shape[1]
         _need(self.filled + tokens <= self.max_length, f"{tokens} tokens behind {self.filled} are more than the {self.max_length} entries that there is room for")
         append(self.pool, self.table, self.lengths, k, v, counts=counts, weights=self.weights)
-        more = tokens if counts is None else counts
-        self.lengths.add_(more)
-        self.positions.add_(more)
+        self._counts.add_(tokens if counts is None else counts)
         self.filled += tokens
+        self.seen += tokens
+
+    def reset(self):
+        """All sequences empty again."""
+        self._counts.zero_()
+        self.filled = self.seen = 0
 
     def attend(self, q, counts=None, scale=None):
         """Attention of the last appended tokens' queries: see :func:`attention`."""

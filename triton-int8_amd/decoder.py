@@ -6,6 +6,9 @@ SDPA) and SwiGLU stay in bf16; ``int8=False`` builds the bf16 twin used for loss
 In the int8 layer the RMSNorms, the rotary embedding and the SwiGLU product run as one kernel each per direction
 (csrc/decoder.hip), and the attention's backward as two (csrc/attention.hip); the twin, tensors those kernels do not take and calls under a tracer or a function transform go through the
 torch expressions, which are also what a backward that is differentiated again is made of.
+
+:meth:`DecoderLayer.serve` runs the layer on new tokens of sequences whose keys and values lie in a 4-bit cache (cache4.py): prompts, parts of them, and single
+tokens.
 """
 import math
 
@@ -238,6 +241,33 @@ class DecoderLayer(torch.nn.Module):
         scale = 1.0 / math.sqrt(self.head_dim)
         a = _attention(q, k, v, scale) if self.int8 else F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale)
         x = x + self.o_proj(a.transpose(1, 2).reshape(B, S, H))
+        h = self.post_norm(x)
+        gate, up = _projections(h, self.gate_proj, self.up_proj)
+        product = _SwiGLUFunction.apply if self.int8 and _kernels_take(gate, up) else _swiglu
+        return x + self.down_proj(product(gate, up))
+
+    @torch.no_grad()
+    def serve(self, x, cache, rotary, counts=None):
+        """The layer's output for new tokens x [batch, tokens, hidden] behind those that went into ``cache`` (a :class:`~triton_int8_amd.cache4.Cache4` of this
+        layer's heads), which they join.  ``rotary``: the tables of :func:`rope_tables` for as many positions as the sequences will have.  ``counts`` int32
+        [batch]: of sequence b only the first so many tokens are new, its other rows mean nothing.
+
+        A budget is kept by calling ``cache.evict(recent)`` between calls: what stays is attended to at the positions that it had."""
+        B, S, H = x.shape
+        cos, sin = rotary
+        if cache.seen + S > cos.shape[0]:
+            raise ValueError(f"{S} tokens behind {cache.seen} have positions beyond the {cos.shape[0]} of the rotary tables")
+        # (clamped: a recorded graph is replayed without the check above)
+        at = (cache.positions[:, None] + torch.arange(S, dtype=torch.int32, device=x.device)).clamp_(max=cos.shape[0] - 1).flatten()
+        cos, sin = cos.index_select(0, at), sin.index_select(0, at)
+        h = self.input_norm(x)
+        q, k, v = (t.view(1, B * S, self.heads, self.head_dim) for t in _projections(h, self.q_proj, self.k_proj, self.v_proj))
+        rotate = _RopeFunction.apply if self.int8 and self.head_dim % 16 == 0 and _kernels_take(q, k, cos, sin) else _rope_pair
+        q, k = rotate(q, k, cos, sin)
+        q, k, v = (t.reshape(B, S, self.heads, self.head_dim) for t in (q, k, v))
+        cache.append(k, v, counts=counts)
+        a = cache.attend(q, counts=counts)
+        x = x + self.o_proj(a.view(B, S, H))
         h = self.post_norm(x)
         gate, up = _projections(h, self.gate_proj, self.up_proj)
         product = _SwiGLUFunction.apply if self.int8 and _kernels_take(gate, up) else _swiglu
