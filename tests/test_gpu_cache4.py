@@ -391,3 +391,71 @@ def test_refusals(C, dev):
     with torch.no_grad():
         C.append(pool, table, one, kv.clone().requires_grad_(True), kv)
     assert not torch.equal(pool, before)
+
+
+def _masked_reference(pool, table, lengths, q, counts, scale, page):
+    """As oracle.attention, for tables with pages that the pool does not have: their entries are not seen."""
+    B, S, H, D = q.shape
+    hkv, pages = pool.shape[1], pool.shape[0]
+    out, lse = torch.zeros(B, S, H, D, dtype=torch.float64), torch.full((B, S, H), float("-inf"), dtype=torch.float64)
+    logits, spread = torch.zeros(B, S, H, dtype=torch.float64), torch.zeros(B, S, H, D, dtype=torch.float64)
+    gains = [[torch.zeros(n, dtype=torch.float64) for _ in range(hkv)] for n in lengths]
+    for b, n in enumerate(lengths):
+        j = torch.arange(n)
+        there = (table[b].long()[j // page] >= 0) & (table[b].long()[j // page] < pages)
+        for h in range(hkv):
+            k, v = oracle.entries(pool, table[b].clamp(0, pages - 1), page, D, h, n)
+            for t in range(counts[b]):
+                sees = there & (j <= n - counts[b] + t)
+                if not sees.any():
+                    continue
+                x = slice(h * (H // hkv), (h + 1) * (H // hkv))
+                rows = q[b, t, x].double()
+                s = (rows @ k[sees].T) * scale
+                p = s.softmax(-1)
+                out[b, t, x], lse[b, t, x] = p @ v[sees], s.logsumexp(-1)
+                logits[b, t, x] = (rows.abs() @ k[sees].abs().T * scale).amax(-1)
+                spread[b, t, x] = p @ v[sees].abs()
+                gains[b][h][sees] += p.sum(0)
+    return out, lse, gains, logits, spread
+
+
+# 4, 32, 36, 64, 65, 200 and 400 rows that share a kv head; several pages that are not there, a whole sequence of them, and one that is there alone
+@pytest.mark.parametrize("tokens,heads", [(1, 4), (8, 4), (9, 4), (16, 4), (65, 1), (50, 4), (100, 4)])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_that_are_not_there(C, dev, tokens, heads, page, dim):
+    gen = torch.Generator().manual_seed(tokens + page)
+    lengths = [700, 333, 128, 640]
+    mine = -(-700 // page)
+    pool, table = _pool(gen, 4 * mine, 1, page, dim), _table(gen, 4, mine, 4 * mine)
+    table[0, 1::3] = torch.tensor([-1, 4 * mine, 1 << 30]).repeat(mine)[:len(table[0, 1::3])]
+    table[2] = -5
+    table[3, :5], table[3, 6:] = 1 << 29, -1
+    weights = torch.rand(4 * mine, 1, page, generator=gen)
+    q = torch.randn(4, tokens, heads, dim, generator=gen).bfloat16()
+    want = _masked_reference(pool, table, lengths, q, [tokens] * 4, 1 / math.sqrt(dim), page)
+    g_weights = weights.to(dev)
+    out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev), weights=g_weights)
+    _check_attention(out, lse, want, dim, 700)
+    rel = 2.0 ** -18 + 4 * (dim + 8) * 2.0 ** -24 * float(want[3].max()) + tokens * heads * 2.0 ** -24      # as in test_attention
+    for b, n in enumerate(lengths):
+        for j in range(n):
+            at = int(table[b, j // page])
+            if 0 <= at < 4 * mine:
+                weights[at, 0, j % page] += want[2][b][0][j]
+    assert bool(((g_weights.cpu().double() - weights.double()).abs() <= rel * weights.double() + 2.0 ** -22 * weights.double()).all())
+
+
+@pytest.mark.parametrize("tokens,heads,hkv", [(9, 4, 1), (13, 8, 2), (64, 3, 3), (33, 1, 1), (2, 40, 2), (128, 2, 1), (257, 1, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_of_every_form(C, dev, tokens, heads, hkv, dim):
+    """33 to 64 rows (two waves share them), 128, 256 and 257; entries shared among many workgroups, and few of them."""
+    gen = torch.Generator().manual_seed(tokens + dim)
+    for page, lengths, counts in ((64, [3000, tokens, 1111], None), (16, [tokens + 1, 700], [tokens, tokens - 1])):
+        batch, mine = len(lengths), -(-max(lengths) // page)
+        pool, table = _pool(gen, batch * mine, hkv, page, dim), _table(gen, batch, mine, batch * mine)
+        q = torch.randn(batch, tokens, heads, dim, generator=gen).bfloat16()
+        want = oracle.attention(pool, table, lengths, q, counts or [tokens] * batch, 1 / math.sqrt(dim), page)
+        out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev), counts=None if counts is None else _ints(counts, dev))
+        _check_attention(out, lse, want, dim, max(lengths))

@@ -1073,6 +1073,12 @@ extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths,
     if (need > workspace_bytes) return fail(TI8_ERR_SHAPE, "%s: %lld bytes of workspace are needed, got %lld", fn, (long long)need, (long long)workspace_bytes);
     if (!aligned16(q) || !aligned16(out) || (reinterpret_cast<uintptr_t>(lse) & 3) || !aligned16(workspace) || q_stride_b % 8 || q_stride_t % 8 || q_stride_h % 8)
         return fail(TI8_ERR_ALIGN, "%s: q, out and the workspace must be 16-byte aligned, q's strides multiples of 8 elements", fn);
+    // weights_kernel: 32-bit offsets within a tile's rows
+    const int64_t group = heads / c.heads, tile_tokens = ROWS / group + 2;
+    const auto within = [&](int64_t st, int64_t sh) { return st >= 0 && sh >= 0 && st <= 0x3fffffff / tile_tokens && sh <= 0x3fffffff / group && tile_tokens * st + group * sh + c.dim <= 0x3fffffff; };
+    if (accumulate && (!within(q_stride_t, q_stride_h) || !within(heads, 1)))
+        return fail(TI8_ERR_SHAPE, "%s: q's strides of %lld and %lld elements between tokens and heads are too large for the weights to be added up", fn,
+                    (long long)q_stride_t, (long long)q_stride_h);
     Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace),
            (int)tokens, (int)heads, (int)(heads / c.heads), scale, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
