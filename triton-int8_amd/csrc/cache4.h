@@ -76,6 +76,10 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return dpp_add<0x143, 0xc>(v);
 }
 
+// 16 bytes that nobody asks for again soon
+__device__ __forceinline__ uint4 stream_load(const void* p) { return __builtin_bit_cast(uint4, __builtin_nontemporal_load(static_cast<const v4i*>(p))); }
+__device__ __forceinline__ void stream_store(void* p, uint4 x) { __builtin_nontemporal_store(__builtin_bit_cast(v4i, x), static_cast<v4i*>(p)); }
+
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 #if defined(__HIP_DEVICE_COMPILE__)
 // the two bf16 that byte I of a word of codes stands for (v_cvt_scalef32_pk_bf16_fp4)

@@ -16,7 +16,8 @@ constexpr int TILE = 16;        // tokens per wave
 // Eight elements per lane: the 32 that share a scale are four neighbouring lanes'.  a = max |x|; e = the exponent byte of the smallest
 // 2^(e - 127) with a <= 6 * 2^(e - 127) = 1.5 * 2^(e - 125): that of a less two, one more where a's fraction is over 1.5.  Dividing by a power of two
 // is exact, so codes do not depend on how the division is carried out.
-// Bound by memory: a wave has the keys and values of all its 16 tokens in flight before it converts the first.
+// Bound by memory: a wave has the keys and values of all its 16 tokens in flight before it converts the first, and past the caches, which they would only
+// fill (4 x 4096 tokens of 32 heads 67 us, 5.0 TB/s; through the caches 90; read back 50 us, 6.8 TB/s, and 82).
 template <int D>
 __global__ __launch_bounds__(64) void append_kernel(const Cache c, const int32_t* starts, const int32_t* counts, int tokens, Rows k, Rows v) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -32,8 +33,8 @@ __global__ __launch_bounds__(64) void append_kernel(const Cache c, const int32_t
         const int t = first + i * PER;
         page[i] = -1;
         if (t < n) {
-            w[i][0] = *reinterpret_cast<const uint4*>(k.p + b * k.sb + t * k.st + h * k.sh + chunk * 8);
-            w[i][1] = *reinterpret_cast<const uint4*>(v.p + b * v.sb + t * v.st + h * v.sh + chunk * 8);
+            w[i][0] = stream_load(k.p + b * k.sb + t * k.st + h * k.sh + chunk * 8);
+            w[i][1] = stream_load(v.p + b * v.sb + t * v.st + h * v.sh + chunk * 8);
             page[i] = page_of(c, b, start + t);
         }
     }
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(64) void read_kernel(const Cache c, const int32_t* 
         if (t >= tokens) break;
 #pragma unroll
         for (int values = 0; values < 2; ++values)
-            *reinterpret_cast<uint4*>((values ? v : k) + (((int64_t)b * tokens + t) * c.heads + h) * D + chunk * 8) = decode8(codes[i][values], scale_of(scales[i][values]));
+            stream_store((values ? v : k) + (((int64_t)b * tokens + t) * c.heads + h) * D + chunk * 8, decode8(codes[i][values], scale_of(scales[i][values])));
     }
 #endif
 }
