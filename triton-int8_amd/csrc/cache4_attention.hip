@@ -33,7 +33,8 @@ struct Args {
     int64_t q_sb, q_st, q_sh;
     uint16_t* out;
     float* lse;
-    float* parts;               // step_kernel: two per workgroup, see Part
+    int2* owners;               // step_kernel: first and last workgroup of every (sequence, head)
+    float* parts;               // two per workgroup, or one per row and split: see Part
     int tokens, heads, group;       // group = query heads per kv head
     float scale;
     int groups;                 // workgroups that share the units
@@ -45,7 +46,7 @@ __device__ __forceinline__ int seen_of(const Args& a, int b) { return count_of(a
 
 // ---- sharing out ---------------------------------------------------------------------------------------------
 
-// What a workgroup has of the units, or a (sequence, head): found by every wave from the lengths, the first 64 of which are read once
+// What a workgroup has of the units: found by every wave from the lengths, the first 64 of which are read once
 template <int UNIT, int EXTRA>     // EXTRA units of every head stand for what beginning and ending it takes
 struct Lengths {
     const Args& a;
@@ -58,17 +59,6 @@ struct Lengths {
         int n = last(upto);
         for (int b0 = 64; b0 < a.c.batch; b0 += 64) n += last(wave_prefix(of(b0 + lane)));
         return n * a.c.heads;
-    }
-    // units in front of sequence b; `own`: those of one of its heads
-    __device__ __forceinline__ int before(int b, int& own) const {
-        int n = 0, b0 = 0, x = first, up = upto;
-        for (; b - b0 >= 64; b0 += 64) {
-            n += last(up);
-            x = of(b0 + 64 + lane);
-            up = wave_prefix(x);
-        }
-        own = __builtin_amdgcn_readlane(x, b - b0);
-        return (n + __builtin_amdgcn_readlane(up, b - b0) - own) * a.c.heads;
     }
     // the sequence that a unit belongs to, the units in front of that sequence and those of one of its heads
     __device__ __forceinline__ int find(int unit, int& before, int& own) const {
@@ -107,7 +97,8 @@ __device__ __forceinline__ float over_rows(float x) {
 //
 // A wave takes 32 entries at a time, on its own: their keys go from memory to registers in the order of the operand (a lane has 32 or 16 neighbouring
 // elements of a key, which share a scale; the order of the elements in the sum is the same on both sides), their values in the same way, as
-// bf16 through 32 rows of LDS that are the wave's own and out again transposed (ds_read_b64_tr_b16).  The next 32 entries' loads are in flight
+// bf16 through 32 rows of LDS that are the wave's own and out again transposed (ds_read_b64_tr_b16); values are read past the caches, which
+// the keys stay in for weights_kernel (8 streams of up to 131072 entries 120 us -> 113).  The next 32 entries' loads are in flight
 // meanwhile.  Four waves of a workgroup take turns and add up at the end, with their workgroups' neighbours through memory.
 
 template <int D>
@@ -173,13 +164,14 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
                 const int row = (j & (c.page - 1)) + r16;
                 const uint8_t *const kc = block + idx::cache4_codes(c.page, D, 0, row) + quarter * (D / 8), *const vc = block + idx::cache4_codes(c.page, D, 1, row) + quarter * (D / 8);
                 if constexpr (D == 128) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(kc), z = *reinterpret_cast<const uint4*>(vc);
+                    const uint4 y = *reinterpret_cast<const uint4*>(kc), z = stream_load(vc);
                     x.k[u][0] = y.x; x.k[u][1] = y.y; x.k[u][2] = y.z; x.k[u][3] = y.w;
                     x.v[u][0] = z.x; x.v[u][1] = z.y; x.v[u][2] = z.z; x.v[u][3] = z.w;
                 } else {
-                    const uint2 y = *reinterpret_cast<const uint2*>(kc), z = *reinterpret_cast<const uint2*>(vc);
+                    const uint2 y = *reinterpret_cast<const uint2*>(kc);
+                    const v2i z = __builtin_nontemporal_load(reinterpret_cast<const v2i*>(vc));
                     x.k[u][0] = y.x; x.k[u][1] = y.y;
-                    x.v[u][0] = z.x; x.v[u][1] = z.y;
+                    x.v[u][0] = z[0]; x.v[u][1] = z[1];
                 }
                 x.ks[u] = block[idx::cache4_scales(c.page, D, 0, row) + quarter * (D / 4) / GROUP];
                 x.vs[u] = block[idx::cache4_scales(c.page, D, 1, row) + quarter * (D / 4) / GROUP];
@@ -298,6 +290,7 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
 
         // the waves' results meet in LDS, 16 rows at a time
         const bool whole = n == per_head;
+        if (unit == 0 && threadIdx.x == 0) a.owners[b * c.heads + h] = make_int2(blockIdx.x, whole ? blockIdx.x : idx::share_of(share, end - left + per_head - 1));
         float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (unit == 0)) * (TILES * 16) * Part<D>::ROW;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -413,12 +406,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const Cache& c = a.c;
     const int rows = a.tokens * a.group, row = blockIdx.x % rows, h = (int)(blockIdx.x / rows) % c.heads, b = (int)(blockIdx.x / rows) / c.heads;
-    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, threadIdx.x & 63);
-    const idx::Share share = idx::share_out(lengths.all(), a.groups);
-    int per_head, begin = lengths.before(b, per_head);
-    begin += h * per_head + EXTRA;
-    per_head -= EXTRA;
-    const int first = idx::share_of(share, begin), last = idx::share_of(share, begin + per_head - 1);
+    const int2 owners = a.owners[b * c.heads + h];
+    const int first = owners.x, last = owners.y;
     if (first == last) return;
     // a workgroup's second part is the one that starts with a head's first unit: here that of the first workgroup
     constexpr int64_t PART = TILES * 16 * Part<D>::ROW;
@@ -974,9 +963,10 @@ PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     p.splits = (int)(splits < 1 ? 1 : splits < most ? splits : most);
     return p;
 }
+int64_t owners_bytes(const Cache& c) { return ((int64_t)c.batch * c.heads * (int64_t)sizeof(int2) + 15) / 16 * 16; }
 int64_t workspace_bytes_of(const Cache& c, int64_t tokens, int64_t heads) {
     const int64_t rows = tokens * (heads / c.heads);
-    if (const int tiles = step_tiles(rows)) return (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 4) * (int64_t)sizeof(float);
+    if (const int tiles = step_tiles(rows)) return owners_bytes(c) + (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 4) * (int64_t)sizeof(float);
     const PromptPlan p = prompt_plan(c, rows);
     return p.splits > 1 ? c.batch * tokens * heads * p.splits * (c.dim + 4) * (int64_t)sizeof(float) : 0;
 }
@@ -1017,6 +1007,8 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
     int e;
     if (tiles) {
         a.groups = step_groups(a.c, tiles);
+        a.owners = reinterpret_cast<int2*>(a.parts);
+        a.parts += owners_bytes(a.c) / (int64_t)sizeof(float);
         e = tiles == 1 ? launch_step<D, 1>(fn, a, st) : launch_step<D, 2>(fn, a, st);
     } else {
         const PromptPlan p = prompt_plan(a.c, rows);
@@ -1079,7 +1071,7 @@ extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths,
     if (accumulate && (!within(q_stride_t, q_stride_h) || !within(heads, 1)))
         return fail(TI8_ERR_SHAPE, "%s: q's strides of %lld and %lld elements between tokens and heads are too large for the weights to be added up", fn,
                     (long long)q_stride_t, (long long)q_stride_h);
-    Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, static_cast<float*>(workspace),
+    Args a{c, lengths, counts, static_cast<const uint16_t*>(q), q_stride_b, q_stride_t, q_stride_h, static_cast<uint16_t*>(out), lse, nullptr, static_cast<float*>(workspace),
            (int)tokens, (int)heads, (int)(heads / c.heads), scale, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     return c.dim == 128 ? launch<128>(fn, a, accumulate != 0, st) : launch<64>(fn, a, accumulate != 0, st);
