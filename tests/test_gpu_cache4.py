@@ -459,3 +459,27 @@ def test_rows_of_every_form(C, dev, tokens, heads, hkv, dim):
         want = oracle.attention(pool, table, lengths, q, counts or [tokens] * batch, 1 / math.sqrt(dim), page)
         out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev), counts=None if counts is None else _ints(counts, dev))
         _check_attention(out, lse, want, dim, max(lengths))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_evict_sequences_of_every_length(C, dev, dim):
+    """Sequences that end anywhere within the entries that a wave moves, shorter and longer than the budget: only what is kept is written, and only to its place."""
+    gen = torch.Generator().manual_seed(dim)
+    page, keep, lengths = 16, 70, list(range(0, 101))
+    mine, new = -(-100 // page), -(-keep // page)
+    pages = len(lengths) * (mine + new)
+    pool = _pool(gen, pages, 1, page, dim, values=False)
+    order = torch.randperm(pages, generator=gen).int()
+    table, new_table = order[:len(lengths) * mine].view(-1, mine), order[len(lengths) * mine:].view(-1, new)
+    weights = torch.rand(pages, 1, page, generator=gen)
+    g_pool, g_weights = pool.to(dev), weights.to(dev)
+    kept, _ = C.evict(g_pool, table.to(dev), _ints(lengths, dev), g_weights, new_table.to(dev), keep=keep, recent=30)
+    p = (*oracle.parts(pool, page, dim), weights)
+    for b, n in enumerate(lengths):
+        j = torch.arange(n)
+        stay = oracle.kept(weights[table[b].long()[j // page], 0, j % page].tolist(), 30, keep)
+        assert kept[b, 0].tolist() == stay + [-1] * (keep - len(stay)), n
+        i, stay = torch.arange(len(stay)), torch.tensor(stay, dtype=torch.int64)
+        for t in p:
+            t[new_table[b].long()[i // page], 0, i % page] = t[table[b].long()[stay // page], 0, stay % page]
+    assert torch.equal(g_pool.cpu(), pool) and torch.equal(g_weights.cpu(), weights)

@@ -225,9 +225,11 @@ __global__ __launch_bounds__(256) void move_kernel(const Cache c, const int32_t*
     uint8_t* into[ROUNDS];
 #pragma unroll
     for (int x = 0; x < ROUNDS; ++x) {
-        const int entry = x * PER + lane / LANES, row = __shfl(r, entry, 64), new_row = __shfl(s, entry, 64);
-        const uint8_t* const block = block_of(c, max(__shfl(from, entry, 64), 0), h);
-        into[x] = __shfl((int)moves, entry, 64) ? block_of(c, __shfl(to, entry, 64), h) + new_row * (D / 2) + (lane % LANES) * 16 : nullptr;
+        // (every lane takes part in what it hears from the others: one that has nothing to move still knows an entry)
+        const int entry = x * PER + lane / LANES, row = __shfl(r, entry, 64), new_row = __shfl(s, entry, 64), page = __shfl(from, entry, 64), new_page = __shfl(to, entry, 64);
+        const bool goes = __shfl((int)moves, entry, 64);
+        const uint8_t* const block = block_of(c, max(page, 0), h);
+        into[x] = goes ? block_of(c, new_page, h) + new_row * (D / 2) + (lane % LANES) * 16 : nullptr;
         // (also of an entry that stays behind: a row of some page)
         codes[x][0] = *reinterpret_cast<const v4i*>(block + idx::cache4_codes(c.page, D, 0, row) + (lane % LANES) * 16);
         codes[x][1] = *reinterpret_cast<const v4i*>(block + idx::cache4_codes(c.page, D, 1, row) + (lane % LANES) * 16);
