@@ -130,6 +130,8 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
         const int page = page_of(c, b, j);
         return page < 0 ? 0u : order_of(c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))]);
     };
+    for (int i = tid; i < BINS; i += SELECT) bins[i] = 0;
+    __syncthreads();
     // eight entries of a thread at a time: their pages, then their weights
     const int held = min(old, HELD);
     for (int j0 = tid; j0 < held; j0 += 8 * SELECT) {
@@ -142,19 +144,26 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
             w[i] = c.weights[((int64_t)((unsigned)page[i] < (unsigned)c.pages ? page[i] : 0) * c.heads + h) * c.page + ((j0 + i * SELECT) & (c.page - 1))];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (j0 + i * SELECT < held) orders[j0 + i * SELECT] = (unsigned)page[i] < (unsigned)c.pages ? order_of(w[i]) : 0u;
+            if (j0 + i * SELECT < held) {
+                const uint32_t u = (unsigned)page[i] < (unsigned)c.pages ? order_of(w[i]) : 0u;
+                orders[j0 + i * SELECT] = u;
+                atomicAdd(&bins[u >> (32 - DIGIT)], 1);
+            }
     }
     const auto order = [&](int j) { return j < HELD ? orders[j] : fetch(j); };
+    for (int j = HELD + tid; j < old; j += SELECT) atomicAdd(&bins[order(j) >> (32 - DIGIT)], 1);
     uint32_t limit = 0;         // the heavy-th largest, as far as it is known
     int left = heavy;           // how many of those that agree with it so far are to stay
     for (int shift = 32 - DIGIT; ; shift = max(shift - DIGIT, 0)) {
-        const int known = shift == 32 - DIGIT ? 32 : shift == 32 - 2 * DIGIT ? 32 - DIGIT : 32 - 2 * DIGIT;        // the bits from here on agree with the limit
-        const uint32_t mask = (1u << (known - shift)) - 1;
-        for (int i = tid; i < BINS; i += SELECT) bins[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < old; j += SELECT) {
-            const uint32_t u = order(j);
-            if (known == 32 || u >> known == limit >> known) atomicAdd(&bins[u >> shift & mask], 1);
+        if (shift < 32 - DIGIT) {
+            const int known = shift == 32 - 2 * DIGIT ? 32 - DIGIT : 32 - 2 * DIGIT;        // the bits from here on agree with the limit
+            const uint32_t mask = (1u << (known - shift)) - 1;
+            for (int i = tid; i < BINS; i += SELECT) bins[i] = 0;
+            __syncthreads();
+            for (int j = tid; j < old; j += SELECT) {
+                const uint32_t u = order(j);
+                if (u >> known == limit >> known) atomicAdd(&bins[u >> shift & mask], 1);
+            }
         }
         __syncthreads();
         // from the largest bin on: a thread has two neighbours
