@@ -420,8 +420,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // ---- many rows: prompts ------------------------------------------------------------------------------------------
 //
 // A wave has 32 rows of queries as the columns of 32 x 32 products (S^T = K Q^T, O^T = V^T P^T: a lane has one row of queries, as above); the waves
-// of a workgroup go through the entries together, 64 at a time, which they turn into bf16 in LDS once for all, two tiles ahead (one, where four waves share
-// a CU with another four); the codes of the tile behind that are on their way meanwhile.
+// of a workgroup go through the entries together, 64 at a time, which they turn into bf16 in LDS once for all, two tiles ahead (one, where a
+// workgroup of four waves shares a CU with others); the codes of the tile behind that are on their way meanwhile.
 // A wave's scores of 32 entries are multiplied while it takes the exponentials of the 32 before, and the maxima of the one's are found while the other's
 // values are multiplied: products and vector instructions of a wave alternate, or they would take turns on all waves, which the tiles keep in step.
 // A head's row blocks lie on one XCD, whose L2 then serves the entries; where there are too few row blocks for the chip, several workgroups share the
@@ -946,19 +946,21 @@ int step_groups(const Cache& c, int tiles) {
 // 64 rows 62 us to 54; two less, 16 streams of 8192 and 32 rows 57 to 76
 int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 0; }
 
-// prompt_kernel: waves of a workgroup, how many of them have the same rows, and how many workgroups share the entries of a row block.  Eight waves convert every
-// entry for 256 rows; four are taken where the eight would hold more rows that are none and the CUs have not all got one.  Up to 64 rows two and two of
-// them share the rows (4 streams of 16384 entries, 64 rows: PAIRED).  Parts are worth it from 4 tiles of entries on.
+// prompt_kernel: waves of a workgroup, how many of them have the same rows, and how many workgroups share the entries of a row block.  Heads of 128: eight waves
+// convert every entry for 256 rows and have a CU to themselves; four, two workgroups of which a CU holds, are taken where the eight would hold more rows
+// that are none and the CUs have not all got one (100 tokens of 4 heads each over 32768 entries, 400 rows in 512 either way: 101 us with four, 93 with eight; 300 rows
+// over 2000 entries: 35.5 in 384, 37.8 in 512).  Heads of 64: four waves, whose registers a CU holds three times (1000 tokens over 2000 entries 45 -> 40 us).
+// Up to 64 rows two and two of the four share the rows (4 streams of 16384 entries, 64 rows: 49 -> 45 us).  Parts are worth it from 4 tiles of entries on.
 struct PromptPlan {
     int waves, shares, blocks, splits;
 };
 PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     const int64_t pairs = (int64_t)c.batch * c.heads, cus = device_cu_count();
     PromptPlan p;
-    p.waves = rows > 128 && (pairs * ((rows + 255) / 256) >= cus || (rows + 255) / 256 * 2 == (rows + 127) / 128) ? 8 : 4;
+    p.waves = c.dim == 128 && rows > 128 && (pairs * ((rows + 255) / 256) >= cus || (rows + 255) / 256 * 2 == (rows + 127) / 128) ? 8 : 4;
     p.shares = rows <= 64 ? 2 : 1;
     p.blocks = (int)((rows * p.shares + p.waves * 32 - 1) / (p.waves * 32));
-    const int64_t groups = pairs * p.blocks, room = cus * (8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
+    const int64_t groups = pairs * p.blocks, room = cus * (c.dim == 64 ? 3 : 8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
     const int64_t splits = room / groups;
     p.splits = (int)(splits < 1 ? 1 : splits < most ? splits : most);
     return p;
@@ -1014,7 +1016,9 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
         const PromptPlan p = prompt_plan(a.c, rows);
         a.blocks = p.blocks;
         a.splits = p.splits;
-        e = p.waves == 8 ? launch_prompt<D, 8, 1>(fn, a, st) : p.shares == 2 ? launch_prompt<D, 4, 2>(fn, a, st) : launch_prompt<D, 4, 1>(fn, a, st);
+        if (p.shares == 2) e = launch_prompt<D, 4, 2>(fn, a, st);
+        else if (D == 128 && p.waves == 8) e = launch_prompt<128, 8, 1>(fn, a, st);
+        else e = launch_prompt<D, 4, 1>(fn, a, st);
     }
     if (e || !accumulate) return e;
     const int64_t units = (int64_t)a.c.batch * a.c.heads * idx::cache4_units(a.c.capacity(), WEIGHTS_UNIT), most = device_cu_count() * 2;
@@ -1030,7 +1034,6 @@ int init_attention() {
     int e = prepare_prompt<128, 8, 1>(fn);
     if (!e) e = prepare_prompt<128, 4, 1>(fn);
     if (!e) e = prepare_prompt<128, 4, 2>(fn);
-    if (!e) e = prepare_prompt<64, 8, 1>(fn);
     if (!e) e = prepare_prompt<64, 4, 1>(fn);
     return e ? e : prepare_prompt<64, 4, 2>(fn);
 }
