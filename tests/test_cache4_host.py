@@ -272,6 +272,7 @@ def test_weights_kernel_waits_for_what_it_issues(tmp_path):
         assert walks, name
         inner = min(walks, key=len)
         issued = re.findall(r"^\s*" + VMEM + r"([^\n]*)", inner, flags=re.M)
-        assert len(issued) == per_tile and all(rest.rstrip().endswith("lds") for _, rest in issued), (name, issued)
+        assert len(issued) == per_tile and all("_lds_" in op or rest.rstrip().endswith("lds") for op, rest in issued), (name, issued)
+        assert len(re.findall(r"vmcnt\(", inner)) == 1, name         # nothing else in the walk waits for loads
         behind = body[body.index(inner) + len(inner):]
         assert re.search(r"s_waitcnt vmcnt\(0\)", behind), name

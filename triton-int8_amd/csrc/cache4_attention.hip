@@ -731,7 +731,6 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 constexpr int COLUMNS = 32, WEIGHT_WAVES = 8, WEIGHTS_UNIT = WEIGHT_WAVES * COLUMNS, ROWS = 64, RING = 3;
 
 #if defined(__HIP_DEVICE_COMPILE__)
-typedef __attribute__((address_space(3))) void lds_void;
 // all but this wave's last N loads have landed, its LDS reads have returned, and the same holds for the other waves
 template <int N>
 __device__ __forceinline__ void wait_and_meet() {
@@ -746,8 +745,10 @@ template <int D>
 __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int UNIT = WEIGHTS_UNIT, STEPS = D / 16, ROW = 2 * D, CHUNKS = D / 8, PASSES = ROWS * CHUNKS / (WEIGHT_WAVES * 64), LOADS = PASSES + 1;
-    __shared__ __attribute__((aligned(1024))) uint8_t queries[RING][ROWS * ROW];
-    __shared__ __attribute__((aligned(1024))) float lses[RING][WEIGHT_WAVES][ROWS];       // every wave has its own
+    __shared__ __attribute__((aligned(1024))) int8_t smem[RING * (ROWS * ROW + WEIGHT_WAVES * ROWS * 4)];
+    const auto queries = [&](int stage) { return smem + stage * (ROWS * ROW); };
+    // times log2(e) once they are there; every wave has its own
+    const auto lses = [&](int stage) { return reinterpret_cast<float*>(smem + RING * ROWS * ROW + (stage * WEIGHT_WAVES + (int)(threadIdx.x >> 6)) * (ROWS * 4)); };
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5;
     const Lengths<UNIT, 0> lengths(a, lane);
@@ -830,8 +831,8 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
         const int first = rows <= ROWS ? 0 : max(unit0 - older, 0) * a.group / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
 
         // A thread's rows are 64 apart from one tile to the next: their heads and offsets are counted on, a division each would take as long as the scores.
-        // Offsets are those from the tile's first token (ti8_cache4_attention checks the strides); behind the last row's end zeros are loaded, and
-        // a row that is none but lies in front of it is some part of q.
+        // Offsets are those from the tile's first token (ti8_cache4_attention checks the strides), and none goes beyond the last row: one that is none is
+        // some part of q.
         struct Place {
             int head;
             uint32_t offset;        // in bytes
@@ -856,24 +857,24 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             at[i].offset += ((lane % CHUNKS) ^ Values<D>::swizzle(row)) * 16;
         }
         const auto issue = [&](int stage) {
-            const int tokens = max(count - token0, 0);      // none are left for the tiles that are asked for behind the last
-            const auto rows_of = [&](const void* base, int64_t st, int64_t sh, int64_t bytes) {
-                const int64_t all = tokens ? (tokens - 1) * st + (a.group - 1) * sh + bytes : 0;
-                return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)min(all, (int64_t)0x7fffffff), 0x00027000);
-            };
-            const __amdgpu_buffer_rsrc_t rq = rows_of(a.q + b * a.q_sb + token0 * a.q_st + h * a.group * a.q_sh, a.q_st * 2, a.q_sh * 2, 2 * D);
-            const __amdgpu_buffer_rsrc_t rl = rows_of(a.lse + ((int64_t)b * a.tokens + token0) * a.heads + h * a.group, a.heads * 4, 4, 4);
+            const int at_token = min(token0, count - 1), tokens = min(count - at_token, ROWS / a.group + 2);
+            const auto last_of = [&](uint32_t st, uint32_t sh) { return (tokens - 1) * st + (a.group - 1) * sh; };
+            const int8_t* const bq = reinterpret_cast<const int8_t*>(a.q + b * a.q_sb + at_token * a.q_st + h * a.group * a.q_sh);
+            const int8_t* const bl = reinterpret_cast<const int8_t*>(a.lse + ((int64_t)b * a.tokens + at_token) * a.heads + h * a.group);
+            const uint32_t rq = last_of(q_st, q_sh) + 2 * D - 16, rl = last_of(lse_st, lse_sh);
             int more = head0 + step_head >= a.group;
             head0 += step_head - (more ? a.group : 0);
             more += step_token;
             token0 += more;
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (lds_void*)(queries[stage] + (i * WEIGHT_WAVES + wave) * 1024), 16, at[i].offset, 0, 0, 0);
-                go_on(at[i], q_st, q_sh, more);
+            for (int i = 0; i < PASSES; ++i)
+                __builtin_amdgcn_global_load_lds(bq + min(at[i].offset, rq), queries(stage) + (i * WEIGHT_WAVES + wave) * 1024, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(bl + min(at_lse.offset, rl), reinterpret_cast<int8_t*>(lses(stage)), 4, 0, 0);
+            if (step_head) {        // (where a tile is whole tokens, offsets from its first stay as they are)
+#pragma unroll
+                for (int i = 0; i < PASSES; ++i) go_on(at[i], q_st, q_sh, more);
+                go_on(at_lse, lse_st, lse_sh, more);
             }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds_void*)lses[stage][wave], 4, at_lse.offset, 0, 0, 0);
-            go_on(at_lse, lse_st, lse_sh, more);
         };
 
         float sum = 0.0f;
@@ -881,30 +882,43 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             // somebody of these rows sees one of the wave's entries
             if (j0 >= length || row0 + ROWS <= (j0 - older) * a.group) return;
             const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32), sees = (j - older) * a.group - row0;        // sees: the first row that sees this lane's entry
-#pragma unroll
-            for (int u = 0; u < ROWS / 32; ++u) {
-                if (row0 + u * 32 >= rows) break;
-                const uint8_t* const from = queries[stage] + (u * 32 + r32) * ROW;
+            const auto scores = [&](int u) {
+                const int8_t* const from = queries(stage) + (u * 32 + r32) * ROW;
                 v16f s;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
                 for (int x = 0; x < STEPS; ++x) s = mfma32(*reinterpret_cast<const v8bf*>(from + ((chunk ^ x) << 4)), k[x], s);
-                const bool edge = row0 + u * 32 < (j0 + COLUMNS - 1 - older) * a.group || row0 + u * 32 + 32 > rows;       // not every row is one and sees every entry
+                return s;
+            };
+            const auto exponentials = [&](const v16f& s, int u, int g, auto edge) {
+                const v4f shift = *reinterpret_cast<const v4f*>(lses(stage) + u * 32 + 8 * g + 4 * half);
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = u * 32 + 8 * g + 4 * half + i;
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -shift[i]));
+                    if (edge) p[i] = row >= sees && row0 + row < rows ? p[i] : 0.0f;
+                }
+                return (p[0] + p[1]) + (p[2] + p[3]);
+            };
+            if (row0 + ROWS <= rows && row0 >= (j0 + COLUMNS - 1 - older) * a.group) {      // every row is one and sees every entry
+#pragma unroll
+                for (int u = 0; u < ROWS / 32; ++u) {
+                    const v16f s = scores(u);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) sum += exponentials(s, u, g, std::false_type{});
+                }
+                return;
+            }
+#pragma unroll
+            for (int u = 0; u < ROWS / 32; ++u) {
+                if (row0 + u * 32 >= rows) break;
+                const v16f s = scores(u);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (row0 + u * 32 + 8 * g >= rows) break;       // (a step's few rows: no exponentials of rows that are none)
-                    const v4f shift = *reinterpret_cast<const v4f*>(lses[stage][wave] + u * 32 + 8 * g + 4 * half) * LOG2E;
-                    float p[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], factor, -shift[i]));
-                    if (edge)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int row = u * 32 + 8 * g + 4 * half + i;
-                            p[i] = row >= sees && row0 + row < rows ? p[i] : 0.0f;
-                        }
-                    sum += (p[0] + p[1]) + (p[2] + p[3]);
+                    sum += exponentials(s, u, g, std::true_type{});
                 }
             }
         };
@@ -913,6 +927,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
                 wait_and_meet<0>();
                 issue(0);
                 wait_and_meet<0>();
+                lses(0)[lane] *= LOG2E;
                 staged_b = b;
                 staged_h = h;
             }
@@ -925,6 +940,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             for (int t = 0, stage = 0; t < tiles; ++t) {
                 wait_and_meet<LOADS>();       // tile t is there, and nobody reads tile t - 1, whose place is the next one's
                 issue(stage == 0 ? RING - 1 : stage - 1);
+                lses(stage)[lane] *= LOG2E;
                 add_up(first + t * ROWS, stage);
                 stage = stage == RING - 1 ? 0 : stage + 1;
             }
