@@ -100,6 +100,11 @@ __device__ __forceinline__ float over_rows(float x) {
 // bf16 through 32 rows of LDS that are the wave's own and out again transposed (ds_read_b64_tr_b16); values are read past the caches, which
 // the keys stay in for weights_kernel (8 streams of up to 131072 entries 120 us -> 113).  The next 32 entries' loads are in flight
 // meanwhile.  Four waves of a workgroup take turns and add up at the end, with their workgroups' neighbours through memory.
+//
+// Bound by memory where there are many entries: 8 streams of up to 131072 entries, 616 MB, 106 to 110 us = 5.6 to 5.8 TB/s (a large copy here: 4.95 TB/s
+// read and written).  A step over a few thousand entries is mostly the kernel's beginning and end: one stream of 8192 entries of one head 6.0 us, of which 1.5
+// are the launch, 1.4 to find the units, 1.3 the first loads, 1.2 the waves' sum.  Not taken: the next head's first loads in front of a head's
+// end (registers spill, slower), four workgroups per CU, 64 rows in registers (see step_tiles).
 
 template <int D>
 struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 16 rows' writes of a chunk and 4 x 4 rows' transposing reads spread over the banks
@@ -115,7 +120,8 @@ struct Part {       // what a workgroup leaves of a (sequence, head) that it has
 };
 
 constexpr int WAVES = 4, ENTRIES = 32;      // waves of a workgroup; entries of a wave's turn
-// Units that beginning and ending a head count for when the units are shared out.  TUNE
+// Units that beginning and ending a head count for when the units are shared out: 16 sequences of 1 to 4096 entries, 32 heads each: 37.5 us with none, 28.6
+// with two, 30.9 with four, 32.4 with six
 constexpr int EXTRA = 2;
 static_assert(idx::CACHE4_UNIT == WAVES * ENTRIES, "a unit is a turn of every wave");
 
@@ -400,7 +406,7 @@ __device__ __forceinline__ void join(const Args& a, const float* one, const floa
 #endif
 }
 
-// Rows whose (sequence, head) several workgroups had: one workgroup each
+// Rows whose (sequence, head) several workgroups had: one workgroup each.  Bound by latency (owners, maxima, parts, one after the other): 3.8 to 5 us
 template <int D, int TILES>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -426,6 +432,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // values are multiplied: products and vector instructions of a wave alternate, or they would take turns on all waves, which the tiles keep in step.
 // A head's row blocks lie on one XCD, whose L2 then serves the entries; where there are too few row blocks for the chip, several workgroups share the
 // entries of one and join_rows_kernel adds them up.
+//
+// Bound by the issue of a SIMD, which products and exponentials share, at the clock that the chip's power allows: 2 x 2048 tokens of 32 heads behind 6144 entries
+// 456 to 470 us = 1.02 to 1.05 PFLOP/s (a matrix product of the library: 1.4 to 1.46).  Short prompts of several lengths: by the longest row block's
+// chain of tiles (2 us each with 256 rows).
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -725,8 +735,13 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 // weights of entry j += sum over rows of exp(s_j - lse): the scores once more, with the entries as columns of 32 x 32 products, so that a lane adds up the
 // rows of one entry.  Units of 256 entries are shared out as for step_kernel; each of eight waves has the keys of 32 in registers and goes through the rows
 // that see them, which the workgroup brings into LDS 64 at a time, two tiles ahead, without a trip through registers.  Every entry has one owner: no
-// atomics, sums in a fixed order.  Bound by latency where there are few rows or few workgroups: a wave's products and exponentials take turns, so there are
-// many waves.
+// atomics, sums in a fixed order.
+//
+// Few rows: bound by the beginning and by memory (32 streams of 2048 entries of 8 heads: 39 MB in 15 us); many: by the issue of a SIMD, as prompt_kernel (8 x 1024 tokens
+// over 4096 entries of 32 heads: 315 us = 0.76 PFLOP/s), and, with one or two units per workgroup, by the units that most rows see.  The loads to LDS
+// are global_load_lds: in front of every read of LDS the compiler waits for all buffer loads to LDS, also for those two tiles ahead (390 us).
+// Not taken: a step's exponentials beside the next scores' products in one wave (354 us: the waves of a SIMD overlap as it is, and registers are short);
+// lse from the attention's parts instead of the joined one, which would save a launch's 4 us but reads all parts of a head in every workgroup.
 
 constexpr int COLUMNS = 32, WEIGHT_WAVES = 8, WEIGHTS_UNIT = WEIGHT_WAVES * COLUMNS, ROWS = 64, RING = 3;
 
@@ -953,7 +968,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
 #endif
 }
 
-// Workgroups of step_kernel: as many as run at a time (four per CU with 16 rows, which the registers allow, two otherwise), and no more than there are units
+// Workgroups of step_kernel: as many as run at a time (three per CU with 16 rows, two with 32: their registers), and no more than there are units
 int step_groups(const Cache& c, int tiles) {
     const int64_t units = (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA), most = device_cu_count() * (tiles == 1 ? 3 : 2);
     return (int)(units < most ? units : most);
