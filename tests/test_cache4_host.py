@@ -73,7 +73,7 @@ ROWS = (FAKE, 2048, 256, 128)
 ])
 def test_arguments_that_are_refused(lib, name, args, code, msg):
     l = lib.lib()
-    assert getattr(l, "ti8_cache4_" + name)(_cache(lib), *args) == code
+    assert getattr(l, "ti8_cache4_" + name)(_cache(lib, table_pages=64, table_stride=64), *args) == code
     assert msg in l.ti8_last_error().decode(), l.ti8_last_error()
 
 
@@ -85,7 +85,8 @@ def test_weights_are_required_where_they_are_used(lib):
 
 def test_workspace_sizes(lib):
     size = lambda tokens, heads, **o: lib.lib().ti8_cache4_attention_workspace(_cache(lib, **o), tokens, heads)
-    assert size(1, 8) > 0 and size(1, 7) == -1 and size(0, 8) == -1 and size(1, 8, head_dim=80) == -1
+    assert size(1, 8, table_pages=64, table_stride=64) > 0 and size(1, 8) == 0          # (short sequences have a workgroup each)
+    assert size(1, 7) == -1 and size(0, 8) == -1 and size(1, 8, head_dim=80) == -1
     assert size(1 << 24, 64) == -1          # more rows than a launch takes
     assert size(1, 2, batch=65535, table_pages=1 << 18, table_stride=1 << 18) == -1
 
@@ -259,7 +260,8 @@ def test_kernels_do_not_spill(tmp_path):
         for name, v in kernels.items():
             assert v["private_segment_fixed_size"] == 0 and v["next_free_vgpr"] <= most, (name, v)
     step = {k: v["next_free_vgpr"] for k, v in kernels.items() if "step_kernel" in k}
-    assert all(n <= 168 for k, n in step.items() if k.endswith("Li1EEEvNS1_4ArgsE")), step          # three workgroups per CU
+    assert all(n <= 168 for k, n in step.items() if re.search("ILi(64|128)ELi1ELb0E", k)), step          # three workgroups per CU
+    assert all(n <= 128 for k, n in step.items() if "ILi64ELi1ELb1E" in k) and len(step) == 8, step      # two of eight waves
     assert all(v["next_free_vgpr"] <= 128 for k, v in kernels.items() if "weights_kernel" in k)       # two of eight waves
 
 

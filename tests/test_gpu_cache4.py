@@ -483,3 +483,49 @@ def test_evict_sequences_of_every_length(C, dev, dim):
         for t in p:
             t[new_table[b].long()[i // page], 0, i % page] = t[table[b].long()[stay // page], 0, stay % page]
     assert torch.equal(g_pool.cpu(), pool) and torch.equal(g_weights.cpu(), weights)
+
+
+@pytest.mark.parametrize("tokens,heads,hkv,page,lengths,counts", [s for s in SIZES if s[0] * s[1] // s[2] <= 32 and max(s[4]) <= 1000], ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_steps_whatever_room_the_table_has(C, dev, tokens, heads, hkv, page, lengths, counts, dim):
+    """The same entries in tables of short and long rows, which decide how they are shared out; some pages are not there, some values are no numbers."""
+    gen = torch.Generator().manual_seed(tokens + heads + dim)
+    batch, mine = len(lengths), -(-max(lengths) // page)
+    pool, table = _pool(gen, batch * mine, hkv, page, dim), _table(gen, batch, mine, batch * mine)
+    for b in range(1, batch, 2):
+        table[b, (mine - 1) // 2] = batch * mine + b
+    q = torch.randn(batch, tokens, heads, dim, generator=gen).bfloat16()
+    want = _masked_reference(pool, table, lengths, q, counts or [tokens] * batch, 1 / math.sqrt(dim), page)
+    q = q.to(dev)
+    ragged = None if counts is None else _ints(counts, dev)
+    for room in (mine * page, 512, 528, 1024, 1280, 2048, 2304, 5120):
+        if room >= mine * page and room % page == 0:
+            wide = torch.full((batch, room // page), -1, dtype=torch.int32)
+            wide[:, :mine] = table
+            weights = torch.zeros(pool.shape[0], hkv, page, device=dev)
+            out, lse = C.attention(pool.to(dev), wide.to(dev), _ints(lengths, dev), q, counts=ragged, weights=weights)
+            _check_attention(out, lse, want, dim, max(lengths))
+            odd = q.clone()
+            odd[0, 0, -1, 3] = float("inf")
+            out2, lse2 = C.attention(pool.to(dev), wide.to(dev), _ints(lengths, dev), odd, counts=ragged)
+            out2[0, 0, -1], lse2[0, 0, -1] = out[0, 0, -1], lse[0, 0, -1]
+            assert torch.equal(out2, out) and torch.equal(lse2, lse)
+
+
+@pytest.mark.parametrize("heads,room", [(100, 512), (100, 528), (200, 512), (200, 528), (86, 2048), (85, 2048), (86, 2064), (128, 1040), (171, 256), (171, 528)])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (64, 20), (128, 1), (128, 20)])
+def test_steps_of_many_heads(C, dev, heads, room, dim, tokens):
+    """Around one, two and more heads per CU, of sequences with none, few and all the entries that there is room for."""
+    gen = torch.Generator().manual_seed(heads + room + dim)
+    page, lengths = 16, [room, 0, room // 3]
+    mine = room // page
+    pool, table = _pool(gen, 2 * mine + 5, heads, page, dim), _table(gen, 3, 2 * mine // 3, 2 * mine + 5)
+    table = torch.cat((table, torch.full((3, mine - table.shape[1]), -1, dtype=torch.int32)), 1)
+    table[0] = torch.randperm(2 * mine + 5, generator=gen)[:mine].int()
+    q = torch.randn(3, tokens, heads, dim, generator=gen).bfloat16()
+    out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev))
+    some = [0, heads // 2, heads - 1]
+    want = oracle.attention(pool[:, some].contiguous(), table, lengths, q[:, :, some], [tokens] * 3, 1 / math.sqrt(dim), page)
+    _check_attention(out[:, :, some], lse[:, :, some], want, dim, room)
+    assert bool((lse[1] == float("-inf")).all()) and not bool(out[1].any())
+    assert bool(torch.isfinite(lse[0, -1]).all()) and bool(torch.isfinite(out).all())

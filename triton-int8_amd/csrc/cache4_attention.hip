@@ -125,32 +125,46 @@ constexpr int WAVES = 4, ENTRIES = 32;      // waves of a workgroup; entries of 
 constexpr int EXTRA = 2;
 static_assert(idx::CACHE4_UNIT == WAVES * ENTRIES, "a unit is a turn of every wave");
 
-template <int D, int TILES>     // TILES * 16 rows
-__global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(const Args a) {
+template <int D, int TILES, bool OWN>     // TILES * 16 rows; whether every (sequence, head) has a workgroup of its own, of twice the waves
+__global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 2 ? 2 : 3) void step_kernel(const Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     using V = Values<D>;
     constexpr int STEPS = D / 32;       // words of codes of an entry that a lane has; products over D
-    constexpr int BLOCKS = D / 16;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * V::BYTES];
-    __shared__ float stats[WAVES][2][16];
+    constexpr int BLOCKS = D / 16, NW = OWN ? 2 * WAVES : WAVES;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * V::BYTES];
+    __shared__ float stats[NW][2][16];
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quarter = lane >> 4;
-    const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, lane);
-    const idx::Share share = idx::share_out(lengths.all(), a.groups);
-    if ((int)blockIdx.x >= share.groups) return;
-    const int begin = idx::share_begin(share, blockIdx.x), end = idx::share_begin(share, blockIdx.x + 1);
-    int before, per_head, b = lengths.find(begin, before, per_head);
-    int length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
-    const int at_begin = (begin - before) % per_head;
-    int h = (begin - before) / per_head, unit = max(at_begin - EXTRA, 0);
-    per_head -= EXTRA;
+    idx::Share share;
+    int b, h, length, per_head, end, left, unit = 0;
+    if constexpr (OWN) {
+        b = blockIdx.x / c.heads;
+        h = blockIdx.x % c.heads;
+        length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
+        per_head = idx::cache4_units(length, NW * ENTRIES);
+        end = left = per_head + EXTRA;
+    } else {
+        const Lengths<idx::CACHE4_UNIT, EXTRA> lengths(a, lane);
+        share = idx::share_out(lengths.all(), a.groups);
+        if ((int)blockIdx.x >= share.groups) return;
+        const int begin = idx::share_begin(share, blockIdx.x);
+        int before;
+        end = idx::share_begin(share, blockIdx.x + 1);
+        b = lengths.find(begin, before, per_head);
+        length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
+        const int at_begin = (begin - before) % per_head;
+        h = (begin - before) / per_head;
+        unit = max(at_begin - EXTRA, 0);
+        left = end - begin - max(EXTRA - at_begin, 0);
+        per_head -= EXTRA;
+    }
     uint8_t* const mine = smem + wave * V::BYTES;
     // (a negative scale: the queries' signs are changed, which is exact.  Above zero, so that what is masked stays at -inf)
     const float factor = fmaxf(fabsf(a.scale) * LOG2E, 0x1p-126f);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
 
-    for (int left = end - begin - max(EXTRA - at_begin, 0); left > 0;) {
-        const int n = min(left, per_head - unit), first = unit * WAVES + wave, last = (unit + n) * WAVES;       // this wave's turns
+    while (left > 0) {
+        const int n = min(left, per_head - unit), first = unit * NW + wave, last = (unit + n) * NW;       // this wave's turns
         const int count = count_of(a.counts, b, a.tokens), rows = count * a.group;
         const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
         struct Turn {
@@ -193,7 +207,7 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
         int page[2];
         pages_of(first, page);
         if (first < last) load(first, page, now);
-        pages_of(min(first + WAVES, last - 1), page);
+        pages_of(min(first + NW, last - 1), page);
 
         // this wave's queries as operands, and up to where each row sees
         v8bf q[TILES][STEPS];
@@ -286,17 +300,17 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
             asm volatile("" ::: "memory");
         };
 
-        for (int turn = first; turn < last; turn += WAVES) {
+        for (int turn = first; turn < last; turn += NW) {
             Turn next;
-            if (turn + WAVES < last) load(turn + WAVES, page, next);
-            pages_of(min(turn + 2 * WAVES, last - 1), page);
+            if (turn + NW < last) load(turn + NW, page, next);
+            pages_of(min(turn + 2 * NW, last - 1), page);
             compute(turn, now);
             now = next;
         }
 
         // the waves' results meet in LDS, 16 rows at a time
-        const bool whole = n == per_head;
-        if (unit == 0 && threadIdx.x == 0) a.owners[b * c.heads + h] = make_int2(blockIdx.x, whole ? blockIdx.x : idx::share_of(share, end - left + per_head - 1));
+        const bool whole = OWN || n == per_head;
+        if (!OWN && unit == 0 && threadIdx.x == 0) a.owners[b * c.heads + h] = make_int2(blockIdx.x, whole ? blockIdx.x : idx::share_of(share, end - left + per_head - 1));
         float* const part = a.parts + ((int64_t)blockIdx.x * 2 + (unit == 0)) * (TILES * 16) * Part<D>::ROW;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
@@ -310,13 +324,13 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
             for (int d = 0; d < BLOCKS; ++d)
                 *reinterpret_cast<v4f*>(mine + r16 * (4 * D) + (((d * 4 + quarter) ^ r16) << 4)) = o[t][d];
             __syncthreads();
-            const int row = threadIdx.x >> 4;
+            const int row = threadIdx.x / (NW * 4), lane_of = threadIdx.x % (NW * 4);
             float m = -INFINITY, l = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w][0][row]);
-            float f[WAVES];
+            for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][0][row]);
+            float f[NW];
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 f[w] = stats[w][0][row] == -INFINITY ? 0.0f : exp2f((stats[w][0][row] - m) * factor);
                 // (a NaN in the sum passes a maximum of -inf)
                 l += stats[w][0][row] == -INFINITY ? stats[w][1][row] : stats[w][1][row] * f[w];
@@ -326,17 +340,18 @@ __global__ __launch_bounds__(WAVES * 64, TILES == 1 ? 3 : 2) void step_kernel(co
             const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + h * a.group + at % a.group;
             const float norm = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-                const int chunk = i * 16 + (threadIdx.x & 15);
+            for (int i = 0; i < (D + NW * 16 - 1) / (NW * 16); ++i) {
+                const int chunk = i * (NW * 4) + lane_of;
+                if (chunk >= D / 4) break;
                 v4f x{0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) x += *reinterpret_cast<const v4f*>(smem + w * V::BYTES + row * (4 * D) + ((chunk ^ row) << 4)) * f[w];
+                for (int w = 0; w < NW; ++w) x += *reinterpret_cast<const v4f*>(smem + w * V::BYTES + row * (4 * D) + ((chunk ^ row) << 4)) * f[w];
                 if (!whole) {
                     if (at < rows) *reinterpret_cast<v4f*>(part + at * Part<D>::ROW + chunk * 4) = x;
                 } else if (at < a.tokens * a.group)
                     *reinterpret_cast<uint2*>(a.out + to * D + chunk * 4) = make_uint2(pack_bf16x2(x[0] * norm, x[1] * norm), pack_bf16x2(x[2] * norm, x[3] * norm));
             }
-            if ((threadIdx.x & 15) == 0) {
+            if (lane_of == 0) {
                 if (!whole) {
                     if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor - UP, l);
                 } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor - UP + __builtin_amdgcn_logf(l)) * LN2;
@@ -973,6 +988,14 @@ int step_groups(const Cache& c, int tiles) {
     const int64_t units = (int64_t)c.batch * c.heads * (idx::cache4_units(c.capacity(), idx::CACHE4_UNIT) + EXTRA), most = device_cu_count() * (tiles == 1 ? 3 : 2);
     return (int)(units < most ? units : most);
 }
+// Whether every (sequence, head) is left to a workgroup of its own, which saves the join and the search for its entries, but nobody helps with a long
+// sequence (us, shared out / each its own; heads of 128, one token).  8 heads of 512 entries 10.6 / 7.8, of 1024 10.5 / 10.3, of 2048 10.8 / 16.7; 256 heads
+// of 1024 18.0 / 12.3, of 2048 23.6 / 19.6 (of 1 to 2048 17.5 / 18.0), of 1 to 4096 19.4 / 30.0; 128 heads of 2048 17.8 / 17.8; in two rounds, 512 heads of
+// 256 entries 15.1 / 11.2, of 512 18.0 / 16.1, of 1024 23.6 / 22.4 (of 1 to 1024 19.2 / 20.2)
+bool step_alone(const Cache& c, int tiles) {
+    const int64_t pairs = (int64_t)c.batch * c.heads, room = device_cu_count() * (c.dim == 64 && tiles == 1 ? 2 : 1);      // (registers)
+    return pairs <= room ? c.capacity() <= (3 * pairs > 2 * room ? 2048 : 1024) : pairs <= 2 * room && c.capacity() <= 512;
+}
 // Row tiles of step_kernel that hold all rows of a kv head (1 or 2), or 0: prompt_kernel.  Four of them take longer than it, 4 streams of 16384 entries and
 // 64 rows 62 us to 54; two less, 16 streams of 8192 and 32 rows 57 to 76
 int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 0; }
@@ -999,14 +1022,23 @@ PromptPlan prompt_plan(const Cache& c, int64_t rows) {
 int64_t owners_bytes(const Cache& c) { return ((int64_t)c.batch * c.heads * (int64_t)sizeof(int2) + 15) / 16 * 16; }
 int64_t workspace_bytes_of(const Cache& c, int64_t tokens, int64_t heads) {
     const int64_t rows = tokens * (heads / c.heads);
-    if (const int tiles = step_tiles(rows)) return owners_bytes(c) + (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 4) * (int64_t)sizeof(float);
+    const int tiles = step_tiles(rows);
+    if (tiles && step_alone(c, tiles)) return 0;
+    if (tiles) return owners_bytes(c) + (int64_t)step_groups(c, tiles) * 2 * tiles * 16 * (c.dim + 4) * (int64_t)sizeof(float);
     const PromptPlan p = prompt_plan(c, rows);
     return p.splits > 1 ? c.batch * tokens * heads * p.splits * (c.dim + 4) * (int64_t)sizeof(float) : 0;
 }
 
 template <int D, int TILES>
-int launch_step(const char* fn, const Args& a, hipStream_t st) {
-    hipLaunchKernelGGL((step_kernel<D, TILES>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
+int launch_step(const char* fn, Args& a, hipStream_t st) {
+    if (step_alone(a.c, TILES)) {
+        hipLaunchKernelGGL((step_kernel<D, TILES, true>), dim3((unsigned)(a.c.batch * a.c.heads)), dim3(2 * WAVES * 64), 0, st, a);
+        return check_launch(fn);
+    }
+    a.groups = step_groups(a.c, TILES);
+    a.owners = reinterpret_cast<int2*>(a.parts);
+    a.parts += owners_bytes(a.c) / (int64_t)sizeof(float);
+    hipLaunchKernelGGL((step_kernel<D, TILES, false>), dim3((unsigned)a.groups), dim3(WAVES * 64), 0, st, a);
     if (int e = check_launch(fn)) return e;
     hipLaunchKernelGGL((join_kernel<D, TILES>), dim3((unsigned)(a.c.batch * a.c.heads * a.tokens * a.group)), dim3(256), 0, st, a);
     return check_launch(fn);
@@ -1039,9 +1071,6 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
     const int tiles = step_tiles(rows);
     int e;
     if (tiles) {
-        a.groups = step_groups(a.c, tiles);
-        a.owners = reinterpret_cast<int2*>(a.parts);
-        a.parts += owners_bytes(a.c) / (int64_t)sizeof(float);
         e = tiles == 1 ? launch_step<D, 1>(fn, a, st) : launch_step<D, 2>(fn, a, st);
     } else {
         const PromptPlan p = prompt_plan(a.c, rows);
