@@ -102,9 +102,12 @@ __device__ __forceinline__ float over_rows(float x) {
 // meanwhile.  Four waves of a workgroup take turns and add up at the end, with their workgroups' neighbours through memory.
 //
 // Bound by memory where there are many entries: 8 streams of up to 131072 entries, 616 MB, 106 to 110 us = 5.6 to 5.8 TB/s (a large copy here: 4.95 TB/s
-// read and written).  A step over a few thousand entries is mostly the kernel's beginning and end: one stream of 8192 entries of one head 6.0 us, of which 1.5
-// are the launch, 1.4 to find the units, 1.3 the first loads, 1.2 the waves' sum.  Not taken: the next head's first loads in front of a head's
-// end (registers spill, slower), four workgroups per CU, 64 rows in registers (see step_tiles).
+// read and written).  A step over a few thousand
+// entries is mostly the kernel's beginning and end: 8 heads of 1021 entries, shared out, 6.0 us (1.5 for the launch, 1.4 to find the units, 1.3 for the
+// first loads, 1.2 for the waves' sum) and 4.2 for the join.  Where tables are short every (sequence, head) is therefore left to one workgroup of eight
+// waves (see step_alone): 1.5 us for 256 entries, which is how long codes take to bf16, to LDS and through two products, one after the other
+// (no faster with the loads of two to four turns ahead).  Not taken: the next head's first loads in front of a head's end (registers spill,
+// slower), four workgroups per CU, 64 rows in registers (see step_tiles).
 
 template <int D>
 struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 16 rows' writes of a chunk and 4 x 4 rows' transposing reads spread over the banks
