@@ -1004,9 +1004,10 @@ bool step_alone(const Cache& c, int tiles) {
 int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 0; }
 
 // prompt_kernel: waves of a workgroup, how many of them have the same rows, and how many workgroups share the entries of a row block.  Heads of 128: eight waves
-// convert every entry for 256 rows and have a CU to themselves; four, two workgroups of which a CU holds, are taken where the eight would hold more rows
-// that are none and the CUs have not all got one (100 tokens of 4 heads each over 32768 entries, 400 rows in 512 either way: 101 us with four, 93 with eight; 300 rows
-// over 2000 entries: 35.5 in 384, 37.8 in 512).  Heads of 64: four waves, whose registers a CU holds three times (1000 tokens over 2000 entries 45 -> 40 us).
+// convert every entry for 256 rows and have a CU to themselves; four, two workgroups of which a CU holds, are taken where the eight would hold 128 more rows that
+// are none (us with four / eight waves, 32 heads: 9 x 600 rows over 2000 entries 211 / 246, 3 x 600 112 / 116, 6 x 1150 214 / 222, 40 x 280 of 8 heads 152 / 190, the worst of
+// 14 sizes 6 x 890 187 / 180; where none are saved, 8 x 512 rows of 8 heads over 4096 entries 173 / 160, 2 x 8192 of 8 heads 493 / 466, 3 x 1024 117 / 117).  Heads
+// of 64: four waves, whose registers a CU holds three times (1000 tokens over 2000 entries 45 -> 40 us).
 // Up to 64 rows two and two of the four share the rows (4 streams of 16384 entries, 64 rows: 49 -> 45 us).  Parts are worth it from 4 tiles of entries on.
 struct PromptPlan {
     int waves, shares, blocks, splits;
@@ -1014,7 +1015,7 @@ struct PromptPlan {
 PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     const int64_t pairs = (int64_t)c.batch * c.heads, cus = device_cu_count();
     PromptPlan p;
-    p.waves = c.dim == 128 && rows > 128 && (pairs * ((rows + 255) / 256) >= cus || (rows + 255) / 256 * 2 == (rows + 127) / 128) ? 8 : 4;
+    p.waves = c.dim == 128 && (rows + 127) / 128 % 2 == 0 ? 8 : 4;
     p.shares = rows <= 64 ? 2 : 1;
     p.blocks = (int)((rows * p.shares + p.waves * 32 - 1) / (p.waves * 32));
     const int64_t groups = pairs * p.blocks, room = cus * (c.dim == 64 ? 3 : 8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
