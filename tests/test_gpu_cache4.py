@@ -529,3 +529,27 @@ def test_steps_of_many_heads(C, dev, heads, room, dim, tokens):
     _check_attention(out[:, :, some], lse[:, :, some], want, dim, room)
     assert bool((lse[1] == float("-inf")).all()) and not bool(out[1].any())
     assert bool(torch.isfinite(lse[0, -1]).all()) and bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("batch,tokens,heads,hkv,page", [(7, 150, 7, 1, 64), (5, 90, 32, 8, 16), (40, 44, 8, 8, 32), (3, 300, 2, 1, 16), (4, 70, 40, 40, 16)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_of_no_and_few_entries_in_tables_of_any_width(C, dev, batch, tokens, heads, hkv, page, dim):
+    """Prompts whose blocks are shared out or left whole by what the table has room for and by what there is: none, a few entries, several tiles."""
+    gen = torch.Generator().manual_seed(batch + tokens + dim)
+    counts = [(0, tokens, tokens // 3, 1)[b % 4] for b in range(batch)]
+    lengths = [n + (0, 0, 200, 500)[(b // 2) % 4] for b, n in enumerate(counts)]
+    lengths[-1] = 0
+    mine = -(-max(lengths) // page)
+    pool, table = _pool(gen, batch * mine, hkv, page, dim), _table(gen, batch, mine, batch * mine)
+    some = [0, hkv - 1] if hkv > 1 else [0]
+    q = torch.randn(batch, tokens, heads, dim, generator=gen).bfloat16()
+    rows = [h * (heads // hkv) + g for h in some for g in range(heads // hkv)]
+    want = oracle.attention(pool[:, some].contiguous(), table, lengths, q[:, :, rows], counts, 1 / math.sqrt(dim), page)
+    for room in (mine, mine + 1, -(-2000 // page), -(-8192 // page), -(-60000 // page)):
+        wide = torch.full((batch, max(room, mine)), -1, dtype=torch.int32)
+        wide[:, :mine] = table
+        out = torch.full_like(q, float("nan"), device=dev)        # (memory that the outputs may come from)
+        del out
+        out, lse = C.attention(pool.to(dev), wide.to(dev), _ints(lengths, dev), q.to(dev), counts=_ints(counts, dev))
+        _check_attention(out[:, :, rows], lse[:, :, rows], want, dim, max(lengths))
+        assert bool(torch.isfinite(out).all())

@@ -6,6 +6,7 @@
 // in any attention on bf16 tensors (that rounding, 2^-9 of each, averages out over the entries; the result is rounded to bf16 anyway).
 //
 // step_kernel: up to 32 rows per kv head (rows = new tokens x heads that share it).  prompt_kernel: more.  weights_kernel: what every entry got.
+#include <algorithm>
 #include <type_traits>
 #include "cache4.h"
 
@@ -38,7 +39,7 @@ struct Args {
     int tokens, heads, group;       // group = query heads per kv head
     float scale;
     int groups;                 // workgroups that share the units
-    int blocks, splits;         // prompt_kernel: row blocks of a kv head, workgroups that share the entries of each
+    int blocks, block_rows, splits, shared_from;         // prompt_kernel: row blocks of a kv head, rows of each, workgroups that share its entries at most, and from how many tiles on
 };
 
 // entries of a sequence that any of its queries sees
@@ -499,6 +500,18 @@ struct Codes {
 // tiles in LDS: three with eight waves, which have a CU to themselves
 template <int NW> constexpr int PROMPT_STAGES = NW == 8 ? 3 : 2;
 
+// What the rows from `row0` on, a block, of a sequence see: tiles of entries, and how many workgroups share them (the others of a.splits have nothing to do).
+// One leaves no parts.
+struct BlockSees {
+    int most, tiles, parts;
+    __device__ __forceinline__ BlockSees(const Args& a, int row0, int count, int length) {
+        const int rows = count * a.group;
+        most = row0 < rows ? max(length - count + (min(row0 + a.block_rows, rows) - 1) / a.group + 1, 0) : 0;
+        tiles = (most + TILE - 1) / TILE;
+        parts = tiles < a.shared_from ? 1 : min(a.splits, (tiles + 3) / 4);
+    }
+};
+
 // NW waves, of which SHARES at a time have the same 32 rows: with two, each takes its own half of every tile, and they add up at the end
 template <int D, int NW, int SHARES>
 __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
@@ -520,9 +533,11 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     const int row0 = block * ROWS_OF, row = row0 + wave % (NW / SHARES) * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
     // entries that this lane's row, any row of the workgroup and any row of the wave sees
     const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
-    const int sees = row < rows ? sees_of(row) : 0, most = row0 < rows ? sees_of(min(row0 + ROWS_OF, rows) - 1) : 0;
+    const int sees = row < rows ? sees_of(row) : 0;
+    const BlockSees block_sees(a, row0, count, length);
+    if (split >= block_sees.parts) return;
     const int wave0 = row0 + wave % (NW / SHARES) * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
-    const int tiles = (most + TILE - 1) / TILE, begin = (int)((int64_t)split * tiles / a.splits), end = (int)((int64_t)(split + 1) * tiles / a.splits);
+    const int tiles = block_sees.tiles, begin = (int)((int64_t)split * tiles / block_sees.parts), end = (int)((int64_t)(split + 1) * tiles / block_sees.parts);
     // entries that every row of the workgroup sees: none where the pool does not have all the pages
     bool gaps = false;
     for (int i = (begin * TILE >> c.log2_page) + threadIdx.x; i < (min(end * TILE, length) + c.page - 1) >> c.log2_page; i += NW * 64)
@@ -715,7 +730,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     }
     if (token >= a.tokens) return;
     const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + head;
-    if (a.splits > 1) {
+    if (block_sees.parts > 1) {
         float* const part = a.parts + (to * a.splits + split) * Part<D>::ROW;
 #pragma unroll
         for (int d = 0; d < BLOCKS; ++d)
@@ -739,13 +754,17 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #endif
 }
 
-// Rows whose entries several workgroups shared
+// Rows whose entries several workgroups shared.  Bound by memory, or by latency where there are few
 template <int D, int GROUPS>
 __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t rows) {
     const int64_t row = (int64_t)blockIdx.x * (1024 / D / GROUPS) + threadIdx.x / (GROUPS * D / 4);
     if (row >= rows) return;
+    const uint32_t token_of = (uint32_t)row / (uint32_t)a.heads, b = token_of / (uint32_t)a.tokens;      // (fewer than 2^31 rows: ti8_cache4_attention)
+    const int at = (int)(token_of % (uint32_t)a.tokens) * a.group + (int)((uint32_t)row % (uint32_t)a.heads) % a.group;
+    const int parts = BlockSees(a, at / a.block_rows * a.block_rows, count_of(a.counts, b, a.tokens), length_of(a.c, a.lengths, b)).parts;
+    if (parts == 1) return;
     const float* const from = a.parts + row * a.splits * Part<D>::ROW;
-    join<D, GROUPS>(a, from, from, Part<D>::ROW, a.splits, row, true);
+    join<D, GROUPS>(a, from, from, Part<D>::ROW, parts, row, true);
 }
 
 // ---- what the entries got ------------------------------------------------------------------------------------------
@@ -1010,7 +1029,7 @@ int step_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 0; }
 // of 64: four waves, whose registers a CU holds three times (1000 tokens over 2000 entries 45 -> 40 us).
 // Up to 64 rows two and two of the four share the rows (4 streams of 16384 entries, 64 rows: 49 -> 45 us).  Parts are worth it from 4 tiles of entries on.
 struct PromptPlan {
-    int waves, shares, blocks, splits;
+    int waves, shares, blocks, splits, shared_from;
 };
 PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     const int64_t pairs = (int64_t)c.batch * c.heads, cus = device_cu_count();
@@ -1019,8 +1038,23 @@ PromptPlan prompt_plan(const Cache& c, int64_t rows) {
     p.shares = rows <= 64 ? 2 : 1;
     p.blocks = (int)((rows * p.shares + p.waves * 32 - 1) / (p.waves * 32));
     const int64_t groups = pairs * p.blocks, room = cus * (c.dim == 64 ? 3 : 8 / p.waves), most = (c.capacity() + 4 * TILE - 1) / (4 * TILE);
-    const int64_t splits = room / groups;
-    p.splits = (int)(splits < 1 ? 1 : splits < most ? splits : most);
+    // One part, or as many as fill the CUs once, twice or three times, by an estimate in us: 2 per tile of entries in a row, parts written and read at two thirds
+    // of the rate of a copy (12 x 280 rows of 8 heads over 4000 entries 134 -> 117 us in three parts, 24 x 64 of 1 to 4000 55 -> 50 in two).  Sequences may be far shorter than their
+    // tables: the kernel leaves a block whole up to half of what two parts, or as many as it takes where two are no gain, need to be worth it (half: lengths differ,
+    // and the longest decides; 64 rows of 8 heads, the first 64 entries of 8192: 27 -> 14 us).
+    const double tiles = (double)c.capacity() / TILE, join = (double)(pairs * rows) * (c.dim + 4) * 8e-6 / 3.3;
+    const auto rounds_of = [&](int64_t splits) { return (double)((groups * splits + room - 1) / room) / (double)splits; };
+    double best = rounds_of(1) * tiles * 2.0;
+    p.splits = 1;
+    p.shared_from = 1;
+    for (int rounds = 1; rounds <= 3; ++rounds) {
+        const int64_t fill = rounds * room / groups, splits = fill < most ? fill : most;
+        if (splits < 2 || rounds_of(splits) * tiles * 2.0 + 3.0 + join * (double)splits >= best) continue;
+        best = rounds_of(splits) * tiles * 2.0 + 3.0 + join * (double)splits;
+        p.splits = (int)splits;
+        const int64_t fewest = 2 * groups <= room ? 2 : splits;
+        p.shared_from = std::max(5, (int)((3.0 + join * (double)fewest) / (4.0 * (rounds_of(1) - rounds_of(fewest)))));
+    }
     return p;
 }
 int64_t owners_bytes(const Cache& c) { return ((int64_t)c.batch * c.heads * (int64_t)sizeof(int2) + 15) / 16 * 16; }
@@ -1079,7 +1113,9 @@ int launch(const char* fn, Args& a, bool accumulate, hipStream_t st) {
     } else {
         const PromptPlan p = prompt_plan(a.c, rows);
         a.blocks = p.blocks;
+        a.block_rows = p.waves / p.shares * 32;
         a.splits = p.splits;
+        a.shared_from = p.shared_from;
         if (p.shares == 2) e = launch_prompt<D, 4, 2>(fn, a, st);
         else if (D == 128 && p.waves == 8) e = launch_prompt<128, 8, 1>(fn, a, st);
         else e = launch_prompt<D, 4, 1>(fn, a, st);
