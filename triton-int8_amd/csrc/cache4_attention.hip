@@ -25,7 +25,7 @@ typedef const __attribute__((address_space(4))) int32_t* constant_ints;        /
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 // Exponentials are carried times 2^UP, which their common divisor takes away again: those of scores far below the maximum stay above 2^-126, below which
 // v_exp_f32 gives zero, for 2^UP further (where sums are put under another maximum exp2f goes on below it).  Up to 2^(8 + UP) each (see step_kernel), their sums stay far below 2^127
-constexpr float UP = 24.0f;
+constexpr float UP = 24.0f;      // (= the 24 in lse_of)
 
 struct Args {
     Cache c;
@@ -80,6 +80,8 @@ struct Lengths {
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ v4f mfma16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v8bf operand(uint4 x) { return __builtin_bit_cast(v8bf, x); }
+// from a row's maximum, times scale log2(e), and its sum (2^UP is taken off the sum, which is exact, and not off the logarithm)
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l * 0x1p-24f)) * LN2; }
 // of the four lanes that have the same place in a row of 16, in each of them
 template <bool SUM>
 __device__ __forceinline__ float over_rows(float x) {
@@ -119,7 +121,7 @@ struct Values {     // 32 rows of D bf16, 16-byte chunks permuted within a row: 
 };
 
 template <int D>
-struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e), less UP) and sums of its rows
+struct Part {       // what a workgroup leaves of a (sequence, head) that it has not got alone: unnormalised results, maxima (times scale log2(e)) and sums of its rows
     static constexpr int ROW = D + 4;       // (16-byte aligned)
 };
 
@@ -357,8 +359,8 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
             }
             if (lane_of == 0) {
                 if (!whole) {
-                    if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor - UP, l);
-                } else if (at < a.tokens * a.group) a.lse[to] = l == 0.0f ? -INFINITY : (m * factor - UP + __builtin_amdgcn_logf(l)) * LN2;
+                    if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor, l);
+                } else if (at < a.tokens * a.group) a.lse[to] = lse_of(m * factor, l);
             }
         }
         left -= n + EXTRA;
@@ -421,7 +423,7 @@ __device__ __forceinline__ void join(const Args& a, const float* one, const floa
     }
     const float norm = l == 0.0f ? 0.0f : 1.0f / l;
     *reinterpret_cast<uint2*>(a.out + row * D + at * 4) = make_uint2(pack_bf16x2(o[0] * norm, o[1] * norm), pack_bf16x2(o[2] * norm, o[3] * norm));
-    if (at == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (at == 0) a.lse[row] = lse_of(m, l);
 #endif
 }
 
@@ -738,7 +740,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
             for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<v4f*>(part + d * 32 + 2 * i + 4 * half) = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
         if (half == 0) {
-            part[D] = top * factor - UP;
+            part[D] = top * factor;
             part[D + 1] = row < rows ? sum : 0.0f;
         }
         return;
@@ -750,7 +752,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<uint2*>(a.out + to * D + d * 32 + 2 * i + 4 * half) = make_uint2(pack_bf16x2(o[d][i] * norm, o[d][i + 1] * norm), pack_bf16x2(o[d][i + 2] * norm, o[d][i + 3] * norm));
-    if (half == 0) a.lse[to] = sum == 0.0f ? -INFINITY : (shift + __builtin_amdgcn_logf(sum)) * LN2;
+    if (half == 0) a.lse[to] = lse_of(top * factor, sum);
 #endif
 }
 
