@@ -1,0 +1,32 @@
+"""Index arithmetic of the 4-bit cache's kernels (csrc/index_math.h), compiled for the host, at sizes that the entry points take."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+CODE = r"""
+#include <cstdint>
+#include "index_math.h"
+extern "C" int first_row(int entry, int older, int group) { return ti8::idx::cache4_first_row(entry, older, group); }
+"""
+
+
+@pytest.fixture(scope="module")
+def index(tmp_path_factory):
+    at = tmp_path_factory.mktemp("cache4_index")
+    (at / "index.cpp").write_text(CODE)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "triton-int8_amd", "csrc"), "-o", str(at / "index.so"), str(at / "index.cpp")], check=True)
+    return ctypes.CDLL(str(at / "index.so"))
+
+
+@pytest.mark.parametrize("group,length,count", [
+    (1, 5, 2), (4, 700, 40), (128, (1 << 24) + 1000, 1), (128, (1 << 30), 70), (4096, (1 << 19) + 70000, 1), (4096, 1 << 20, 3), (4096, 1 << 30, 1 << 18), (7, 3, 9)])
+def test_first_row_that_sees_an_entry(index, group, length, count):
+    """Every row sees the entries in front of the tokens' own, however many there are; of the others those from their own token on."""
+    older = length - count
+    entries = sorted({e for e in (0, 1, length // 3, older - 1, older, older + 1, older + count // 2, length - 1, length + 30) if 0 <= e})
+    for entry in entries:
+        assert index.first_row(entry, older, group) == max(entry - older, 0) * group

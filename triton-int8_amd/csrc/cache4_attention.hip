@@ -882,7 +882,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             fetch(now);
         }
         // from the first token that sees the unit's first entry, where the rows do not all fit into a tile
-        const int first = rows <= ROWS ? 0 : max(unit0 - older, 0) * a.group / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
+        const int first = rows <= ROWS ? 0 : idx::cache4_first_row(unit0, older, a.group) / 32 * 32, tiles = (rows - first + ROWS - 1) / ROWS;
 
         // A thread's rows are 64 apart from one tile to the next: their heads and offsets are counted on, a division each would take as long as the scores.
         // Offsets are those from the tile's first token (ti8_cache4_attention checks the strides), and none goes beyond the last row: one that is none is
@@ -934,8 +934,8 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
         float sum = 0.0f;
         const auto add_up = [&](int row0, int stage) {
             // somebody of these rows sees one of the wave's entries
-            if (j0 >= length || row0 + ROWS <= (j0 - older) * a.group) return;
-            const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32), sees = (j - older) * a.group - row0;        // sees: the first row that sees this lane's entry
+            if (j0 >= length || row0 + ROWS <= idx::cache4_first_row(j0, older, a.group)) return;
+            const int chunk = half * (D / 16) ^ Values<D>::swizzle(r32), sees = idx::cache4_first_row(j, older, a.group) - row0;        // sees: the first row that sees this lane's entry
             const auto scores = [&](int u) {
                 const int8_t* const from = queries(stage) + (u * 32 + r32) * ROW;
                 v16f s;
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
                 }
                 return (p[0] + p[1]) + (p[2] + p[3]);
             };
-            if (row0 + ROWS <= rows && row0 >= (j0 + COLUMNS - 1 - older) * a.group) {      // every row is one and sees every entry
+            if (row0 + ROWS <= rows && row0 >= idx::cache4_first_row(j0 + COLUMNS - 1, older, a.group)) {      // every row is one and sees every entry
 #pragma unroll
                 for (int u = 0; u < ROWS / 32; ++u) {
                     const v16f s = scores(u);

@@ -483,6 +483,10 @@ TI8_HD int share_of(const Share& s, int unit) {
     return unit < longer ? unit / (s.each + 1) : s.more + (unit - longer) / s.each;
 }
 
+// The weights' pass: the first row of a kv head that sees an entry, the tokens' own entries being those from `older` on.  Entries in front of them are seen by every
+// row: the distance is cut first, times the group it passes 32 bits (4096 heads that share one from 2^19 entries on).  At most (tokens + 31) group
+TI8_HD int cache4_first_row(int entry, int older, int group) { return imax(entry - older, 0) * group; }
+
 // Attention of many rows: workgroup -> (sequence, kv head) pair and its block (and part).  A pair's blocks lie on one XCD, whose L2 then serves the entries; an
 // XCD has the last block of all its pairs first, which sees the most entries (one prompt of 4096 tokens and 32 heads 248 us with a pair's blocks behind each
 // other).  The grid has round8(pairs) * blocks workgroups; those of a pair beyond the last do nothing.
