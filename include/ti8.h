@@ -541,7 +541,8 @@ int ti8_cache4_read(const ti8_cache4* c, const int32_t* starts, const int32_t* c
  * j <= lengths[b] - counts[b] + i.
  *   out bf16 and lse float, dense [batch][tokens][heads][head_dim] and [batch][tokens][heads]: out = sum_j p_j v_j, p_j = exp(scale q k_j - lse),
  *   lse = log sum_j exp(scale q k_j).  Rows that see nothing and rows from counts[b] on: out 0, lse -inf.
- *   accumulate != 0: weights of every entry j += the sum of its p_j over the queries and the heads that share its kv head.  q's strides of
+ *   accumulate != 0: weights of every entry j += the sum of its p_j over the queries and the heads that share its kv head; an entry whose page several
+ *   sequences name (a common beginning) gets the sums of all of them, which are added one after the other in no fixed order.  q's strides of
  *   64 / (heads / kv_heads) + 2 tokens and of the heads that share a kv head together stay below 2^30 elements (TI8_ERR_SHAPE else).
  *   workspace: ti8_cache4_attention_workspace bytes (-1 for sizes it does not take), 16-byte aligned, contents undefined before and after. */
 int64_t ti8_cache4_attention_workspace(const ti8_cache4* c, int64_t tokens, int64_t heads);

@@ -1,11 +1,13 @@
-"""Index arithmetic of the 4-bit cache's kernels (csrc/index_math.h), compiled for the host, at sizes that the entry points take."""
+"""Index arithmetic of the 4-bit cache's kernels (csrc/index_math.h), compiled for the host, at sizes that the entry points take, and what their code holds."""
 import ctypes
 import os
+import re
 import subprocess
 
 import pytest
 
 from conftest import ROOT
+from test_kernel_resources import kernel_bodies
 
 CODE = r"""
 #include <cstdint>
@@ -30,3 +32,11 @@ def test_first_row_that_sees_an_entry(index, group, length, count):
     entries = sorted({e for e in (0, 1, length // 3, older - 1, older, older + 1, older + count // 2, length - 1, length + 30) if 0 <= e})
     for entry in entries:
         assert index.first_row(entry, older, group) == max(entry - older, 0) * group
+
+
+def test_weights_are_added_to_and_never_stored(tmp_path):
+    """Two sequences may name a page: nothing between a weight's load and its store gets lost if it is neither loaded nor stored."""
+    bodies = kernel_bodies("cache4_attention.hip", tmp_path, "weights_kernel")
+    assert len(bodies) == 2
+    for name, body in bodies.items():
+        assert re.search(r"^\s*global_atomic_add_f32 ", body, flags=re.M) and not re.search(r"^\s*(global|buffer|flat)_store", body, flags=re.M), name

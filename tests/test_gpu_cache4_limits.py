@@ -48,3 +48,31 @@ def test_weights_of_many_entries_that_many_heads_share(C, dev, heads, length):
     assert not bool(got[length:].any())
     assert bool(((got[:length] - want).abs() <= (rel + 2.0 ** -23) * want).all()), float(((got[:length] - want).abs() / want).max())
     assert abs(float(want.sum()) - heads) < 1e-6 * heads
+
+
+@pytest.mark.parametrize("tokens,heads,hkv", [(1, 4, 2), (6, 8, 1), (40, 4, 2), (150, 2, 2)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_weights_of_pages_that_sequences_share(C, dev, tokens, heads, hkv, dim, page):
+    """Sequences with a common beginning, one of which comes upon a page twice: weights get what all of them give."""
+    gen = torch.Generator().manual_seed(tokens + dim)
+    lengths, common = [800, 500, 650, 700, 513], 448
+    batch, mine = len(lengths), -(-800 // page)
+    pool, table = _pool(gen, batch * mine, hkv, page, dim), _table(gen, batch, mine, batch * mine)
+    table[:, :common // page] = table[0, :common // page]
+    table[3, common // page] = table[3, 0]
+    weights = torch.rand(pool.shape[0], hkv, page, generator=gen)
+    q = torch.randn(batch, tokens, heads, dim, generator=gen).bfloat16()
+    want = oracle.attention(pool, table, lengths, q, [tokens] * batch, 1 / math.sqrt(dim), page)
+    expected = weights.double()
+    for b, n in enumerate(lengths):
+        j = torch.arange(n)
+        for h in range(hkv):
+            expected[:, h].index_put_((table[b].long()[j // page], j % page), want[2][b][h], accumulate=True)
+    # as in test_attention, and a rounding for each addition to a weight
+    rel = 2.0 ** -18 + 4 * (dim + 8) * 2.0 ** -24 * float(want[3].max()) + tokens * heads * 2.0 ** -24
+    bound = rel * (expected - weights) + (batch + 2) * 2.0 ** -24 * expected
+    for _ in range(3):
+        got = weights.to(dev)
+        out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev), weights=got)
+        _check_attention(out, lse, want, dim, max(lengths))
+        assert bool(((got.cpu().double() - expected).abs() <= bound).all()), float(((got.cpu().double() - expected).abs() / expected).max())

@@ -114,7 +114,8 @@ def attention(pool, table, lengths, q, counts=None, scale=None, weights=None):
     is a multiple of the pool's kv heads; neighbouring heads share one.  ``scale``: 1 / sqrt(head_dim) by default.
 
     Returns (out bf16 like q, lse float32 [batch, tokens, heads], the logarithms of the sums of the exponentials); rows that see nothing and rows that
-    are no queries are zeros with an lse of -inf.  With ``weights``, every entry's probabilities over queries and heads are added to its weight."""
+    are no queries are zeros with an lse of -inf.  With ``weights``, every entry's probabilities over queries and heads are added to its weight; one whose page
+    several sequences name gets those of all of them, in no fixed order (only there may the last bits differ from call to call)."""
     made = _natively("cache4_attention", pool, table, lengths, q, counts, weights, scale)
     if made is not None:
         return tuple(made)

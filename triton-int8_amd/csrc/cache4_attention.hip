@@ -773,8 +773,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 //
 // weights of entry j += sum over rows of exp(s_j - lse): the scores once more, with the entries as columns of 32 x 32 products, so that a lane adds up the
 // rows of one entry.  Units of 256 entries are shared out as for step_kernel; each of eight waves has the keys of 32 in registers and goes through the rows
-// that see them, which the workgroup brings into LDS 64 at a time, two tiles ahead, without a trip through registers.  Every entry has one owner: no
-// atomics, sums in a fixed order.
+// that see them, which the workgroup brings into LDS 64 at a time, two tiles ahead, without a trip through registers.  An entry of a sequence has one owner, which adds
+// its rows up in a fixed order; the sum goes to the weight as an atomic addition, because sequences with a common beginning may share its pages (then
+// the order of their additions is open, otherwise a weight gets one).
 //
 // Few rows: bound by the beginning and by memory (32 streams of 2048 entries of 8 heads: 39 MB in 15 us); many: by the issue of a SIMD, as prompt_kernel (8 x 1024 tokens
 // over 4096 entries of 32 heads: 315 us = 0.76 PFLOP/s), and, with one or two units per workgroup, by the units that most rows see.  The loads to LDS
@@ -826,12 +827,11 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
     now.sequence(a, lengths.find(begin, before, per_head));
     now.h = (begin - before) / per_head;
     now.unit = (begin - before) % per_head;
-    // the keys, and what the entries have: a lane has half of an entry's elements, whole groups of 32 or one.  The next unit's are on their way
+    // the keys, and where the entries' weights lie: a lane has half of an entry's elements, whole groups of 32 or one.  The next unit's are on their way
     // while one is worked on
     uint4 codes[D / 64];
     uint32_t bytes[D / 64];
     float* weight;
-    float has;
     const auto fetch = [&](const Unit& u) {
         const int j0 = u.unit * UNIT + wave * COLUMNS, j = j0 + r32;
         const constant_ints table = (constant_ints)(c.table + u.b * c.table_stride);
@@ -851,7 +851,6 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             if (!there) bytes[g] = 0;
         }
         weight = there ? c.weights + block * c.page + row : nullptr;
-        has = c.weights[block * c.page + row];
     };
     fetch(now);
     int staged_b = -1, staged_h = -1;       // the head whose queries lie in LDS, all of them
@@ -870,7 +869,6 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             }
         }
         float* const this_weight = weight;
-        const float had = has;
         if (--left > 0) {
             if (++now.unit == now.per_head) {
                 now.unit = 0;
@@ -1001,7 +999,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
             __builtin_amdgcn_s_waitcnt(0);      // the loads behind the last tile: LDS may be another workgroup's once the wave has ended
         }
         sum = over_halves<true>(sum);
-        if (this_weight && half == 0) *this_weight = had + sum;
+        if (this_weight && half == 0) unsafeAtomicAdd(this_weight, sum);       // (device memory: global_atomic_add_f32)
         if (left <= 0) break;
     }
 #endif
