@@ -552,7 +552,8 @@ int ti8_cache4_attention(const ti8_cache4* c, const int32_t* lengths, const int3
 /* Every sequence and kv head cut down to `keep` entries: the `recent` newest (0 <= recent <= keep) and the heaviest of the others by `weights`
  * (among equals the older one; NaN counts as heavier than any number), which become entries 0 .. in their old order, in the pages of new_table
  * int32 [batch][new_pages] (rows new_stride apart; new_pages * page_size >= keep; other pages than those of `table`).  Their weights go with them.
- * new_lengths[b] = min(lengths[b], keep); kept int32 [batch][kv_heads][keep]: which entry each of them was, -1 behind the last. */
+ * Entries of pages that the pool does not have are not there: none of them is kept, also of the `recent` newest, and the lengths go down by them.
+ * new_lengths[b] = min(entries that are there, keep); kept int32 [batch][kv_heads][keep]: which entry each of them was, -1 behind the last. */
 int ti8_cache4_evict(const ti8_cache4* c, const int32_t* lengths, const int32_t* new_table, int64_t new_pages, int64_t new_stride,
                      int64_t keep, int64_t recent, int32_t* kept, int32_t* new_lengths, ti8_stream_t stream);
 

@@ -76,3 +76,92 @@ def test_weights_of_pages_that_sequences_share(C, dev, tokens, heads, hkv, dim, 
         out, lse = C.attention(pool.to(dev), table.to(dev), _ints(lengths, dev), q.to(dev), weights=got)
         _check_attention(out, lse, want, dim, max(lengths))
         assert bool(((got.cpu().double() - expected).abs() <= bound).all()), float(((got.cpu().double() - expected).abs() / expected).max())
+
+
+def _check_evict(C, dev, gen, page, dim, hkv, lengths, keep, recent, weights, table, pool, new_table):
+    """Eviction where some pages are not there: their entries are left out.  Everything that is not written stays as it was."""
+    pages = pool.shape[0]
+    g_pool, g_weights = pool.to(dev), weights.to(dev)
+    kept, new_lengths = C.evict(g_pool, table.to(dev), _ints(lengths, dev), g_weights, new_table.to(dev), keep=keep, recent=recent)
+    p = (*oracle.parts(pool, page, dim), weights)
+    sizes = []
+    for b, n in enumerate(lengths):
+        j = torch.arange(n)
+        at = table[b].long()[j // page]
+        there = (at >= 0) & (at < pages)
+        old, new = j[there & (j < n - recent)], j[there & (j >= n - recent)]
+        sizes.append(min(int(there.sum()), keep))
+        for h in range(hkv):
+            w = weights[at[old], h, old % page].double().nan_to_num(nan=float("inf"))
+            heavy = old[w.sort(descending=True, stable=True).indices[:sizes[-1] - len(new)]].sort().values
+            stay = torch.cat((heavy, new))
+            assert kept[b, h].tolist() == stay.tolist() + [-1] * (keep - len(stay)), (b, h)
+            i = torch.arange(len(stay))
+            for t in p:
+                t[new_table[b].long()[i // page], h, i % page] = t[at[stay], h, stay % page]
+    assert new_lengths.tolist() == sizes
+    assert torch.equal(g_pool.cpu(), pool) and torch.equal(g_weights.cpu(), weights)
+
+
+@pytest.mark.parametrize("page,dim,hkv,lengths,keep,recent", [
+    (16, 64, 2, [300, 1, 0, 16, 17, 299, 150], 100, 40), (64, 128, 1, [2049, 700, 1000], 640, 640), (16, 128, 3, [100, 90, 7], 60, 0), (32, 64, 1, [500, 64], 500, 100),
+    (256, 128, 1, [3000, 5000], 1500, 1234)])
+@pytest.mark.parametrize("holes", ["old", "recent", "everywhere", "all", "all but one"])
+def test_evict_leaves_out_what_is_not_there(C, dev, page, dim, hkv, lengths, keep, recent, holes):
+    gen = torch.Generator().manual_seed(page + dim)
+    batch, mine, new = len(lengths), -(-max(lengths) // page), -(-keep // page)
+    pages = batch * (mine + new)
+    pool = _pool(gen, pages, hkv, page, dim, values=False)
+    order = torch.randperm(pages, generator=gen).int()
+    table, new_table = order[:batch * mine].view(batch, mine).clone(), order[batch * mine:].view(batch, new)
+    weights = torch.rand(pages, hkv, page, generator=gen)
+    for b, n in enumerate(lengths):
+        slots = torch.arange(mine)
+        first = max(0, n - recent) // page
+        gone = {"old": (slots < first) & (slots % 3 == 1), "recent": (slots >= first) & (slots % 2 == 0), "everywhere": torch.rand(mine, generator=gen) < 0.4,
+                "all": slots >= 0, "all but one": slots != min(2, (max(n, 1) - 1) // page)}[holes]
+        table[b, gone] = torch.tensor([-1, pages, 1 << 30])[b % 3].int()
+    _check_evict(C, dev, gen, page, dim, hkv, lengths, keep, recent, weights, table, pool, new_table)
+
+
+@pytest.mark.parametrize("kind", ["few", "equal", "random"])
+@pytest.mark.parametrize("holes", [False, True])
+def test_evict_more_entries_than_lds_holds(C, dev, kind, holes):
+    """Orders beyond the 32768 that stay in LDS, with weights that are equal on both sides of it."""
+    gen = torch.Generator().manual_seed(7)
+    page, dim, hkv, lengths, keep, recent = 64, 64, 2, [40000, 32769, 70001], 35000, 500
+    batch, mine, new = 3, -(-70001 // page), -(-keep // page)
+    pages = batch * (mine + new)
+    pool = _pool(gen, pages, hkv, page, dim, values=False)
+    order = torch.randperm(pages, generator=gen).int()
+    table, new_table = order[:batch * mine].view(batch, mine).clone(), order[batch * mine:].view(batch, new)
+    weights = {"few": torch.randint(0, 3, (pages, hkv, page), generator=gen) * 0.5, "equal": torch.full((pages, hkv, page), 0.25),
+               "random": torch.rand(pages, hkv, page, generator=gen)}[kind]
+    if holes:
+        table[:, 5::7] = -1
+    _check_evict(C, dev, gen, page, dim, hkv, lengths, keep, recent, weights, table, pool, new_table)
+
+
+def test_what_is_not_there_is_not_seen_after_an_eviction(C, dev):
+    """The places of a new page that nothing was moved to hold whatever was there before: numbers that are none, here."""
+    gen = torch.Generator().manual_seed(5)
+    page, dim, lengths = 16, 128, [130, 100]
+    pool, table = _pool(gen, 40, 1, page, dim), _table(gen, 2, 9, 30)
+    for s in oracle.parts(pool[30:], page, dim)[2:]:
+        s.fill_(255)
+    table[0, 2:4], table[1, 5:] = -1, 1 << 20
+    new_table = torch.arange(30, 40, dtype=torch.int32).view(2, 5)
+    weights = torch.rand(40, 1, page, generator=gen)
+    q = torch.randn(2, 1, 4, dim, generator=gen).bfloat16().to(dev)
+    g_pool, g_table, g_new = pool.to(dev), table.to(dev), new_table.to(dev)
+    kept, new_lengths = C.evict(g_pool, g_table, _ints(lengths, dev), weights.to(dev), g_new, keep=80, recent=80)
+    assert new_lengths.tolist() == [80, 80]
+    out, lse = C.attention(g_pool, g_new, new_lengths, q)
+    after = g_pool.cpu()
+    want = oracle.attention(after, new_table, new_lengths.tolist(), q.cpu(), [1, 1], 1 / math.sqrt(dim), page)
+    assert bool(torch.isfinite(out).all())
+    _check_attention(out, lse, want, dim, 80)
+    for b, n in enumerate(lengths):         # and they are the entries that were there before
+        j = kept[b, 0].cpu().long()
+        for x, y in zip(oracle.entries(after, new_table[b], page, dim, 0, 80), oracle.entries(pool, table[b].clamp(0, 39), page, dim, 0, n)):
+            assert torch.equal(x, y[j]) and bool((table[b].long()[j // page] < 40).all()) and bool((table[b].long()[j // page] >= 0).all())

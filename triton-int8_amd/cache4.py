@@ -138,7 +138,8 @@ def attention(pool, table, lengths, q, counts=None, scale=None, weights=None):
 def evict(pool, table, lengths, weights, new_table, *, keep, recent):
     """Every sequence and kv head cut down to ``keep`` entries: the ``recent`` newest and the heaviest of the others by ``weights`` (among equals the
     older one), in their old order, with their weights, in the pages that ``new_table`` int32 [batch, pages] names.  Those must be
-    others than the sequences' present ones, which are only read.  Sequences of up to ``keep`` entries move as they are.
+    others than the sequences' present ones, which are only read.  Sequences of up to ``keep`` entries move as they are.  Entries of pages that the pool does not
+    have are not there: they are left out and do not count.
 
     Returns (kept int32 [batch, kv_heads, keep], which entry each of them was, -1 behind the last; the new lengths int32 [batch])."""
     made = _natively("cache4_evict", pool, table, lengths, weights, new_table, keep, recent)

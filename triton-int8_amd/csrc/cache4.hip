@@ -109,30 +109,42 @@ constexpr int DIGIT = 11, BINS = 1 << DIGIT;
 
 // Which entries of a (sequence, head) stay: one workgroup each.  The `heavy`-th largest weight of the old entries is found from the top, eleven bits of its
 // order at a time (a histogram of those that agree so far; of the first eleven two are the weight's own, which spreads weights of a size over the bins), then
-// the entries are gone through in order: those above it stay, and the first of those equal to it.  Bound by latency: the weights are read once and
+// the entries are gone through in order: those above it stay, and the first of those equal to it.  Entries of pages that the pool does not have are not there: where a
+// table has such pages, entries are counted first and the recent ones placed one by one; among the old ones theirs is an order of 0, below that of every
+// weight, and no more are looked for than are there.  Bound by latency: the weights are read once and
 // kept in LDS, and a wave writes what stays of its own part of the entries (16 x 8 heads of up to 16384 entries, 2.9 MB of weights:
 // 20 us, the longest sequence's; 8 x 8 heads of 2112 entries 9.2 us).
 __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int32_t* lengths, int keep, int recent, int32_t* kept, int32_t* new_lengths) {
     extern __shared__ uint32_t orders[];
-    __shared__ int bins[BINS], found[2], sums[2][SELECT_WAVES];
+    __shared__ int bins[BINS], found[2], sums[2][SELECT_WAVES], missing;
     const int b = blockIdx.x / c.heads, h = blockIdx.x % c.heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n = length_of(c, lengths, b), stay = min(n, keep);
+    const int n = length_of(c, lengths, b), old = n - min(recent, n), pages = (n + c.page - 1) >> c.log2_page;
     int32_t* const mine = kept + ((int64_t)b * c.heads + h) * keep;
-    if (h == 0 && tid == 0) new_lengths[b] = stay;
-    for (int i = stay + tid; i < keep; i += SELECT) mine[i] = -1;
-    if (n <= keep) {
-        for (int i = tid; i < n; i += SELECT) mine[i] = i;
-        return;
+    const uint64_t below = (1ull << lane) - 1;
+    const auto absent = [&](int page) { return (unsigned)c.table[b * c.table_stride + page] >= (unsigned)c.pages; };
+    const int a_page = c.table[b * c.table_stride + min(tid, max(pages - 1, 0))];        // (looked at behind the weights' loads)
+    for (int i = tid; i < BINS; i += SELECT) bins[i] = 0;
+    if (tid == 0) missing = 0;
+    __syncthreads();
+    const auto any_missing = [&] {
+        bool is = pages > 0 && (unsigned)a_page >= (unsigned)c.pages;
+        for (int i = tid + SELECT; i < pages; i += SELECT) is |= absent(i);
+        if (is) missing = 1;
+        __syncthreads();
+        return missing != 0;
+    };
+    if (n <= keep || n - old == keep) {
+        if (!any_missing()) {         // all of them, or the recent ones alone
+            const int stay = min(n, keep);
+            if (h == 0 && tid == 0) new_lengths[b] = stay;
+            for (int i = tid; i < keep; i += SELECT) mine[i] = i < stay ? n - stay + i : -1;
+            return;
+        }
     }
-    const int old = n - min(recent, n), heavy = stay - (n - old);
-    for (int j = old + tid; j < n; j += SELECT) mine[heavy + j - old] = j;
-    if (heavy == 0) return;
     const auto fetch = [&](int j) {
         const int page = page_of(c, b, j);
         return page < 0 ? 0u : order_of(c.weights[((int64_t)page * c.heads + h) * c.page + (j & (c.page - 1))]);
     };
-    for (int i = tid; i < BINS; i += SELECT) bins[i] = 0;
-    __syncthreads();
     // eight entries of a thread at a time: their pages, then their weights
     const int held = min(old, HELD);
     for (int j0 = tid; j0 < held; j0 += 8 * SELECT) {
@@ -153,6 +165,48 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
     }
     const auto order = [&](int j) { return j < HELD ? orders[j] : fetch(j); };
     for (int j = HELD + tid; j < old; j += SELECT) atomicAdd(&bins[order(j) >> (32 - DIGIT)], 1);
+    const bool gaps = any_missing();        // (and the first histogram is complete)
+    int there = n, newest = n - old;        // entries, those of them that are recent
+    if (gaps) {
+        if (tid < 2) found[tid] = 0;
+        __syncthreads();
+        int gone = 0, gone_newest = 0;
+        for (int i = tid; i < pages; i += SELECT)
+            if (absent(i)) {
+                const int first = i << c.log2_page, end = min(first + c.page, n);
+                gone += end - first;
+                gone_newest += max(end - max(first, old), 0);
+            }
+        atomicAdd(&found[0], gone);
+        atomicAdd(&found[1], gone_newest);
+        __syncthreads();
+        there -= found[0];
+        newest -= found[1];
+    }
+    const int stay = min(there, keep), heavy = stay - newest;
+    if (h == 0 && tid == 0) new_lengths[b] = stay;
+    for (int i = stay + tid; i < keep; i += SELECT) mine[i] = -1;
+    if (gaps) {
+        int place = heavy;
+        for (int j0 = old; j0 < n; j0 += SELECT) {
+            const bool is = j0 + tid < n && !absent((j0 + tid) >> c.log2_page);
+            const uint64_t of = __ballot(is);
+            __syncthreads();
+            if (lane == 0) sums[0][wave] = __popcll(of);
+            __syncthreads();
+            int before = 0, all = 0;
+            for (int w = 0; w < SELECT_WAVES; ++w) {
+                before += w < wave ? sums[0][w] : 0;
+                all += sums[0][w];
+            }
+            if (is) mine[place + before + __popcll(of & below)] = j0 + tid;
+            place += all;
+        }
+        if (heavy == 0) return;
+        __syncthreads();
+    } else {
+        for (int j = old + tid; j < n; j += SELECT) mine[heavy + j - old] = j;
+    }
     uint32_t limit = 0;         // the heavy-th largest, as far as it is known
     int left = heavy;           // how many of those that agree with it so far are to stay
     for (int shift = 32 - DIGIT; ; shift = max(shift - DIGIT, 0)) {
@@ -165,8 +219,8 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
                 const uint32_t u = order(j);
                 if (u >> known == limit >> known) atomicAdd(&bins[u >> shift & mask], 1);
             }
+            __syncthreads();
         }
-        __syncthreads();
         // from the largest bin on: a thread has two neighbours
         const int top = BINS - 1 - 2 * tid, x = bins[top], y = bins[top - 1];
         int upto = wave_prefix(x + y);
@@ -203,7 +257,6 @@ __global__ __launch_bounds__(SELECT) void select_kernel(const Cache c, const int
         above += sums[0][w];
         equal += sums[1][w];
     }
-    const uint64_t below = (1ull << lane) - 1;
     for (int j0 = from; j0 < to; j0 += 64) {
         const bool in = j0 + lane < to;
         const uint32_t u = in ? order(j0 + lane) : 0;
