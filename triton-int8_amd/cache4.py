@@ -188,7 +188,7 @@ class Cache4:
         tokens = k.shape[1]
         _need(self.filled + tokens <= self.max_length, f"{tokens} tokens behind {self.filled} are more than the {self.max_length} entries that there is room for")
         append(self.pool, self.table, self.lengths, k, v, counts=counts, weights=self.weights)
-        self._counts.add_(tokens if counts is None else counts)
+        self._counts.add_(tokens if counts is None else counts.clamp(0, tokens))        # (as the kernel takes them)
         self.filled += tokens
         self.seen += tokens
 
