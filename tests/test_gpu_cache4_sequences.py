@@ -24,3 +24,32 @@ def test_counts_of_more_and_less_than_the_tokens(C, dev):
     want = oracle.attention(cache.pool.cpu(), cache.table.cpu(), [12, 7, 9], q, [5, 0, 2], 1 / math.sqrt(64), 16)
     assert bool(torch.isfinite(out).all())
     _check_attention(out, lse, want, 64, 12)
+
+
+@pytest.mark.parametrize("int8,scheme", [(True, "block_channel"), (True, "double_channel"), (True, "row_block"), (False, "block_channel")])
+def test_blank_rows_change_nothing(dev, int8, scheme):
+    """Rows behind a sequence's tokens share blocks of 128 rows, and a scale, with other sequences' tokens: taken for blank, they may hold anything."""
+    import triton_int8_amd as T
+    gen = torch.Generator().manual_seed(2)
+    layer = T.DecoderLayer(hidden=512, heads=4, mlp=1024, int8=int8, scheme=scheme, device=dev)
+    with torch.no_grad():
+        for p in layer.parameters():
+            if p.dim() == 2:
+                p.copy_((torch.randn(p.shape, generator=gen) * p.shape[1] ** -0.5).bfloat16())
+    rotary = T.decoder.rope_tables(64, 128, dev)
+    x = torch.randn(4, 40, 512, generator=gen).bfloat16().to(dev)
+    counts = [40, 3, 0, 17]
+    padding = torch.arange(40, device=dev)[None] >= torch.tensor(counts, device=dev)[:, None]
+    results = []
+    for fill in (0.0, 1.0, -3e4, float("inf"), float("nan")):
+        cache = T.Cache4(4, 64, 4, 128, page_size=16, budget=64, device=dev)
+        cache.pool.zero_()
+        prompt = x.masked_fill(padding[..., None], fill)
+        before = prompt.clone()
+        out = layer.serve(prompt, cache, rotary, counts=_ints(counts, dev), blank=True)
+        assert torch.equal(prompt.view(torch.int16), before.view(torch.int16))        # the caller's tensor stays as it is
+        assert bool(torch.isfinite(out).all()) and not bool(out[padding].any())
+        results.append((out, cache.pool.clone(), cache.weights.clone(), layer.serve(x[:, :1], cache, rotary)))
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)

@@ -247,10 +247,12 @@ class DecoderLayer(torch.nn.Module):
         return x + self.down_proj(product(gate, up))
 
     @torch.no_grad()
-    def serve(self, x, cache, rotary, counts=None):
+    def serve(self, x, cache, rotary, counts=None, blank=False):
         """The layer's output for new tokens x [batch, tokens, hidden] behind those that went into ``cache`` (a :class:`~triton_int8_amd.cache4.Cache4` of this
         layer's heads), which they join.  ``rotary``: the tables of :func:`rope_tables` for as many positions as the sequences will have.  ``counts`` int32
-        [batch]: of sequence b only the first so many tokens are new, its other rows mean nothing.
+        [batch]: of sequence b only the first so many rows are new tokens, the others go into no cache and what comes out of them means nothing.  They are rows of the call
+        all the same: where the linears' int8 codes share a scale among 128 rows (``block_channel``), an outlier in such a row coarsens the codes of tokens beside
+        it, and a NaN spoils them.  ``blank``: they are taken for zeros, which change nothing, and give zeros; for rows that may hold anything.
 
         A budget is kept by calling ``cache.evict(recent)`` between calls: what stays is attended to at the positions that it had."""
         B, S, H = x.shape
@@ -258,7 +260,11 @@ class DecoderLayer(torch.nn.Module):
         if cache.seen + S > cos.shape[0]:
             raise ValueError(f"{S} tokens behind {cache.seen} have positions beyond the {cos.shape[0]} of the rotary tables")
         # (clamped: a recorded graph is replayed without the check above)
-        at = (cache.positions[:, None] + torch.arange(S, dtype=torch.int32, device=x.device)).clamp_(max=cos.shape[0] - 1).flatten()
+        token = torch.arange(S, dtype=torch.int32, device=x.device)
+        at = (cache.positions[:, None] + token).clamp_(max=cos.shape[0] - 1).flatten()
+        if blank and counts is not None:
+            # zeros all the way: norms, projections, attention and products of a row of zeros are zeros, which no scale that it shares with tokens notices
+            x = x.masked_fill((token >= counts[:, None])[:, :, None], 0.0)
         cos, sin = cos.index_select(0, at), sin.index_select(0, at)
         h = self.input_norm(x)
         q, k, v = (t.view(1, B * S, self.heads, self.head_dim) for t in _projections(h, self.q_proj, self.k_proj, self.v_proj))
