@@ -53,3 +53,23 @@ def test_blank_rows_change_nothing(dev, int8, scheme):
     for other in results[1:]:
         for a, b in zip(results[0], other):
             assert torch.equal(a, b)
+
+
+def test_serving_goes_on_while_there_is_room(dev):
+    """Drafts of which most are no tokens in the end: neither the cache nor the rotary tables run out before the sequences need them."""
+    import triton_int8_amd as T
+    layer = T.DecoderLayer(hidden=256, heads=2, mlp=512, int8=False, device=dev)
+    rotary = T.decoder.rope_tables(24, 128, dev)
+    gen = torch.Generator().manual_seed(3)
+    cache = T.Cache4(2, 20, 2, 128, page_size=16, budget=12, device=dev)
+    for i in range(9):
+        layer.serve(torch.randn(2, 4, 256, generator=gen).bfloat16().to(dev), cache, rotary, counts=_ints([2, i % 2], dev))
+    assert cache.lengths.tolist() == [18, 4]
+    cache.evict(4)
+    layer.serve(torch.randn(2, 6, 256, generator=gen).bfloat16().to(dev), cache, rotary, counts=_ints([6, 0], dev))
+    assert cache.lengths.tolist() == [18, 4] and cache.positions.tolist() == [24, 4]
+    with pytest.raises(ValueError, match="rotary"):
+        layer.serve(torch.randn(2, 1, 256, generator=gen).bfloat16().to(dev), cache, rotary)
+    x = torch.randn(2, 3, 256, generator=gen).bfloat16().to(dev)
+    with pytest.raises(ValueError, match="room"):
+        cache.append(*(t.view(2, 3, 2, 128) for t in (x, x)), counts=_ints([3, 3], dev))

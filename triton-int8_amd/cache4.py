@@ -180,17 +180,30 @@ class Cache4:
         self.spare = torch.arange(batch * mine, pages, dtype=torch.int32, device=device).view(batch, spare) if spare else None
         self._counts = torch.zeros((2, batch), dtype=torch.int32, device=device)
         self.lengths, self.positions = self._counts
-        # entries and tokens of the longest sequence, as far as the host knows (all tokens of a call counted, replays of a graph not)
+        # entries and tokens of the longest sequence, as far as the host knows (all tokens of a call counted, replays of a graph not); see look()
         self.filled = self.seen = 0
+
+    def look(self):
+        """``filled`` and ``seen`` as the GPU has them, which is waited for."""
+        self.filled, self.seen = self._counts.amax(1).tolist()
+
+    def after(self, tokens, counts=None):
+        """What ``filled`` and ``seen`` will be behind so many new tokens of every sequence (of sequence b ``counts[b]``), as the GPU has it; while a graph is
+        recorded as the host has it."""
+        if self.pool.is_cuda and torch.cuda.is_current_stream_capturing():
+            return self.filled + tokens, self.seen + tokens
+        return (self._counts + (tokens if counts is None else counts.clamp(0, tokens))).amax(1).tolist()
 
     def append(self, k, v, counts=None):
         """New tokens, bf16 [batch, tokens, kv_heads, head_dim], behind the entries of each sequence (of sequence b the first ``counts[b]``)."""
         tokens = k.shape[1]
-        _need(self.filled + tokens <= self.max_length, f"{tokens} tokens behind {self.filled} are more than the {self.max_length} entries that there is room for")
+        filled, seen = self.filled + tokens, self.seen + tokens
+        if filled > self.max_length:        # before a call is refused: sequences may have got fewer tokens than the host counts
+            filled, seen = self.after(tokens, counts)
+        _need(filled <= self.max_length, f"{tokens} tokens are more than there is room for: a sequence would have {filled} entries of {self.max_length}")
         append(self.pool, self.table, self.lengths, k, v, counts=counts, weights=self.weights)
         self._counts.add_(tokens if counts is None else counts.clamp(0, tokens))        # (as the kernel takes them)
-        self.filled += tokens
-        self.seen += tokens
+        self.filled, self.seen = filled, seen
 
     def reset(self):
         """All sequences empty again."""

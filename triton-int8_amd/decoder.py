@@ -257,7 +257,8 @@ class DecoderLayer(torch.nn.Module):
         A budget is kept by calling ``cache.evict(recent)`` between calls: what stays is attended to at the positions that it had."""
         B, S, H = x.shape
         cos, sin = rotary
-        if cache.seen + S > cos.shape[0]:
+        # (as in Cache4.append: the GPU is asked before a call is refused)
+        if cache.seen + S > cos.shape[0] and cache.after(S, counts)[1] > cos.shape[0]:
             raise ValueError(f"{S} tokens behind {cache.seen} have positions beyond the {cos.shape[0]} of the rotary tables")
         # (clamped: a recorded graph is replayed without the check above)
         token = torch.arange(S, dtype=torch.int32, device=x.device)
