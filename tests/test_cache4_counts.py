@@ -51,3 +51,30 @@ def test_the_host_can_look(C):
     cache.lengths.fill_(1)      # as an eviction does
     cache.look()
     assert (cache.filled, cache.seen) == (1, 2)
+
+
+def test_tokens_are_taken_back(C):
+    cache = _cache(C)
+    _new(cache, 8, [8, 2, 0])
+    cache.take_back(1)
+    assert cache.lengths.tolist() == cache.positions.tolist() == [7, 1, 0]
+    cache.take_back(torch.tensor([3, 5, -2], dtype=torch.int32))
+    assert cache.lengths.tolist() == cache.positions.tolist() == [4, 0, 0]
+    cache.positions.add_(10)        # entries that an eviction dropped
+    cache.take_back(9)
+    assert cache.lengths.tolist() == [0, 0, 0] and cache.positions.tolist() == [10, 10, 10]
+    for tokens in (1.0, torch.tensor([1, 1]), torch.tensor([1, 1, 1]), [1, 1, 1]):
+        with pytest.raises(ValueError, match="tokens"):
+            cache.take_back(tokens)
+    _new(cache, 20)
+    assert (cache.filled, cache.seen) == (20, 30)
+
+
+@pytest.mark.parametrize("index", [1, [1], torch.tensor([False, True, False]), slice(1, 2)], ids=str)
+def test_some_sequences_begin_again(C, index):
+    cache = _cache(C)
+    _new(cache, 20)
+    cache.reset(index)
+    assert cache.lengths.tolist() == cache.positions.tolist() == [20, 0, 20]
+    _new(cache, 20, [0, 20, 0])
+    assert cache.lengths.tolist() == [20, 20, 20]

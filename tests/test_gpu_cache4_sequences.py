@@ -73,3 +73,30 @@ def test_serving_goes_on_while_there_is_room(dev):
     x = torch.randn(2, 3, 256, generator=gen).bfloat16().to(dev)
     with pytest.raises(ValueError, match="room"):
         cache.append(*(t.view(2, 3, 2, 128) for t in (x, x)), counts=_ints([3, 3], dev))
+
+
+def test_rejected_drafts_and_sequences_that_begin_again(C, dev):
+    """Entries that were taken back are not seen, and written over by the next tokens, whose weights begin at zero."""
+    gen = torch.Generator().manual_seed(4)
+    rand = lambda *shape: torch.randn(*shape, generator=gen).bfloat16().to(dev)  # noqa: E731
+    k, v, q = rand(2, 30, 2, 64), rand(2, 30, 2, 64), rand(2, 2, 4, 64)
+    drafted, straight = (C.Cache4(2, 40, 2, 64, page_size=16, budget=40, device=dev) for _ in range(2))
+    drafted.append(k[:, :20], v[:, :20])
+    drafted.append(rand(2, 6, 2, 64), rand(2, 6, 2, 64))
+    drafted.attend(rand(2, 6, 4, 64))
+    drafted.take_back(_ints([6, 2], dev))
+    drafted.take_back(_ints([0, 4], dev))
+    drafted.weights.zero_()
+    straight.append(k[:, :20], v[:, :20])
+    for cache in (drafted, straight):
+        cache.append(k[:, 20:22], v[:, 20:22])
+    assert torch.equal(drafted.attend(q), straight.attend(q)) and torch.equal(drafted.lengths, straight.lengths)
+    for cache in (drafted, straight):
+        cache.reset(1)
+        cache.append(k[:, 22:], v[:, 22:], counts=_ints([0, 8], dev))
+        assert cache.lengths.tolist() == cache.positions.tolist() == [22, 8]
+    assert torch.equal(drafted.attend(q), straight.attend(q))
+    seen = torch.arange(48, device=dev) < drafted.lengths[:, None]
+    for a, b in ((drafted, straight),):
+        wa, wb = (c.weights[c.table.long()].transpose(1, 2).flatten(2).transpose(1, 2)[seen] for c in (a, b))
+        assert torch.equal(wa, wb)

@@ -205,8 +205,21 @@ class Cache4:
         self._counts.add_(tokens if counts is None else counts.clamp(0, tokens))        # (as the kernel takes them)
         self.filled, self.seen = filled, seen
 
-    def reset(self):
-        """All sequences empty again."""
+    def take_back(self, tokens):
+        """The newest tokens out again, as drafted ones that were rejected: so many of every sequence, or int32 [batch]; no more than it has entries.  What they gave
+        to other entries' weights stays there."""
+        if isinstance(tokens, int):
+            self._counts.sub_(self.lengths.clamp(max=max(tokens, 0)))
+            return
+        _need(isinstance(tokens, torch.Tensor) and tokens.dtype == torch.int32 and tokens.shape == self.lengths.shape and tokens.device == self.lengths.device,
+              f"tokens must be a number or an int32 tensor {tuple(self.lengths.shape)} on {self.lengths.device}")
+        self._counts.sub_(self.lengths.minimum(tokens.clamp(min=0)))
+
+    def reset(self, sequences=None):
+        """All sequences empty again, or those that an index names (numbers, or bool [batch])."""
+        if sequences is not None:
+            self._counts[:, sequences] = 0
+            return
         self._counts.zero_()
         self.filled = self.seen = 0
 
