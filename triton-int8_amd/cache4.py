@@ -4,12 +4,14 @@ entries that got the least attention (csrc/cache4.hip, csrc/cache4_attention.hip
 The functions take the cache as the tensors that it consists of: ``pool`` uint8 [pages, kv_heads, page_size * (head_dim + head_dim // 16)] (see
 ``include/ti8.h`` for a page's layout), a page table int32 [batch, pages of a sequence], lengths int32 [batch] and, where attention is added up,
 ``weights`` float32 [pages, kv_heads, page_size].  :class:`Cache4` holds them for a batch of sequences.  Lengths, starts and counts are read on the
-GPU only, so all of it may be captured into a graph.  There are no gradients: tensors that require one are refused while gradients are recorded.
+GPU only, so all of it may be captured into a graph.  There are no gradients: tensors that require one are refused while gradients are recorded, and
+so are tensors with a tangent, and tracing.
 """
 import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from .ops import _need, _stream
@@ -50,15 +52,21 @@ def _cache(pool, table, weights, head_dim, batch):
     if weights is not None:
         _need(isinstance(weights, torch.Tensor) and weights.dtype == torch.float32 and weights.shape == (pages, heads, page) and weights.is_contiguous()
               and _on_this_gpu(weights), f"weights must be a contiguous float32 tensor {(pages, heads, page)} on the current GPU")
+        _no_gradient(weights, "weights")
     at, width, stride = _table(table, "table", batch)
     return _lib.Cache4(pool.data_ptr(), at, None if weights is None else weights.data_ptr(), pages, heads, page, head_dim, batch, width, stride)
+
+
+def _no_gradient(t, name):
+    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a cache does not give: call it under torch.no_grad()")
+    _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent, which a cache does not carry on")
 
 
 def _rows(x, name):
     """bf16 [batch, tokens, heads, head_dim] as the kernels read it, and its strides."""
     _need(isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and x.dim() == 4 and x.numel() > 0 and _on_this_gpu(x),
           f"{name} must be a non-empty bfloat16 tensor [batch, tokens, heads, head_dim] on the current GPU")
-    _need(not (x.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a cache does not give: call it under torch.no_grad()")
+    _no_gradient(x, name)
     B, S, H, _ = x.shape
     sb, ss, sh, one = x.stride()
     sb, ss, sh = 0 if B == 1 else sb, 0 if S == 1 else ss, 0 if H == 1 else sh      # (of a dimension of one a stride means nothing)
@@ -71,11 +79,10 @@ def _rows(x, name):
 def _natively(name, *args):
     """A call with its checks, allocations and launches made from C++, or None where it takes the Python way, which says what is wrong."""
     native = _lib.native()
-    if native is None:
-        return None
-    out = getattr(native, name)(*args, _stream())
+    out = None if native is None else getattr(native, name)(*args, _stream())
     if type(out) is tuple:
         raise _lib.failed(*out)
+    _need(out is not None or torch._C._get_tracing_state() is None, "calls on a cache cannot be traced: what they launch would not be recorded")
     return out
 
 

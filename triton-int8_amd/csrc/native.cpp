@@ -166,6 +166,9 @@ PyObject* linear_call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 c10::DeviceIndex current_device() { return c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index(); }
 
+// Whether a gradient or a tangent is asked for
+bool derived(const at::Tensor& t) { return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
+
 struct CacheCall {
     const c10::DeviceIndex device = current_device();
     ti8_cache4 c = {};
@@ -192,7 +195,7 @@ struct CacheCall {
         if (page * entry != pool.size(2) || (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)) return false;
         c.batch = batch;
         if (!rows_of(table, &c.table_pages, &c.table_stride)) return false;
-        if (weights.defined() && (!here(weights, at::kFloat, 3) || !weights.is_contiguous() || weights.size(0) != pool.size(0) || weights.size(1) != pool.size(1) || weights.size(2) != page)) return false;
+        if (weights.defined() && (!here(weights, at::kFloat, 3) || derived(weights) || !weights.is_contiguous() || weights.size(0) != pool.size(0) || weights.size(1) != pool.size(1) || weights.size(2) != page)) return false;
         c.pool = pool.data_ptr();
         c.table = static_cast<const int32_t*>(table.data_ptr());
         c.weights = weights.defined() ? static_cast<float*>(weights.data_ptr()) : nullptr;
@@ -204,7 +207,7 @@ struct CacheCall {
     }
     // bf16 [batch][tokens][heads][head_dim] that is read in place; strides between batches, tokens and heads
     bool tokens_of(const at::Tensor& t, int64_t (&strides)[3]) const {
-        if (!here(t, at::kBFloat16, 4) || t.numel() == 0 || (t.requires_grad() && at::GradMode::is_enabled())) return false;
+        if (!here(t, at::kBFloat16, 4) || t.numel() == 0 || derived(t)) return false;
         int64_t any = 0;
         for (int i = 0; i < 3; ++i) any |= strides[i] = t.size(i) == 1 ? 0 : t.stride(i);
         return t.stride(3) == 1 && !(any & 7) && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
