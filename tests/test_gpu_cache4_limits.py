@@ -165,3 +165,49 @@ def test_what_is_not_there_is_not_seen_after_an_eviction(C, dev):
         j = kept[b, 0].cpu().long()
         for x, y in zip(oracle.entries(after, new_table[b], page, dim, 0, 80), oracle.entries(pool, table[b].clamp(0, 39), page, dim, 0, n)):
             assert torch.equal(x, y[j]) and bool((table[b].long()[j // page] < 40).all()) and bool((table[b].long()[j // page] >= 0).all())
+
+
+# steps with a workgroup for each head and shared out, rows that two waves share, prompts of four and eight waves, entries shared among workgroups
+ROWS = [(1, 2, 2, 600), (1, 2, 2, 5000), (7, 4, 1, 600), (7, 4, 1, 5000), (50, 1, 1, 600), (50, 1, 1, 9000), (100, 2, 2, 600), (250, 1, 1, 600), (250, 2, 2, 9000)]
+
+
+@pytest.mark.parametrize("tokens,heads,hkv,room", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("values", ["one", "all", "some", "late"])
+def test_values_as_large_as_are_stored(C, dev, tokens, heads, hkv, room, dim, values):
+    """Up to 1.5 2^127: a single entry's come out as they are, and sums of many, of either sign and beside small ones, as the definition has them; rows that are
+    none are zeros."""
+    gen = torch.Generator().manual_seed(tokens + dim)
+    page, lengths, counts = 32, [1, 600, 333, 597], [1, tokens, max(tokens - 3, 0), tokens // 2]
+    mine = -(-600 // page)
+    pool, table = _pool(gen, 4 * mine, hkv, page, dim), _table(gen, 4, mine, 4 * mine)
+    scales = oracle.parts(pool, page, dim)[3]
+    if values == "some":        # here and there a group of 32, of any size
+        some = torch.rand(scales.shape, generator=gen) < 0.05
+        scales[some] = torch.randint(180, 253, (int(some.sum()),), generator=gen, dtype=torch.uint8)
+    elif values == "late":      # the last entries alone, behind many of usual size
+        for b, n in enumerate(lengths):
+            for j in range(max(0, n - 3), n):
+                scales[int(table[b, j // page]), :, j % page] = 252
+    else:
+        scales.fill_({"one": 127 + 110, "all": 252}[values])
+    if values == "one":
+        lengths = [1] * 4
+        counts = [1, min(tokens, 1), 0, 1]
+    if values == "all":         # all positive for some entries' elements: sums of equal signs
+        oracle.parts(pool, page, dim)[1][:, :, ::2] &= 0x77
+    wide = torch.full((4, -(-room // page)), -1, dtype=torch.int32)
+    wide[:, :mine] = table
+    q = torch.randn(4, tokens, heads, dim, generator=gen).bfloat16()
+    want = oracle.attention(pool, table, lengths, q, counts, 1 / math.sqrt(dim), page)
+    weights = torch.zeros(4 * mine, hkv, page, device=dev)
+    out, lse = C.attention(pool.to(dev), wide.to(dev), _ints(lengths, dev), q.to(dev), counts=_ints(counts, dev), weights=weights)
+    assert bool(torch.isfinite(out).all()), out[~torch.isfinite(out)][:4]
+    _check_attention(out, lse, want, dim, max(lengths))
+    if values == "one":
+        for b in range(4):
+            for h in range(hkv):
+                v = oracle.entries(pool, table[b], page, dim, h, 1)[1][0]
+                for t in range(counts[b]):
+                    for head in range(h * (heads // hkv), (h + 1) * (heads // hkv)):
+                        assert torch.equal(out[b, t, head].cpu().double(), v)

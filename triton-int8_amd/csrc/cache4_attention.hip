@@ -26,6 +26,11 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 // Exponentials are carried times 2^UP, which their common divisor takes away again: those of scores far below the maximum stay above 2^-126, below which
 // v_exp_f32 gives zero, for 2^UP further (where sums are put under another maximum exp2f goes on below it).  Up to 2^(8 + UP) each (see step_kernel), their sums stay far below 2^127
 constexpr float UP = 24.0f;      // (= the 24 in lse_of)
+// With values below 2^63 their products' sums stay below 2^127, too (2^32 of an exponential, 2^30 entries).  A wave that comes upon a larger one (a scale of BIG or more) goes on
+// with exponentials, and the sums so far, times 2^-DOWN of that, which the largest values have room for; those below 2^-86 of a row's largest then vanish.  A part in memory has
+// DOWN in its maximum.
+constexpr uint32_t BIG = 190;
+constexpr float DOWN = 64.0f, DOWN_FACTOR = 0x1p-64f, DOWN_AWAY = 0x1p64f;
 
 struct Args {
     Cache c;
@@ -233,6 +238,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
 
         v4f o[TILES][BLOCKS];
         float top[TILES], shift[TILES], sum[TILES];      // maximum, what is taken from a score times factor, sum of this lane's entries
+        float up = UP;
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             top[t] = -INFINITY;
@@ -264,7 +270,8 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
                     *reinterpret_cast<uint4*>(mine + row * V::ROW + (((quarter * STEPS + i) ^ V::swizzle(row)) << 4)) = decode8(x.v[u][i], scale);
             }
             const int j0 = turn * ENTRIES;
-            if (j0 + ENTRIES > all_see || x.absent)
+            const bool big = __any(max(x.vs[0], x.vs[1]) >= BIG);
+            if (j0 + ENTRIES > all_see || x.absent || big) {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -272,6 +279,17 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (j0 + u * 16 + quarter * 4 + i >= sees[t] || (x.absent >> u & 1)) s[t][u][i] = -INFINITY;
+                if (big && up == UP) {
+                    up -= DOWN;
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        shift[t] += DOWN;
+                        sum[t] *= DOWN_FACTOR;
+#pragma unroll
+                        for (int d = 0; d < BLOCKS; ++d) o[t][d] *= DOWN_FACTOR;
+                    }
+                }
+            }
             v8bf p[TILES];
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
@@ -281,7 +299,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
                 if (__any((largest - top[t]) * factor > 8.0f)) {
                     const float higher = fmaxf(top[t], largest), shrink = higher == -INFINITY ? 1.0f : exp2f((top[t] - higher) * factor);
                     top[t] = higher;
-                    shift[t] = higher == -INFINITY ? 0.0f : higher * factor - UP;
+                    shift[t] = higher == -INFINITY ? 0.0f : higher * factor - up;
                     sum[t] *= shrink;
 #pragma unroll
                     for (int d = 0; d < BLOCKS; ++d) o[t][d] *= shrink;
@@ -324,7 +342,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
             __syncthreads();
             if (quarter == 0) {
                 stats[wave][0][r16] = top[t];
-                stats[wave][1][r16] = total;
+                stats[wave][1][r16] = up == UP ? total : -total;      // (the sign says how they are carried)
             }
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d)
@@ -335,12 +353,18 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
 #pragma unroll
             for (int w = 0; w < NW; ++w) m = fmaxf(m, stats[w][0][row]);
             float f[NW];
+            bool down = false;
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
                 f[w] = stats[w][0][row] == -INFINITY ? 0.0f : exp2f((stats[w][0][row] - m) * factor);
-                // (a NaN in the sum passes a maximum of -inf)
-                l += stats[w][0][row] == -INFINITY ? stats[w][1][row] : stats[w][1][row] * f[w];
+                down |= stats[w][1][row] < 0.0f;
             }
+            if (__any(down))
+#pragma unroll
+                for (int w = 0; w < NW; ++w) f[w] *= down && !(stats[w][1][row] < 0.0f) ? DOWN_FACTOR : 1.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w)        // (a NaN in the sum passes a maximum of -inf)
+                l += stats[w][0][row] == -INFINITY ? stats[w][1][row] : fabsf(stats[w][1][row]) * f[w];
             const int at = t * 16 + row, token = at / a.group;
             if (at >= rows) l = 0.0f;       // (no query: zeros were multiplied)
             const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + h * a.group + at % a.group;
@@ -359,8 +383,8 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
             }
             if (lane_of == 0) {
                 if (!whole) {
-                    if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor, l);
-                } else if (at < a.tokens * a.group) a.lse[to] = lse_of(m * factor, l);
+                    if (at < rows) *reinterpret_cast<float2*>(part + at * Part<D>::ROW + D) = make_float2(m * factor + (down ? DOWN : 0.0f), l);
+                } else if (at < a.tokens * a.group) a.lse[to] = lse_of(m * factor, down ? l * DOWN_AWAY : l);
             }
         }
         left -= n + EXTRA;
@@ -523,6 +547,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     constexpr int STAGES = PROMPT_STAGES<NW>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];        // [STAGES][keys, values]
     __shared__ __attribute__((aligned(16))) int absent[STAGES][4];        // whether the pool does not have the page of 16 entries of a tile
+    __shared__ int any_big;     // whether some values so far have a scale of BIG or more
     const Cache& c = a.c;
     const idx::AttentionPlace place = idx::cache4_place(blockIdx.x, c.batch * c.heads, a.blocks * a.splits);
     if (place.pair >= c.batch * c.heads) return;
@@ -532,7 +557,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     constexpr int ROWS_OF = NW / SHARES * 32;
     const int mine_of = wave / (NW / SHARES);      // which half of a tile, with two shares
     const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), rows = count * a.group;
-    const int row0 = block * ROWS_OF, row = row0 + wave % (NW / SHARES) * 32 + r32, token = row / a.group, head = h * a.group + row % a.group;
+    const int row0 = block * ROWS_OF, row = row0 + wave % (NW / SHARES) * 32 + r32;
     // entries that this lane's row, any row of the workgroup and any row of the wave sees
     const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
     const int sees = row < rows ? sees_of(row) : 0;
@@ -540,6 +565,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     if (split >= block_sees.parts) return;
     const int wave0 = row0 + wave % (NW / SHARES) * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
     const int tiles = block_sees.tiles, begin = (int)((int64_t)split * tiles / block_sees.parts), end = (int)((int64_t)(split + 1) * tiles / block_sees.parts);
+    if (threadIdx.x == 0) any_big = 0;
     // entries that every row of the workgroup sees: none where the pool does not have all the pages
     bool gaps = false;
     for (int i = (begin * TILE >> c.log2_page) + threadIdx.x; i < (min(end * TILE, length) + c.page - 1) >> c.log2_page; i += NW * 64)
@@ -553,7 +579,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + token * a.q_st + head * a.q_sh + s * 16 + half * 8);
+        if (row < rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + (row / a.group) * a.q_st + (h * a.group + row % a.group) * a.q_sh + s * 16 + half * 8);
         q[s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
     }
     v16f o[BLOCKS];
@@ -561,7 +587,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    float top = -INFINITY, shift = 0.0f, sum = 0.0f;
+    float top = -INFINITY, shift = 0.0f, sum = 0.0f, up = UP;
 
     Codes<D> raw[PARTS];
     int there[PARTS];
@@ -583,6 +609,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         for (int i = 0; i < PARTS; ++i) {
             const int p = wave + i * NW, at = (p & 3) * 16 + r16;
             uint8_t* const to = smem + (stage * 2 + (p >> 2)) * T::BYTES + at * T::ROW;
+            if (p >= 4 && __any(raw[i].scale >= BIG)) any_big = 1;
             const float scale = scale_of(raw[i].scale);
 #pragma unroll
             for (int w = 0; w < Codes<D>::WORDS; ++w)
@@ -619,11 +646,16 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         for (int i = 1; i < 16; ++i) m = __builtin_amdgcn_fmed3f(m, s[i], INFINITY);
         return over_halves<false>(m);
     };
-    const auto raise = [&](float largest) {
-        if (__any((largest - top) * factor > 8.0f)) {       // see step_kernel
-            const float higher = fmaxf(top, largest), shrink = higher == -INFINITY ? 1.0f : exp2f((top - higher) * factor);
+    const auto raise = [&](float largest, int big) {
+        if (__any((largest - top) * factor > 8.0f || big)) {       // see step_kernel
+            const float higher = fmaxf(top, largest);
+            float shrink = higher == -INFINITY ? 1.0f : exp2f((top - higher) * factor);
+            if (__any(big) && up == UP) {
+                up -= DOWN;
+                shrink *= DOWN_FACTOR;
+            }
             top = higher;
-            shift = higher == -INFINITY ? 0.0f : higher * factor - UP;
+            shift = higher == -INFINITY ? 0.0f : higher * factor - up;
             sum *= shrink;
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d) o[d] *= shrink;
@@ -655,15 +687,17 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     };
     // from the scores of a half tile (s) to the next one's, of half u of a tile in `ahead`; the values are half `of` of `stage`
     v16f s;
-    const auto step = [&](int stage, int of, int ahead, int u, int tile, int gone, auto masked) {
+    // (with `last` they are those of the next tile, and the first multiplied by its values)
+    const auto step = [&](int stage, int of, int ahead, int u, int tile, int gone, auto masked, auto last) {
         v8bf p[2];
+        const int big = last ? any_big : 0;     // (the next tile was converted before the waves last met)
         v16f other = scores(ahead, u);
         exponentials(s, p);
         if (masked) mask(other, tile, u, gone);
         const float largest = largest_of(other);
         add_values(stage, of, p);
         s = other;
-        raise(largest);
+        raise(largest, big);
     };
 
     if (begin < end) {
@@ -679,7 +713,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         if (begin < mine) {
             s = scores(0, SHARES == 2 ? mine_of : 0);
             mask(s, begin, SHARES == 2 ? mine_of : 0, gone_of(0));
-            raise(largest_of(s));
+            raise(largest_of(s), __builtin_amdgcn_readfirstlane(any_big));
         }
         int stage = 0;
         const auto walk = [&](int from, int to, auto masked) {
@@ -689,10 +723,10 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
                 const int into = STAGES == 3 ? (next + 1 == STAGES ? 0 : next + 1) : next, ready = tile + STAGES - 1;
                 if (ready < end) convert(ready, into);
                 if (ready + 1 < end) load(ready + 1);
-                if (SHARES == 1 && tile < mine) step(stage, 0, stage, 1, tile, masked ? gone_of(stage) : 0, masked);
+                if (SHARES == 1 && tile < mine) step(stage, 0, stage, 1, tile, masked ? gone_of(stage) : 0, masked, std::false_type{});
                 if (STAGES == 2) __syncthreads();       // the next tile is there
                 const int of = SHARES == 2 ? mine_of : 1, u = SHARES == 2 ? mine_of : 0;
-                if (tile + 1 < mine) step(stage, of, next, u, tile + 1, masked ? gone_of(next) : 0, masked);
+                if (tile + 1 < mine) step(stage, of, next, u, tile + 1, masked ? gone_of(next) : 0, masked, std::true_type{});
                 else if (tile < mine) {
                     v8bf p[2];
                     exponentials(s, p);
@@ -705,6 +739,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         const int clear = min(max(all / TILE - 1, begin), end);
         walk(begin, clear, std::false_type{});
         walk(clear, end, std::true_type{});
+        raise(-INFINITY, __builtin_amdgcn_readfirstlane(any_big));        // (a wave whose rows see none of the last tiles: all waves carry alike)
     }
     sum = over_halves<true>(sum);
     if constexpr (SHARES == 2) {
@@ -728,8 +763,11 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * fa + meet[(d * 16 + i) * 64] * fb;
         top = higher;
-        shift = higher == -INFINITY ? 0.0f : higher * factor - UP;
     }
+    // (the row is found anew, from the lane: kept in registers it would be spilled)
+    int lane_of = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(lane_of));
+    const int half_of = lane_of >> 5, row_of = row0 + wave % (NW / SHARES) * 32 + (lane_of & 31), token = row_of / a.group, head = h * a.group + row_of % a.group;
     if (token >= a.tokens) return;
     const int64_t to = ((int64_t)b * a.tokens + token) * a.heads + head;
     if (block_sees.parts > 1) {
@@ -738,21 +776,21 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
         for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<v4f*>(part + d * 32 + 2 * i + 4 * half) = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
-        if (half == 0) {
-            part[D] = top * factor;
-            part[D + 1] = row < rows ? sum : 0.0f;
+                *reinterpret_cast<v4f*>(part + d * 32 + 2 * i + 4 * half_of) = v4f{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+        if (half_of == 0) {
+            part[D] = top * factor + (UP - up);
+            part[D + 1] = row_of < rows ? sum : 0.0f;
         }
         return;
     }
-    if (row >= rows) sum = 0.0f;
+    if (row_of >= rows) sum = 0.0f;
     const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint2*>(a.out + to * D + d * 32 + 2 * i + 4 * half) = make_uint2(pack_bf16x2(o[d][i] * norm, o[d][i + 1] * norm), pack_bf16x2(o[d][i + 2] * norm, o[d][i + 3] * norm));
-    if (half == 0) a.lse[to] = lse_of(top * factor, sum);
+            *reinterpret_cast<uint2*>(a.out + to * D + d * 32 + 2 * i + 4 * half_of) = make_uint2(pack_bf16x2(o[d][i] * norm, o[d][i + 1] * norm), pack_bf16x2(o[d][i + 2] * norm, o[d][i + 3] * norm));
+    if (half_of == 0) a.lse[to] = lse_of(top * factor, up == UP ? sum : sum * DOWN_AWAY);
 #endif
 }
 
