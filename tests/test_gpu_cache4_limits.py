@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import cache4 as oracle
-from test_gpu_cache4 import C, _check_attention, _ints, _pool, _table  # noqa: F401
+from test_gpu_cache4 import C, _check_attention, _ints, _masked_reference, _pool, _table  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -211,3 +211,29 @@ def test_values_as_large_as_are_stored(C, dev, tokens, heads, hkv, room, dim, va
                 for t in range(counts[b]):
                     for head in range(h * (heads // hkv), (h + 1) * (heads // hkv)):
                         assert torch.equal(out[b, t, head].cpu().double(), v)
+
+
+@pytest.mark.parametrize("tokens,heads,hkv", [(1, 2, 2), (5, 4, 2), (12, 2, 1), (50, 1, 1), (100, 2, 2), (300, 1, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lengths_beyond_the_table(C, dev, tokens, heads, hkv, dim):
+    """Entries that the table has no room for are not seen; up to where a query sees the others goes by the length that the sequence says it has."""
+    gen = torch.Generator().manual_seed(tokens + dim)
+    page, room = 16, 208
+    lengths, counts = [room + 1, room + 3, room + tokens + 40, room, 2 ** 31 - 1], [tokens, max(tokens - 1, 1), tokens, tokens, tokens]
+    pool, table = _pool(gen, 5 * room // page, hkv, page, dim), _table(gen, 5, room // page, 5 * room // page)
+    q = torch.randn(5, tokens, heads, dim, generator=gen).bfloat16()
+    said = [min(n, room + 1000) for n in lengths]
+    wide = torch.full((5, -(-(room + 1000) // page)), -1, dtype=torch.int32)
+    wide[:, :room // page] = table
+    want = _masked_reference(pool, wide, said, q, counts, 1 / math.sqrt(dim), page)
+    for narrow in (table, wide[:, :40]):        # (pages that are none: what there is room for then)
+        weights = torch.zeros(pool.shape[0], hkv, page, device=dev)
+        out, lse = C.attention(pool.to(dev), narrow.to(dev), _ints(lengths, dev), q.to(dev), counts=_ints(counts, dev), weights=weights)
+        _check_attention(out, lse, want, dim, room)
+        expected = torch.zeros(pool.shape[0], hkv, page, dtype=torch.float64)
+        j = torch.arange(room)
+        for b in range(5):
+            for h in range(hkv):
+                expected[table[b].long()[j // page], h, j % page] += want[2][b][h][:room]
+        rel = 2.0 ** -18 + 4 * (dim + 8) * 2.0 ** -24 * float(want[3].max()) + tokens * heads * 2.0 ** -24      # as in test_attention
+        assert bool(((weights.cpu().double() - expected).abs() <= (rel + 2.0 ** -22) * expected).all())

@@ -47,8 +47,9 @@ struct Args {
     int blocks, block_rows, splits, shared_from;         // prompt_kernel: row blocks of a kv head, rows of each, workgroups that share its entries at most, and from how many tiles on
 };
 
-// entries of a sequence that any of its queries sees
+// entries of a sequence that any of its queries sees, and those that it says it has, whether or not the table has room for them
 __device__ __forceinline__ int seen_of(const Args& a, int b) { return count_of(a.counts, b, a.tokens) ? length_of(a.c, a.lengths, b) : 0; }
+__device__ __forceinline__ int total_of(const Args& a, int b) { return min(max(a.lengths[b], 0), 1 << 30); }
 
 // ---- sharing out ---------------------------------------------------------------------------------------------
 
@@ -147,11 +148,15 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
     const Cache& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quarter = lane >> 4;
     idx::Share share;
-    int b, h, length, per_head, end, left, unit = 0;
+    int b, h, total, length, per_head, end, left, unit = 0;
+    const auto read_length = [&] {
+        total = __builtin_amdgcn_readfirstlane(total_of(a, b));
+        length = __builtin_amdgcn_readfirstlane(count_of(a.counts, b, a.tokens)) ? min(total, c.capacity()) : 0;
+    };
     if constexpr (OWN) {
         b = blockIdx.x / c.heads;
         h = blockIdx.x % c.heads;
-        length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
+        read_length();
         per_head = idx::cache4_units(length, NW * ENTRIES);
         end = left = per_head + EXTRA;
     } else {
@@ -162,7 +167,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
         int before;
         end = idx::share_begin(share, blockIdx.x + 1);
         b = lengths.find(begin, before, per_head);
-        length = __builtin_amdgcn_readfirstlane(seen_of(a, b));
+        read_length();
         const int at_begin = (begin - before) % per_head;
         h = (begin - before) / per_head;
         unit = max(at_begin - EXTRA, 0);
@@ -176,7 +181,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
 
     while (left > 0) {
         const int n = min(left, per_head - unit), first = unit * NW + wave, last = (unit + n) * NW;       // this wave's turns
-        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group;
+        const int count = count_of(a.counts, b, a.tokens), rows = count * a.group, older = total - count;
         const constant_ints table = (constant_ints)(c.table + b * c.table_stride);
         struct Turn {
             uint32_t k[2][STEPS], v[2][STEPS], ks[2], vs[2];
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
             const int row = t * 16 + r16, token = row / a.group, head = h * a.group + row % a.group;
-            sees[t] = row < rows ? length - count + token + 1 : 0;
+            sees[t] = row < rows ? min(older + token + 1, length) : 0;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 uint4 x = make_uint4(0, 0, 0, 0);
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
                 q[t][s] = operand(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
             }
         }
-        const int all_see = length - count + 1;         // entries that every row sees
+        const int all_see = min(older + 1, length);         // entries that every row sees
 
         v4f o[TILES][BLOCKS];
         float top[TILES], shift[TILES], sum[TILES];      // maximum, what is taken from a score times factor, sum of this lane's entries
@@ -391,7 +396,8 @@ __global__ __launch_bounds__(OWN ? 2 * WAVES * 64 : WAVES * 64, OWN || TILES == 
         unit = 0;
         if (++h == c.heads && left > 0) {
             h = 0;
-            length = __builtin_amdgcn_readfirstlane(seen_of(a, ++b));
+            ++b;
+            read_length();
             per_head = idx::cache4_units(length, idx::CACHE4_UNIT);
         }
         __syncthreads();        // nobody writes values while somebody still adds up
@@ -530,9 +536,9 @@ template <int NW> constexpr int PROMPT_STAGES = NW == 8 ? 3 : 2;
 // One leaves no parts.
 struct BlockSees {
     int most, tiles, parts;
-    __device__ __forceinline__ BlockSees(const Args& a, int row0, int count, int length) {
+    __device__ __forceinline__ BlockSees(const Args& a, int row0, int count, int older, int length) {
         const int rows = count * a.group;
-        most = row0 < rows ? max(length - count + (min(row0 + a.block_rows, rows) - 1) / a.group + 1, 0) : 0;
+        most = row0 < rows ? max(min(older + (min(row0 + a.block_rows, rows) - 1) / a.group + 1, length), 0) : 0;
         tiles = (most + TILE - 1) / TILE;
         parts = tiles < a.shared_from ? 1 : min(a.splits, (tiles + 3) / 4);
     }
@@ -556,12 +562,12 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_kernel(const Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r32 = lane & 31, half = lane >> 5, r16 = lane & 15, quarter = lane >> 4;
     constexpr int ROWS_OF = NW / SHARES * 32;
     const int mine_of = wave / (NW / SHARES);      // which half of a tile, with two shares
-    const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), rows = count * a.group;
+    const int count = count_of(a.counts, b, a.tokens), length = length_of(c, a.lengths, b), older = total_of(a, b) - count, rows = count * a.group;
     const int row0 = block * ROWS_OF, row = row0 + wave % (NW / SHARES) * 32 + r32;
     // entries that this lane's row, any row of the workgroup and any row of the wave sees
-    const auto sees_of = [&](int r) { return max(length - count + r / a.group + 1, 0); };
+    const auto sees_of = [&](int r) { return max(min(older + r / a.group + 1, length), 0); };
     const int sees = row < rows ? sees_of(row) : 0;
-    const BlockSees block_sees(a, row0, count, length);
+    const BlockSees block_sees(a, row0, count, older, length);
     if (split >= block_sees.parts) return;
     const int wave0 = row0 + wave % (NW / SHARES) * 32, wave_most = wave0 < rows ? sees_of(min(wave0 + 32, rows) - 1) : 0;
     const int tiles = block_sees.tiles, begin = (int)((int64_t)split * tiles / block_sees.parts), end = (int)((int64_t)(split + 1) * tiles / block_sees.parts);
@@ -801,7 +807,8 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
     if (row >= rows) return;
     const uint32_t token_of = (uint32_t)row / (uint32_t)a.heads, b = token_of / (uint32_t)a.tokens;      // (fewer than 2^31 rows: ti8_cache4_attention)
     const int at = (int)(token_of % (uint32_t)a.tokens) * a.group + (int)((uint32_t)row % (uint32_t)a.heads) % a.group;
-    const int parts = BlockSees(a, at / a.block_rows * a.block_rows, count_of(a.counts, b, a.tokens), length_of(a.c, a.lengths, b)).parts;
+    const int count = count_of(a.counts, b, a.tokens);
+    const int parts = BlockSees(a, at / a.block_rows * a.block_rows, count, total_of(a, b) - count, length_of(a.c, a.lengths, b)).parts;
     if (parts == 1) return;
     const float* const from = a.parts + row * a.splits * Part<D>::ROW;
     join<D, GROUPS>(a, from, from, Part<D>::ROW, parts, row, true);
@@ -852,11 +859,13 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
     const int step_token = ROWS / a.group, step_head = ROWS % a.group;
     struct Unit {
-        int b, h, unit, length, count, per_head;
+        int b, h, unit, length, count, older, per_head;
         __device__ __forceinline__ void sequence(const Args& a, int b_) {
             b = b_;
             count = a.counts ? min(max(((constant_ints)a.counts)[b], 0), a.tokens) : a.tokens;
-            length = count ? min(max(((constant_ints)a.lengths)[b], 0), a.c.capacity()) : 0;
+            const int total = max(((constant_ints)a.lengths)[b], 0);
+            length = count ? min(total, a.c.capacity()) : 0;
+            older = min(total, 1 << 30) - count;      // entry older + t is token t's own
             per_head = idx::cache4_units(length, UNIT);
         }
     };
@@ -893,7 +902,7 @@ __global__ __launch_bounds__(WEIGHT_WAVES * 64, 4) void weights_kernel(const Arg
     fetch(now);
     int staged_b = -1, staged_h = -1;       // the head whose queries lie in LDS, all of them
     while (true) {
-        const int b = now.b, h = now.h, length = now.length, count = now.count, rows = count * a.group, older = length - count;      // entry older + t is token t's own
+        const int b = now.b, h = now.h, length = now.length, count = now.count, rows = count * a.group, older = now.older;
         const int unit0 = now.unit * UNIT, j0 = unit0 + wave * COLUMNS, j = j0 + r32;
         v8bf k[STEPS];      // the queries' elements are taken in the same order
 #pragma unroll
