@@ -539,7 +539,7 @@ int ti8_cache4_read(const ti8_cache4* c, const int32_t* starts, const int32_t* c
 /* Attention over the cache: q bf16 [batch][tokens][heads][head_dim] (strides as above; heads a multiple of kv_heads, neighbouring heads share
  * a kv head), the last counts[b] of lengths[b] entries being those of the queries' own tokens: query i of sequence b sees entries
  * j <= lengths[b] - counts[b] + i.
- *   out bf16 and lse float, dense [batch][tokens][heads][head_dim] and [batch][tokens][heads]: out = sum_j p_j v_j, p_j = exp(scale q k_j - lse),
+ *   out bf16 and lse float, dense [batch][tokens][heads][head_dim] and [batch][tokens][heads]: out = sum_j p_j v_j, p_j = exp(scale q k_j - lse) (|scale| <= 2^127),
  *   lse = log sum_j exp(scale q k_j).  Rows that see nothing and rows from counts[b] on: out 0, lse -inf.  Results are as finite as what is stored; where
  *   values of 2^63 and more are among it, a p_j below 2^-86 of its row's largest may count as zero.
  *   accumulate != 0: weights of every entry j += the sum of its p_j over the queries and the heads that share its kv head; an entry whose page several

@@ -40,3 +40,13 @@ def test_weights_are_added_to_and_never_stored(tmp_path):
     assert len(bodies) == 2
     for name, body in bodies.items():
         assert re.search(r"^\s*global_atomic_add_f32 ", body, flags=re.M) and not re.search(r"^\s*(global|buffer|flat)_store", body, flags=re.M), name
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38, -2e38])
+def test_scales_that_are_refused(scale):
+    """With one that is no number all entries would get the same, without a word."""
+    import triton_int8_amd
+    lib, fake = triton_int8_amd._lib, 0x10000
+    cache = lib.Cache4(pool=fake, table=fake, weights=fake, pages=8, kv_heads=2, page_size=64, head_dim=128, batch=3, table_pages=4, table_stride=4)
+    assert lib.lib().ti8_cache4_attention(cache, fake, None, 5, 8, fake, 2048, 256, 128, scale, 0, fake, fake, fake, 1 << 40, None) == 2
+    assert b"scale" in lib.lib().ti8_last_error()

@@ -77,3 +77,16 @@ def test_tracing(C, dev, cache, native, monkeypatch):
         with pytest.raises(ValueError, match="traced"):
             torch.jit.trace(call, (x,), check_trace=False)
     assert torch.equal(cache.pool, before)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 1e39, -(2 ** 200)])
+def test_scales(C, dev, cache, native, scale, monkeypatch):
+    import triton_int8_amd as T
+    if not native:
+        monkeypatch.setattr(T._lib, "native", lambda: None)
+    x = torch.ones(1, 3, 2, 64, dtype=torch.bfloat16, device=dev)
+    cache.append(x, x)
+    with pytest.raises(ValueError, match="scale"):
+        C.attention(cache.pool, cache.table, cache.lengths, x, scale=scale)
+    assert torch.equal(cache.attend(x, scale=1), cache.attend(x, scale=1.0))

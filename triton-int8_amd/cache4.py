@@ -130,6 +130,8 @@ def attention(pool, table, lengths, q, counts=None, scale=None, weights=None):
     B, S, H, D = q.shape
     c = _cache(pool, table, weights, D, B)
     _need(H % c.kv_heads == 0, f"{H} heads are no multiple of {c.kv_heads} kv heads")
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    _need(abs(scale) <= 2.0 ** 127, f"scale must be a number of up to 2^127 in magnitude, got {scale}")
     lengths = _ints(lengths, "lengths", B)
     counts = None if counts is None else _ints(counts, "counts", B)
     need = _lib.lib().ti8_cache4_attention_workspace(c, S, H)
@@ -137,7 +139,7 @@ def attention(pool, table, lengths, q, counts=None, scale=None, weights=None):
     dev = q.device
     out, lse = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=dev), torch.empty((B, S, H), dtype=torch.float32, device=dev)
     workspace = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    _lib.call("ti8_cache4_attention", c, lengths, counts, S, H, q.data_ptr(), *at_q, 1.0 / math.sqrt(D) if scale is None else scale, weights is not None,
+    _lib.call("ti8_cache4_attention", c, lengths, counts, S, H, q.data_ptr(), *at_q, scale, weights is not None,
               out.data_ptr(), lse.data_ptr(), workspace.data_ptr() if need else None, need, _stream())
     return out, lse
 

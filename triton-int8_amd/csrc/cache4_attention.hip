@@ -1210,6 +1210,7 @@ extern "C" int ti8_cache4_attention(const ti8_cache4* p, const int32_t* lengths,
     const int64_t need = ti8_cache4_attention_workspace(p, tokens, heads);
     if (need < 0) return fail(TI8_ERR_SHAPE, "%s: need tokens > 0 and heads a multiple of kv_heads, and no more rows than a launch takes; got tokens=%lld heads=%lld", fn,
                               (long long)tokens, (long long)heads);
+    if (!(scale >= -0x1p127f && scale <= 0x1p127f)) return fail(TI8_ERR_SHAPE, "%s: scale must be a number of up to 2^127 in magnitude, got %g", fn, (double)scale);
     if (!q || !lengths || !out || !lse || (accumulate && !c.weights) || (need && !workspace))
         return fail(TI8_ERR_NULL, "%s: q, lengths, out and lse are required, the weights to add up as well, and the workspace", fn);
     if (need > workspace_bytes) return fail(TI8_ERR_SHAPE, "%s: %lld bytes of workspace are needed, got %lld", fn, (long long)need, (long long)workspace_bytes);

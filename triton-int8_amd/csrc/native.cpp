@@ -292,6 +292,7 @@ PyObject* cache4_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int64_t need = cache4_attention_workspace(&call.c, q.size(1), q.size(2));
     if (need < 0) Py_RETURN_NONE;
     const float scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)q.size(3))) : (float)PyFloat_AS_DOUBLE(args[6]);
+    if (!(std::fabs(scale) <= 0x1p127f)) Py_RETURN_NONE;
     int status;
     {
         const GilReleased released;
