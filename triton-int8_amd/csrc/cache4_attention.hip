@@ -110,8 +110,8 @@ __device__ __forceinline__ float over_rows(float x) {
 // the keys stay in for weights_kernel (8 streams of up to 131072 entries 120 us -> 113).  The next 32 entries' loads are in flight
 // meanwhile.  Four waves of a workgroup take turns and add up at the end, with their workgroups' neighbours through memory.
 //
-// Bound by memory where there are many entries: 8 streams of up to 131072 entries, 616 MB, 106 to 110 us = 5.6 to 5.8 TB/s (a large copy here: 4.95 TB/s
-// read and written).  A step over a few thousand
+// Bound by memory where there are many entries, and nearly by the issue of instructions: 8 streams of up to 131072 entries, 616 MB, 108 to 113 us = 5.5 to 5.7 TB/s (a large copy
+// here: 4.95 TB/s read and written); a SIMD issues in 0.84 of its cycles.  A step over a few thousand
 // entries is mostly the kernel's beginning and end: 8 heads of 1021 entries, shared out, 6.0 us (1.5 for the launch, 1.4 to find the units, 1.3 for the
 // first loads, 1.2 for the waves' sum) and 4.2 for the join.  Where tables are short every (sequence, head) is therefore left to one workgroup of eight
 // waves (see step_alone): 1.5 us for 256 entries, which is how long codes take to bf16, to LDS and through two products, one after the other
@@ -484,8 +484,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // A head's row blocks lie on one XCD, whose L2 then serves the entries; where there are too few row blocks for the chip, several workgroups share the
 // entries of one and join_rows_kernel adds them up.
 //
-// Bound by the issue of a SIMD, which products and exponentials share, at the clock that the chip's power allows: 2 x 2048 tokens of 32 heads behind 6144 entries
-// 456 to 470 us = 1.02 to 1.05 PFLOP/s (a matrix product of the library: 1.4 to 1.46).  Short prompts of several lengths: by the longest row block's
+// 2 x 2048 tokens of 32 heads behind 6144 entries 462 to 472 us = 1.02 to 1.04 PFLOP/s (a matrix product of the library: 1.4 to 1.46).  No unit is full: of the cycles the
+// matrix pipe has 0.42, the vector unit 0.44 (half of the former's beside the latter: 0.65 together), LDS 0.53, of which half are bank conflicts; waves
+// wait 0.37 of their time.  Short prompts of several lengths: bound by the longest row block's
 // chain of tiles (2 us each with 256 rows).
 
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -822,7 +823,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Args a, int64_t ro
 // its rows up in a fixed order; the sum goes to the weight as an atomic addition, because sequences with a common beginning may share its pages (then
 // the order of their additions is open, otherwise a weight gets one).
 //
-// Few rows: bound by the beginning and by memory (32 streams of 2048 entries of 8 heads: 39 MB in 15 us); many: by the issue of a SIMD, as prompt_kernel (8 x 1024 tokens
+// Few rows: bound by the beginning and by memory (32 streams of 2048 entries of 8 heads: 39 MB in 15 us); many: by the issue of a SIMD, 0.87 of its cycles (8 x 1024 tokens
 // over 4096 entries of 32 heads: 315 us = 0.76 PFLOP/s), and, with one or two units per workgroup, by the units that most rows see.  The loads to LDS
 // are global_load_lds: in front of every read of LDS the compiler waits for all buffer loads to LDS, also for those two tiles ahead (390 us).
 // Not taken: a step's exponentials beside the next scores' products in one wave (354 us: the waves of a SIMD overlap as it is, and registers are short);
@@ -1059,7 +1060,9 @@ int step_groups(const Cache& c, int tiles) {
 }
 // Whether every (sequence, head) is left to a workgroup of its own, which saves the join and the search for its entries, but nobody helps with a long
 // sequence (us, shared out / each its own; heads of 128, one token).  8 heads of 512 entries 10.6 / 7.8, of 1024 10.5 / 10.3, of 2048 10.8 / 16.7; 256 heads
-// of 1024 18.0 / 12.3, of 2048 23.6 / 19.6 (of 1 to 2048 17.5 / 18.0), of 1 to 4096 19.4 / 30.0; 128 heads of 2048 17.8 / 17.8; in two rounds, 512 heads of
+// of 1024 18.0 / 12.3, of 2048 23.6 / 19.6 (of 1 to 2048 17.5 / 18.0), of 2560 26.5 / 22.5 (of 1 to 2560 19.4 / 21.5), of 4096 34.6 / 31.9 (of 1 to 4096 19.4 / 30.5); 192 heads of 2560
+// 22.7 / 21.6, of 4096 28.6 / 31.0; 128 heads of 2048 17.8 / 17.8, of 2560 18.7 / 21.0.  So 2048 is where sequences of several lengths, and 128 heads, take as long either
+// way; the host sees the room alone, and full sequences of 256 heads beyond it would lose less than those of several lengths gain.  In two rounds, 512 heads of
 // 256 entries 15.1 / 11.2, of 512 18.0 / 16.1, of 1024 23.6 / 22.4 (of 1 to 1024 19.2 / 20.2)
 bool step_alone(const Cache& c, int tiles) {
     const int64_t pairs = (int64_t)c.batch * c.heads, room = device_cu_count() * (c.dim == 64 && tiles == 1 ? 2 : 1);      // (registers)
