@@ -559,6 +559,51 @@ int ti8_cache4_evict(const ti8_cache4* c, const int32_t* lengths, const int32_t*
                      int64_t keep, int64_t recent, int32_t* kept, int32_t* new_lengths, ti8_stream_t stream);
 
 /* ---------------------------------------------------------------------------------
+ * Tensors in 4 bits with shared scales ("mx4") and their product (no counterpart in the reference).
+ *   [rows][cols] elements.  A code is a 4-bit float (bit 3 the sign, magnitudes 0 .5 1 1.5 2 3 4 6), the even element in the low half of its byte; 32
+ *   neighbours of a row share a scale byte e, which stands for 2^(e - 127): e the smallest of 1 .. 252 with their largest magnitude at most 6 * 2^(e - 127)
+ *   (252 where there is none: what is beyond 1.5 * 2^127 counts as that), or 255 where one of them is an infinity or a NaN (their codes are zeros then, and they
+ *   stand for NaN).  An element is rounded to the nearest code, of two the even one.
+ *   A row takes whole tiles of 256 elements, zeros behind its end; tiles = (cols + 255) / 256:
+ *   codes   uint8 [rows][tiles * 128], rows ld bytes apart (a multiple of 16), 16-byte aligned
+ *   scales  uint8 [tiles][rows][8], tiles scale_ld bytes apart (a multiple of 8), 8-byte aligned */
+typedef struct {
+    void* codes;
+    void* scales;
+    int64_t ld, scale_ld;
+} ti8_mx4;
+/* x bf16 [rows][cols] (ldx, any alignment) quantised by its rows (by_rows: [rows][cols]), by its columns (by_columns: the transposed tensor [cols][rows]), or
+ * both from one read; either may be NULL. */
+int ti8_mx4_quant(const void* x, int64_t ldx, int64_t rows, int64_t cols, const ti8_mx4* by_rows, const ti8_mx4* by_columns, ti8_stream_t stream);
+/* y bf16 [rows][cols] (ldy): the values that the codes stand for, exactly */
+int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, void* y, int64_t ldy, ti8_stream_t stream);
+/* C[b] = A[b] B[b]^T, A [M][K] and B [N][K]: batch b of A is the rows from b * rows_a on of `a` (0: all batches share A), of B likewise; C bf16 (wide: float)
+ * [M][N], rows ldc and batches bsc elements apart.  Products and sums in fp32, rounded once.  K up to 2^22; behind K both operands hold zeros up to
+ * the end of the tile. */
+int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc,
+                    int64_t batch, int64_t M, int64_t N, int64_t K, int wide, ti8_stream_t stream);
+/* A decoder layer's step from one linear's output to the next one's operand: h = bf16(x + residual) (residual and h NULL: h is x), rstd = 1 / sqrt(mean(h^2) + eps)
+ * (float [rows]; the mean in 64 bits), y = bf16(bf16(h * rstd) * w), and y quantised: into 4 bits (mx4.codes not NULL), or into int8 codes q [rows][dim] with the
+ * arithmetic of ti8_quant_row (s, group 0 or 128, qflags and inv_mode as there).  h may be the memory of x or residual.
+ * dim a multiple of 8 up to 16384 (of 128 with q); x, residual, h and w 16-byte aligned, leading dimensions multiples of 8. */
+typedef struct {
+    const void* x; int64_t ldx;
+    const void* residual; int64_t ldr;
+    const void* w;
+    void* h; int64_t ldh;
+    float* rstd;
+    int64_t rows, dim;
+    double eps;
+    ti8_mx4 mx4;
+    int8_t* q; int64_t ldq;
+    float* s;
+    int group, qflags, inv_mode;
+} ti8_rmsnorm_quant_args;
+int ti8_rmsnorm_quant(const ti8_rmsnorm_quant_args* a, ti8_stream_t stream);
+/* y bf16 [rows][cols] (ldy) = q * s: what the codes of ti8_quant_row stand for, s [rows] (group 0) or [rows][cols / 128] (group 128); cols % 8 == 0 */
+int ti8_dequant_row(const int8_t* q, int64_t ldq, const float* s, int64_t rows, int64_t cols, int group, void* y, int64_t ldy, ti8_stream_t stream);
+
+/* ---------------------------------------------------------------------------------
  * Measurement aid (no counterpart in the reference; used by bench.py --probe mfma): a loop of nothing
  * but v_mfma_i32_32x32x32_i8 on `workgroups` workgroups of 8 waves, `iters` x 16 MFMAs per wave,
  * operands all zero or pseudo-random, optionally with the block-channel promotion's vector work

@@ -11,7 +11,7 @@ top-level shim of that name loads this package).
 """
 from . import _lib  # noqa: F401
 from . import (block_channel_bwd33, block_channel_fwd32, cache4, decoder, double_channel_bwd33, double_channel_fwd32,
-               double_channel_triton_bwd, double_channel_triton_fwd, fused_bwd33, fused_fwd32, graph, latency, linear, ops,
+               double_channel_triton_bwd, double_channel_triton_fwd, fused_bwd33, fused_fwd32, graph, latency, linear, mx4, ops,
                tilelang_block_channel_bwd, tilelang_block_channel_fwd)
 from ._common import calc_diff
 from ._lib import init, last_gemm_kernel
@@ -19,5 +19,6 @@ from .cache4 import Cache4
 from .decoder import DecoderLayer
 from .graph import GraphedStep
 from .linear import Int8Linear, Int8LinearFunction, linear_fwd_bwd
+from .mx4 import Mx4Linear
 
 __version__ = "0.1.0"

@@ -55,6 +55,17 @@ class Cache4(ctypes.Structure):
                 ("batch", _i64), ("table_pages", _i64), ("table_stride", _i64)]
 
 
+class Mx4(ctypes.Structure):
+    """ti8_mx4 of include/ti8.h."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("ld", _i64), ("scale_ld", _i64)]
+
+
+class RmsnormQuantArgs(ctypes.Structure):
+    """ti8_rmsnorm_quant_args of include/ti8.h."""
+    _fields_ = [("x", _vp), ("ldx", _i64), ("residual", _vp), ("ldr", _i64), ("w", _vp), ("h", _vp), ("ldh", _i64), ("rstd", _vp), ("rows", _i64), ("dim", _i64),
+                ("eps", ctypes.c_double), ("mx4", Mx4), ("q", _vp), ("ldq", _i64), ("s", _vp), ("group", _int), ("qflags", _int), ("inv_mode", _int)]
+
+
 # name -> argument types, in the order of include/ti8.h
 PROTOTYPES = {
     "ti8_quant_block": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
@@ -90,6 +101,11 @@ PROTOTYPES = {
     "ti8_cache4_read": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _vp, _vp, _vp],
     "ti8_cache4_attention": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _f32, _int, _vp, _vp, _vp, _i64, _vp],
     "ti8_cache4_evict": [ctypes.POINTER(Cache4), _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
+    "ti8_mx4_quant": [_vp, _i64, _i64, _i64, ctypes.POINTER(Mx4), ctypes.POINTER(Mx4), _vp],
+    "ti8_mx4_dequant": [ctypes.POINTER(Mx4), _i64, _i64, _vp, _i64, _vp],
+    "ti8_mx4_gemm_nt": [ctypes.POINTER(Mx4), _i64, ctypes.POINTER(Mx4), _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp],
+    "ti8_rmsnorm_quant": [ctypes.POINTER(RmsnormQuantArgs), _vp],
+    "ti8_dequant_row": [_vp, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp],
     "ti8_probe_mfma": [_vp, _i64, _vp, _int, _int, _int, _int, _vp],
 }
 EXPORTS = ["ti8_version", "ti8_last_error", "ti8_arch", "ti8_init", "ti8_last_gemm_kernel", "ti8_linear_fwd_bwd_workspace", "ti8_linear_workspace", "ti8_linear_group_workspace",

@@ -741,5 +741,27 @@ TI8_HD bool decode_narrow(int64_t N, int64_t K, int64_t rows, bool by_rows, int 
     return N / 16 <= num_cu && (rows <= 4 || (nk >= 24 && (!by_rows || nk <= 96)));
 }
 
+// ---- tensors in 4 bits with shared scales (mx4_quant.hip, mx4_gemm.hip) ------------------------------------------------------------------
+// A row takes whole tiles of 256 elements: 128 bytes of codes, 8 scales (one per 32 elements).
+constexpr int MX4_TILE = 256, MX4_TILE_BYTES = 128, MX4_TILE_SCALES = 8;
+TI8_HD int64_t mx4_tiles(int64_t cols) { return (cols + MX4_TILE - 1) / MX4_TILE; }
+TI8_HD int64_t mx4_code_at(int64_t row, int64_t ld, int64_t tile, int octet) { return row * ld + tile * MX4_TILE_BYTES + octet * 4; }
+TI8_HD int64_t mx4_scale_at(int64_t tile, int64_t scale_ld, int64_t row, int group) { return tile * scale_ld + row * MX4_TILE_SCALES + group; }
+
+// workgroup -> block of consecutive work, a contiguous range of it on every XCD
+TI8_HD int64_t xcd_range(int64_t block, int64_t blocks) {
+    const int64_t xcd = block & 7, rest = blocks & 7;
+    return xcd * (blocks >> 3) + (xcd < rest ? xcd : rest) + (block >> 3);
+}
+
+// quantiser by rows: 256 threads, a tile of 32 rows x 256 columns; thread t has octet t % 32 of rows t / 32 + 8 i, i < 4
+constexpr int MX4_ROW_BLOCK = 32;
+// quantiser by columns: waves of 32 rows x 256 columns; lane l has octet l % 32 of rows 16 (l / 32) .. + 15
+TI8_HD int mx4_col_chunk(int wave, int octet, int waves) { return wave ^ (octet & (waves - 1)); }     // where 16 bytes of a column lie in its LDS line
+
+// product: rows of an operand that a workgroup's loads go to stay within it
+TI8_HD int mx4_row(int row, int rows) { return row < rows ? row : rows - 1; }
+TI8_HD uint32_t mx4_chunk_swizzle(int row) { return (uint32_t)((row & 7) ^ ((row >> 3) & 1)); }
+
 }  // namespace idx
 }  // namespace ti8

@@ -674,6 +674,65 @@ def rmsnorm(x, weight, eps):
     return y, rstd
 
 
+def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV_RCP_OF_SCALE):
+    """``h = x + residual`` (bf16), ``y = bf16(h * rstd) * weight`` over the last dim and y quantised, in one pass: the step from a linear's output to the next one's operand.
+    ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
+    multiple of 8 (with "int8" of 128) up to 16384.
+
+    Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean in 64 bits: no code depends on an order of
+    summation.  Quantised tensors have no gradients: x, weight and residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and,
+    the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
+    _need(to in ("mx4", "int8"), f"`to` must be 'mx4' or 'int8', got {to!r}")
+    _need(group in (0, 128) and (group == 0 or to == "int8"), f"group must be 0 or, with 'int8', 128, got {group}")
+    for t, name in ((x, "x"), (weight, "weight")) + (() if residual is None else ((residual, "residual"),)):
+        _check_bf16(t, name)
+        _need(t.get_device() == torch._C._cuda_getDevice(), f"{name} must be on the current GPU")
+        _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a quantised tensor does not give: call this under torch.no_grad()")
+    dim = x.shape[-1] if x.dim() else 0
+    _need(x.numel() > 0 and dim % (8 if to == "mx4" else 128) == 0 and dim <= 16384,
+          f"x must be non-empty and its last dim a multiple of {8 if to == 'mx4' else 128} up to 16384, got {tuple(x.shape)}")
+    _need(tuple(weight.shape) == (dim,) and (residual is None or residual.shape == x.shape),
+          f"shapes do not fit: x {tuple(x.shape)}, weight {tuple(weight.shape)}" + ("" if residual is None else f", residual {tuple(residual.shape)}"))
+    lead = x.shape[:-1]
+    x2, r2 = rows16(x.reshape(-1, dim)), None if residual is None else rows16(residual.reshape(-1, dim))
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    rows, dev = x2.shape[0], x.device
+    _need(rows <= 1 << 28, f"up to 2^28 rows, got {rows}")
+    rstd = torch.empty(lead, dtype=torch.float32, device=dev)
+    h = None if residual is None else torch.empty((*lead, dim), dtype=torch.bfloat16, device=dev)
+    a = _lib.RmsnormQuantArgs(x=x2.data_ptr(), ldx=dim if rows == 1 else x2.stride(0), w=weight.data_ptr(), rstd=rstd.data_ptr(), rows=rows, dim=dim, eps=eps, group=group, inv_mode=inv_mode)
+    if residual is not None:
+        a.residual, a.ldr, a.h, a.ldh = r2.data_ptr(), dim if rows == 1 else r2.stride(0), h.data_ptr(), dim
+    if to == "mx4":
+        tiles = -(-dim // 256)
+        q, s = torch.empty((*lead, tiles * 128), dtype=torch.uint8, device=dev), torch.empty((tiles, rows, 8), dtype=torch.uint8, device=dev)
+        a.mx4 = _lib.Mx4(q.data_ptr(), s.data_ptr(), tiles * 128, rows * 8)
+    else:
+        q = torch.empty((*lead, dim), dtype=torch.int8, device=dev)
+        s = torch.empty((*lead, dim // 128) if group else lead, dtype=torch.float32, device=dev)
+        a.q, a.ldq, a.s, a.qflags = q.data_ptr(), dim, s.data_ptr(), Q_CLAMP
+    _lib.call("ti8_rmsnorm_quant", ctypes.byref(a), _stream())
+    return (q, s, rstd) if residual is None else (q, s, rstd, h)
+
+
+def dequant_row(q, s):
+    """bf16 [.., cols]: ``q * s``, what codes int8 [.., cols] of :func:`quant_row` with scales float32 [..] or, of groups of 128, [.., cols / 128] stand for."""
+    _need(isinstance(q, torch.Tensor) and isinstance(s, torch.Tensor) and _on_gpu(q) and _on_gpu(s) and q.get_device() == s.get_device() == torch._C._cuda_getDevice(),
+          "q and s must be tensors on the current GPU")
+    _need(q.dtype == torch.int8 and s.dtype == torch.float32 and q.dim() >= 1 and q.numel() > 0 and q.shape[-1] % 8 == 0,
+          f"q must be a non-empty int8 tensor whose last dim is a multiple of 8, s float32; got {tuple(q.shape)} {q.dtype}, {s.dtype}")
+    cols, lead = q.shape[-1], tuple(q.shape[:-1])
+    by_group = tuple(s.shape) != lead
+    _need(not by_group or (cols % 128 == 0 and tuple(s.shape) == (*lead, cols // 128)), f"scales {tuple(s.shape)} do not fit codes {tuple(q.shape)}")
+    q, s = q.contiguous(), s.contiguous()
+    if q.data_ptr() % 8:
+        q = q.clone()
+    y = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    _lib.call("ti8_dequant_row", q.data_ptr(), cols, s.data_ptr(), q.numel() // cols, cols, 128 if by_group else 0, y.data_ptr(), cols, _stream())
+    return y
+
+
 def rmsnorm_backward(dy, x, weight, rstd):
     """dx and the weight's gradient with the bits that autograd gives for the torch expression."""
     dx = torch.empty_like(x)
