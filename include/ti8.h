@@ -581,7 +581,10 @@ int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, void* y, int64
  * [M][N], rows ldc and batches bsc elements apart.  Products and sums in fp32, rounded once.  K up to 2^22; behind K both operands hold zeros up to
  * the end of the tile. */
 int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc,
-                    int64_t batch, int64_t M, int64_t N, int64_t K, int wide, ti8_stream_t stream);
+                    int64_t batch, int64_t M, int64_t N, int64_t K, int wide, void* workspace, int64_t workspace_bytes, ti8_stream_t stream);
+/* bytes of workspace that the call above needs (0: none; -1 for sizes it does not take), 16-byte aligned, contents undefined before and after: few tiles over a
+ * long K are shared among workgroups, whose parts are added up in order */
+int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K);
 /* A decoder layer's step from one linear's output to the next one's operand: h = bf16(x + residual) (residual and h NULL: h is x), rstd = 1 / sqrt(mean(h^2) + eps)
  * (float [rows]; the mean in 64 bits), y = bf16(bf16(h * rstd) * w), and y quantised: into 4 bits (mx4.codes not NULL), or into int8 codes q [rows][dim] with the
  * arithmetic of ti8_quant_row (s, group 0 or 128, qflags and inv_mode as there).  h may be the memory of x or residual.

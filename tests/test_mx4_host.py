@@ -35,7 +35,7 @@ def test_tensors_that_are_refused(lib, other, code, msg):
     refused(lib, "ti8_mx4_quant", code, msg, FAKE, 64, 512, 64, None, bad, None)
     refused(lib, "ti8_mx4_dequant", code, msg, bad, 64, 512, FAKE, 512, None)
     for a, b in ((bad, good), (good, bad)):
-        refused(lib, "ti8_mx4_gemm_nt", code, msg, a, 0, b, 0, FAKE, 64, 0, 1, 64, 64, 512, 0, None)
+        refused(lib, "ti8_mx4_gemm_nt", code, msg, a, 0, b, 0, FAKE, 64, 0, 1, 64, 64, 512, 0, None, 0, None)
     if other != dict(codes=None):
         refused(lib, "ti8_rmsnorm_quant", code, msg, norm(lib, dim=512, ldx=512, ldr=512, ldh=512, mx4=bad), None)
 
@@ -54,7 +54,7 @@ def test_quant(lib, args, code, msg):
     (dict(rows_a=64, batch=2), 2, "scale_ld"), (dict(c=FAKE + 1), 3, "aligned"), (dict(c=FAKE + 2, wide=1), 3, "aligned")], ids=str)
 def test_gemm(lib, change, code, msg):
     v = {**dict(rows_a=0, rows_b=0, c=FAKE, ldc=64, bsc=0, batch=1, M=64, N=64, K=512, wide=0), **change}
-    refused(lib, "ti8_mx4_gemm_nt", code, msg, mx(lib), v["rows_a"], mx(lib), v["rows_b"], v["c"], v["ldc"], v["bsc"], v["batch"], v["M"], v["N"], v["K"], v["wide"], None)
+    refused(lib, "ti8_mx4_gemm_nt", code, msg, mx(lib), v["rows_a"], mx(lib), v["rows_b"], v["c"], v["ldc"], v["bsc"], v["batch"], v["M"], v["N"], v["K"], v["wide"], None, 0, None)
 
 
 def norm(lib, **other):
@@ -90,7 +90,7 @@ def test_dequant_row(lib, args, code, msg):
 def test_missing_arguments_are_refused(lib):
     refused(lib, "ti8_rmsnorm_quant", 1, "required", None, None)
     refused(lib, "ti8_mx4_dequant", 1, "required", None, 64, 512, FAKE, 512, None)
-    refused(lib, "ti8_mx4_gemm_nt", 1, "required", None, 0, mx(lib), 0, FAKE, 64, 0, 1, 64, 64, 512, 0, None)
+    refused(lib, "ti8_mx4_gemm_nt", 1, "required", None, 0, mx(lib), 0, FAKE, 64, 0, 1, 64, 64, 512, 0, None, 0, None)
     refused(lib, "ti8_mx4_dequant", 2, "ldy", mx(lib), 64, 512, FAKE, 511, None)
     refused(lib, "ti8_mx4_dequant", 3, "aligned", mx(lib), 64, 512, FAKE + 1, 512, None)
 

@@ -763,5 +763,48 @@ TI8_HD int mx4_col_chunk(int wave, int octet, int waves) { return wave ^ (octet 
 TI8_HD int mx4_row(int row, int rows) { return row < rows ? row : rows - 1; }
 TI8_HD uint32_t mx4_chunk_swizzle(int row) { return (uint32_t)((row & 7) ^ ((row >> 3) & 1)); }
 
+// K tiles that part `p` of a contraction over nk takes (1 <= parts <= nk: none of them is empty)
+struct Mx4Part {
+    int first, tiles;
+};
+TI8_HD Mx4Part mx4_part(int p, int parts, int nk) {
+    const int each = nk / parts, more = nk % parts;
+    return {p * each + imin(p, more), each + (p < more ? 1 : 0)};
+}
+
+// Which kernel multiplies [M][K] and [N][K], K in nk tiles, and in how many parts along K.
+enum { MX4_FEW_16 = 0, MX4_FEW_32 = 1, MX4_TILES_32 = 2, MX4_TILES_64 = 3, MX4_TILES_128 = 4, MX4_TILES_128_TWO = 5, MX4_TILES_256 = 6 };
+struct Mx4Plan {
+    int kernel, parts;
+};
+// us that a round of `tiles` output tiles takes per K tile: `slots` of them have the chip full, up to `free` take no longer than one
+TI8_HD double mx4_rounds(int64_t tiles, int64_t slots, int64_t free, double one, double full) {
+    const int64_t rest = tiles % slots;
+    return (double)(tiles / slots) * full + (rest == 0 ? 0.0 : rest <= free ? one : one + (full - one) * (double)(rest - free) / (double)(slots - free));
+}
+TI8_HD Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t nk, int64_t batch, int cus) {
+    if (M <= 32 && (N + 15) / 16 * batch <= cus) return {M <= 16 ? MX4_FEW_16 : MX4_FEW_32, 1};
+    Mx4Plan best{MX4_TILES_256, 1};
+    double least = 1e30;
+    const auto consider = [&](int kernel, int64_t bm, int64_t bn, int64_t slots, int64_t free, double one, double full) {
+        const int64_t tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * batch;
+        for (int parts = 1; parts <= 8 && (parts == 1 || (nk >= 4 * parts && tiles * parts <= cus)); parts *= 2) {
+            double t = (double)((nk + parts - 1) / parts) * mx4_rounds(tiles * parts, slots, free, one, full);
+            if (parts > 1) t += 2.5 + (double)(batch * M * N) * (8.0 * parts + 2.0) / 4e6;
+            if (t < least) {
+                least = t;
+                best = {kernel, parts};
+            }
+        }
+    };
+    const int64_t c = cus;
+    if (M <= 64) consider(MX4_TILES_32, 32, 64, 2 * c, c, 0.29, 0.50);
+    consider(MX4_TILES_64, 64, 64, 2 * c, c, 0.31, 0.56);
+    consider(MX4_TILES_128, 128, 128, c, c, 0.61, 0.68);
+    consider(MX4_TILES_128_TWO, 128, 128, 2 * c, c, 0.75, 1.22);
+    consider(MX4_TILES_256, 256, 256, c, c / 4, 1.25, 2.10);
+    return best;
+}
+
 }  // namespace idx
 }  // namespace ti8

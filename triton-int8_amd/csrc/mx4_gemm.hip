@@ -19,6 +19,8 @@ struct Gemm {
     int64_t rows_a, rows_b;             // rows between batches
     int64_t ldc, bsc;
     int M, N, nk, tiles_m, tiles_n, wide;
+    int parts;                          // workgroups that share the contraction of a tile: C is then fp32, one after the other `part` elements apart
+    int64_t part;
 };
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -35,23 +37,48 @@ __device__ __forceinline__ v16f multiply(const v4i& b, const v4i& a, const v16f&
 #endif
 }
 
-// One BM x BN tile of C on WM x WN waves
-template <int BM, int BN, int WM, int WN>
+// Order of one step of a K tile: one LDS read and one load from memory, while there are any, behind each matrix instruction; nothing of another step among them.
+// (Left to itself the compiler reads a step's fragments right before it needs them: 8192 x 14336 x 4096 243 us.)
+template <int NMFMA, int NDS, int NVM>
+__device__ __forceinline__ void interleave() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int DS = (NDS + NMFMA - 1) / NMFMA, VM = (NVM + NMFMA - 1) / NMFMA;
+#pragma unroll
+    for (int q = 0; q < NMFMA; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (q * DS < NDS) __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
+        if (q * VM < NVM) __builtin_amdgcn_sched_group_barrier(0x020, VM, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS
+constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
+constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
+constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14
+
+template <int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int A_INSTR = BM / 8 / NW, B_INSTR = BN / 8 / NW, A_BYTES = BM * 128, B_BYTES = BN * 128;
+    constexpr int SA_INSTR = (BM / 32 + NW - 1) / NW, SB_INSTR = (BN / 32 + NW - 1) / NW, S_BYTES = (BM + BN) * 8, RING = scale_stages(STAGES);
+    constexpr bool WHOLE = TM * TN <= 2;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     uint8_t* const ldsA = smem;
-    uint8_t* const ldsB = smem + 2 * A_BYTES;
+    uint8_t* const ldsB = smem + STAGES * A_BYTES;
+    uint8_t* const ldsS = ldsB + STAGES * B_BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     const idx::TileCoord tc = idx::gemm_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, idx::gemm_group_rows(BM), false);
     const int m0 = tc.tile_m * BM, n0 = tc.tile_n * BN;
     const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
     const int rows_a = min(g.M - m0, BM), rows_b = min(g.N - n0, BN);
 
+    const idx::Mx4Part part = idx::mx4_part(blockIdx.y, g.parts, g.nk);
+    const int last = part.tiles - 1;
     // global -> LDS: an instruction of a wave covers 8 rows, lane l lands at byte 16 l of them; rows beyond the operand repeat its last
-    const uint8_t *at_a = g.A + first_a * g.lda, *at_b = g.B + first_b * g.ldb;
+    const uint8_t *at_a = g.A + first_a * g.lda + part.first * 128, *at_b = g.B + first_b * g.ldb + part.first * 128;
     uint32_t off_a[A_INSTR], off_b[B_INSTR];
 #pragma unroll
     for (int i = 0; i < A_INSTR; ++i) {
@@ -63,19 +90,40 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
         const int r = (wave * B_INSTR + i) * 8 + (lane >> 3);
         off_b[i] = (uint32_t)(idx::mx4_row(r, rows_b) * (int)g.ldb) + (((uint32_t)(lane & 7) ^ idx::mx4_chunk_swizzle(r)) * 16);
     }
-    const auto issue = [&](int kt, int buf) {
-        const uint8_t *a = at_a + (int64_t)kt * 128, *b = at_b + (int64_t)kt * 128;
+    constexpr int LOADS = A_INSTR + B_INSTR, FIRST = LOADS / 2;
+    const auto issue = [&](int kt, int stage, int from, int to) {
+        const uint8_t *a = at_a + (int64_t)min(kt, last) * 128, *b = at_b + (int64_t)min(kt, last) * 128;
 #pragma unroll
-        for (int i = 0; i < A_INSTR; ++i) {
-            uint32_t o = off_a[i];
+        for (int i = 0; i < LOADS; ++i) {
+            if (i < from || i >= to) continue;
+            const bool of_a = i < A_INSTR;
+            uint32_t o = of_a ? off_a[of_a ? i : 0] : off_b[of_a ? 0 : i - A_INSTR];
+            asm volatile("" : "+v"(o));     // (a uniform address and a 32-bit offset, not a sum in 64 bits)
+            if (of_a) __builtin_amdgcn_global_load_lds(a + o, ldsA + stage * A_BYTES + (wave * A_INSTR + i) * 1024, 16, 0, 0);
+            else __builtin_amdgcn_global_load_lds(b + o, ldsB + stage * B_BYTES + (wave * B_INSTR + i - A_INSTR) * 1024, 16, 0, 0);
+        }
+    };
+    // scales of a tile: 32 rows to an instruction, lane l lands at byte 4 l of their 256
+    const uint8_t *scales_a = g.SA + first_a * 8 + part.first * g.sla, *scales_b = g.SB + first_b * 8 + part.first * g.slb;
+    uint32_t soff_a[SA_INSTR], soff_b[SB_INSTR];
+#pragma unroll
+    for (int i = 0; i < SA_INSTR; ++i) soff_a[i] = idx::mx4_row((wave + i * NW) % (BM / 32) * 32 + (lane >> 1), rows_a) * 8 + (lane & 1) * 4;
+#pragma unroll
+    for (int i = 0; i < SB_INSTR; ++i) soff_b[i] = idx::mx4_row((wave + i * NW) % (BN / 32) * 32 + (lane >> 1), rows_b) * 8 + (lane & 1) * 4;
+    const auto issue_scales = [&](int kt) {
+        const uint8_t *a = scales_a + min(kt, last) * g.sla, *b = scales_b + min(kt, last) * g.slb;
+        uint8_t* const slot = ldsS + kt % RING * S_BYTES;
+#pragma unroll
+        for (int i = 0; i < SA_INSTR; ++i) {
+            uint32_t o = soff_a[i];
             asm volatile("" : "+v"(o));
-            __builtin_amdgcn_global_load_lds(a + o, ldsA + buf * A_BYTES + (wave * A_INSTR + i) * 1024, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(a + o, slot + (wave + i * NW) % (BM / 32) * 256, 4, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < B_INSTR; ++i) {
-            uint32_t o = off_b[i];
+        for (int i = 0; i < SB_INSTR; ++i) {
+            uint32_t o = soff_b[i];
             asm volatile("" : "+v"(o));
-            __builtin_amdgcn_global_load_lds(b + o, ldsB + buf * B_BYTES + (wave * B_INSTR + i) * 1024, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(b + o, slot + BM * 8 + (wave + i * NW) % (BN / 32) * 256, 4, 0, 0);
         }
     };
 
@@ -86,12 +134,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) chunk[ks] = ((half * 4 + ks) ^ sw) * 16;
     const uint8_t *frag_a = ldsA + (wm * TM * 32 + row) * 128, *frag_b = ldsB + (wn * TN * 32 + row) * 128;
-    const uint8_t *scales_a = g.SA + first_a * 8, *scales_b = g.SB + first_b * 8;
-    uint32_t soff_a[TM], soff_b[TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) soff_a[i] = idx::mx4_row((wm * TM + i) * 32 + row, rows_a) * 8 + half * 4;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) soff_b[j] = idx::mx4_row((wn * TN + j) * 32 + row, rows_b) * 8 + half * 4;
+    const uint8_t *scale_a = ldsS + (wm * TM * 32 + row) * 8 + half * 4, *scale_b = ldsS + BM * 8 + (wn * TN * 32 + row) * 8 + half * 4;
 
     v16f acc[TM][TN];
 #pragma unroll
@@ -102,50 +145,122 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     v4i a[2][TM], b[2][TN];
     int sa[TM], sb[TN], na[TM], nb[TN];
-    const auto frags = [&](int set, int buf, int ks) {
+    const auto frags = [&](int set, int stage, int ks) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[set][i] = *reinterpret_cast<const v4i*>(frag_a + buf * A_BYTES + i * 4096 + chunk[ks]);
+        for (int i = 0; i < TM; ++i) a[set][i] = *reinterpret_cast<const v4i*>(frag_a + stage * A_BYTES + i * 4096 + chunk[ks]);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) b[set][j] = *reinterpret_cast<const v4i*>(frag_b + buf * B_BYTES + j * 4096 + chunk[ks]);
+        for (int j = 0; j < TN; ++j) b[set][j] = *reinterpret_cast<const v4i*>(frag_b + stage * B_BYTES + j * 4096 + chunk[ks]);
     };
     const auto scales = [&](int kt) {
-        const uint8_t *pa = scales_a + kt * g.sla, *pb = scales_b + kt * g.slb;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) na[i] = *reinterpret_cast<const int*>(pa + soff_a[i]);
+        for (int i = 0; i < TM; ++i) na[i] = *reinterpret_cast<const int*>(scale_a + kt % RING * S_BYTES + i * 256);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) nb[j] = *reinterpret_cast<const int*>(pb + soff_b[j]);
+        for (int j = 0; j < TN; ++j) nb[j] = *reinterpret_cast<const int*>(scale_b + kt % RING * S_BYTES + j * 256);
     };
 
-    const int last = g.nk - 1;
-    scales(0);
-    issue(0, 0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    issue(min(1, last), 1);
-    frags(0, 0, 0);
-    for (int kt = 0; kt <= last; ++kt) {
-        const int cur = kt & 1;
+    constexpr int SCALE_LOADS = SA_INSTR + SB_INSTR;
+    if constexpr (WHOLE) {
+        // Few matrix instructions to a tile: all of the next tile's fragments are read beside them (a step at a time every step waits for LDS; 64 x 4096 x 4096
+        // 7.1 us).  Tile kt + STAGES is asked for once everybody has tile kt in registers.
+        constexpr int BEHIND = (STAGES - 2) * (LOADS + SCALE_LOADS);
+        static_assert((STAGES - 1) * (LOADS + SCALE_LOADS) < 64 && RING >= STAGES, "vmcnt has six bits");
+        v4i wa[2][TM][4], wb[2][TN][4];
+        int ws[2][TM], wt[2][TN];
+        const auto read = [&](int set, int stage, int kt) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) sa[i] = na[i];
+            for (int i = 0; i < TM; ++i) ws[set][i] = *reinterpret_cast<const int*>(scale_a + kt % RING * S_BYTES + i * 256);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) sb[j] = nb[j];
-        scales(min(kt + 1, last));
-#define TI8_STEP(KS)                                                                                                          \
+            for (int j = 0; j < TN; ++j) wt[set][j] = *reinterpret_cast<const int*>(scale_b + kt % RING * S_BYTES + j * 256);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) wa[set][i][ks] = *reinterpret_cast<const v4i*>(frag_a + stage * A_BYTES + i * 4096 + chunk[ks]);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) wb[set][j][ks] = *reinterpret_cast<const v4i*>(frag_b + stage * B_BYTES + j * 4096 + chunk[ks]);
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < STAGES; ++t) {
+            issue(t, t, 0, LOADS);
+            issue_scales(t);
+        }
+        __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 1) * (LOADS + SCALE_LOADS), 0x70));
+        asm volatile("s_barrier" ::: "memory");
+        read(0, 0, 0);
+        int cur = 0, kt = 0;
+#define TI8_STEP(KS, SET)                                                                                                     \
     _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j) acc[i][j] =                 \
-        multiply<KS>(b[KS & 1][j], a[KS & 1][i], acc[i][j], sb[j], sa[i]);
-        frags(1, cur, 1);
-        TI8_STEP(0)
-        frags(0, cur, 2);
-        TI8_STEP(1)
-        frags(1, cur, 3);
-        TI8_STEP(2)
-        // the next tile and its scales are there, and nobody reads this one any more (its last fragments are in registers)
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        issue(min(kt + 2, last), cur);
-        frags(0, cur ^ 1, 0);
-        TI8_STEP(3)
+        multiply<KS>(wb[SET][j][KS], wa[SET][i][KS], acc[i][j], wt[SET][j], ws[SET][i]);
+#define TI8_TILE(SET)                                                                                                         \
+    {                                                                                                                         \
+        const int next = cur + 1 == STAGES ? 0 : cur + 1;                                                                     \
+        __builtin_amdgcn_s_waitcnt(waitcnt(BEHIND, 0x70));                                                                    \
+        asm volatile("s_barrier" ::: "memory");                                                                               \
+        issue(kt + STAGES, cur, 0, LOADS);                                                                                    \
+        issue_scales(kt + STAGES);                                                                                            \
+        read(1 - SET, next, kt + 1);                                                                                          \
+        __builtin_amdgcn_sched_barrier(0);                                                                                    \
+        TI8_STEP(0, SET) TI8_STEP(1, SET) TI8_STEP(2, SET) TI8_STEP(3, SET)                                                   \
+        __builtin_amdgcn_sched_barrier(0);                                                                                    \
+        cur = next;                                                                                                           \
+        ++kt;                                                                                                                 \
+    }
+        for (;;) {
+            TI8_TILE(0)
+            if (kt > last) break;
+            TI8_TILE(1)
+            if (kt > last) break;
+        }
+#undef TI8_TILE
 #undef TI8_STEP
+    } else {
+        // Codes of tile kt + STAGES are asked for once tile kt has been read, half of them a step later, scales of tile kt + STAGES + 1 before that.  What may be on its
+        // way when a tile's third step ends, behind the last codes of the next one: those of STAGES - 2 tiles and scales of STAGES - 1.  (Loads past the last tile
+        // repeat it: no branches in the loop.)
+        constexpr int BEHIND = (STAGES - 2) * LOADS + (STAGES - 1) * SCALE_LOADS;
+        static_assert(BEHIND < 64, "vmcnt has six bits");
+#pragma unroll
+        for (int t = 0; t <= STAGES; ++t) issue_scales(t);
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t) issue(t, t, 0, LOADS);
+        issue(STAGES - 1, STAGES - 1, 0, FIRST);
+        __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 2) * LOADS + FIRST, 0x70));
+        asm volatile("s_barrier" ::: "memory");
+        frags(0, 0, 0);
+        scales(0);
+        int cur = 0, fill = STAGES - 1;       // stages of tile kt and of the one that is being fetched
+        for (int kt = 0; kt <= last; ++kt) {
+            const int next = cur + 1 == STAGES ? 0 : cur + 1;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sa[i] = na[i];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) sb[j] = nb[j];
+#define TI8_STEP(KS)                                                                                                          \
+        _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j) acc[i][j] =                 \
+            multiply<KS>(b[KS & 1][j], a[KS & 1][i], acc[i][j], sb[j], sa[i]);
+            frags(1, cur, 1);
+            issue(kt + STAGES - 1, fill, FIRST, LOADS);
+            TI8_STEP(0)
+            interleave<TM * TN, TM + TN, LOADS - FIRST>();
+            frags(0, cur, 2);
+            issue_scales(kt + STAGES + 1);
+            TI8_STEP(1)
+            interleave<TM * TN, TM + TN, SCALE_LOADS>();
+            frags(1, cur, 3);
+            TI8_STEP(2)
+            interleave<TM * TN, TM + TN, 0>();
+            // the next tile is there, and nobody reads this one any more (its last fragments are in registers)
+            __builtin_amdgcn_s_waitcnt(waitcnt(BEHIND, 0x70));       // lgkmcnt(0)
+            asm volatile("s_barrier" ::: "memory");                  // (not __syncthreads(), which would wait for all loads)
+            issue(kt + STAGES, cur, 0, FIRST);
+            frags(0, next, 0);
+            scales(kt + 1);
+            TI8_STEP(3)
+            interleave<TM * TN, 2 * (TM + TN), FIRST>();
+#undef TI8_STEP
+            fill = cur;
+            cur = next;
+        }
     }
     __builtin_amdgcn_s_waitcnt(0);      // (loads past the last tile, repeated into LDS)
     __syncthreads();
@@ -153,7 +268,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
     // lane: row m = l % 32 of a 32 x 32 block of C, columns 8 (r / 4) + 4 (l / 32) + r % 4
     const int cols = g.N - n0 - wn * TN * 32;
     if (g.wide) {
-        float* const C = static_cast<float*>(g.C) + blockIdx.z * g.bsc + n0 + wn * TN * 32;
+        float* const C = static_cast<float*>(g.C) + blockIdx.y * g.part + blockIdx.z * g.bsc + n0 + wn * TN * 32;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int m = m0 + (wm * TM + i) * 32 + row;
@@ -178,7 +293,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
     }
     // through LDS, a wave's 32 rows at a time, so that a row is written in one piece
     constexpr int WIDTH = TN * 32, PITCH = WIDTH * 2 + 16, LPR = WIDTH / 8, RPI = 64 / LPR;
-    static_assert(32 * PITCH * NW <= 2 * (A_BYTES + B_BYTES), "the waves' rows fit the operands' buffers");
+    static_assert(32 * PITCH * NW <= STAGES * (A_BYTES + B_BYTES), "the waves' rows fit the operands' buffers");
     uint8_t* const mine = smem + wave * 32 * PITCH;
     uint16_t* const C = static_cast<uint16_t*>(g.C) + blockIdx.z * g.bsc + n0 + wn * WIDTH;
     const int n = (lane % LPR) * 8;
@@ -202,17 +317,166 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
 #endif
 }
 
-template <int BM, int BN, int WM, int WN>
-int launch(const char* fn, Gemm g, int64_t batch, hipStream_t st) {
-    constexpr int LDS = 2 * (BM + BN) * 128;
+// Few rows of A: the weight passes once from memory straight into registers.  A workgroup has 16 NB rows of B and 16 MB of A, its waves take turns at the K
+// tiles and add up their parts in LDS, in order.  v_mfma_scale_f32_16x16x128_f8f6f4: lane l supplies row l % 16 and 32 of 128 elements, chunk l / 16 of each half
+// of a tile, so that four lanes read 64 bytes of a row in one piece.
+__device__ __forceinline__ v4f multiply16(const v4i& b, const v4i& a, const v4f& c, int sb, int sa) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1),
+                                                            __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1), c, 4, 4, 0, sb, 0, sa);
+#else
+    (void)b; (void)a; (void)sb; (void)sa;
+    return c;
+#endif
+}
+
+template <int MB, int NB, int NW>
+__global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemm g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int BLOCK = MB * NB * 256;        // elements of C here
+    extern __shared__ __attribute__((aligned(16))) float parts[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * MB);
+    const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
+    const uint8_t *pa[MB], *pb[NB], *qa[MB], *qb[NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+        const int64_t r = first_a + idx::mx4_row(i * 16 + row, g.M - m0);
+        pa[i] = g.A + r * g.lda + q * 16;
+        qa[i] = g.SA + r * 8;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int64_t r = first_b + idx::mx4_row(j * 16 + row, g.N - n0);
+        pb[j] = g.B + r * g.ldb + q * 16;
+        qb[j] = g.SB + r * 8;
+    }
+    struct Set {
+        v4i a[MB][2], b[NB][2];
+        uint2 sa[MB], sb[NB];
+    };
+    const auto load = [&](Set& s, int kt) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            s.b[j][0] = *reinterpret_cast<const v4i*>(pb[j] + kt * 128);
+            s.b[j][1] = *reinterpret_cast<const v4i*>(pb[j] + kt * 128 + 64);
+            s.sb[j] = *reinterpret_cast<const uint2*>(qb[j] + kt * g.slb);
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+            s.a[i][0] = *reinterpret_cast<const v4i*>(pa[i] + kt * 128);
+            s.a[i][1] = *reinterpret_cast<const v4i*>(pa[i] + kt * 128 + 64);
+            s.sa[i] = *reinterpret_cast<const uint2*>(qa[i] + kt * g.sla);
+        }
+    };
+    v4f acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto product = [&](const Set& s) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = multiply16(s.b[j][0], s.a[i][0], acc[i][j], s.sb[j].x >> (8 * q), s.sa[i].x >> (8 * q));
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = multiply16(s.b[j][1], s.a[i][1], acc[i][j], s.sb[j].y >> (8 * q), s.sa[i].y >> (8 * q));
+    };
+    // two tiles of a wave on their way at a time
+    Set even, odd;
+    int kt = wave;
+    if (kt < g.nk) load(even, kt);
+    while (kt < g.nk) {
+        if (kt + NW < g.nk) load(odd, kt + NW);
+        product(even);
+        kt += NW;
+        if (kt >= g.nk) break;
+        if (kt + NW < g.nk) load(even, kt + NW);
+        product(odd);
+        kt += NW;
+    }
+    // lane: row m = l % 16 of a 16 x 16 block of C, columns 4 (l / 16) .. + 3: blocks of C in LDS as [wave][i][m][16 NB columns]
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) *reinterpret_cast<v4f*>(parts + wave * BLOCK + (i * 16 + row) * (16 * NB) + j * 16 + q * 4) = acc[i][j];
+    __syncthreads();
+    for (int e = threadIdx.x * 4; e < BLOCK; e += 64 * NW * 4) {
+        v4f sum = *reinterpret_cast<const v4f*>(parts + e);
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+            const v4f x = *reinterpret_cast<const v4f*>(parts + w * BLOCK + e);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += x[c];
+        }
+        const int m = m0 + e / (16 * NB), n = n0 + e % (16 * NB);
+        if (m >= g.M) break;
+        const int64_t at = blockIdx.z * g.bsc + m * g.ldc + n;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (n + c >= g.N) break;
+            if (g.wide) static_cast<float*>(g.C)[at + c] = sum[c];
+            else static_cast<uint16_t*>(g.C)[at + c] = (uint16_t)f32_to_bf16_bits(sum[c]);
+        }
+    }
+#else
+    (void)g;
+#endif
+}
+
+template <int MB, int NB, int NW>
+int launch_few(const char* fn, const Gemm& g, int64_t batch, hipStream_t st) {
+    constexpr int LDS = MB * NB * 1024 * NW;
     static OncePerDevice once;
-    const auto kernel = gemm_kernel<BM, BN, WM, WN>;
+    const auto kernel = few_rows_kernel<MB, NB, NW>;
+    if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
+    kernel<<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB)), (unsigned)((g.M + 16 * MB - 1) / (16 * MB)), (unsigned)batch), dim3(64 * NW), LDS, st>>>(g);
+    return check_launch(fn);
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES>
+int launch(const char* fn, Gemm g, int64_t batch, hipStream_t st) {
+    constexpr int LDS = gemm_lds(BM, BN, STAGES);
+    static_assert(LDS <= 160 * 1024, "LDS of a CU");
+    static OncePerDevice once;
+    const auto kernel = gemm_kernel<BM, BN, WM, WN, STAGES>;
     if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
     g.tiles_m = (g.M + BM - 1) / BM;
     g.tiles_n = (g.N + BN - 1) / BN;
     if ((int64_t)g.tiles_m * g.tiles_n > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(g);
+    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(g);
     return check_launch(fn);
+}
+
+// The parts of a contraction added up in order: [parts][batch][M][N] in fp32 -> C
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ from, int parts, int64_t part, int64_t rows, int M, int N, void* C, int64_t ldc, int64_t bsc, int wide) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int64_t quads = (N + 3) >> 2, at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / quads;
+    if (row >= rows) return;
+    const int n = (int)(at - row * quads) * 4, left = N - n;
+    typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* p = from + row * N + n;
+    for (int s = 0; s < parts; ++s, p += part) {
+        v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (left >= 4) {
+            x = *reinterpret_cast<const v4f_any*>(p);
+        } else {
+            for (int c = 0; c < left; ++c) x[c] = p[c];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += x[c];
+    }
+    const int64_t to = row / M * bsc + row % M * ldc + n;
+    for (int c = 0; c < 4 && c < left; ++c) {
+        if (wide) static_cast<float*>(C)[to + c] = sum[c];
+        else static_cast<uint16_t*>(C)[to + c] = (uint16_t)f32_to_bf16_bits(sum[c]);
+    }
+#else
+    (void)from; (void)parts; (void)part; (void)rows; (void)M; (void)N; (void)C; (void)ldc; (void)bsc; (void)wide;
+#endif
 }
 
 }  // namespace
@@ -221,8 +485,14 @@ int launch(const char* fn, Gemm g, int64_t batch, hipStream_t st) {
 
 using namespace ti8;
 
+extern "C" int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || batch > 65535 || M > (1 << 28) || N > (1 << 28) || K > (1 << 22)) return -1;
+    const idx::Mx4Plan plan = idx::mx4_plan(M, N, idx::mx4_tiles(K), batch, device_cu_count());
+    return plan.parts > 1 ? plan.parts * batch * M * N * 4 : 0;
+}
+
 extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc, int64_t batch, int64_t M, int64_t N,
-                               int64_t K, int wide, ti8_stream_t stream) {
+                               int64_t K, int wide, void* workspace, int64_t workspace_bytes, ti8_stream_t stream) {
     const char* const fn = "ti8_mx4_gemm_nt";
     if (!a || !b || !c) return fail(TI8_ERR_NULL, "%s: a, b and c are required", fn);
     if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || batch > 65535 || M > (1 << 28) || N > (1 << 28) || K > (1 << 22) || ldc < N || bsc < 0 || (rows_a != 0 && rows_a < M) ||
@@ -235,6 +505,32 @@ extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* 
     if (int e = mx4::check(fn, "b", b, (batch - 1) * rows_b + N, K, tb)) return e;
     if (ta.ld > (1 << 22) || tb.ld > (1 << 22)) return fail(TI8_ERR_SHAPE, "%s: rows of codes may be up to 2^22 bytes apart", fn);
     if (reinterpret_cast<uintptr_t>(c) & (wide ? 3 : 1)) return fail(TI8_ERR_ALIGN, "%s: c must be aligned to its elements", fn);
-    const mx4::Gemm g{ta.codes, tb.codes, ta.scales, tb.scales, c, ta.ld, tb.ld, ta.scale_ld, tb.scale_ld, rows_a, rows_b, ldc, bsc, (int)M, (int)N, (int)idx::mx4_tiles(K), 0, 0, wide ? 1 : 0};
-    return mx4::launch<128, 128, 2, 2>(fn, g, batch, static_cast<hipStream_t>(stream));
+    const idx::Mx4Plan plan = idx::mx4_plan(M, N, idx::mx4_tiles(K), batch, device_cu_count());
+    const int64_t need = plan.parts > 1 ? plan.parts * batch * M * N * 4 : 0;
+    if (need && (!workspace || workspace_bytes < need)) return fail(TI8_ERR_NULL, "%s: a workspace of %lld bytes is required", fn, (long long)need);
+    if (need && !aligned16(workspace)) return fail(TI8_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
+    mx4::Gemm g{ta.codes, tb.codes, ta.scales, tb.scales, c, ta.ld, tb.ld, ta.scale_ld, tb.scale_ld, rows_a, rows_b, ldc, bsc, (int)M, (int)N, (int)idx::mx4_tiles(K), 0, 0, wide ? 1 : 0, plan.parts, 0};
+    if (need) {
+        g.C = workspace;
+        g.wide = 1;
+        g.ldc = N;
+        g.bsc = M * N;
+        g.part = batch * M * N;
+    }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    int e = TI8_OK;
+    switch (plan.kernel) {
+        case idx::MX4_FEW_16: e = mx4::launch_few<1, 1, 8>(fn, g, batch, st); break;
+        case idx::MX4_FEW_32: e = mx4::launch_few<2, 1, 8>(fn, g, batch, st); break;
+        case idx::MX4_TILES_32: e = mx4::launch<32, 64, 1, 2, 4>(fn, g, batch, st); break;
+        case idx::MX4_TILES_64: e = mx4::launch<64, 64, 2, 2, 4>(fn, g, batch, st); break;
+        case idx::MX4_TILES_128: e = mx4::launch<128, 128, 2, 2, 3>(fn, g, batch, st); break;
+        case idx::MX4_TILES_128_TWO: e = mx4::launch<128, 128, 2, 2, 2>(fn, g, batch, st); break;
+        default: e = mx4::launch<256, 256, 2, 4, 2>(fn, g, batch, st); break;
+    }
+    if (e || !need) return e;
+    const int64_t blocks = (batch * M * ((N + 3) / 4) + 255) / 256;
+    if (blocks > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    mx4::join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float*>(workspace), plan.parts, g.part, batch * M, (int)M, (int)N, c, ldc, bsc, wide ? 1 : 0);
+    return check_launch(fn);
 }

@@ -1,4 +1,4 @@
-// The host side of a layer call (ops.linear_call) and of the calls on the 4-bit cache (cache4.py) as one Python call each: outputs, workspace and argument
+// The host side of a layer call (ops.linear_call), of the calls on the 4-bit cache (cache4.py) and of those on tensors in 4 bits (mx4.py) as one Python call each: outputs, workspace and argument
 // block, then the library's entry points.  It makes the same allocations and calls as the Python that it stands in for.  Calls with anything out of the ordinary
 // (subclasses of Tensor, other dtypes, tensors that are not on a GPU) return None and take the Python way, which says what is wrong.
 #define PY_SSIZE_T_CLEAN
@@ -28,6 +28,12 @@ decltype(&ti8_cache4_read) cache4_read_entry = nullptr;
 decltype(&ti8_cache4_attention) cache4_attention_entry = nullptr;
 decltype(&ti8_cache4_attention_workspace) cache4_attention_workspace = nullptr;
 decltype(&ti8_cache4_evict) cache4_evict_entry = nullptr;
+decltype(&ti8_mx4_quant) mx4_quant_entry = nullptr;
+decltype(&ti8_mx4_dequant) mx4_dequant_entry = nullptr;
+decltype(&ti8_mx4_gemm_nt) mx4_gemm_entry = nullptr;
+decltype(&ti8_mx4_gemm_nt_workspace) mx4_gemm_workspace = nullptr;
+decltype(&ti8_rmsnorm_quant) rmsnorm_quant_entry = nullptr;
+decltype(&ti8_dequant_row) dequant_row_entry = nullptr;
 PyObject* parameter_class = nullptr;
 
 // *out = the tensor behind `o` (undefined for None); false if it is not a plain tensor
@@ -335,6 +341,218 @@ PyObject* cache4_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- tensors in 4 bits: every function returns None for what mx4.py (ops.py) has to look at, else what its call returns, or (name, status) -------------
+
+constexpr int64_t MX4_ROWS = 1 << 28, MX4_CONTRACTED = 1 << 22;
+
+bool on(const at::Tensor& t, at::ScalarType type, c10::DeviceIndex device) {
+    return t.defined() && t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.numel() > 0;
+}
+bool at_multiple(const at::Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
+
+// room for a tensor in 4 bits
+struct Mx4Out {
+    at::Tensor codes, scales;
+    ti8_mx4 mx = {};
+    Mx4Out() = default;
+    Mx4Out(at::IntArrayRef lead, int64_t rows, int64_t cols, const at::TensorOptions& bytes) {
+        const int64_t tiles = (cols + 255) / 256;
+        std::vector<int64_t> sizes(lead.begin(), lead.end());
+        sizes.push_back(tiles * 128);
+        codes = at::empty(sizes, bytes);
+        scales = at::empty({tiles, rows, 8}, bytes);
+        mx = ti8_mx4{codes.data_ptr(), scales.data_ptr(), tiles * 128, rows * 8};
+    }
+};
+
+// codes [rows][bytes] or [batch][rows][bytes] with their scales, where they are read in place
+bool mx4_operand(const at::Tensor& codes, const at::Tensor& scales, c10::DeviceIndex device, ti8_mx4* mx) {
+    if (!on(codes, at::kByte, device) || !on(scales, at::kByte, device) || (codes.dim() != 2 && codes.dim() != 3) || scales.dim() != 3) return false;
+    const int64_t bytes = codes.size(-1), rows = codes.numel() / bytes, tiles = bytes / 128;
+    if (bytes % 128 || scales.size(0) != tiles || scales.size(1) != rows || scales.size(2) != 8 || !at_multiple(codes, 16) || !at_multiple(scales, 8)) return false;
+    int64_t ld = bytes, scale_ld = rows * 8;
+    if (!codes.is_contiguous()) {
+        if (codes.dim() != 2 || codes.stride(1) != 1 || codes.stride(0) % 16 || codes.stride(0) < bytes) return false;
+        ld = codes.stride(0);
+    }
+    if (!scales.is_contiguous()) {
+        if (scales.stride(2) != 1 || (rows > 1 && scales.stride(1) != 8) || (tiles > 1 && (scales.stride(0) % 8 || scales.stride(0) < rows * 8))) return false;
+        if (tiles > 1) scale_ld = scales.stride(0);
+    }
+    *mx = ti8_mx4{codes.data_ptr(), scales.data_ptr(), ld, scale_ld};
+    return true;
+}
+
+// mx4_quant(x [.., cols], by rows, by columns (x a matrix), stream) -> [codes, scales] or [codes, scales, codes, scales]
+PyObject* mx4_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor x;
+    at::Tensor* const tensors[] = {&x};
+    int64_t by_rows, by_columns, stream;
+    if (nargs != 4 || !tensors_of(args, tensors, 1) || !number(args[1], &by_rows) || !number(args[2], &by_columns) || !number(args[3], &stream)) Py_RETURN_NONE;
+    if (!on(x, at::kBFloat16, current_device()) || x.dim() < 1 || (x.dim() != 2 && (by_columns || !x.is_contiguous()))) Py_RETURN_NONE;
+    const int64_t C = x.size(-1), R = x.numel() / C, ldx = x.dim() != 2 || R == 1 ? C : x.stride(0);
+    if (x.stride(-1) != 1 || ldx < C || R > MX4_ROWS || C > MX4_ROWS) Py_RETURN_NONE;
+    Mx4Out rows, cols;
+    int status;
+    {
+        const GilReleased released;
+        const auto bytes = at::TensorOptions().dtype(at::kByte).device(x.device());
+        if (by_rows) rows = Mx4Out(x.sizes().slice(0, x.dim() - 1), R, C, bytes);
+        if (by_columns) cols = Mx4Out({C}, C, R, bytes);
+        status = mx4_quant_entry(x.data_ptr(), ldx, R, C, by_rows ? &rows.mx : nullptr, by_columns ? &cols.mx : nullptr, stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_quant", status);
+    if (by_rows && by_columns) return Py_BuildValue("[NNNN]", wrap(rows.codes), wrap(rows.scales), wrap(cols.codes), wrap(cols.scales));
+    const Mx4Out& made = by_rows ? rows : cols;
+    return Py_BuildValue("[NN]", wrap(made.codes), wrap(made.scales));
+    END_HANDLE_TH_ERRORS
+}
+
+// mx4_dequant(codes [rows, bytes], scales, cols, stream) -> y
+PyObject* mx4_dequant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor codes, scales, y;
+    at::Tensor* const tensors[] = {&codes, &scales};
+    int64_t cols, stream;
+    ti8_mx4 mx;
+    if (nargs != 4 || !tensors_of(args, tensors, 2) || !number(args[2], &cols) || !number(args[3], &stream) || !mx4_operand(codes, scales, current_device(), &mx)) Py_RETURN_NONE;
+    const int64_t rows = codes.size(0);
+    if (codes.dim() != 2 || cols <= 0 || codes.size(1) != (cols + 255) / 256 * 128 || rows > MX4_ROWS) Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        y = at::empty({rows, cols}, at::TensorOptions().dtype(at::kBFloat16).device(codes.device()));
+        status = mx4_dequant_entry(&mx, rows, cols, y.data_ptr(), cols, stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_dequant", status);
+    return wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// mx4_gemm_nt(A, scales of A, B, scales of B, whether in fp32, stream) -> C
+PyObject* mx4_gemm_nt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor A, sA, B, sB, out;
+    at::Tensor* const tensors[] = {&A, &sA, &B, &sB};
+    int64_t wide, stream;
+    ti8_mx4 a, b;
+    const c10::DeviceIndex device = current_device();
+    if (nargs != 6 || !tensors_of(args, tensors, 4) || !number(args[4], &wide) || !number(args[5], &stream) || !mx4_operand(A, sA, device, &a) || !mx4_operand(B, sB, device, &b)) Py_RETURN_NONE;
+    const int64_t K = A.size(-1) * 2, N = B.size(-2), rows = A.numel() / A.size(-1);
+    if (B.size(-1) * 2 != K || (B.dim() == 3 && (A.dim() != 3 || A.size(0) != B.size(0)))) Py_RETURN_NONE;
+    const int64_t batch = B.dim() == 3 ? B.size(0) : 1, M = rows / batch;      // (one weight for all batches: their rows are rows of one product)
+    if (M > MX4_ROWS || N > MX4_ROWS || K > MX4_CONTRACTED || batch > 65535) Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        const auto type = at::TensorOptions().dtype(wide ? at::kFloat : at::kBFloat16).device(A.device());
+        out = A.dim() == 2 ? at::empty({M, N}, type) : at::empty({A.size(0), A.size(1), N}, type);
+        const int64_t need = mx4_gemm_workspace(batch, M, N, K);
+        c10::optional<Workspace> workspace;
+        if (need > 0) workspace.emplace(need, A.device(), at::TensorOptions().dtype(at::kByte).device(A.device()));
+        status = mx4_gemm_entry(&a, batch > 1 ? M : 0, &b, batch > 1 ? N : 0, out.data_ptr(), N, M * N, batch, M, N, K, wide ? 1 : 0, workspace ? workspace->p : nullptr, need,
+                                stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_gemm_nt", status);
+    return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// rmsnorm_quant(x, weight, residual, eps, whether in 4 bits, group, inv_mode, qflags, stream) -> [q, s, rstd] or [q, s, rstd, h]
+PyObject* rmsnorm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor x, w, r, q, s, rstd, h;
+    at::Tensor* const tensors[] = {&x, &w, &r};
+    int64_t mx, group, inv_mode, qflags, stream;
+    if (nargs != 9 || !tensors_of(args, tensors, 3) || !PyFloat_CheckExact(args[3]) || !number(args[4], &mx) || !number(args[5], &group) || !number(args[6], &inv_mode) ||
+        !number(args[7], &qflags) || !number(args[8], &stream))
+        Py_RETURN_NONE;
+    const c10::DeviceIndex device = current_device();
+    const auto dense = [&](const at::Tensor& t) { return on(t, at::kBFloat16, device) && t.is_contiguous() && at_multiple(t, 16) && !derived(t); };
+    if (!dense(x) || !dense(w) || (r.defined() && (!dense(r) || r.sizes() != x.sizes())) || x.dim() < 1 || w.dim() != 1) Py_RETURN_NONE;
+    const int64_t dim = x.size(-1), rows = x.numel() / dim;
+    if (w.size(0) != dim || dim % (mx ? 8 : 128) || dim > 16384 || rows > MX4_ROWS || (group != 0 && (group != 128 || mx))) Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        const auto options = at::TensorOptions().device(x.device());
+        const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+        ti8_rmsnorm_quant_args a = {};
+        Mx4Out out;
+        rstd = at::empty(lead, options.dtype(at::kFloat));
+        if (r.defined()) h = at::empty(x.sizes(), options.dtype(at::kBFloat16));
+        if (mx) {
+            out = Mx4Out(lead, rows, dim, options.dtype(at::kByte));
+            q = out.codes;
+            s = out.scales;
+            a.mx4 = out.mx;
+        } else {
+            q = at::empty(x.sizes(), options.dtype(at::kChar));
+            std::vector<int64_t> sizes(lead.begin(), lead.end());
+            if (group) sizes.push_back(dim / 128);
+            s = at::empty(sizes, options.dtype(at::kFloat));
+            a.q = static_cast<int8_t*>(q.data_ptr());
+            a.ldq = dim;
+            a.s = static_cast<float*>(s.data_ptr());
+        }
+        a.x = x.data_ptr(); a.ldx = dim;
+        a.w = w.data_ptr();
+        if (r.defined()) {
+            a.residual = r.data_ptr(); a.ldr = dim;
+            a.h = h.data_ptr(); a.ldh = dim;
+        }
+        a.rstd = static_cast<float*>(rstd.data_ptr());
+        a.rows = rows; a.dim = dim; a.eps = PyFloat_AS_DOUBLE(args[3]);
+        a.group = (int)group; a.qflags = (int)qflags; a.inv_mode = (int)inv_mode;
+        status = rmsnorm_quant_entry(&a, stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_rmsnorm_quant", status);
+    if (r.defined()) return Py_BuildValue("[NNNN]", wrap(q), wrap(s), wrap(rstd), wrap(h));
+    return Py_BuildValue("[NNN]", wrap(q), wrap(s), wrap(rstd));
+    END_HANDLE_TH_ERRORS
+}
+
+// dequant_row(q, s, stream) -> y
+PyObject* dequant_row(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor q, s, y;
+    at::Tensor* const tensors[] = {&q, &s};
+    int64_t stream;
+    if (nargs != 3 || !tensors_of(args, tensors, 2) || !number(args[2], &stream)) Py_RETURN_NONE;
+    const c10::DeviceIndex device = current_device();
+    if (!on(q, at::kChar, device) || !on(s, at::kFloat, device) || q.dim() < 1 || !q.is_contiguous() || !s.is_contiguous() || !at_multiple(q, 8)) Py_RETURN_NONE;
+    const int64_t cols = q.size(-1), rows = q.numel() / cols;
+    const at::IntArrayRef lead = q.sizes().slice(0, q.dim() - 1);
+    const bool by_group = s.sizes() != lead;
+    if (cols % 8 || rows > MX4_ROWS || cols > MX4_ROWS ||
+        (by_group && (cols % 128 || s.dim() != q.dim() || s.sizes().slice(0, q.dim() - 1) != lead || s.size(-1) != cols / 128)))
+        Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        y = at::empty(q.sizes(), at::TensorOptions().dtype(at::kBFloat16).device(q.device()));
+        status = dequant_row_entry(static_cast<const int8_t*>(q.data_ptr()), cols, static_cast<const float*>(s.data_ptr()), rows, cols, by_group ? 128 : 0, y.data_ptr(), cols,
+                                   stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_dequant_row", status);
+    return wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// set_up_mx4(addresses of ti8_mx4_quant, ti8_mx4_dequant, ti8_mx4_gemm_nt, ti8_mx4_gemm_nt_workspace, ti8_rmsnorm_quant, ti8_dequant_row)
+PyObject* set_up_mx4(PyObject*, PyObject* args) {
+    unsigned long long q, d, g, w, n, r;
+    if (!PyArg_ParseTuple(args, "KKKKKK", &q, &d, &g, &w, &n, &r)) return nullptr;
+    mx4_quant_entry = reinterpret_cast<decltype(mx4_quant_entry)>(q);
+    mx4_dequant_entry = reinterpret_cast<decltype(mx4_dequant_entry)>(d);
+    mx4_gemm_entry = reinterpret_cast<decltype(mx4_gemm_entry)>(g);
+    mx4_gemm_workspace = reinterpret_cast<decltype(mx4_gemm_workspace)>(w);
+    rmsnorm_quant_entry = reinterpret_cast<decltype(rmsnorm_quant_entry)>(n);
+    dequant_row_entry = reinterpret_cast<decltype(dequant_row_entry)>(r);
+    Py_RETURN_NONE;
+}
+
 // set_up_cache4(addresses of ti8_cache4_append, _read, _attention, _attention_workspace, _evict)
 PyObject* set_up_cache4(PyObject*, PyObject* args) {
     unsigned long long a, r, t, w, e;
@@ -366,8 +584,14 @@ PyMethodDef methods[] = {
     {"cache4_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache4_read)), METH_FASTCALL, nullptr},
     {"cache4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache4_attention)), METH_FASTCALL, nullptr},
     {"cache4_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache4_evict)), METH_FASTCALL, nullptr},
+    {"mx4_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_quant)), METH_FASTCALL, nullptr},
+    {"mx4_dequant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_dequant)), METH_FASTCALL, nullptr},
+    {"mx4_gemm_nt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_gemm_nt)), METH_FASTCALL, nullptr},
+    {"rmsnorm_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rmsnorm_quant)), METH_FASTCALL, nullptr},
+    {"dequant_row", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_row)), METH_FASTCALL, nullptr},
     {"set_up", set_up, METH_VARARGS, nullptr},
     {"set_up_cache4", set_up_cache4, METH_VARARGS, nullptr},
+    {"set_up_mx4", set_up_mx4, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -378,8 +602,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 // library's argument blocks are read and written here without a call)
 PyMODINIT_FUNC PyInit__native(void) {
     PyObject* const m = PyModule_Create(&module);
-    PyObject* const built_for = Py_BuildValue("(s(ii)nnn)", TI8_BUILT_FOR_TORCH, PY_MAJOR_VERSION, PY_MINOR_VERSION, (Py_ssize_t)sizeof(ti8_linear_args), (Py_ssize_t)sizeof(ti8_gemm_problem),
-                                              (Py_ssize_t)sizeof(ti8_cache4));
+    PyObject* const built_for = Py_BuildValue("(s(ii)nnnnn)", TI8_BUILT_FOR_TORCH, PY_MAJOR_VERSION, PY_MINOR_VERSION, (Py_ssize_t)sizeof(ti8_linear_args), (Py_ssize_t)sizeof(ti8_gemm_problem),
+                                              (Py_ssize_t)sizeof(ti8_cache4), (Py_ssize_t)sizeof(ti8_mx4), (Py_ssize_t)sizeof(ti8_rmsnorm_quant_args));
     if (m && (!built_for || PyModule_AddObject(m, "built_for", built_for) < 0)) {
         Py_XDECREF(built_for);
         Py_DECREF(m);

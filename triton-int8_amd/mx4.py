@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .ops import _need, _stream
+from .ops import _natively, _need, _stream
 
 __all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "linear_fwd_bwd", "quant_col_t", "quant_row", "quant_row_col_t"]
 
@@ -62,6 +62,9 @@ def _quant(x, by_rows, by_columns):
 
 def quant_row(x):
     """``x`` bf16 [.., cols] in 4 bits, groups along the last dim: ``(codes, scales)``."""
+    made = _natively("mx4_quant", x, 1, 0)
+    if made is not None:
+        return tuple(made)
     _bf16(x, "x")
     codes, scales = _quant(x.reshape(-1, x.shape[-1]), True, False)[0]
     return codes.view(*x.shape[:-1], codes.shape[-1]), scales
@@ -69,12 +72,18 @@ def quant_row(x):
 
 def quant_col_t(x):
     """The transpose of ``x`` [R, C] in 4 bits, groups along its columns: ``quant_row(x.T)`` without the transpose in bf16."""
+    made = _natively("mx4_quant", x, 0, 1)
+    if made is not None:
+        return tuple(made)
     _bf16(x, "x", 2)
     return _quant(x, False, True)[1]
 
 
 def quant_row_col_t(x):
     """``(codes, scales)`` of ``x`` [R, C] and of its transpose from one read: the same bits as :func:`quant_row` and :func:`quant_col_t`."""
+    made = _natively("mx4_quant", x, 1, 1)
+    if made is not None:
+        return tuple(made)
     _bf16(x, "x", 2)
     rows, cols = _quant(x, True, True)
     return *rows, *cols
@@ -98,6 +107,9 @@ def _operand(codes, scales, name):
 
 def dequant(codes, scales, cols):
     """The values, bf16 [.., cols], that codes [.., tiles * 128] and scales stand for (exact)."""
+    y = _natively("mx4_dequant", codes, scales, cols)
+    if y is not None:
+        return y
     _need(isinstance(codes, torch.Tensor) and codes.dim() >= 1 and codes.numel() > 0, "codes must be a non-empty uint8 tensor [.., tiles * 128]")
     _need(isinstance(cols, int) and cols > 0 and codes.shape[-1] == _tiles(cols) * 128, f"{cols} columns have {_tiles(cols) * 128 if isinstance(cols, int) else '?'} bytes of codes, got {codes.shape[-1]}")
     flat = codes.reshape(-1, codes.shape[-1])
@@ -112,6 +124,9 @@ def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
     """``A B^T`` of tensors in 4 bits: A [M, ..] or [batch, M, ..], B [N, ..] (that all batches share) or [batch, N, ..]; bf16 or float32, [M, N] or [batch, M, N].
     Added up in fp32 in a fixed order and rounded once."""
     _need(out_dtype in (torch.bfloat16, torch.float32), f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    out = _natively("mx4_gemm_nt", A, sA, B, sB, int(out_dtype == torch.float32))
+    if out is not None:
+        return out
     A, sA, a = _operand(A, sA, "A")
     B, sB, b = _operand(B, sB, "B")
     _need(A.shape[-1] == B.shape[-1], f"A has {A.shape[-1] // 128} tiles along the contraction, B {B.shape[-1] // 128}")
@@ -123,7 +138,10 @@ def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
     if rows_b == 0:         # one weight for all batches: their rows are rows of one product
         M, batch = M * batch, 1
     _need(batch <= 65535 and M <= MOST_ROWS, f"a product takes up to 65535 batches and 2^28 rows, got {batch} and {M}")
-    _lib.call("ti8_mx4_gemm_nt", a, rows_a if batch > 1 else 0, b, rows_b if batch > 1 else 0, out.data_ptr(), N, M * N, batch, M, N, K, int(out_dtype == torch.float32), _stream())
+    need = _lib.lib().ti8_mx4_gemm_nt_workspace(batch, M, N, K)
+    workspace = torch.empty((need,), dtype=torch.uint8, device=A.device) if need > 0 else None
+    _lib.call("ti8_mx4_gemm_nt", a, rows_a if batch > 1 else 0, b, rows_b if batch > 1 else 0, out.data_ptr(), N, M * N, batch, M, N, K, int(out_dtype == torch.float32),
+              None if workspace is None else workspace.data_ptr(), need, _stream())
     return out
 
 

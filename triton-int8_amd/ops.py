@@ -674,6 +674,15 @@ def rmsnorm(x, weight, eps):
     return y, rstd
 
 
+def _natively(name, *args):
+    """A call with its checks, allocations and launch made from C++, or None where it takes the Python way, which says what is wrong."""
+    native = _lib.native()
+    out = None if native is None else getattr(native, name)(*args, _stream())
+    if type(out) is tuple:
+        raise _lib.failed(*out)
+    return out
+
+
 def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV_RCP_OF_SCALE):
     """``h = x + residual`` (bf16), ``y = bf16(h * rstd) * weight`` over the last dim and y quantised, in one pass: the step from a linear's output to the next one's operand.
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
@@ -682,6 +691,9 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
     Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean in 64 bits: no code depends on an order of
     summation.  Quantised tensors have no gradients: x, weight and residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and,
     the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
+    made = _natively("rmsnorm_quant", x, weight, residual, eps, int(to == "mx4"), group, inv_mode, Q_CLAMP) if to in ("mx4", "int8") else None
+    if made is not None:
+        return tuple(made)
     _need(to in ("mx4", "int8"), f"`to` must be 'mx4' or 'int8', got {to!r}")
     _need(group in (0, 128) and (group == 0 or to == "int8"), f"group must be 0 or, with 'int8', 128, got {group}")
     for t, name in ((x, "x"), (weight, "weight")) + (() if residual is None else ((residual, "residual"),)):
@@ -718,6 +730,9 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
 
 def dequant_row(q, s):
     """bf16 [.., cols]: ``q * s``, what codes int8 [.., cols] of :func:`quant_row` with scales float32 [..] or, of groups of 128, [.., cols / 128] stand for."""
+    y = _natively("dequant_row", q, s)
+    if y is not None:
+        return y
     _need(isinstance(q, torch.Tensor) and isinstance(s, torch.Tensor) and _on_gpu(q) and _on_gpu(s) and q.get_device() == s.get_device() == torch._C._cuda_getDevice(),
           "q and s must be tensors on the current GPU")
     _need(q.dtype == torch.int8 and s.dtype == torch.float32 and q.dim() >= 1 and q.numel() > 0 and q.shape[-1] % 8 == 0,
