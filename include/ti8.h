@@ -573,8 +573,13 @@ typedef struct {
     int64_t ld, scale_ld;
 } ti8_mx4;
 /* x bf16 [rows][cols] (ldx, any alignment) quantised by its rows (by_rows: [rows][cols]), by its columns (by_columns: the transposed tensor [cols][rows]), or
- * both from one read; either may be NULL. */
-int ti8_mx4_quant(const void* x, int64_t ldx, int64_t rows, int64_t cols, const ti8_mx4* by_rows, const ti8_mx4* by_columns, ti8_stream_t stream);
+ * both from one read: what has no codes (NULL) is not made.  `operands` is a HOST array; 2 or 3 of them, each both ways, go in one launch, with the same bits. */
+typedef struct {
+    const void* x; int64_t ldx;
+    int64_t rows, cols;
+    ti8_mx4 by_rows, by_columns;
+} ti8_mx4_operand;
+int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_stream_t stream);
 /* y bf16 [rows][cols] (ldy): the values that the codes stand for, exactly */
 int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, void* y, int64_t ldy, ti8_stream_t stream);
 /* C[b] = A[b] B[b]^T, A [M][K] and B [N][K]: batch b of A is the rows from b * rows_a on of `a` (0: all batches share A), of B likewise; C bf16 (wide: float)
@@ -585,6 +590,13 @@ int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t 
 /* bytes of workspace that the call above needs (0: none; -1 for sizes it does not take), 16-byte aligned, contents undefined before and after: few tiles over a
  * long K are shared among workgroups, whose parts are added up in order */
 int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K);
+/* One training step of a layer, every product in 4 bits: Y = X W^T, dX = dY W, dW = dY^T X, i.e. ti8_mx4_quant of X, W and dY both ways in one launch and three
+ * times ti8_mx4_gemm_nt.  X bf16 [T][K] (ldx), W bf16 [N][K] (ldw), dY bf16 [T][N] (lddy), any alignment -> Y [T][N], dX [T][K], dW [N][K], dense bf16; any T, K and N
+ * up to 2^22.  The outputs may be the inputs' memory.  workspace: ti8_mx4_linear_fwd_bwd_workspace bytes (-1 for sizes it does not take), 256-byte aligned, contents
+ * undefined before and after. */
+int64_t ti8_mx4_linear_fwd_bwd_workspace(int64_t T, int64_t K, int64_t N);
+int ti8_mx4_linear_fwd_bwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* dY, int64_t lddy, void* Y, void* dX, void* dW,
+                           int64_t T, int64_t K, int64_t N, void* workspace, int64_t workspace_bytes, ti8_stream_t stream);
 /* A decoder layer's step from one linear's output to the next one's operand: h = bf16(x + residual) (residual and h NULL: h is x), rstd = 1 / sqrt(mean(h^2) + eps)
  * (float [rows]; the mean in 64 bits), y = bf16(bf16(h * rstd) * w), and y quantised: into 4 bits (mx4.codes not NULL), or into int8 codes q [rows][dim] with the
  * arithmetic of ti8_quant_row (s, group 0 or 128, qflags and inv_mode as there).  h may be the memory of x or residual.

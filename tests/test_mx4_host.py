@@ -24,6 +24,11 @@ def refused(lib, name, code, msg, *args):
     assert msg in text and (name in text or text.startswith("unknown")), text       # (what all quantisers have in common)
 
 
+def operand(lib, **other):
+    fields = dict(x=FAKE, ldx=512, rows=64, cols=512)
+    return lib.Mx4Operand(**{**fields, **other})
+
+
 TENSORS = [(dict(codes=None), 1, "required"), (dict(scales=None), 1, "required"), (dict(ld=128), 2, "ld"), (dict(scale_ld=504), 2, "scale_ld"), (dict(codes=FAKE + 8), 3, "aligned"),
            (dict(scales=FAKE + 4), 3, "8-byte"), (dict(ld=264), 3, "ld"), (dict(scale_ld=516), 3, "scale_ld")]
 
@@ -31,8 +36,9 @@ TENSORS = [(dict(codes=None), 1, "required"), (dict(scales=None), 1, "required")
 @pytest.mark.parametrize("other,code,msg", TENSORS, ids=str)
 def test_tensors_that_are_refused(lib, other, code, msg):
     bad, good = mx(lib, **other), mx(lib)
-    refused(lib, "ti8_mx4_quant", code, msg, FAKE, 512, 64, 512, bad, None, None)
-    refused(lib, "ti8_mx4_quant", code, msg, FAKE, 64, 512, 64, None, bad, None)
+    if other != dict(codes=None):
+        refused(lib, "ti8_mx4_quant", code, msg, operand(lib, by_rows=bad), 1, None)
+        refused(lib, "ti8_mx4_quant", code, msg, operand(lib, ldx=64, rows=512, cols=64, by_columns=bad), 1, None)
     refused(lib, "ti8_mx4_dequant", code, msg, bad, 64, 512, FAKE, 512, None)
     for a, b in ((bad, good), (good, bad)):
         refused(lib, "ti8_mx4_gemm_nt", code, msg, a, 0, b, 0, FAKE, 64, 0, 1, 64, 64, 512, 0, None, 0, None)
@@ -45,7 +51,38 @@ def test_tensors_that_are_refused(lib, other, code, msg):
     ((FAKE, 511, 64, 512, 1, 1), 2, "ldx"), ((FAKE, 512, (1 << 28) + 1, 512, 1, 1), 2, "2^28"), ((FAKE + 1, 512, 64, 512, 1, 0), 3, "aligned")])
 def test_quant(lib, args, code, msg):
     x, ldx, rows, cols, by_rows, by_columns = args
-    refused(lib, "ti8_mx4_quant", code, msg, x, ldx, rows, cols, mx(lib) if by_rows else None, mx(lib, 512, 64) if by_columns else None, None)
+    o = operand(lib, x=x, ldx=ldx, rows=rows, cols=cols, by_rows=mx(lib) if by_rows else lib.Mx4(), by_columns=mx(lib, 512, 64) if by_columns else lib.Mx4())
+    refused(lib, "ti8_mx4_quant", code, msg, o, 1, None)
+
+
+def test_quant_of_several(lib):
+    both = operand(lib, by_rows=mx(lib), by_columns=mx(lib, 512, 64))
+    for count in (0, 4, -1):
+        refused(lib, "ti8_mx4_quant", 2, "operands", (lib.Mx4Operand * 4)(*[both] * 4), count, None)
+    refused(lib, "ti8_mx4_quant", 1, "by rows and by columns", (lib.Mx4Operand * 2)(both, operand(lib, by_rows=mx(lib))), 2, None)
+    refused(lib, "ti8_mx4_quant", 2, "ldx", (lib.Mx4Operand * 2)(both, operand(lib, ldx=5, by_rows=mx(lib), by_columns=mx(lib, 512, 64))), 2, None)
+
+
+@pytest.mark.parametrize("change,code,msg", [
+    (dict(X=None), 1, "required"), (dict(dW=None), 1, "required"), (dict(workspace=None), 1, "required"), (dict(T=0), 2, "T"), (dict(K=(1 << 22) + 1), 2, "2^22"), (dict(N=-3), 2, "N"),
+    (dict(bytes=4096), 1, "workspace of"), (dict(workspace=FAKE + 16), 3, "256-byte"), (dict(dX=FAKE + 1), 3, "2-byte"), (dict(W=FAKE + 1), 3, "ti8_mx4_quant"),
+    (dict(lddy=99), 2, "ti8_mx4_quant")], ids=str)
+def test_step(lib, change, code, msg):
+    v = {**dict(X=FAKE, W=FAKE, dY=FAKE, Y=FAKE, dX=FAKE, dW=FAKE, T=50, K=200, N=100, lddy=100, workspace=FAKE, bytes=1 << 30), **change}
+    got = lib.lib().ti8_mx4_linear_fwd_bwd(v["X"], 200, v["W"], 200, v["dY"], v["lddy"], v["Y"], v["dX"], v["dW"], v["T"], v["K"], v["N"], v["workspace"], v["bytes"], None)
+    assert got == code and msg in lib.lib().ti8_last_error().decode()
+
+
+def test_workspaces(lib):
+    """Long contractions over few tiles are shared out; sizes that are not taken have no workspace."""
+    l = lib.lib()
+    assert l.ti8_mx4_gemm_nt_workspace(1, 8192, 8192, 4096) == 0 and l.ti8_mx4_gemm_nt_workspace(1, 1, 1, 1) == 0
+    assert l.ti8_mx4_gemm_nt_workspace(1, 100, 100, 16384) in (2 * 40000, 4 * 40000, 8 * 40000)
+    assert l.ti8_mx4_gemm_nt_workspace(0, 1, 1, 1) == l.ti8_mx4_gemm_nt_workspace(1, 1, 1, 1 << 23) == -1
+    assert l.ti8_mx4_linear_fwd_bwd_workspace(0, 1, 1) == l.ti8_mx4_linear_fwd_bwd_workspace(1, 1 << 23, 1) == -1
+    T, K, N = 300, 520, 1000
+    held = sum(r * -(-c // 256) * 136 for r, c in ((T, K), (K, T), (N, K), (K, N), (T, N), (N, T)))
+    assert held <= l.ti8_mx4_linear_fwd_bwd_workspace(T, K, N) <= held + 13 * 256 + l.ti8_mx4_gemm_nt_workspace(1, N, K, T) + l.ti8_mx4_gemm_nt_workspace(1, T, N, K) + l.ti8_mx4_gemm_nt_workspace(1, T, K, N)
 
 
 @pytest.mark.parametrize("change,code,msg", [
@@ -229,12 +266,12 @@ def test_gradients_that_are_not_wanted_are_not_computed(recorded):
     y, = T.mx4.Mx4LinearFunction.apply(x, w)
     calls.clear()
     y.sum().backward()
-    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][4] is None
+    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][0].by_rows.codes is None
     w.requires_grad_(False)
     y, = T.mx4.Mx4LinearFunction.apply(x.requires_grad_(), w)
     calls.clear()
     y.sum().backward()
-    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][5] is None
+    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][0].by_columns.codes is None
     # one of several outputs that nobody uses
     a, b = torch.nn.Parameter(bf(24, 40)), torch.nn.Parameter(bf(8, 40))
     y, z = T.mx4.Mx4LinearFunction.apply(x, a, b)

@@ -763,6 +763,10 @@ TI8_HD int mx4_col_chunk(int wave, int octet, int waves) { return wave ^ (octet 
 TI8_HD int mx4_row(int row, int rows) { return row < rows ? row : rows - 1; }
 TI8_HD uint32_t mx4_chunk_swizzle(int row) { return (uint32_t)((row & 7) ^ ((row >> 3) & 1)); }
 
+// What may be on its way when a tile has to have arrived: the loads that are issued behind its last codes, those of STAGES - 2 tiles of codes and of STAGES - 1 of
+// scales.  (Order: scales of t + 1, codes of t, scales of t + 2, codes of t + 1, ..; a tile is waited for behind the scales of the tile STAGES further.)
+constexpr int mx4_behind(int stages, int loads, int scale_loads) { return (stages - 2) * loads + (stages - 1) * scale_loads; }
+
 // K tiles that part `p` of a contraction over nk takes (1 <= parts <= nk: none of them is empty)
 struct Mx4Part {
     int first, tiles;

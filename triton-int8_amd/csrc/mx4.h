@@ -40,14 +40,52 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 __device__ __forceinline__ uint4 load16(const uint16_t* p) { return __builtin_bit_cast(uint4, *reinterpret_cast<const u32x4_any*>(p)); }
 __device__ __forceinline__ void store16(uint16_t* p, const uint4& v) { *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, v); }
 #pragma clang diagnostic pop
-// eight elements of which the first `left` exist (any number), zeros for the others
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int64_t left) {
-    if (left >= 8) return load16(p);
+// Elements col .. col + 7 of a row of `cols` elements (at least 8), zeros for those that it does not have; without a branch, so that several are on their way at
+// once: what lies across the row's end is read from its last eight and shifted.
+__device__ __forceinline__ uint4 load8_of(const uint16_t* row, int64_t col, int64_t cols) {
+    const int64_t left = cols - col;
+    uint4 v = load16(row + (left >= 8 ? col : left > 0 ? cols - 8 : 0));
+    const int gone = left >= 8 ? 0 : left > 0 ? 8 - (int)left : 8;
+    if (gone & 4) v = make_uint4(v.z, v.w, 0, 0);
+    if (gone & 2) v = make_uint4(v.y, v.z, v.w, 0);
+    if (gone & 1) v = make_uint4((v.x >> 16) | (v.y << 16), (v.y >> 16) | (v.z << 16), (v.z >> 16) | (v.w << 16), v.w >> 16);
+    if (gone == 8) v = make_uint4(0, 0, 0, 0);
+    return v;
+}
+// the same of rows of up to 7 elements
+__device__ __forceinline__ uint4 load_short(const uint16_t* row, int64_t col, int64_t cols) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+        if (col + j < cols) w[j >> 1] |= (uint32_t)row[col + j] << (16 * (j & 1));
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// N rows from `row0` on, `step` apart, zeros where there are none.  `split`: the lanes' octets may lie across the rows' end.
+template <int N>
+__device__ __forceinline__ void load_rows(uint4 (&v)[N], const uint16_t* x, int64_t ldx, int64_t row0, int step, int64_t rows, int64_t col, int64_t cols, bool split) {
+    if (!split) {
+        const int64_t at = col < cols ? col : cols - 8;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t row = row0 + i * step;
+            v[i] = load16(x + (row < rows ? row : rows - 1) * ldx + at);
+        }
+    } else if (cols >= 8) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t row = row0 + i * step;
+            v[i] = load8_of(x + (row < rows ? row : rows - 1) * ldx, col, cols);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t row = row0 + i * step;
+            v[i] = load_short(x + (row < rows ? row : rows - 1) * ldx, col, cols);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (row0 + i * step >= rows || col >= cols) v[i] = make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void store8(uint16_t* p, const uint4& v, int64_t left) {
     if (left >= 8) return store16(p, v);
@@ -68,6 +106,17 @@ __device__ __forceinline__ uint32_t largest2(const uint4& v) {
 __device__ __forceinline__ uint32_t halves_max(uint32_t m) { return max(m & 0xffffu, m >> 16); }
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_umax(uint32_t v) { return max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false)); }
+// pk_max over the lanes whose numbers differ in bit 4 or bit 5, in all of them
+__device__ __forceinline__ uint32_t pk_max_16(uint32_t m) {
+    const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    return pk_max(r[0], r[1]);
+}
+__device__ __forceinline__ uint32_t pk_max_32(uint32_t m) {
+    const auto r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return pk_max(r[0], r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_pk_max(uint32_t v) { return pk_max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false)); }
 // over four neighbouring lanes, in all of them
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) { return dpp_umax<0x4E>(dpp_umax<0xB1>(v)); }
 
@@ -86,6 +135,12 @@ __device__ __forceinline__ uint32_t encode2(uint32_t old, uint32_t pair, float s
 __device__ __forceinline__ uint32_t encode8(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t byte) {
     const float scale = scale_of(byte);
     const uint32_t w = encode2<3>(encode2<2>(encode2<1>(encode2<0>(0u, a, scale), b, scale), c, scale), d, scale);
+    return byte == NAN_SCALE ? 0u : w;
+}
+// four of them
+__device__ __forceinline__ uint32_t encode4(uint32_t a, uint32_t b, uint32_t byte) {
+    const float scale = scale_of(byte);
+    const uint32_t w = encode2<1>(encode2<0>(0u, a, scale), b, scale);
     return byte == NAN_SCALE ? 0u : w;
 }
 #endif

@@ -6,6 +6,7 @@
 // supplies row l % 32 of its operand and 32 elements of the 64 that it contracts.  Which 32 is free as long as both operands agree: step ks of a tile takes
 // chunk ks from lanes below 32 and chunk 4 + ks from the others, so that a lane's four scales of a tile are one word, and the step's number picks the byte.
 // The operands change places (the instruction's rows are C's columns), so that a lane holds four neighbouring elements of a row of C.
+#include <type_traits>
 #include "mx4.h"
 
 namespace ti8 {
@@ -183,6 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
         for (int t = 0; t < STAGES; ++t) {
             issue(t, t, 0, LOADS);
             issue_scales(t);
+            __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 1) * (LOADS + SCALE_LOADS), 0x70));
         asm volatile("s_barrier" ::: "memory");
@@ -214,17 +216,23 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
 #undef TI8_TILE
 #undef TI8_STEP
     } else {
-        // Codes of tile kt + STAGES are asked for once tile kt has been read, half of them a step later, scales of tile kt + STAGES + 1 before that.  What may be on its
-        // way when a tile's third step ends, behind the last codes of the next one: those of STAGES - 2 tiles and scales of STAGES - 1.  (Loads past the last tile
-        // repeat it: no branches in the loop.)
-        constexpr int BEHIND = (STAGES - 2) * LOADS + (STAGES - 1) * SCALE_LOADS;
-        static_assert(BEHIND < 64, "vmcnt has six bits");
+        // Codes of tile kt + STAGES are asked for once tile kt has been read, half of them a step later, scales of tile kt + STAGES + 1 before that (and so in front of the
+        // loop: what is waited for is counted from the end).  (Loads past the last tile repeat it: no branches in the loop.)
+        constexpr int BEHIND = idx::mx4_behind(STAGES, LOADS, SCALE_LOADS);
+        static_assert(BEHIND + FIRST < 64, "vmcnt has six bits");
+        issue_scales(0);
+        issue_scales(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t <= STAGES; ++t) issue_scales(t);
-#pragma unroll
-        for (int t = 0; t < STAGES - 1; ++t) issue(t, t, 0, LOADS);
+        for (int t = 0; t < STAGES - 1; ++t) {
+            issue(t, t, 0, LOADS);
+            __builtin_amdgcn_sched_barrier(0);
+            issue_scales(t + 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         issue(STAGES - 1, STAGES - 1, 0, FIRST);
-        __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 2) * LOADS + FIRST, 0x70));
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(waitcnt(BEHIND + FIRST, 0x70));
         asm volatile("s_barrier" ::: "memory");
         frags(0, 0, 0);
         scales(0);
@@ -265,53 +273,48 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
     __builtin_amdgcn_s_waitcnt(0);      // (loads past the last tile, repeated into LDS)
     __syncthreads();
 
-    // lane: row m = l % 32 of a 32 x 32 block of C, columns 8 (r / 4) + 4 (l / 32) + r % 4
-    const int cols = g.N - n0 - wn * TN * 32;
-    if (g.wide) {
-        float* const C = static_cast<float*>(g.C) + blockIdx.y * g.part + blockIdx.z * g.bsc + n0 + wn * TN * 32;
+    // Lane: row m = l % 32 of a 32 x 32 block of C, columns 8 q + 4 (l / 32) + c in register 4 q + c.  Through LDS, 32 rows of a wave's at a time, so that a row is
+    // written in one piece
+    const int64_t first_c = blockIdx.y * g.part + blockIdx.z * g.bsc + (int64_t)(m0 + wm * TM * 32) * g.ldc + n0 + wn * TN * 32;
+    const int rows_left = g.M - m0 - wm * TM * 32, cols_left = g.N - n0 - wn * TN * 32;
+    const auto write = [&](auto wide, auto put) {
+        constexpr int SIZE = decltype(wide)::value ? 4 : 2, WIDTH = TN * 32, PITCH = WIDTH * SIZE + 16, PER = 16 / SIZE, LPR = WIDTH / PER, RPI = 64 / LPR;
+        static_assert(32 * PITCH * NW <= STAGES * (A_BYTES + B_BYTES), "the waves' rows fit the operands' buffers");
+        uint8_t* const mine = smem + wave * 32 * PITCH;
+        const int n = (lane % LPR) * PER;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const int m = m0 + (wm * TM + i) * 32 + row;
-            if (m >= g.M) continue;
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int n = j * 32 + 8 * q + 4 * half;
-                    float* const to = C + m * g.ldc + n;
-                    if (n + 4 <= cols) {
-                        typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
-                        *reinterpret_cast<v4f_any*>(to) = v4f{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (n + c < cols) to[c] = acc[i][j][4 * q + c];
-                    }
+                    uint8_t* const to = mine + row * PITCH + (j * 32 + 8 * q + 4 * half) * SIZE;
+                    const v4f x = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    if constexpr (SIZE == 4) *reinterpret_cast<v4f*>(to) = x;
+                    else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
                 }
+#pragma unroll
+            for (int u = 0; u < 32 / RPI; ++u) {
+                const int r = u * RPI + lane / LPR;
+                const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + n * SIZE);
+                if (i * 32 + r < rows_left) put(first_c + (i * 32 + r) * g.ldc + n, v, cols_left - n);
+            }
         }
-        return;
-    }
-    // through LDS, a wave's 32 rows at a time, so that a row is written in one piece
-    constexpr int WIDTH = TN * 32, PITCH = WIDTH * 2 + 16, LPR = WIDTH / 8, RPI = 64 / LPR;
-    static_assert(32 * PITCH * NW <= STAGES * (A_BYTES + B_BYTES), "the waves' rows fit the operands' buffers");
-    uint8_t* const mine = smem + wave * 32 * PITCH;
-    uint16_t* const C = static_cast<uint16_t*>(g.C) + blockIdx.z * g.bsc + n0 + wn * WIDTH;
-    const int n = (lane % LPR) * 8;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<uint2*>(mine + row * PITCH + (j * 32 + 8 * q + 4 * half) * 2) =
-                    make_uint2(pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
-#pragma unroll
-        for (int u = 0; u < 32 / RPI; ++u) {
-            const int r = u * RPI + lane / LPR, m = m0 + (wm * TM + i) * 32 + r;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + n * 2);
-            if (m < g.M) store8(C + m * g.ldc + n, v, cols - n);
-        }
-    }
+    };
+    if (g.wide)
+        write(std::true_type(), [&](int64_t at, const uint4& v, int left) {
+            typedef u32x4 u32x4_word __attribute__((aligned(4)));
+            uint32_t* const to = static_cast<uint32_t*>(g.C) + at;
+            if (left >= 4) {
+                *reinterpret_cast<u32x4_word*>(to) = __builtin_bit_cast(u32x4, v);
+            } else {
+                if (left > 0) to[0] = v.x;
+                if (left > 1) to[1] = v.y;
+                if (left > 2) to[2] = v.z;
+            }
+        });
+    else
+        write(std::false_type(), [&](int64_t at, const uint4& v, int left) { store8(static_cast<uint16_t*>(g.C) + at, v, left); });
 #else
     (void)g;
 #endif
@@ -533,4 +536,76 @@ extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* 
     if (blocks > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     mx4::join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float*>(workspace), plan.parts, g.part, batch * M, (int)M, (int)N, c, ldc, bsc, wide ? 1 : 0);
     return check_launch(fn);
+}
+
+namespace {
+// Where a step's operands lie in its workspace: X, W and dY by rows and by columns, and behind them what the products need
+struct Mx4Step {
+    ti8_mx4_operand o[3];
+    int64_t products, bytes;
+    bool ok;
+};
+Mx4Step mx4_step(int64_t T, int64_t K, int64_t N, char* base) {
+    Mx4Step s{};
+    s.ok = T > 0 && K > 0 && N > 0 && T <= (1 << 22) && K <= (1 << 22) && N <= (1 << 22);
+    if (!s.ok) return s;
+    const auto take = [&](int64_t bytes) {
+        char* const at = base + s.bytes;
+        s.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    const auto room = [&](int64_t rows, int64_t cols) {
+        const int64_t tiles = idx::mx4_tiles(cols);
+        ti8_mx4 t;
+        t.ld = tiles * idx::MX4_TILE_BYTES;
+        t.scale_ld = rows * idx::MX4_TILE_SCALES;
+        t.codes = take(rows * t.ld);
+        t.scales = take(tiles * t.scale_ld);
+        return t;
+    };
+    const int64_t rows[3] = {T, N, T}, cols[3] = {K, K, N};
+    for (int i = 0; i < 3; ++i) {
+        s.o[i].rows = rows[i];
+        s.o[i].cols = cols[i];
+        s.o[i].by_rows = room(rows[i], cols[i]);
+        s.o[i].by_columns = room(cols[i], rows[i]);
+    }
+    const int64_t sizes[3][3] = {{T, N, K}, {T, K, N}, {N, K, T}};
+    for (const auto& p : sizes) {
+        const int64_t need = ti8_mx4_gemm_nt_workspace(1, p[0], p[1], p[2]);
+        if (need > s.products) s.products = need;
+    }
+    take(s.products);
+    return s;
+}
+}  // namespace
+
+extern "C" int64_t ti8_mx4_linear_fwd_bwd_workspace(int64_t T, int64_t K, int64_t N) {
+    const Mx4Step s = mx4_step(T, K, N, nullptr);
+    return s.ok ? s.bytes : -1;
+}
+
+extern "C" int ti8_mx4_linear_fwd_bwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* dY, int64_t lddy, void* Y, void* dX, void* dW,
+                                      int64_t T, int64_t K, int64_t N, void* workspace, int64_t workspace_bytes, ti8_stream_t stream) {
+    const char* const fn = "ti8_mx4_linear_fwd_bwd";
+    if (!X || !W || !dY || !Y || !dX || !dW || !workspace) return fail(TI8_ERR_NULL, "%s: X, W, dY, Y, dX, dW and workspace are required", fn);
+    Mx4Step s = mx4_step(T, K, N, static_cast<char*>(workspace));
+    if (!s.ok) return fail(TI8_ERR_SHAPE, "%s: need T, K, N in 1 .. 2^22; got T=%lld K=%lld N=%lld", fn, (long long)T, (long long)K, (long long)N);
+    if (workspace_bytes < s.bytes) return fail(TI8_ERR_NULL, "%s: a workspace of %lld bytes is required, got %lld", fn, (long long)s.bytes, (long long)workspace_bytes);
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255) || ((reinterpret_cast<uintptr_t>(Y) | reinterpret_cast<uintptr_t>(dX) | reinterpret_cast<uintptr_t>(dW)) & 1))
+        return fail(TI8_ERR_ALIGN, "%s: the workspace must be 256-byte aligned, outputs 2-byte", fn);
+    const void* const x[3] = {X, W, dY};
+    const int64_t ld[3] = {ldx, ldw, lddy};
+    for (int i = 0; i < 3; ++i) {
+        s.o[i].x = x[i];
+        s.o[i].ldx = ld[i];
+    }
+    // (from here on everything is checked that the calls below check, but for the inputs' leading dimensions and alignment, which the first of them checks before it
+    // launches anything)
+    if (int e = ti8_mx4_quant(s.o, 3, stream)) return e;
+    char* const products = static_cast<char*>(workspace) + (s.bytes - (s.products + 255) / 256 * 256);
+    const ti8_mx4_operand &x4 = s.o[0], &w4 = s.o[1], &d4 = s.o[2];
+    if (int e = ti8_mx4_gemm_nt(&x4.by_rows, 0, &w4.by_rows, 0, Y, N, 0, 1, T, N, K, 0, products, s.products, stream)) return e;
+    if (int e = ti8_mx4_gemm_nt(&d4.by_rows, 0, &w4.by_columns, 0, dX, K, 0, 1, T, K, N, 0, products, s.products, stream)) return e;
+    return ti8_mx4_gemm_nt(&d4.by_columns, 0, &x4.by_columns, 0, dW, K, 0, 1, N, K, T, 0, products, s.products, stream);
 }

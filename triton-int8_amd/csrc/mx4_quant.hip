@@ -9,21 +9,27 @@ namespace {
 
 constexpr int THREADS = 256;
 
-struct QuantArgs {
+struct QuantOperand {
     const uint16_t* x;
     int64_t ldx, R, C;
     Tensor rows, cols;
+    int64_t first;          // of the launch's workgroups
+    int strips;             // workgroups along the columns
+};
+constexpr int QUANT_MAX = 3;
+struct QuantArgs {
+    QuantOperand o[QUANT_MAX];
+    int count;
 };
 
 // By rows: 32 rows x 256 columns per workgroup; a row's 512 bytes are read by half a wave, a group's maximum is over four lanes.
-__global__ __launch_bounds__(THREADS) void quant_row_kernel(QuantArgs g) {
+// 14336 x 4096: 24 us (6.1 TB/s).
+__global__ __launch_bounds__(THREADS) void quant_row_kernel(QuantOperand g) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int64_t tiles = idx::mx4_tiles(g.C), tile = blockIdx.x % tiles, row0 = (int64_t)(blockIdx.x / tiles) * idx::MX4_ROW_BLOCK + (threadIdx.x >> 5);
+    const int64_t tiles = idx::mx4_tiles(g.C), tile = blockIdx.x % tiles, first = (int64_t)(blockIdx.x / tiles) * idx::MX4_ROW_BLOCK, row0 = first + (threadIdx.x >> 5);
     const int octet = threadIdx.x & 31;
-    const int64_t col = tile * idx::MX4_TILE + octet * 8;
     uint4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = row0 + 8 * i < g.R ? load8(g.x + (row0 + 8 * i) * g.ldx + col, g.C - col) : make_uint4(0, 0, 0, 0);
+    load_rows<4>(v, g.x, g.ldx, row0, 8, g.R, tile * idx::MX4_TILE + octet * 8, g.C, (g.C & 7) && (tile + 1) * idx::MX4_TILE > g.C);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = row0 + 8 * i;
@@ -37,32 +43,39 @@ __global__ __launch_bounds__(THREADS) void quant_row_kernel(QuantArgs g) {
 #endif
 }
 
-// By columns (the transposed tensor's rows), with ROWS both ways from the same read: 32 rows x 256 columns per wave, a lane has 8 columns of 16 rows in
-// registers.  A column's group is two lanes' (l and l + 32); its codes go through LDS, from where lines of a column are written.
-template <int NW, bool ROWS>
-__global__ __launch_bounds__(64 * NW) void quant_cols_kernel(QuantArgs g) {
+// By columns (the transposed tensor's rows), with ROWS both ways from the same read, up to three tensors in a launch.  A wave has 32 rows x 512 / RB columns in
+// registers, a lane 8 columns of 32 / RB rows: a column's group is RB lanes', a row's four neighbours'.  A column's codes go through LDS, from where 16 NW
+// bytes of it are written in one piece.
+template <int NW, int RB, bool ROWS>
+__global__ __launch_bounds__(64 * NW, 4) void quant_cols_kernel(QuantArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int LINE = NW * 16;                       // bytes of a column's codes here
-    __shared__ __attribute__((aligned(16))) uint8_t lines[idx::MX4_TILE * LINE];
-    __shared__ __attribute__((aligned(16))) uint8_t row_scales[32 * NW * 8], col_scales[idx::MX4_TILE * NW];
-    const int64_t tiles = idx::mx4_tiles(g.C), tile = blockIdx.x % tiles, chunk = blockIdx.x / tiles;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, octet = lane & 31, half = lane >> 5;
-    const int64_t col = tile * idx::MX4_TILE + octet * 8, first = chunk * (32 * NW), row0 = first + wave * 32 + half * 16;
-    uint4 v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = row0 + i < g.R ? load8(g.x + (row0 + i) * g.ldx + col, g.C - col) : make_uint4(0, 0, 0, 0);
+    constexpr int OCTETS = 64 / RB, COLS = OCTETS * 8, RPL = 32 / RB, ROWS_HERE = 32 * NW, GROUPS = COLS / 32, LINE = NW * 16;
+    __shared__ __attribute__((aligned(16))) uint8_t lines[COLS * LINE];
+    __shared__ __attribute__((aligned(16))) uint8_t row_scales[ROWS_HERE * GROUPS], col_scales[COLS * NW];
+    const int64_t block = blockIdx.x;
+    int which = 0;
+    if (args.count > 1 && block >= args.o[1].first) which = 1;
+    if (args.count > 2 && block >= args.o[2].first) which = 2;
+    const QuantOperand& g = args.o[which];
+    const int64_t R = g.R, C = g.C, at_block = block - g.first, chunk = at_block / g.strips, first = chunk * ROWS_HERE, col0 = (at_block - chunk * g.strips) * COLS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, octet = lane % OCTETS, part = lane / OCTETS;
+    const int64_t row0 = first + wave * 32 + part * RPL;
+    uint4 v[RPL];
+    load_rows<RPL>(v, g.x, g.ldx, row0, 1, R, col0 + octet * 8, C, (C & 7) && col0 + COLS > C);
+    const int64_t tile = col0 / idx::MX4_TILE;
+    const int tile_octet = (int)(col0 % idx::MX4_TILE) / 8;
     if (ROWS) {
+        uint8_t* const codes = g.rows.codes + idx::mx4_code_at(row0, g.rows.ld, tile, tile_octet + octet);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < RPL; ++i) {
             const uint32_t byte = scale_byte(quad_max(halves_max(largest2(v[i]))));
-            if (row0 + i < g.R)
-                *reinterpret_cast<uint32_t*>(g.rows.codes + idx::mx4_code_at(row0 + i, g.rows.ld, tile, octet)) = encode8(v[i].x, v[i].y, v[i].z, v[i].w, byte);
-            if ((octet & 3) == 0) row_scales[(wave * 32 + half * 16 + i) * 8 + (octet >> 2)] = (uint8_t)byte;
+            if (row0 + i < R) *reinterpret_cast<uint32_t*>(codes + i * g.rows.ld) = encode8(v[i].x, v[i].y, v[i].z, v[i].w, byte);
+            if ((octet & 3) == 0) row_scales[(wave * 32 + part * RPL + i) * GROUPS + (octet >> 2)] = (uint8_t)byte;
         }
     }
     uint32_t m[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < RPL; ++i) {
         m[0] = pk_max(m[0], v[i].x & MAGNITUDE);
         m[1] = pk_max(m[1], v[i].y & MAGNITUDE);
         m[2] = pk_max(m[2], v[i].z & MAGNITUDE);
@@ -70,7 +83,9 @@ __global__ __launch_bounds__(64 * NW) void quant_cols_kernel(QuantArgs g) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        m[j] = pk_max(m[j], (uint32_t)__shfl_xor((int)m[j], 32, 64));
+        if (OCTETS == 8) m[j] = dpp_pk_max<0x128>(m[j]);      // (row_ror:8)
+        if (OCTETS <= 16) m[j] = pk_max_16(m[j]);
+        m[j] = pk_max_32(m[j]);
 #pragma unroll
         for (int odd = 0; odd < 2; ++odd) {
             const uint32_t byte = scale_byte(odd ? m[j] >> 16 : m[j] & 0xffffu);
@@ -78,38 +93,56 @@ __global__ __launch_bounds__(64 * NW) void quant_cols_kernel(QuantArgs g) {
                 const uint32_t a = j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w, b = j == 0 ? v[i + 1].x : j == 1 ? v[i + 1].y : j == 2 ? v[i + 1].z : v[i + 1].w;
                 return odd ? (a >> 16) | (b & 0xffff0000u) : (a & 0xffffu) | (b << 16);
             };
-            const uint2 w = make_uint2(encode8(pair(0), pair(2), pair(4), pair(6), byte), encode8(pair(8), pair(10), pair(12), pair(14), byte));
             const int c = octet * 8 + 2 * j + odd;
-            *reinterpret_cast<uint2*>(lines + c * LINE + idx::mx4_col_chunk(wave, octet, NW) * 16 + half * 8) = w;
-            if (half == 0) col_scales[c * NW + wave] = (uint8_t)byte;
+            uint8_t* const to = lines + c * LINE + idx::mx4_col_chunk(wave, octet, NW) * 16 + part * (RPL / 2);
+            if constexpr (RPL == 4) {
+                *reinterpret_cast<uint16_t*>(to) = (uint16_t)encode4(pair(0), pair(2), byte);
+            } else {
+#pragma unroll
+                for (int w = 0; w < RPL / 8; ++w) reinterpret_cast<uint32_t*>(to)[w] = encode8(pair(8 * w), pair(8 * w + 2), pair(8 * w + 4), pair(8 * w + 6), byte);
+            }
+            if (part == 0) col_scales[c * NW + wave] = (uint8_t)byte;
         }
     }
     __syncthreads();
-    if (ROWS) {
-        const int64_t row = first + threadIdx.x;
-        if (threadIdx.x < 32 * NW && row < g.R)
-            *reinterpret_cast<uint2*>(g.rows.scales + idx::mx4_scale_at(tile, g.rows.scale_ld, row, 0)) = *reinterpret_cast<const uint2*>(row_scales + threadIdx.x * 8);
+    if (ROWS && threadIdx.x < ROWS_HERE && first + threadIdx.x < R) {
+        uint8_t* const to = g.rows.scales + idx::mx4_scale_at(tile, g.rows.scale_ld, first + threadIdx.x, tile_octet / 4);
+        if (GROUPS == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(row_scales + threadIdx.x * GROUPS);
+        else if (GROUPS == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(row_scales + threadIdx.x * GROUPS);
+        else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(row_scales + threadIdx.x * GROUPS);
     }
     const int64_t row_tile = first / idx::MX4_TILE;
-    const int within = (int)(first % idx::MX4_TILE) / 2, group = (int)(first % idx::MX4_TILE) / 32;
+    const int within = (int)(first % idx::MX4_TILE);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {       // 256 columns of NW pieces of 16 bytes
+    for (int u = 0; u < COLS / 64; ++u) {       // NW pieces of 16 bytes to a column
         const int piece = u * 64 * NW + threadIdx.x, c = piece / NW, p = piece % NW;
-        const int64_t at = tile * idx::MX4_TILE + c;
-        if (at < g.C)
-            *reinterpret_cast<uint4*>(g.cols.codes + at * g.cols.ld + row_tile * idx::MX4_TILE_BYTES + within + p * 16) =
+        if (col0 + c < C)
+            *reinterpret_cast<uint4*>(g.cols.codes + idx::mx4_code_at(col0 + c, g.cols.ld, row_tile, within / 8) + p * 16) =
                 *reinterpret_cast<const uint4*>(lines + c * LINE + idx::mx4_col_chunk(p, c >> 3, NW) * 16);
     }
-    for (int c = threadIdx.x; c < idx::MX4_TILE; c += 64 * NW) {
-        const int64_t at = tile * idx::MX4_TILE + c;
-        if (at >= g.C) break;
-        uint8_t* to = g.cols.scales + idx::mx4_scale_at(row_tile, g.cols.scale_ld, at, group);
+    for (int c = threadIdx.x; c < COLS && col0 + c < C; c += 64 * NW) {
+        uint8_t* const to = g.cols.scales + idx::mx4_scale_at(row_tile, g.cols.scale_ld, col0 + c, within / 32);
         if (NW == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(col_scales + c * NW);
+        else if (NW == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(col_scales + c * NW);
         else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(col_scales + c * NW);
     }
 #else
-    (void)g;
+    (void)args;
 #endif
+}
+
+// Workgroups over all of x^T's tiles (those behind its last rows make the zeros up to the end of a tile) and, with them, over all columns of x
+template <int NW, int RB, bool ROWS>
+void launch_cols(QuantArgs g, hipStream_t st) {
+    constexpr int COLS = 512 / RB;
+    int64_t blocks = 0;
+    for (int i = 0; i < g.count; ++i) {
+        QuantOperand& o = g.o[i];
+        o.first = blocks;
+        o.strips = (int)(ROWS ? idx::mx4_tiles(o.C) * (idx::MX4_TILE / COLS) : (o.C + COLS - 1) / COLS);
+        blocks += o.strips * idx::mx4_tiles(o.R) * (8 / NW);
+    }
+    quant_cols_kernel<NW, RB, ROWS><<<dim3((unsigned)blocks), dim3(64 * NW), 0, st>>>(g);
 }
 
 // The values back, exact in bf16
@@ -291,33 +324,42 @@ bool grid_ok(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
 
 using namespace ti8;
 
-extern "C" int ti8_mx4_quant(const void* x, int64_t ldx, int64_t rows, int64_t cols, const ti8_mx4* by_rows, const ti8_mx4* by_columns, ti8_stream_t stream) {
+extern "C" int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_stream_t stream) {
     const char* const fn = "ti8_mx4_quant";
-    if (!x || (!by_rows && !by_columns)) return fail(TI8_ERR_NULL, "%s: x and one of by_rows and by_columns are required", fn);
-    if (rows <= 0 || cols <= 0 || rows > (1 << 28) || cols > (1 << 28) || (rows > 1 && ldx < cols))
-        return fail(TI8_ERR_SHAPE, "%s: need rows, cols in 1 .. 2^28 and ldx >= cols; got rows=%lld cols=%lld ldx=%lld", fn, (long long)rows, (long long)cols, (long long)ldx);
-    if (reinterpret_cast<uintptr_t>(x) & 1) return fail(TI8_ERR_ALIGN, "%s: x must be 2-byte aligned", fn);
-    mx4::QuantArgs g{static_cast<const uint16_t*>(x), ldx, rows, cols, {}, {}};
-    if (by_rows)
-        if (int e = mx4::check(fn, "by_rows", by_rows, rows, cols, g.rows)) return e;
-    if (by_columns)
-        if (int e = mx4::check(fn, "by_columns", by_columns, cols, rows, g.cols)) return e;
+    if (!operands) return fail(TI8_ERR_NULL, "%s: operands are required", fn);
+    if (count < 1 || count > mx4::QUANT_MAX) return fail(TI8_ERR_SHAPE, "%s: need 1 to %d operands, got %d", fn, mx4::QUANT_MAX, count);
+    mx4::QuantArgs g;
+    g.count = count;
+    int64_t elements = 0;
+    for (int i = 0; i < count; ++i) {
+        const ti8_mx4_operand& o = operands[i];
+        if (!o.x || (!o.by_rows.codes && !o.by_columns.codes)) return fail(TI8_ERR_NULL, "%s: x and one of by_rows and by_columns are required", fn);
+        if (count > 1 && (!o.by_rows.codes || !o.by_columns.codes)) return fail(TI8_ERR_NULL, "%s: several operands are quantised by rows and by columns", fn);
+        if (o.rows <= 0 || o.cols <= 0 || o.rows > (1 << 28) || o.cols > (1 << 28) || (o.rows > 1 && o.ldx < o.cols) || o.rows * o.cols > (1ll << 40))
+            return fail(TI8_ERR_SHAPE, "%s: need rows, cols in 1 .. 2^28, up to 2^40 elements and ldx >= cols; got rows=%lld cols=%lld ldx=%lld", fn, (long long)o.rows,
+                        (long long)o.cols, (long long)o.ldx);
+        if (reinterpret_cast<uintptr_t>(o.x) & 1) return fail(TI8_ERR_ALIGN, "%s: x must be 2-byte aligned", fn);
+        g.o[i] = {static_cast<const uint16_t*>(o.x), o.ldx, o.rows, o.cols, {}, {}, 0, 0};
+        if (o.by_rows.codes)
+            if (int e = mx4::check(fn, "by_rows", &o.by_rows, o.rows, o.cols, g.o[i].rows)) return e;
+        if (o.by_columns.codes)
+            if (int e = mx4::check(fn, "by_columns", &o.by_columns, o.cols, o.rows, g.o[i].cols)) return e;
+        elements += idx::mx4_tiles(o.rows) * idx::mx4_tiles(o.cols) * idx::MX4_TILE * idx::MX4_TILE;
+    }
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t tiles = idx::mx4_tiles(cols);
-    if (!by_columns) {
-        const int64_t blocks = tiles * ((rows + idx::MX4_ROW_BLOCK - 1) / idx::MX4_ROW_BLOCK);
+    if (!operands[0].by_columns.codes) {
+        const int64_t blocks = idx::mx4_tiles(g.o[0].C) * ((g.o[0].R + idx::MX4_ROW_BLOCK - 1) / idx::MX4_ROW_BLOCK);
         if (!mx4::grid_ok(blocks)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-        mx4::quant_row_kernel<<<dim3((unsigned)blocks), dim3(mx4::THREADS), 0, st>>>(g);
+        mx4::quant_row_kernel<<<dim3((unsigned)blocks), dim3(mx4::THREADS), 0, st>>>(g.o[0]);
         return check_launch(fn);
     }
-    // a workgroup per 256 x 256 elements, per 64 x 256 where that would leave CUs without one
-    const int64_t large = tiles * idx::mx4_tiles(rows);
-    const bool small = large < 2 * device_cu_count();
-    const int64_t blocks = small ? 4 * large : large;
-    if (!mx4::grid_ok(blocks)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    const auto go = [&](auto kernel, int waves) { kernel<<<dim3((unsigned)blocks), dim3(64 * waves), 0, st>>>(g); };
-    if (small) by_rows ? go(mx4::quant_cols_kernel<2, true>, 2) : go(mx4::quant_cols_kernel<2, false>, 2);
-    else by_rows ? go(mx4::quant_cols_kernel<8, true>, 8) : go(mx4::quant_cols_kernel<8, false>, 8);
+    if (!mx4::grid_ok(elements / (64 * 64))) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    // Up to four workgroups of 64 x 64 elements per CU: small ones, whose code is a quarter as long (it is read from memory too); behind that 128 or 256 rows of a
+    // column to a workgroup, whose codes are written in longer pieces.  us, both ways, small / large: 200 x 300 4.3 / 5.8, 1001 x 1016 4.6 / 5.1, 1000 x 2560 5.3 / 5.6,
+    // 2048 x 4096 9.4 / 8.5, 14336 x 4096 44 / 37 (4.9 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
+    const bool small = elements < (int64_t)16384 * device_cu_count(), rows = operands[0].by_rows.codes;
+    if (small) rows ? mx4::launch_cols<2, 8, true>(g, st) : mx4::launch_cols<2, 8, false>(g, st);
+    else rows ? mx4::launch_cols<4, 4, true>(g, st) : mx4::launch_cols<8, 4, false>(g, st);
     return check_launch(fn);
 }
 

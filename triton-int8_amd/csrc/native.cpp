@@ -6,7 +6,9 @@
 #include <cmath>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/util/SmallVector.h>
 #include <ATen/detail/CUDAHooksInterface.h>
 #include <ATen/ops/narrow.h>
 #include <ATen/TracerMode.h>
@@ -32,6 +34,8 @@ decltype(&ti8_mx4_quant) mx4_quant_entry = nullptr;
 decltype(&ti8_mx4_dequant) mx4_dequant_entry = nullptr;
 decltype(&ti8_mx4_gemm_nt) mx4_gemm_entry = nullptr;
 decltype(&ti8_mx4_gemm_nt_workspace) mx4_gemm_workspace = nullptr;
+decltype(&ti8_mx4_linear_fwd_bwd) mx4_step_entry = nullptr;
+decltype(&ti8_mx4_linear_fwd_bwd_workspace) mx4_step_workspace = nullptr;
 decltype(&ti8_rmsnorm_quant) rmsnorm_quant_entry = nullptr;
 decltype(&ti8_dequant_row) dequant_row_entry = nullptr;
 PyObject* parameter_class = nullptr;
@@ -350,17 +354,22 @@ bool on(const at::Tensor& t, at::ScalarType type, c10::DeviceIndex device) {
 }
 bool at_multiple(const at::Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 
+// A new tensor on the current device, from the allocator that tensors come from (what at::empty comes down to; without the dispatcher, which takes as long)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+    return at::detail::empty_generic(sizes, at::detail::getCUDAHooks().getCUDADeviceAllocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, c10::nullopt);
+}
+
 // room for a tensor in 4 bits
 struct Mx4Out {
     at::Tensor codes, scales;
     ti8_mx4 mx = {};
     Mx4Out() = default;
-    Mx4Out(at::IntArrayRef lead, int64_t rows, int64_t cols, const at::TensorOptions& bytes) {
+    Mx4Out(at::IntArrayRef lead, int64_t rows, int64_t cols) {
         const int64_t tiles = (cols + 255) / 256;
-        std::vector<int64_t> sizes(lead.begin(), lead.end());
+        c10::SmallVector<int64_t, 4> sizes(lead.begin(), lead.end());
         sizes.push_back(tiles * 128);
-        codes = at::empty(sizes, bytes);
-        scales = at::empty({tiles, rows, 8}, bytes);
+        codes = fresh(sizes, at::kByte);
+        scales = fresh({tiles, rows, 8}, at::kByte);
         mx = ti8_mx4{codes.data_ptr(), scales.data_ptr(), tiles * 128, rows * 8};
     }
 };
@@ -397,10 +406,10 @@ PyObject* mx4_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        const auto bytes = at::TensorOptions().dtype(at::kByte).device(x.device());
-        if (by_rows) rows = Mx4Out(x.sizes().slice(0, x.dim() - 1), R, C, bytes);
-        if (by_columns) cols = Mx4Out({C}, C, R, bytes);
-        status = mx4_quant_entry(x.data_ptr(), ldx, R, C, by_rows ? &rows.mx : nullptr, by_columns ? &cols.mx : nullptr, stream_of(stream));
+        if (by_rows) rows = Mx4Out(x.sizes().slice(0, x.dim() - 1), R, C);
+        if (by_columns) cols = Mx4Out({C}, C, R);
+        const ti8_mx4_operand o = {x.data_ptr(), ldx, R, C, rows.mx, cols.mx};
+        status = mx4_quant_entry(&o, 1, stream_of(stream));
     }
     if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_quant", status);
     if (by_rows && by_columns) return Py_BuildValue("[NNNN]", wrap(rows.codes), wrap(rows.scales), wrap(cols.codes), wrap(cols.scales));
@@ -422,7 +431,7 @@ PyObject* mx4_dequant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        y = at::empty({rows, cols}, at::TensorOptions().dtype(at::kBFloat16).device(codes.device()));
+        y = fresh({rows, cols}, at::kBFloat16);
         status = mx4_dequant_entry(&mx, rows, cols, y.data_ptr(), cols, stream_of(stream));
     }
     if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_dequant", status);
@@ -446,8 +455,8 @@ PyObject* mx4_gemm_nt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        const auto type = at::TensorOptions().dtype(wide ? at::kFloat : at::kBFloat16).device(A.device());
-        out = A.dim() == 2 ? at::empty({M, N}, type) : at::empty({A.size(0), A.size(1), N}, type);
+        const at::ScalarType type = wide ? at::kFloat : at::kBFloat16;
+        out = A.dim() == 2 ? fresh({M, N}, type) : fresh({A.size(0), A.size(1), N}, type);
         const int64_t need = mx4_gemm_workspace(batch, M, N, K);
         c10::optional<Workspace> workspace;
         if (need > 0) workspace.emplace(need, A.device(), at::TensorOptions().dtype(at::kByte).device(A.device()));
@@ -456,6 +465,32 @@ PyObject* mx4_gemm_nt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_gemm_nt", status);
     return wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// mx4_linear_fwd_bwd(X, W, dY, stream) -> [Y, dX, dW]
+PyObject* mx4_linear_fwd_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    at::Tensor X, W, dY, Y, dX, dW;
+    at::Tensor* const tensors[] = {&X, &W, &dY};
+    int64_t stream;
+    if (nargs != 4 || !tensors_of(args, tensors, 3) || !number(args[3], &stream)) Py_RETURN_NONE;
+    for (const at::Tensor* t : tensors)
+        if (!on(*t, at::kBFloat16, current_device()) || t->dim() != 2 || t->stride(1) != 1 || t->stride(0) < t->size(1)) Py_RETURN_NONE;
+    const int64_t T = X.size(0), K = X.size(1), N = W.size(0), need = mx4_step_workspace(T, K, N);
+    if (W.size(1) != K || dY.size(0) != T || dY.size(1) != N || need < 0) Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        Y = fresh({T, N}, at::kBFloat16);
+        dX = fresh({T, K}, at::kBFloat16);
+        dW = fresh({N, K}, at::kBFloat16);
+        const Workspace workspace(need, X.device(), at::TensorOptions().dtype(at::kByte).device(X.device()));
+        status = mx4_step_entry(X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), dY.data_ptr(), dY.stride(0), Y.data_ptr(), dX.data_ptr(), dW.data_ptr(), T, K, N,
+                                workspace.p, need, stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_linear_fwd_bwd", status);
+    return Py_BuildValue("[NNN]", wrap(Y), wrap(dX), wrap(dW));
     END_HANDLE_TH_ERRORS
 }
 
@@ -476,22 +511,21 @@ PyObject* rmsnorm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        const auto options = at::TensorOptions().device(x.device());
         const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
         ti8_rmsnorm_quant_args a = {};
         Mx4Out out;
-        rstd = at::empty(lead, options.dtype(at::kFloat));
-        if (r.defined()) h = at::empty(x.sizes(), options.dtype(at::kBFloat16));
+        rstd = fresh(lead, at::kFloat);
+        if (r.defined()) h = fresh(x.sizes(), at::kBFloat16);
         if (mx) {
-            out = Mx4Out(lead, rows, dim, options.dtype(at::kByte));
+            out = Mx4Out(lead, rows, dim);
             q = out.codes;
             s = out.scales;
             a.mx4 = out.mx;
         } else {
-            q = at::empty(x.sizes(), options.dtype(at::kChar));
-            std::vector<int64_t> sizes(lead.begin(), lead.end());
+            q = fresh(x.sizes(), at::kChar);
+            c10::SmallVector<int64_t, 4> sizes(lead.begin(), lead.end());
             if (group) sizes.push_back(dim / 128);
-            s = at::empty(sizes, options.dtype(at::kFloat));
+            s = fresh(sizes, at::kFloat);
             a.q = static_cast<int8_t*>(q.data_ptr());
             a.ldq = dim;
             a.s = static_cast<float*>(s.data_ptr());
@@ -531,7 +565,7 @@ PyObject* dequant_row(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        y = at::empty(q.sizes(), at::TensorOptions().dtype(at::kBFloat16).device(q.device()));
+        y = fresh(q.sizes(), at::kBFloat16);
         status = dequant_row_entry(static_cast<const int8_t*>(q.data_ptr()), cols, static_cast<const float*>(s.data_ptr()), rows, cols, by_group ? 128 : 0, y.data_ptr(), cols,
                                    stream_of(stream));
     }
@@ -540,10 +574,13 @@ PyObject* dequant_row(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
-// set_up_mx4(addresses of ti8_mx4_quant, ti8_mx4_dequant, ti8_mx4_gemm_nt, ti8_mx4_gemm_nt_workspace, ti8_rmsnorm_quant, ti8_dequant_row)
+// set_up_mx4(addresses of ti8_mx4_quant, ti8_mx4_dequant, ti8_mx4_gemm_nt, ti8_mx4_gemm_nt_workspace, ti8_mx4_linear_fwd_bwd,
+// ti8_mx4_linear_fwd_bwd_workspace, ti8_rmsnorm_quant, ti8_dequant_row)
 PyObject* set_up_mx4(PyObject*, PyObject* args) {
-    unsigned long long q, d, g, w, n, r;
-    if (!PyArg_ParseTuple(args, "KKKKKK", &q, &d, &g, &w, &n, &r)) return nullptr;
+    unsigned long long q, d, g, w, t, u, n, r;
+    if (!PyArg_ParseTuple(args, "KKKKKKKK", &q, &d, &g, &w, &t, &u, &n, &r)) return nullptr;
+    mx4_step_entry = reinterpret_cast<decltype(mx4_step_entry)>(t);
+    mx4_step_workspace = reinterpret_cast<decltype(mx4_step_workspace)>(u);
     mx4_quant_entry = reinterpret_cast<decltype(mx4_quant_entry)>(q);
     mx4_dequant_entry = reinterpret_cast<decltype(mx4_dequant_entry)>(d);
     mx4_gemm_entry = reinterpret_cast<decltype(mx4_gemm_entry)>(g);
@@ -587,6 +624,7 @@ PyMethodDef methods[] = {
     {"mx4_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_quant)), METH_FASTCALL, nullptr},
     {"mx4_dequant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_dequant)), METH_FASTCALL, nullptr},
     {"mx4_gemm_nt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_gemm_nt)), METH_FASTCALL, nullptr},
+    {"mx4_linear_fwd_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_linear_fwd_bwd)), METH_FASTCALL, nullptr},
     {"rmsnorm_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rmsnorm_quant)), METH_FASTCALL, nullptr},
     {"dequant_row", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_row)), METH_FASTCALL, nullptr},
     {"set_up", set_up, METH_VARARGS, nullptr},
@@ -603,7 +641,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 PyMODINIT_FUNC PyInit__native(void) {
     PyObject* const m = PyModule_Create(&module);
     PyObject* const built_for = Py_BuildValue("(s(ii)nnnnn)", TI8_BUILT_FOR_TORCH, PY_MAJOR_VERSION, PY_MINOR_VERSION, (Py_ssize_t)sizeof(ti8_linear_args), (Py_ssize_t)sizeof(ti8_gemm_problem),
-                                              (Py_ssize_t)sizeof(ti8_cache4), (Py_ssize_t)sizeof(ti8_mx4), (Py_ssize_t)sizeof(ti8_rmsnorm_quant_args));
+                                              (Py_ssize_t)sizeof(ti8_cache4), (Py_ssize_t)sizeof(ti8_mx4_operand), (Py_ssize_t)sizeof(ti8_rmsnorm_quant_args));
     if (m && (!built_for || PyModule_AddObject(m, "built_for", built_for) < 0)) {
         Py_XDECREF(built_for);
         Py_DECREF(m);

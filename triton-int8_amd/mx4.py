@@ -56,7 +56,8 @@ def _quant(x, by_rows, by_columns):
     _need(max(R, C) <= MOST_ROWS, f"a tensor in 4 bits has up to 2^28 rows and columns, got {R} x {C}")
     rows = _empty(R, C, x.device) if by_rows else None
     cols = _empty(C, R, x.device) if by_columns else None
-    _lib.call("ti8_mx4_quant", x.data_ptr(), ldx, R, C, None if rows is None else rows[2], None if cols is None else cols[2], _stream())
+    nothing = _lib.Mx4()
+    _lib.call("ti8_mx4_quant", _lib.Mx4Operand(x.data_ptr(), ldx, R, C, nothing if rows is None else rows[2], nothing if cols is None else cols[2]), 1, _stream())
     return None if rows is None else rows[:2], None if cols is None else cols[:2]
 
 
@@ -150,6 +151,11 @@ def _fit(X2, W, dY2=None):
           f"shapes do not fit: X {tuple(X2.shape)}, W {tuple(W.shape)}" + ("" if dY2 is None else f", dY {tuple(dY2.shape)}"))
 
 
+def _dense_rows(x):
+    """x itself where its rows are dense and do not overlap, else a copy."""
+    return x if (x.stride(1) == 1 or x.shape[1] == 1) and x.stride(0) >= x.shape[1] else x.clone(memory_format=torch.contiguous_format)
+
+
 def linear_fwd_bwd(X, W, dY):
     """One forward and backward of a layer, every product in 4 bits: ``(Y, dX, dW)`` for X bf16 [.., K], W bf16 [N, K] and dY bf16 [.., N].  The operands of
     dX = dY W are in 4 bits along N, those of dW = dY^T X along the tokens."""
@@ -158,12 +164,20 @@ def linear_fwd_bwd(X, W, dY):
     _fit(X2, W, dY2)
     if X2.shape[0] == 0:    # nothing to multiply: empty Y and dX, a zero weight gradient (as torch.nn.functional.linear gives)
         return X.new_empty((*X.shape[:-1], N)), torch.empty_like(X), torch.zeros_like(W)
-    for t, name in ((X2, "X"), (W, "W"), (dY2, "dY")):
-        _bf16(t, name)
-    x, sx, xt, sxt = quant_row_col_t(X2)
-    w, sw, wt, swt = quant_row_col_t(W)
-    d, sd, dt, sdt = quant_row_col_t(dY2)
-    return gemm_nt(x, sx, w, sw).view(*X.shape[:-1], N), gemm_nt(d, sd, wt, swt).view(X.shape), gemm_nt(dt, sdt, xt, sxt)
+    made = _natively("mx4_linear_fwd_bwd", X2, W, dY2)
+    if made is None:
+        for t, name in ((X2, "X"), (W, "W"), (dY2, "dY")):
+            _bf16(t, name)
+        X2, W, dY2 = (_dense_rows(t) for t in (X2, W, dY2))
+        T, dev = X2.shape[0], X2.device
+        need = _lib.lib().ti8_mx4_linear_fwd_bwd_workspace(T, K, N)
+        _need(need >= 0, f"a step takes up to 2^22 tokens and features, got {T}, {K} and {N}")
+        made = [torch.empty(shape, dtype=torch.bfloat16, device=dev) for shape in ((T, N), (T, K), (N, K))]
+        workspace = ops._workspace(need, dev)
+        _lib.call("ti8_mx4_linear_fwd_bwd", X2.data_ptr(), X2.stride(0), W.data_ptr(), W.stride(0), dY2.data_ptr(), dY2.stride(0), *(t.data_ptr() for t in made), T, K, N,
+                  workspace.data_ptr(), need, _stream())
+    Y, dX, dW = made
+    return Y.view(*X.shape[:-1], N), dX.view(X.shape), dW
 
 
 def _column_sum(x):
