@@ -1,7 +1,8 @@
-"""Llama-style decoder layer whose seven linears run on the INT8 path (forward and backward):
+"""Llama-style decoder layer whose seven linears run on the INT8 path, or in 4 bits (forward and backward):
 the training step either side of the hot path, as BASELINE config 5 describes it (hidden 4096,
 32 heads, MLP 14336, bf16 elsewhere).  RMSNorm, rotary embedding, causal attention (torch
-SDPA) and SwiGLU stay in bf16; ``int8=False`` builds the bf16 twin used for loss/grad parity.
+SDPA) and SwiGLU stay in bf16; ``int8=False`` builds the bf16 twin used for loss/grad parity, ``scheme="mx4"`` a layer of
+:class:`~triton_int8_amd.mx4.Mx4Linear`.
 
 In the int8 layer the RMSNorms, the rotary embedding and the SwiGLU product run as one kernel each per direction
 (csrc/decoder.hip), and the attention's backward as two (csrc/attention.hip); the twin, tensors those kernels do not take and calls under a tracer or a function transform go through the
@@ -15,7 +16,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import mx4, ops
 from .linear import Int8Linear, LinearGroupFunction, _one_group
 
 __all__ = ["DecoderLayer", "rope_tables"]
@@ -185,6 +186,8 @@ def _attention(q, k, v, scale):
 
 def _projections(x, *layers):
     """The layers' outputs for the same x."""
+    if mx4.all_as_written(layers):
+        return mx4.linears(x, layers)
     if _one_group(x, layers) and _kernels_take(x, *(m.weight for m in layers)):
         return LinearGroupFunction.apply(x, *(m.weight for m in layers))
     return tuple(m(x) for m in layers)
@@ -206,6 +209,10 @@ class RMSNorm(torch.nn.Module):
         return _rmsnorm(x, self.weight, self.eps)
 
 
+# the norm's call, to be told from one that replaces part of it
+_NORM_CALL = (RMSNorm.forward, RMSNorm.__call__, RMSNorm._call_impl)
+
+
 class DecoderLayer(torch.nn.Module):
     def __init__(self, hidden=4096, heads=32, mlp=14336, int8=True, scheme="block_channel", device=None):
         super().__init__()
@@ -213,6 +220,8 @@ class DecoderLayer(torch.nn.Module):
         self.hidden, self.heads, self.head_dim = hidden, heads, hidden // heads
 
         def lin(i, o):
+            if int8 and scheme == "mx4":
+                return mx4.Mx4Linear(i, o, device=device)
             if int8:
                 return Int8Linear(i, o, bias=False, scheme=scheme, device=device)
             m = torch.nn.Linear(i, o, bias=False, device=device, dtype=torch.bfloat16)
@@ -223,6 +232,27 @@ class DecoderLayer(torch.nn.Module):
         self.gate_proj, self.up_proj, self.down_proj = lin(hidden, mlp), lin(hidden, mlp), lin(mlp, hidden)
         self.int8 = int8
         self.input_norm, self.post_norm = RMSNorm(hidden, device=device, fused=int8), RMSNorm(hidden, device=device, fused=int8)
+
+    def _linears(self):
+        return self.q_proj, self.k_proj, self.v_proj, self.o_proj, self.gate_proj, self.up_proj, self.down_proj
+
+    def pack(self):
+        """The weights of a layer in 4 bits kept in 4 bits, for :meth:`serve` alone (:meth:`~triton_int8_amd.mx4.Mx4Linear.pack`); returns the layer."""
+        if not all(isinstance(m, mx4.Mx4Linear) for m in self._linears()):
+            raise ValueError('pack() is for a layer of scheme "mx4"')
+        for m in self._linears():
+            m.pack()
+        return self
+
+    def _norm_quantises(self, x):
+        """Whether norms and what quantises their results for the projections behind them may be one kernel each (ops.rmsnorm_quant)."""
+        return (mx4.all_as_written(self._linears()) and mx4._as_written((self.input_norm, self.post_norm), RMSNorm, _NORM_CALL)
+                and self.hidden % 8 == 0 and self.hidden <= 16384 and _kernels_take(x, self.input_norm.weight, self.post_norm.weight))
+
+    def _normed(self, x, norm, layers, residual=None):
+        """What layers make of the norm of x (+ residual): (their outputs, that sum)."""
+        q, s, _, *h = ops.rmsnorm_quant(x, norm.weight, norm.eps, residual=residual)
+        return mx4._served(q.view(-1, q.shape[-1]), s, x.shape[:-1], layers), h[0] if h else x
 
     def copy_weights_from(self, other):
         """Share initial values with another layer (int8 layer <-> bf16 twin)."""
@@ -267,15 +297,21 @@ class DecoderLayer(torch.nn.Module):
             # zeros all the way: norms, projections, attention and products of a row of zeros are zeros, which no scale that it shares with tokens notices
             x = x.masked_fill((token >= counts[:, None])[:, :, None], 0.0)
         cos, sin = cos.index_select(0, at), sin.index_select(0, at)
-        h = self.input_norm(x)
-        q, k, v = (t.view(1, B * S, self.heads, self.head_dim) for t in _projections(h, self.q_proj, self.k_proj, self.v_proj))
+        in_4_bits = self._norm_quantises(x)
+        if in_4_bits:
+            qkv, _ = self._normed(x, self.input_norm, (self.q_proj, self.k_proj, self.v_proj))
+        else:
+            qkv = _projections(self.input_norm(x), self.q_proj, self.k_proj, self.v_proj)
+        q, k, v = (t.view(1, B * S, self.heads, self.head_dim) for t in qkv)
         rotate = _RopeFunction.apply if self.int8 and self.head_dim % 16 == 0 and _kernels_take(q, k, cos, sin) else _rope_pair
         q, k = rotate(q, k, cos, sin)
         q, k, v = (t.reshape(B, S, self.heads, self.head_dim) for t in (q, k, v))
         cache.append(k, v, counts=counts)
-        a = cache.attend(q, counts=counts)
-        x = x + self.o_proj(a.view(B, S, H))
-        h = self.post_norm(x)
-        gate, up = _projections(h, self.gate_proj, self.up_proj)
+        a = self.o_proj(cache.attend(q, counts=counts).view(B, S, H))
+        if in_4_bits:
+            (gate, up), x = self._normed(a, self.post_norm, (self.gate_proj, self.up_proj), residual=x)
+        else:
+            x = x + a
+            gate, up = _projections(self.post_norm(x), self.gate_proj, self.up_proj)
         product = _SwiGLUFunction.apply if self.int8 and _kernels_take(gate, up) else _swiglu
         return x + self.down_proj(product(gate, up))

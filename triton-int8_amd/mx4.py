@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 from .ops import _natively, _need, _stream
 
-__all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "linear_fwd_bwd", "quant_col_t", "quant_row", "quant_row_col_t"]
+__all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "linear_fwd_bwd", "linears", "quant_col_t", "quant_row", "quant_row_col_t"]
 
 TILE = 256                  # elements of a row that take 128 bytes of codes and 8 scales
 MOST_ROWS = 1 << 28
@@ -220,27 +220,24 @@ class Mx4LinearFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *dys):
         wants_x, wants = ctx.needs_input_grad[0], ctx.needs_input_grad[1:]
-        kept = list(ctx.saved_tensors)
+        kept = ctx.saved_tensors
         K, tokens = ctx.shape[-1], ctx.shape[:-1].numel()
-        x = (kept.pop(0), kept.pop(0)) if kept and any(wants) else None
-        dx, dws = None, []
-        for i, d in enumerate(dys):
-            w = (kept.pop(0), kept.pop(0)) if kept and wants_x else None
-            if d is None:       # (an output that nobody uses: its weight has no gradient)
-                dws.append(None)
+        x, of_weights = kept[:2 * any(wants)], kept[2 * any(wants):]
+        dx, dws = None, [None] * len(dys)
+        # the last layer's part first, as autograd adds up those of separate calls
+        for i in reversed(range(len(dys))):
+            if dys[i] is None:       # (an output that nobody uses: its weight has no gradient)
                 continue
             if tokens == 0:
-                dws.append(d.new_zeros((ctx.features[i], K)) if wants[i] else None)
+                dx, dws[i] = dys[i].new_empty((0, K)), dys[i].new_zeros((ctx.features[i], K)) if wants[i] else None
                 continue
-            d2 = d.reshape(tokens, ctx.features[i])
-            rows, cols = _quant(d2, wants_x, wants[i])
+            rows, cols = _quant(dys[i].reshape(tokens, ctx.features[i]), wants_x, wants[i])
             if wants_x:
-                part = gemm_nt(*rows, *w)
+                part = gemm_nt(*rows, *of_weights[2 * i:2 * i + 2])
                 dx = part if dx is None else dx.add_(part)
-            dws.append(gemm_nt(*cols, *x) if wants[i] else None)
-        if wants_x and dx is None and any(d is not None for d in dys):
-            dx = next(d for d in dys if d is not None).new_empty((0, K))
-        return (None if dx is None else dx.view(ctx.shape), *dws)
+            if wants[i]:
+                dws[i] = gemm_nt(*cols, *x)
+        return (dx.view(ctx.shape) if wants_x and dx is not None else None, *dws)
 
 
 class _BiasFunction(torch.autograd.Function):
@@ -258,6 +255,38 @@ class _BiasFunction(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             db = _column_sum(d2) if d2.shape[0] else d2.new_zeros(d2.shape[1:])
         return d, db
+
+
+def _served(codes, scales, shape, layers):
+    """Outputs [*shape, out_features] of layers whose input is already in 4 bits."""
+    ys = (gemm_nt(codes, scales, *m.quantised()).view(*shape, m.out_features) for m in layers)
+    return tuple(y if m.bias is None else y + m.bias for y, m in zip(ys, layers))
+
+
+def linears(x, layers):
+    """The outputs of several :class:`Mx4Linear` for the same x, which is quantised once; the bits of separate calls."""
+    for m in layers:
+        _need(x.shape[-1] == m.in_features, f"expected {m.in_features} input features, got {x.shape[-1]}")
+    if torch.is_grad_enabled() and (x.requires_grad or any(not m.packed and m.weight.requires_grad for m in layers)):
+        _need(not any(m.packed for m in layers), "a packed layer serves the forward only: call it under torch.no_grad()")
+        ys = Mx4LinearFunction.apply(x, *(m.weight for m in layers))
+        return tuple(y if m.bias is None else _BiasFunction.apply(y, m.bias) for y, m in zip(ys, layers))
+    if x.numel() == 0:
+        return tuple(x.new_empty((*x.shape[:-1], m.out_features)) for m in layers)
+    return _served(*quant_row(x.reshape(-1, x.shape[-1])), x.shape[:-1], layers)
+
+
+def _as_written(modules, cls, call):
+    """Whether calls of these modules do just what their class does: no hooks, nothing replaced."""
+    if torch.nn.modules.module._has_any_global_hook() or (cls.forward, cls.__call__, cls._call_impl) != call:
+        return False
+    for m in modules:
+        own = m.__dict__
+        if type(m) is not cls or "forward" in own or "_call_impl" in own or m._compiled_call_impl is not None:
+            return False
+        if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
+            return False
+    return True
 
 
 class Mx4Linear(torch.nn.Module):
@@ -292,15 +321,16 @@ class Mx4Linear(torch.nn.Module):
         return (self.codes, self.scales) if self.packed else quant_row(self.weight.detach())
 
     def forward(self, x):
-        _need(x.shape[-1] == self.in_features, f"expected {self.in_features} input features, got {x.shape[-1]}")
-        if torch.is_grad_enabled() and (x.requires_grad or (not self.packed and self.weight.requires_grad)):
-            _need(not self.packed, "a packed layer serves the forward only: call it under torch.no_grad()")
-            y, = Mx4LinearFunction.apply(x, self.weight)
-            return y if self.bias is None else _BiasFunction.apply(y, self.bias)
-        if x.numel() == 0:
-            return x.new_empty((*x.shape[:-1], self.out_features))
-        y = gemm_nt(*quant_row(x.reshape(-1, x.shape[-1])), *self.quantised()).view(*x.shape[:-1], self.out_features)
-        return y if self.bias is None else y + self.bias
+        return linears(x, (self,))[0]
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, packed={self.packed}"
+
+
+# the module's call, to be told from one that replaces part of it
+_CALL = (Mx4Linear.forward, Mx4Linear.__call__, Mx4Linear._call_impl)
+
+
+def all_as_written(layers):
+    """Whether modules are :class:`Mx4Linear` whose calls do just what that does: then several may be one call."""
+    return _as_written(layers, Mx4Linear, _CALL)
