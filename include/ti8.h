@@ -590,9 +590,20 @@ int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t 
 /* bytes of workspace that the call above needs (0: none; -1 for sizes it does not take), 16-byte aligned, contents undefined before and after: few tiles over a
  * long K are shared among workgroups, whose parts are added up in order */
 int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K);
-/* One training step of a layer, every product in 4 bits: Y = X W^T, dX = dY W, dW = dY^T X, i.e. ti8_mx4_quant of X, W and dY both ways in one launch and three
- * times ti8_mx4_gemm_nt.  X bf16 [T][K] (ldx), W bf16 [N][K] (ldw), dY bf16 [T][N] (lddy), any alignment -> Y [T][N], dX [T][K], dW [N][K], dense bf16; any T, K and N
- * up to 2^22.  The outputs may be the inputs' memory.  workspace: ti8_mx4_linear_fwd_bwd_workspace bytes (-1 for sizes it does not take), 256-byte aligned, contents
+/* Up to 3 such products (batch 1), in one launch where that is faster: the bits of separate calls but for the order in which long contractions are added up.  `problems` is a HOST
+ * array.  workspace: the bytes that ti8_mx4_gemm_nt_multi_workspace gives for these sizes (it reads nothing else), -1 for those that are not taken.  Outputs share no
+ * memory with each other. */
+typedef struct {
+    ti8_mx4 a, b;
+    void* c; int64_t ldc;
+    int64_t M, N, K;
+    int wide;
+} ti8_mx4_gemm_problem;
+int64_t ti8_mx4_gemm_nt_multi_workspace(const ti8_mx4_gemm_problem* problems, int count);
+int ti8_mx4_gemm_nt_multi(const ti8_mx4_gemm_problem* problems, int count, void* workspace, int64_t workspace_bytes, ti8_stream_t stream);
+/* One training step of a layer, every product in 4 bits: Y = X W^T, dX = dY W, dW = dY^T X, i.e. ti8_mx4_quant of X, W and dY both ways in one launch and
+ * ti8_mx4_gemm_nt_multi of the three.  X bf16 [T][K] (ldx), W bf16 [N][K] (ldw), dY bf16 [T][N] (lddy), any alignment -> Y [T][N], dX [T][K], dW [N][K], dense bf16; any T, K and N
+ * up to 2^22.  The outputs may be the inputs' memory, and share none with each other.  workspace: ti8_mx4_linear_fwd_bwd_workspace bytes (-1 for sizes it does not take), 256-byte aligned, contents
  * undefined before and after. */
 int64_t ti8_mx4_linear_fwd_bwd_workspace(int64_t T, int64_t K, int64_t N);
 int ti8_mx4_linear_fwd_bwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* dY, int64_t lddy, void* Y, void* dX, void* dW,

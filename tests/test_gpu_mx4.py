@@ -193,8 +193,23 @@ def test_layer_forward_and_backward(M, dev, tokens, k, n):
     xd = x.to(dev).requires_grad_()
     y = layer(xd)
     y.backward(dy.to(dev))
-    for g, h, name in zip((y, xd.grad, layer.weight.grad), got, ("Y", "dX", "dW")):
-        assert bits_equal(g.detach(), h), name
+    for g, (v, mag), depth, name in zip((y, xd.grad, layer.weight.grad), want, (k, n, tokens), ("Y", "dX", "dW")):
+        close(g.detach(), v, mag, depth, name)
     with torch.no_grad():
-        assert bits_equal(layer(xd), got[0])
-        assert bits_equal(layer.pack()(xd), got[0]) and layer.weight is None and [n for n, _ in layer.named_buffers()] == ["codes", "scales"]
+        assert bits_equal(layer(xd), y.detach())
+        assert bits_equal(layer.pack()(xd), y.detach()) and layer.weight is None and [n for n, _ in layer.named_buffers()] == ["codes", "scales"]
+
+
+TOGETHER = [[(3, 64, 512), (3, 200, 512), (3, 16, 512)], [(30, 5000, 300), (30, 4000, 300)], [(100, 333, 1000), (257, 100, 40), (40, 1000, 5000)], [(1, 7, 256), (300, 300, 300), (20, 20, 20)],
+            [(5, 5, 16384), (8, 8, 10)], [(1000, 513, 700)], [(2050, 1030, 520), (1030, 520, 2050), (2050, 520, 1030)]]
+
+
+@pytest.mark.parametrize("sizes", TOGETHER, ids=str)
+def test_products_together(M, dev, sizes):
+    gen = make_gen(len(sizes))
+    inputs = [(tensor(gen, m, k), tensor(gen, n, k, spread=False)) for m, n, k in sizes]
+    got = M.gemm_nt_multi([(*M.quant_row(a.to(dev)), *M.quant_row(b.to(dev))) for a, b in inputs])
+    assert len(got) == len(sizes)
+    for c, (a, b), (m, n, k) in zip(got, inputs, sizes):
+        assert c.dtype == torch.bfloat16 and c.shape == (m, n)
+        close(c, *oracle.gemm_nt(oracle.rounded(a), oracle.rounded(b)), k, (m, n, k))

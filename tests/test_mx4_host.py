@@ -73,6 +73,29 @@ def test_step(lib, change, code, msg):
     assert got == code and msg in lib.lib().ti8_last_error().decode()
 
 
+def problem(lib, **other):
+    fields = dict(a=mx(lib), b=mx(lib), c=FAKE, ldc=64, M=64, N=64, K=512, wide=0)
+    return lib.Mx4GemmProblem(**{**fields, **other})
+
+
+@pytest.mark.parametrize("other,code,msg", [
+    (dict(c=None), 1, "required"), (dict(M=0), 2, "M"), (dict(K=(1 << 22) + 1), 2, "2^22"), (dict(ldc=63), 2, "ldc"), (dict(c=FAKE + 1), 3, "aligned"), (dict(N=65, ldc=65), 2, "scale_ld"),
+    (dict(K=513), 2, "ld")], ids=str)
+def test_several_products(lib, other, code, msg):
+    for at in range(3):
+        problems = (lib.Mx4GemmProblem * 3)(*(problem(lib, **(other if i == at else {})) for i in range(3)))
+        refused(lib, "ti8_mx4_gemm_nt_multi", code, msg, problems, 3, None, 0, None)
+    for count in (0, 4, -1):
+        refused(lib, "ti8_mx4_gemm_nt_multi", 2, "products", (lib.Mx4GemmProblem * 4)(*[problem(lib)] * 4), count, None, 0, None)
+        assert lib.lib().ti8_mx4_gemm_nt_multi_workspace((lib.Mx4GemmProblem * 4)(*[problem(lib)] * 4), count) == -1
+    refused(lib, "ti8_mx4_gemm_nt_multi", 1, "required", None, 1, None, 0, None)
+    long = lib.Mx4GemmProblem(mx(lib, 100, 16384), mx(lib, 100, 16384), FAKE, 100, 100, 100, 16384, 0)
+    need = lib.lib().ti8_mx4_gemm_nt_multi_workspace(long, 1)
+    assert need == lib.lib().ti8_mx4_gemm_nt_workspace(1, 100, 100, 16384) > 0
+    refused(lib, "ti8_mx4_gemm_nt_multi", 1, "workspace of", long, 1, FAKE, need - 1, None)
+    refused(lib, "ti8_mx4_gemm_nt_multi", 3, "16-byte", long, 1, FAKE + 8, need, None)
+
+
 def test_workspaces(lib):
     """Long contractions over few tiles are shared out; sizes that are not taken have no workspace."""
     l = lib.lib()
@@ -182,6 +205,9 @@ def test_python_refusals(recorded):
         M.linear_fwd_bwd(bf(5, 300), bf(7, 300), bf(6, 7))
     with pytest.raises(ValueError, match="positive"):
         M.Mx4Linear(0, 4)
+    for problems, msg in (([], "between 1 and 3"), ([(q, s, q, s)] * 4, "between 1 and 3"), ([(q, s, q, s), (q, s, q1, s1)], "as many tiles"), ([(q3, s3, q, s)], "matrices")):
+        with pytest.raises(ValueError, match=msg):
+            M.gemm_nt_multi(problems)
 
 
 def test_python_refusals_of_the_norm(recorded):
@@ -266,15 +292,15 @@ def test_gradients_that_are_not_wanted_are_not_computed(recorded):
     y, = T.mx4.Mx4LinearFunction.apply(x, w)
     calls.clear()
     y.sum().backward()
-    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][0].by_rows.codes is None
+    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt_multi"] and calls[0][1][0].by_rows.codes is None
     w.requires_grad_(False)
     y, = T.mx4.Mx4LinearFunction.apply(x.requires_grad_(), w)
     calls.clear()
     y.sum().backward()
-    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt"] and calls[0][1][0].by_columns.codes is None
+    assert names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt_multi"] and calls[0][1][0].by_columns.codes is None
     # one of several outputs that nobody uses
     a, b = torch.nn.Parameter(bf(24, 40)), torch.nn.Parameter(bf(8, 40))
     y, z = T.mx4.Mx4LinearFunction.apply(x, a, b)
     calls.clear()
     z.sum().backward()
-    assert a.grad is None and b.grad.shape == (8, 40) and names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt", "ti8_mx4_gemm_nt"]
+    assert a.grad is None and b.grad.shape == (8, 40) and names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt_multi"]

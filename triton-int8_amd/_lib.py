@@ -65,6 +65,11 @@ class Mx4Operand(ctypes.Structure):
     _fields_ = [("x", _vp), ("ldx", _i64), ("rows", _i64), ("cols", _i64), ("by_rows", Mx4), ("by_columns", Mx4)]
 
 
+class Mx4GemmProblem(ctypes.Structure):
+    """ti8_mx4_gemm_problem of include/ti8.h."""
+    _fields_ = [("a", Mx4), ("b", Mx4), ("c", _vp), ("ldc", _i64), ("M", _i64), ("N", _i64), ("K", _i64), ("wide", _int)]
+
+
 class RmsnormQuantArgs(ctypes.Structure):
     """ti8_rmsnorm_quant_args of include/ti8.h."""
     _fields_ = [("x", _vp), ("ldx", _i64), ("residual", _vp), ("ldr", _i64), ("w", _vp), ("h", _vp), ("ldh", _i64), ("rstd", _vp), ("rows", _i64), ("dim", _i64),
@@ -109,6 +114,7 @@ PROTOTYPES = {
     "ti8_mx4_quant": [ctypes.POINTER(Mx4Operand), _int, _vp],
     "ti8_mx4_dequant": [ctypes.POINTER(Mx4), _i64, _i64, _vp, _i64, _vp],
     "ti8_mx4_gemm_nt": [ctypes.POINTER(Mx4), _i64, ctypes.POINTER(Mx4), _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp],
+    "ti8_mx4_gemm_nt_multi": [ctypes.POINTER(Mx4GemmProblem), _int, _vp, _i64, _vp],
     "ti8_mx4_linear_fwd_bwd": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp],
     "ti8_rmsnorm_quant": [ctypes.POINTER(RmsnormQuantArgs), _vp],
     "ti8_dequant_row": [_vp, _i64, _vp, _i64, _i64, _int, _vp, _i64, _vp],
@@ -116,7 +122,7 @@ PROTOTYPES = {
 }
 EXPORTS = ["ti8_version", "ti8_last_error", "ti8_arch", "ti8_init", "ti8_last_gemm_kernel", "ti8_linear_fwd_bwd_workspace", "ti8_linear_workspace", "ti8_linear_group_workspace",
            "ti8_rmsnorm_bwd_workspace", "ti8_column_sum_workspace", "ti8_attention_bwd_workspace", "ti8_cache4_attention_workspace", "ti8_mx4_gemm_nt_workspace",
-           "ti8_mx4_linear_fwd_bwd_workspace"] + list(PROTOTYPES)
+           "ti8_mx4_gemm_nt_multi_workspace", "ti8_mx4_linear_fwd_bwd_workspace"] + list(PROTOTYPES)
 
 # enums of include/ti8.h
 Q_CLAMP, Q_EPS_ADD, Q_SCALE_BF16, Q_HAD128, Q_WS_PINGPONG, Q_WS_SECOND, Q_TORCH_ROUND, Q_TORCH_BF16, Q_WS_IS_ZERO, Q_SCALE_T = 1, 2, 4, 8, 16, 32, 64, 128, 256, 512
@@ -174,6 +180,8 @@ def lib():
         l.ti8_cache4_attention_workspace.argtypes = [ctypes.POINTER(Cache4), _i64, _i64]
         l.ti8_mx4_gemm_nt_workspace.restype = _i64
         l.ti8_mx4_gemm_nt_workspace.argtypes = [_i64] * 4
+        l.ti8_mx4_gemm_nt_multi_workspace.restype = _i64
+        l.ti8_mx4_gemm_nt_multi_workspace.argtypes = [ctypes.POINTER(Mx4GemmProblem), _int]
         l.ti8_mx4_linear_fwd_bwd_workspace.restype = _i64
         l.ti8_mx4_linear_fwd_bwd_workspace.argtypes = [_i64] * 3
         for name, args in PROTOTYPES.items():
@@ -238,14 +246,14 @@ def native():
         try:
             spec = importlib.util.spec_from_file_location("_native", NATIVE_PATH)
             module = importlib.util.module_from_spec(spec)
-            here = (str(torch.__version__), sys.version_info[:2], ctypes.sizeof(LinearArgs), ctypes.sizeof(GemmProblem), ctypes.sizeof(Cache4), ctypes.sizeof(Mx4Operand), ctypes.sizeof(RmsnormQuantArgs))
+            here = (str(torch.__version__), sys.version_info[:2], ctypes.sizeof(LinearArgs), ctypes.sizeof(GemmProblem), ctypes.sizeof(Cache4), ctypes.sizeof(Mx4Operand), ctypes.sizeof(Mx4GemmProblem), ctypes.sizeof(RmsnormQuantArgs))
             built_for = getattr(module, "built_for", None)
             if built_for != here:
                 raise ImportError(f"{NATIVE_PATH} was built for {built_for}, this is {here}")
             address = lambda name: ctypes.cast(getattr(lib(), name), _vp).value
             module.set_up(address("ti8_linear"), address("ti8_linear_quantise"), address("ti8_gemm_i8_nt_multi"), torch.nn.Parameter)
             module.set_up_cache4(*(address("ti8_cache4_" + name) for name in ("append", "read", "attention", "attention_workspace", "evict")))
-            module.set_up_mx4(*(address("ti8_" + name) for name in ("mx4_quant", "mx4_dequant", "mx4_gemm_nt", "mx4_gemm_nt_workspace", "mx4_linear_fwd_bwd",
+            module.set_up_mx4(*(address("ti8_" + name) for name in ("mx4_quant", "mx4_dequant", "mx4_gemm_nt", "mx4_gemm_nt_workspace", "mx4_gemm_nt_multi", "mx4_gemm_nt_multi_workspace", "mx4_linear_fwd_bwd",
                                                                 "mx4_linear_fwd_bwd_workspace", "rmsnorm_quant", "dequant_row")))
             _native = module
         except ImportError:

@@ -24,6 +24,13 @@ struct Gemm {
     int64_t part;
 };
 
+// Up to three products of a launch: number i has the workgroups from first[i] on (multiples of 8: workgroups go round the XCDs)
+constexpr int TOGETHER = 3;
+struct Gemms {
+    Gemm g[TOGETHER];
+    int first[TOGETHER + 1], count;
+};
+
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -60,8 +67,11 @@ constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * s
 constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14
 
 template <int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
+__global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemms all) {
 #if defined(__HIP_DEVICE_COMPILE__)
+    const int which = idx::gemm_multi_pick(blockIdx.x, all.first[1], all.first[2], all.count), block = blockIdx.x - all.first[which];
+    const Gemm& g = all.g[which];
+    if (block >= g.tiles_m * g.tiles_n) return;
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int A_INSTR = BM / 8 / NW, B_INSTR = BN / 8 / NW, A_BYTES = BM * 128, B_BYTES = BN * 128;
     constexpr int SA_INSTR = (BM / 32 + NW - 1) / NW, SB_INSTR = (BN / 32 + NW - 1) / NW, S_BYTES = (BM + BN) * 8, RING = scale_stages(STAGES);
@@ -71,7 +81,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
     uint8_t* const ldsB = smem + STAGES * A_BYTES;
     uint8_t* const ldsS = ldsB + STAGES * B_BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-    const idx::TileCoord tc = idx::gemm_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, idx::gemm_group_rows(BM), false);
+    const idx::TileCoord tc = idx::gemm_tile_of(block, g.tiles_m, g.tiles_n, idx::gemm_group_rows(BM), all.count > 1);
     const int m0 = tc.tile_m * BM, n0 = tc.tile_n * BN;
     const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
     const int rows_a = min(g.M - m0, BM), rows_b = min(g.N - n0, BN);
@@ -316,7 +326,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemm g) {
     else
         write(std::false_type(), [&](int64_t at, const uint4& v, int left) { store8(static_cast<uint16_t*>(g.C) + at, v, left); });
 #else
-    (void)g;
+    (void)all;
 #endif
 }
 
@@ -334,12 +344,15 @@ __device__ __forceinline__ v4f multiply16(const v4i& b, const v4i& a, const v4f&
 }
 
 template <int MB, int NB, int NW>
-__global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemm g) {
+__global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemms all) {
 #if defined(__HIP_DEVICE_COMPILE__)
+    const int which = idx::gemm_multi_pick(blockIdx.x, all.first[1], all.first[2], all.count);
+    const Gemm& g = all.g[which];
     constexpr int BLOCK = MB * NB * 256;        // elements of C here
     extern __shared__ __attribute__((aligned(16))) float parts[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * MB);
+    const int n0 = (blockIdx.x - all.first[which]) * (16 * NB), m0 = blockIdx.y * (16 * MB);
+    if (n0 >= g.N || m0 >= g.M) return;
     const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
     const uint8_t *pa[MB], *pb[NB], *qa[MB], *qb[NB];
 #pragma unroll
@@ -425,31 +438,50 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemm g) {
         }
     }
 #else
-    (void)g;
+    (void)all;
 #endif
 }
 
+// the workgroups of each product, and all of them
+template <class Blocks>
+int64_t share_out(Gemms& all, const Blocks& blocks) {
+    int64_t total = 0;
+    for (int i = 0; i <= TOGETHER; ++i) {
+        all.first[i] = (int)total;
+        if (i < all.count) total += (blocks(all.g[i]) + 7) / 8 * 8;
+        if (total > 0x3fffffff) return -1;
+    }
+    return all.count > 1 ? total : blocks(all.g[0]);
+}
+
 template <int MB, int NB, int NW>
-int launch_few(const char* fn, const Gemm& g, int64_t batch, hipStream_t st) {
+int launch_few(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     constexpr int LDS = MB * NB * 1024 * NW;
     static OncePerDevice once;
     const auto kernel = few_rows_kernel<MB, NB, NW>;
     if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
-    kernel<<<dim3((unsigned)((g.N + 16 * NB - 1) / (16 * NB)), (unsigned)((g.M + 16 * MB - 1) / (16 * MB)), (unsigned)batch), dim3(64 * NW), LDS, st>>>(g);
+    int most = 0;
+    for (int i = 0; i < all.count; ++i) most = all.g[i].M > most ? all.g[i].M : most;
+    const int64_t strips = share_out(all, [](const Gemm& g) { return (int64_t)(g.N + 16 * NB - 1) / (16 * NB); });
+    if (strips < 0) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    kernel<<<dim3((unsigned)strips, (unsigned)((most + 16 * MB - 1) / (16 * MB)), (unsigned)batch), dim3(64 * NW), LDS, st>>>(all);
     return check_launch(fn);
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES>
-int launch(const char* fn, Gemm g, int64_t batch, hipStream_t st) {
+int launch(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     constexpr int LDS = gemm_lds(BM, BN, STAGES);
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
     static OncePerDevice once;
     const auto kernel = gemm_kernel<BM, BN, WM, WN, STAGES>;
     if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
-    g.tiles_m = (g.M + BM - 1) / BM;
-    g.tiles_n = (g.N + BN - 1) / BN;
-    if ((int64_t)g.tiles_m * g.tiles_n > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(g);
+    const int64_t tiles = share_out(all, [](Gemm& g) {
+        g.tiles_m = (g.M + BM - 1) / BM;
+        g.tiles_n = (g.N + BN - 1) / BN;
+        return (int64_t)g.tiles_m * g.tiles_n;
+    });
+    if (tiles < 0 || tiles > 0x3fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    kernel<<<dim3((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(all);
     return check_launch(fn);
 }
 
@@ -488,60 +520,133 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ fro
 
 using namespace ti8;
 
-extern "C" int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || batch > 65535 || M > (1 << 28) || N > (1 << 28) || K > (1 << 22)) return -1;
-    const idx::Mx4Plan plan = idx::mx4_plan(M, N, idx::mx4_tiles(K), batch, device_cu_count());
-    return plan.parts > 1 ? plan.parts * batch * M * N * 4 : 0;
+namespace ti8 {
+namespace mx4 {
+namespace {
+int launch_plan(const char* fn, int kernel, const Gemms& all, int64_t batch, hipStream_t st) {
+    switch (kernel) {
+        case idx::MX4_FEW_16: return launch_few<1, 1, 8>(fn, all, batch, st);
+        case idx::MX4_FEW_32: return launch_few<2, 1, 8>(fn, all, batch, st);
+        case idx::MX4_TILES_32: return launch<32, 64, 1, 2, 4>(fn, all, batch, st);
+        case idx::MX4_TILES_64: return launch<64, 64, 2, 2, 4>(fn, all, batch, st);
+        case idx::MX4_TILES_128: return launch<128, 128, 2, 2, 3>(fn, all, batch, st);
+        case idx::MX4_TILES_128_TWO: return launch<128, 128, 2, 2, 2>(fn, all, batch, st);
+        default: return launch<256, 256, 2, 4, 2>(fn, all, batch, st);
+    }
 }
 
-extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc, int64_t batch, int64_t M, int64_t N,
-                               int64_t K, int wide, void* workspace, int64_t workspace_bytes, ti8_stream_t stream) {
-    const char* const fn = "ti8_mx4_gemm_nt";
-    if (!a || !b || !c) return fail(TI8_ERR_NULL, "%s: a, b and c are required", fn);
+int64_t parts_bytes(const idx::Mx4Plan& plan, int64_t elements) { return plan.parts > 1 ? plan.parts * elements * 4 : 0; }
+
+// What is checked of a product, and its description
+int describe(const char* fn, const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc, int64_t batch, int64_t M, int64_t N,
+             int64_t K, int wide, Gemm& g) {
+    if (!c) return fail(TI8_ERR_NULL, "%s: a, b and c are required", fn);
     if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || batch > 65535 || M > (1 << 28) || N > (1 << 28) || K > (1 << 22) || ldc < N || bsc < 0 || (rows_a != 0 && rows_a < M) ||
         (rows_b != 0 && rows_b < N))
         return fail(TI8_ERR_SHAPE, "%s: need M, N in 1 .. 2^28, K in 1 .. 2^22, batch in 1 .. 65535, ldc >= N and batches of as many rows; got M=%lld N=%lld K=%lld batch=%lld ldc=%lld "
                     "rows_a=%lld rows_b=%lld", fn, (long long)M, (long long)N, (long long)K, (long long)batch, (long long)ldc, (long long)rows_a, (long long)rows_b);
     // (the last row that any batch reads)
-    mx4::Tensor ta, tb;
-    if (int e = mx4::check(fn, "a", a, (batch - 1) * rows_a + M, K, ta)) return e;
-    if (int e = mx4::check(fn, "b", b, (batch - 1) * rows_b + N, K, tb)) return e;
+    Tensor ta, tb;
+    if (int e = check(fn, "a", a, (batch - 1) * rows_a + M, K, ta)) return e;
+    if (int e = check(fn, "b", b, (batch - 1) * rows_b + N, K, tb)) return e;
     if (ta.ld > (1 << 22) || tb.ld > (1 << 22)) return fail(TI8_ERR_SHAPE, "%s: rows of codes may be up to 2^22 bytes apart", fn);
     if (reinterpret_cast<uintptr_t>(c) & (wide ? 3 : 1)) return fail(TI8_ERR_ALIGN, "%s: c must be aligned to its elements", fn);
-    const idx::Mx4Plan plan = idx::mx4_plan(M, N, idx::mx4_tiles(K), batch, device_cu_count());
-    const int64_t need = plan.parts > 1 ? plan.parts * batch * M * N * 4 : 0;
+    g = Gemm{ta.codes, tb.codes, ta.scales, tb.scales, c, ta.ld, tb.ld, ta.scale_ld, tb.scale_ld, rows_a, rows_b, ldc, bsc, (int)M, (int)N, (int)idx::mx4_tiles(K), 0, 0, wide ? 1 : 0, 1, 0};
+    return TI8_OK;
+}
+}  // namespace
+}  // namespace mx4
+}  // namespace ti8
+
+extern "C" int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || batch <= 0 || batch > 65535 || M > (1 << 28) || N > (1 << 28) || K > (1 << 22)) return -1;
+    return mx4::parts_bytes(idx::mx4_plan(M, N, idx::mx4_tiles(K), batch, device_cu_count()), batch * M * N);
+}
+
+extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t rows_b, void* c, int64_t ldc, int64_t bsc, int64_t batch, int64_t M, int64_t N,
+                               int64_t K, int wide, void* workspace, int64_t workspace_bytes, ti8_stream_t stream) {
+    const char* const fn = "ti8_mx4_gemm_nt";
+    if (!a || !b) return fail(TI8_ERR_NULL, "%s: a, b and c are required", fn);
+    mx4::Gemms all;
+    all.count = 1;
+    mx4::Gemm& g = all.g[0];
+    if (int e = mx4::describe(fn, a, rows_a, b, rows_b, c, ldc, bsc, batch, M, N, K, wide, g)) return e;
+    const idx::Mx4Plan plan = idx::mx4_plan(M, N, g.nk, batch, device_cu_count());
+    const int64_t need = mx4::parts_bytes(plan, batch * M * N);
     if (need && (!workspace || workspace_bytes < need)) return fail(TI8_ERR_NULL, "%s: a workspace of %lld bytes is required", fn, (long long)need);
     if (need && !aligned16(workspace)) return fail(TI8_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
-    mx4::Gemm g{ta.codes, tb.codes, ta.scales, tb.scales, c, ta.ld, tb.ld, ta.scale_ld, tb.scale_ld, rows_a, rows_b, ldc, bsc, (int)M, (int)N, (int)idx::mx4_tiles(K), 0, 0, wide ? 1 : 0, plan.parts, 0};
     if (need) {
         g.C = workspace;
         g.wide = 1;
         g.ldc = N;
         g.bsc = M * N;
+        g.parts = plan.parts;
         g.part = batch * M * N;
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    int e = TI8_OK;
-    switch (plan.kernel) {
-        case idx::MX4_FEW_16: e = mx4::launch_few<1, 1, 8>(fn, g, batch, st); break;
-        case idx::MX4_FEW_32: e = mx4::launch_few<2, 1, 8>(fn, g, batch, st); break;
-        case idx::MX4_TILES_32: e = mx4::launch<32, 64, 1, 2, 4>(fn, g, batch, st); break;
-        case idx::MX4_TILES_64: e = mx4::launch<64, 64, 2, 2, 4>(fn, g, batch, st); break;
-        case idx::MX4_TILES_128: e = mx4::launch<128, 128, 2, 2, 3>(fn, g, batch, st); break;
-        case idx::MX4_TILES_128_TWO: e = mx4::launch<128, 128, 2, 2, 2>(fn, g, batch, st); break;
-        default: e = mx4::launch<256, 256, 2, 4, 2>(fn, g, batch, st); break;
-    }
-    if (e || !need) return e;
-    const int64_t blocks = (batch * M * ((N + 3) / 4) + 255) / 256;
+    const int64_t blocks = need ? (batch * M * ((N + 3) / 4) + 255) / 256 : 0;
     if (blocks > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (int e = mx4::launch_plan(fn, plan.kernel, all, batch, st)) return e;
+    if (!need) return TI8_OK;
     mx4::join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float*>(workspace), plan.parts, g.part, batch * M, (int)M, (int)N, c, ldc, bsc, wide ? 1 : 0);
     return check_launch(fn);
+}
+
+extern "C" int64_t ti8_mx4_gemm_nt_multi_workspace(const ti8_mx4_gemm_problem* problems, int count) {
+    if (!problems || count < 1 || count > mx4::TOGETHER) return -1;
+    int64_t sizes[mx4::TOGETHER][3], most = 0;
+    for (int i = 0; i < count; ++i) {
+        const ti8_mx4_gemm_problem& p = problems[i];
+        const int64_t need = ti8_mx4_gemm_nt_workspace(1, p.M, p.N, p.K);
+        if (need < 0) return -1;
+        if (need > most) most = need;
+        sizes[i][0] = p.M;
+        sizes[i][1] = p.N;
+        sizes[i][2] = idx::mx4_tiles(p.K);
+    }
+    return count > 1 && idx::mx4_plan_together(sizes, count, device_cu_count()) >= 0 ? 0 : most;
+}
+
+extern "C" int ti8_mx4_gemm_nt_multi(const ti8_mx4_gemm_problem* problems, int count, void* workspace, int64_t workspace_bytes, ti8_stream_t stream) {
+    const char* const fn = "ti8_mx4_gemm_nt_multi";
+    if (!problems) return fail(TI8_ERR_NULL, "%s: problems are required", fn);
+    if (count < 1 || count > mx4::TOGETHER) return fail(TI8_ERR_SHAPE, "%s: need 1 to %d products, got %d", fn, mx4::TOGETHER, count);
+    mx4::Gemms all;
+    all.count = count;
+    int64_t sizes[mx4::TOGETHER][3];
+    // the longest contractions first: the short ones fill up what they leave
+    int order[mx4::TOGETHER] = {0, 1, 2};
+    for (int i = 1; i < count; ++i)
+        for (int j = i; j > 0 && problems[order[j]].K > problems[order[j - 1]].K; --j) {
+            const int t = order[j];
+            order[j] = order[j - 1];
+            order[j - 1] = t;
+        }
+    for (int i = 0; i < count; ++i) {
+        const ti8_mx4_gemm_problem& p = problems[order[i]];
+        if (int e = mx4::describe(fn, &p.a, 0, &p.b, 0, p.c, p.ldc, 0, 1, p.M, p.N, p.K, p.wide, all.g[i])) return e;
+        int64_t* const size = sizes[order[i]];     // (in the caller's order, as the workspace was asked for: the plan's sums are the same)
+        size[0] = p.M;
+        size[1] = p.N;
+        size[2] = all.g[i].nk;
+    }
+    const int kernel = count > 1 ? idx::mx4_plan_together(sizes, count, device_cu_count()) : -1;
+    if (kernel >= 0) return mx4::launch_plan(fn, kernel, all, 1, static_cast<hipStream_t>(stream));
+    const int64_t need = ti8_mx4_gemm_nt_multi_workspace(problems, count);
+    if (need && (!workspace || workspace_bytes < need)) return fail(TI8_ERR_NULL, "%s: a workspace of %lld bytes is required", fn, (long long)need);
+    if (need && !aligned16(workspace)) return fail(TI8_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", fn);
+    for (int i = 0; i < count; ++i) {
+        const ti8_mx4_gemm_problem& p = problems[i];
+        if (int e = ti8_mx4_gemm_nt(&p.a, 0, &p.b, 0, p.c, p.ldc, 0, 1, p.M, p.N, p.K, p.wide, workspace, workspace_bytes, stream)) return e;
+    }
+    return TI8_OK;
 }
 
 namespace {
 // Where a step's operands lie in its workspace: X, W and dY by rows and by columns, and behind them what the products need
 struct Mx4Step {
     ti8_mx4_operand o[3];
+    ti8_mx4_gemm_problem p[3];
     int64_t products, bytes;
     bool ok;
 };
@@ -570,11 +675,11 @@ Mx4Step mx4_step(int64_t T, int64_t K, int64_t N, char* base) {
         s.o[i].by_rows = room(rows[i], cols[i]);
         s.o[i].by_columns = room(cols[i], rows[i]);
     }
-    const int64_t sizes[3][3] = {{T, N, K}, {T, K, N}, {N, K, T}};
-    for (const auto& p : sizes) {
-        const int64_t need = ti8_mx4_gemm_nt_workspace(1, p[0], p[1], p[2]);
-        if (need > s.products) s.products = need;
-    }
+    const ti8_mx4_operand &x = s.o[0], &w = s.o[1], &d = s.o[2];
+    s.p[0] = {x.by_rows, w.by_rows, nullptr, N, T, N, K, 0};
+    s.p[1] = {d.by_rows, w.by_columns, nullptr, K, T, K, N, 0};
+    s.p[2] = {d.by_columns, x.by_columns, nullptr, K, N, K, T, 0};
+    s.products = ti8_mx4_gemm_nt_multi_workspace(s.p, 3);
     take(s.products);
     return s;
 }
@@ -604,8 +709,7 @@ extern "C" int ti8_mx4_linear_fwd_bwd(const void* X, int64_t ldx, const void* W,
     // launches anything)
     if (int e = ti8_mx4_quant(s.o, 3, stream)) return e;
     char* const products = static_cast<char*>(workspace) + (s.bytes - (s.products + 255) / 256 * 256);
-    const ti8_mx4_operand &x4 = s.o[0], &w4 = s.o[1], &d4 = s.o[2];
-    if (int e = ti8_mx4_gemm_nt(&x4.by_rows, 0, &w4.by_rows, 0, Y, N, 0, 1, T, N, K, 0, products, s.products, stream)) return e;
-    if (int e = ti8_mx4_gemm_nt(&d4.by_rows, 0, &w4.by_columns, 0, dX, K, 0, 1, T, K, N, 0, products, s.products, stream)) return e;
-    return ti8_mx4_gemm_nt(&d4.by_columns, 0, &x4.by_columns, 0, dW, K, 0, 1, N, K, T, 0, products, s.products, stream);
+    void* const to[3] = {Y, dX, dW};
+    for (int i = 0; i < 3; ++i) s.p[i].c = to[i];
+    return ti8_mx4_gemm_nt_multi(s.p, 3, products, s.products, stream);
 }

@@ -34,6 +34,8 @@ decltype(&ti8_mx4_quant) mx4_quant_entry = nullptr;
 decltype(&ti8_mx4_dequant) mx4_dequant_entry = nullptr;
 decltype(&ti8_mx4_gemm_nt) mx4_gemm_entry = nullptr;
 decltype(&ti8_mx4_gemm_nt_workspace) mx4_gemm_workspace = nullptr;
+decltype(&ti8_mx4_gemm_nt_multi) mx4_multi_entry = nullptr;
+decltype(&ti8_mx4_gemm_nt_multi_workspace) mx4_multi_workspace = nullptr;
 decltype(&ti8_mx4_linear_fwd_bwd) mx4_step_entry = nullptr;
 decltype(&ti8_mx4_linear_fwd_bwd_workspace) mx4_step_workspace = nullptr;
 decltype(&ti8_rmsnorm_quant) rmsnorm_quant_entry = nullptr;
@@ -468,6 +470,45 @@ PyObject* mx4_gemm_nt(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// mx4_gemm_nt_multi(A, scales of A, B, scales of B, of the next product likewise .., stream) -> [C ..] in bf16
+PyObject* mx4_gemm_nt_multi(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const int count = (int)(nargs - 1) / 4;
+    int64_t stream;
+    if (count < 1 || count > 3 || nargs != 4 * count + 1 || !number(args[4 * count], &stream)) Py_RETURN_NONE;
+    at::Tensor t[12], out[3];
+    at::Tensor* tensors[12];
+    for (int i = 0; i < 4 * count; ++i) tensors[i] = &t[i];
+    if (!tensors_of(args, tensors, 4 * count)) Py_RETURN_NONE;
+    ti8_mx4_gemm_problem p[3] = {};
+    for (int i = 0; i < count; ++i) {
+        const at::Tensor *A = &t[4 * i], *B = &t[4 * i + 2];
+        if (!mx4_operand(A[0], A[1], current_device(), &p[i].a) || !mx4_operand(B[0], B[1], current_device(), &p[i].b) || A->dim() != 2 || B->dim() != 2 || A->size(1) != B->size(1)) Py_RETURN_NONE;
+        p[i].M = A->size(0);
+        p[i].N = p[i].ldc = B->size(0);
+        p[i].K = A->size(1) * 2;
+    }
+    const int64_t need = mx4_multi_workspace(p, count);
+    if (need < 0) Py_RETURN_NONE;
+    int status;
+    {
+        const GilReleased released;
+        c10::optional<Workspace> workspace;
+        if (need > 0) workspace.emplace(need, t[0].device(), at::TensorOptions().dtype(at::kByte).device(t[0].device()));
+        for (int i = 0; i < count; ++i) {
+            out[i] = fresh({p[i].M, p[i].N}, at::kBFloat16);
+            p[i].c = out[i].data_ptr();
+        }
+        status = mx4_multi_entry(p, count, workspace ? workspace->p : nullptr, need, stream_of(stream));
+    }
+    if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_gemm_nt_multi", status);
+    PyObject* const list = PyList_New(count);
+    if (!list) return nullptr;
+    for (int i = 0; i < count; ++i) PyList_SET_ITEM(list, i, wrap(out[i]));
+    return list;
+    END_HANDLE_TH_ERRORS
+}
+
 // mx4_linear_fwd_bwd(X, W, dY, stream) -> [Y, dX, dW]
 PyObject* mx4_linear_fwd_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -574,11 +615,13 @@ PyObject* dequant_row(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
-// set_up_mx4(addresses of ti8_mx4_quant, ti8_mx4_dequant, ti8_mx4_gemm_nt, ti8_mx4_gemm_nt_workspace, ti8_mx4_linear_fwd_bwd,
+// set_up_mx4(addresses of ti8_mx4_quant, ti8_mx4_dequant, ti8_mx4_gemm_nt, ti8_mx4_gemm_nt_workspace, ti8_mx4_gemm_nt_multi, ti8_mx4_gemm_nt_multi_workspace, ti8_mx4_linear_fwd_bwd,
 // ti8_mx4_linear_fwd_bwd_workspace, ti8_rmsnorm_quant, ti8_dequant_row)
 PyObject* set_up_mx4(PyObject*, PyObject* args) {
-    unsigned long long q, d, g, w, t, u, n, r;
-    if (!PyArg_ParseTuple(args, "KKKKKKKK", &q, &d, &g, &w, &t, &u, &n, &r)) return nullptr;
+    unsigned long long q, d, g, w, m, v, t, u, n, r;
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKK", &q, &d, &g, &w, &m, &v, &t, &u, &n, &r)) return nullptr;
+    mx4_multi_entry = reinterpret_cast<decltype(mx4_multi_entry)>(m);
+    mx4_multi_workspace = reinterpret_cast<decltype(mx4_multi_workspace)>(v);
     mx4_step_entry = reinterpret_cast<decltype(mx4_step_entry)>(t);
     mx4_step_workspace = reinterpret_cast<decltype(mx4_step_workspace)>(u);
     mx4_quant_entry = reinterpret_cast<decltype(mx4_quant_entry)>(q);
@@ -624,6 +667,7 @@ PyMethodDef methods[] = {
     {"mx4_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_quant)), METH_FASTCALL, nullptr},
     {"mx4_dequant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_dequant)), METH_FASTCALL, nullptr},
     {"mx4_gemm_nt", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_gemm_nt)), METH_FASTCALL, nullptr},
+    {"mx4_gemm_nt_multi", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_gemm_nt_multi)), METH_FASTCALL, nullptr},
     {"mx4_linear_fwd_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx4_linear_fwd_bwd)), METH_FASTCALL, nullptr},
     {"rmsnorm_quant", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rmsnorm_quant)), METH_FASTCALL, nullptr},
     {"dequant_row", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_row)), METH_FASTCALL, nullptr},
@@ -640,8 +684,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 // library's argument blocks are read and written here without a call)
 PyMODINIT_FUNC PyInit__native(void) {
     PyObject* const m = PyModule_Create(&module);
-    PyObject* const built_for = Py_BuildValue("(s(ii)nnnnn)", TI8_BUILT_FOR_TORCH, PY_MAJOR_VERSION, PY_MINOR_VERSION, (Py_ssize_t)sizeof(ti8_linear_args), (Py_ssize_t)sizeof(ti8_gemm_problem),
-                                              (Py_ssize_t)sizeof(ti8_cache4), (Py_ssize_t)sizeof(ti8_mx4_operand), (Py_ssize_t)sizeof(ti8_rmsnorm_quant_args));
+    PyObject* const built_for = Py_BuildValue("(s(ii)nnnnnn)", TI8_BUILT_FOR_TORCH, PY_MAJOR_VERSION, PY_MINOR_VERSION, (Py_ssize_t)sizeof(ti8_linear_args), (Py_ssize_t)sizeof(ti8_gemm_problem),
+                                              (Py_ssize_t)sizeof(ti8_cache4), (Py_ssize_t)sizeof(ti8_mx4_operand), (Py_ssize_t)sizeof(ti8_mx4_gemm_problem), (Py_ssize_t)sizeof(ti8_rmsnorm_quant_args));
     if (m && (!built_for || PyModule_AddObject(m, "built_for", built_for) < 0)) {
         Py_XDECREF(built_for);
         Py_DECREF(m);

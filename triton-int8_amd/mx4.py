@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, ops
 from .ops import _natively, _need, _stream
 
-__all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "linear_fwd_bwd", "linears", "quant_col_t", "quant_row", "quant_row_col_t"]
+__all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "gemm_nt_multi", "linear_fwd_bwd", "linears", "quant_col_t", "quant_row", "quant_row_col_t"]
 
 TILE = 256                  # elements of a row that take 128 bytes of codes and 8 scales
 MOST_ROWS = 1 << 28
@@ -146,6 +146,29 @@ def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
     return out
 
 
+def gemm_nt_multi(problems):
+    """Up to three products ``(A, sA, B, sB)`` of matrices, in one launch where that is faster: a list of bf16 matrices.  What :func:`gemm_nt` gives, but for the order
+    in which long contractions may be added up."""
+    _need(1 <= len(problems) <= 3, f"between 1 and 3 products, got {len(problems)}")
+    made = _natively("mx4_gemm_nt_multi", *(t for p in problems for t in p))
+    if made is not None:
+        return made
+    descs, outs, keep = (_lib.Mx4GemmProblem * len(problems))(), [], []
+    for i, (A, sA, B, sB) in enumerate(problems):
+        A, sA, a = _operand(A, sA, "A")
+        B, sB, b = _operand(B, sB, "B")
+        _need(A.dim() == B.dim() == 2 and A.shape[1] == B.shape[1], f"need matrices of as many tiles along the contraction, got codes {tuple(A.shape)} and {tuple(B.shape)}")
+        M, N, K = A.shape[0], B.shape[0], A.shape[1] * 2
+        _need(max(M, N) <= MOST_ROWS and K <= MOST_CONTRACTED, f"a product takes up to 2^28 rows and contracts up to 2^22 elements, got {M}, {N} and {K}")
+        outs.append(torch.empty((M, N), dtype=torch.bfloat16, device=A.device))
+        descs[i] = _lib.Mx4GemmProblem(a, b, outs[-1].data_ptr(), N, M, N, K, 0)
+        keep.append((A, sA, B, sB))     # (copies stay alive until the launch is queued)
+    need = _lib.lib().ti8_mx4_gemm_nt_multi_workspace(descs, len(problems))
+    workspace = torch.empty((need,), dtype=torch.uint8, device=outs[0].device) if need > 0 else None
+    _lib.call("ti8_mx4_gemm_nt_multi", descs, len(problems), None if workspace is None else workspace.data_ptr(), need, _stream())
+    return outs
+
+
 def _fit(X2, W, dY2=None):
     _need(W.dim() == 2 and X2.shape[1] == W.shape[1] and (dY2 is None or tuple(dY2.shape) == (X2.shape[0], W.shape[0])),
           f"shapes do not fit: X {tuple(X2.shape)}, W {tuple(W.shape)}" + ("" if dY2 is None else f", dY {tuple(dY2.shape)}"))
@@ -186,6 +209,12 @@ def _column_sum(x):
     return ops.column_sum(x if cols % 32 == 0 else torch.nn.functional.pad(x, (0, -cols % 32)))[:cols]
 
 
+def _products(codes, scales, views, shape):
+    """Outputs [*shape, features] for an input in 4 bits and the forward's views of several weights: three to a launch."""
+    ys = [y for i in range(0, len(views), 3) for y in gemm_nt_multi([(codes, scales, *v) for v in views[i:i + 3]])]
+    return tuple(y.view(*shape, y.shape[1]) for y in ys)
+
+
 class Mx4LinearFunction(torch.autograd.Function):
     """The products of one x with several weights, each ``x W^T`` with all of its operands, and those of its gradients, in 4 bits; x is quantised once.
     The backward reads what the forward quantised: neither x nor the weights are kept."""
@@ -201,7 +230,7 @@ class Mx4LinearFunction(torch.autograd.Function):
         if x2.shape[0] == 0:
             return tuple(x.new_empty((*x.shape[:-1], n)) for n in ctx.features)
         _bf16(x, "x")
-        kept, ys = [], []
+        kept, views = [], []
         if any(ctx.needs_input_grad[1:]):
             xq, xs, *kept = quant_row_col_t(x2)
         else:
@@ -212,9 +241,9 @@ class Mx4LinearFunction(torch.autograd.Function):
                 kept += transposed
             else:
                 q, s = quant_row(w)
-            ys.append(gemm_nt(xq, xs, q, s).view(*x.shape[:-1], w.shape[0]))
+            views.append((q, s))
         ctx.save_for_backward(*kept)
-        return tuple(ys)
+        return _products(xq, xs, views, x.shape[:-1])
 
     @staticmethod
     @once_differentiable
@@ -226,17 +255,17 @@ class Mx4LinearFunction(torch.autograd.Function):
         dx, dws = None, [None] * len(dys)
         # the last layer's part first, as autograd adds up those of separate calls
         for i in reversed(range(len(dys))):
-            if dys[i] is None:       # (an output that nobody uses: its weight has no gradient)
+            if dys[i] is None or not (wants_x or wants[i]):     # (an output that nobody uses: its weight has no gradient)
                 continue
             if tokens == 0:
                 dx, dws[i] = dys[i].new_empty((0, K)), dys[i].new_zeros((ctx.features[i], K)) if wants[i] else None
                 continue
             rows, cols = _quant(dys[i].reshape(tokens, ctx.features[i]), wants_x, wants[i])
+            made = gemm_nt_multi(([(*rows, *of_weights[2 * i:2 * i + 2])] if wants_x else []) + ([(*cols, *x)] if wants[i] else []))
             if wants_x:
-                part = gemm_nt(*rows, *of_weights[2 * i:2 * i + 2])
-                dx = part if dx is None else dx.add_(part)
+                dx = made[0] if dx is None else dx.add_(made[0])
             if wants[i]:
-                dws[i] = gemm_nt(*cols, *x)
+                dws[i] = made[-1]
         return (dx.view(ctx.shape) if wants_x and dx is not None else None, *dws)
 
 
@@ -259,12 +288,12 @@ class _BiasFunction(torch.autograd.Function):
 
 def _served(codes, scales, shape, layers):
     """Outputs [*shape, out_features] of layers whose input is already in 4 bits."""
-    ys = (gemm_nt(codes, scales, *m.quantised()).view(*shape, m.out_features) for m in layers)
+    ys = _products(codes, scales, [m.quantised() for m in layers], shape)
     return tuple(y if m.bias is None else y + m.bias for y, m in zip(ys, layers))
 
 
 def linears(x, layers):
-    """The outputs of several :class:`Mx4Linear` for the same x, which is quantised once; the bits of separate calls."""
+    """The outputs of several :class:`Mx4Linear` for the same x, which is quantised once, three products to a launch."""
     for m in layers:
         _need(x.shape[-1] == m.in_features, f"expected {m.in_features} input features, got {x.shape[-1]}")
     if torch.is_grad_enabled() and (x.requires_grad or any(not m.packed and m.weight.requires_grad for m in layers)):
