@@ -31,6 +31,18 @@ struct Gemms {
     int first[TOGETHER + 1], count;
 };
 
+// This workgroup's product, and its number there.  A launch of one product is a kernel of its own: looking the product up takes 0.6 us before the first load
+// (16 x 4096 x 4096 5.0 us / 4.5, 128 x 4096 x 4096 7.7 / 7.2).
+__device__ __forceinline__ const Gemm& product_of(const Gemm& g, int& block) {
+    block = blockIdx.x;
+    return g;
+}
+__device__ __forceinline__ const Gemm& product_of(const Gemms& all, int& block) {
+    const int which = idx::gemm_multi_pick(blockIdx.x, all.first[1], all.first[2], all.count);
+    block = blockIdx.x - all.first[which];
+    return all.g[which];
+}
+
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -66,12 +78,13 @@ constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
 constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
 constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14
 
-template <int BM, int BN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemms all) {
+template <int BM, int BN, int WM, int WN, int STAGES, class Products>
+__global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int which = idx::gemm_multi_pick(blockIdx.x, all.first[1], all.first[2], all.count), block = blockIdx.x - all.first[which];
-    const Gemm& g = all.g[which];
-    if (block >= g.tiles_m * g.tiles_n) return;
+    constexpr bool MANY = std::is_same<Products, Gemms>::value;
+    int block;
+    const Gemm& g = product_of(products, block);
+    if (MANY && block >= g.tiles_m * g.tiles_n) return;
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int A_INSTR = BM / 8 / NW, B_INSTR = BN / 8 / NW, A_BYTES = BM * 128, B_BYTES = BN * 128;
     constexpr int SA_INSTR = (BM / 32 + NW - 1) / NW, SB_INSTR = (BN / 32 + NW - 1) / NW, S_BYTES = (BM + BN) * 8, RING = scale_stages(STAGES);
@@ -81,7 +94,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemms all) {
     uint8_t* const ldsB = smem + STAGES * A_BYTES;
     uint8_t* const ldsS = ldsB + STAGES * B_BYTES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-    const idx::TileCoord tc = idx::gemm_tile_of(block, g.tiles_m, g.tiles_n, idx::gemm_group_rows(BM), all.count > 1);
+    const idx::TileCoord tc = idx::gemm_tile_of(block, g.tiles_m, g.tiles_n, idx::gemm_group_rows(BM), MANY);
     const int m0 = tc.tile_m * BM, n0 = tc.tile_n * BN;
     const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
     const int rows_a = min(g.M - m0, BM), rows_b = min(g.N - n0, BN);
@@ -326,7 +339,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Gemms all) {
     else
         write(std::false_type(), [&](int64_t at, const uint4& v, int left) { store8(static_cast<uint16_t*>(g.C) + at, v, left); });
 #else
-    (void)all;
+    (void)products;
 #endif
 }
 
@@ -343,15 +356,15 @@ __device__ __forceinline__ v4f multiply16(const v4i& b, const v4i& a, const v4f&
 #endif
 }
 
-template <int MB, int NB, int NW>
-__global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemms all) {
+template <int MB, int NB, int NW, class Products>
+__global__ __launch_bounds__(64 * NW) void few_rows_kernel(Products products) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int which = idx::gemm_multi_pick(blockIdx.x, all.first[1], all.first[2], all.count);
-    const Gemm& g = all.g[which];
+    int block;
+    const Gemm& g = product_of(products, block);
     constexpr int BLOCK = MB * NB * 256;        // elements of C here
     extern __shared__ __attribute__((aligned(16))) float parts[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, q = lane >> 4;
-    const int n0 = (blockIdx.x - all.first[which]) * (16 * NB), m0 = blockIdx.y * (16 * MB);
+    const int n0 = block * (16 * NB), m0 = blockIdx.y * (16 * MB);
     if (n0 >= g.N || m0 >= g.M) return;
     const int64_t first_a = blockIdx.z * g.rows_a + m0, first_b = blockIdx.z * g.rows_b + n0;
     const uint8_t *pa[MB], *pb[NB], *qa[MB], *qb[NB];
@@ -438,7 +451,7 @@ __global__ __launch_bounds__(64 * NW) void few_rows_kernel(Gemms all) {
         }
     }
 #else
-    (void)all;
+    (void)products;
 #endif
 }
 
@@ -457,14 +470,16 @@ int64_t share_out(Gemms& all, const Blocks& blocks) {
 template <int MB, int NB, int NW>
 int launch_few(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     constexpr int LDS = MB * NB * 1024 * NW;
-    static OncePerDevice once;
-    const auto kernel = few_rows_kernel<MB, NB, NW>;
-    if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
+    static_assert(LDS <= 64 * 1024, "no limit to raise");
     int most = 0;
     for (int i = 0; i < all.count; ++i) most = all.g[i].M > most ? all.g[i].M : most;
     const int64_t strips = share_out(all, [](const Gemm& g) { return (int64_t)(g.N + 16 * NB - 1) / (16 * NB); });
     if (strips < 0) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    kernel<<<dim3((unsigned)strips, (unsigned)((most + 16 * MB - 1) / (16 * MB)), (unsigned)batch), dim3(64 * NW), LDS, st>>>(all);
+    const dim3 grid((unsigned)strips, (unsigned)((most + 16 * MB - 1) / (16 * MB)), (unsigned)batch), block(64 * NW);
+    if (all.count > 1)
+        few_rows_kernel<MB, NB, NW, Gemms><<<grid, block, LDS, st>>>(all);
+    else
+        few_rows_kernel<MB, NB, NW, Gemm><<<grid, block, LDS, st>>>(all.g[0]);
     return check_launch(fn);
 }
 
@@ -472,17 +487,19 @@ template <int BM, int BN, int WM, int WN, int STAGES>
 int launch(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     constexpr int LDS = gemm_lds(BM, BN, STAGES);
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
-    static OncePerDevice once;
-    const auto kernel = gemm_kernel<BM, BN, WM, WN, STAGES>;
-    if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
     const int64_t tiles = share_out(all, [](Gemm& g) {
         g.tiles_m = (g.M + BM - 1) / BM;
         g.tiles_n = (g.N + BN - 1) / BN;
         return (int64_t)g.tiles_m * g.tiles_n;
     });
     if (tiles < 0 || tiles > 0x3fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    kernel<<<dim3((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(all);
-    return check_launch(fn);
+    const auto run = [&](auto kernel, OncePerDevice& once, const auto& products) {
+        if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
+        kernel<<<dim3((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(products);
+        return check_launch(fn);
+    };
+    static OncePerDevice one, many;
+    return all.count > 1 ? run(gemm_kernel<BM, BN, WM, WN, STAGES, Gemms>, many, all) : run(gemm_kernel<BM, BN, WM, WN, STAGES, Gemm>, one, all.g[0]);
 }
 
 // The parts of a contraction added up in order: [parts][batch][M][N] in fp32 -> C
