@@ -776,20 +776,21 @@ TI8_HD Mx4Part mx4_part(int p, int parts, int nk) {
     return {p * each + imin(p, more), each + (p < more ? 1 : 0)};
 }
 
-// Which kernel multiplies [M][K] and [N][K], K in nk tiles, and in how many parts along K.  us behind the launch's own 2.5 (measured with weights that come from
-// memory and with those that do not): `slots` tiles have the chip full and take `full` per K tile, up to `free` of them no longer than one, `one`.
+// Which kernel multiplies [M][K] and [N][K], K in nk tiles, and in how many parts along K.  In us, behind the launch's own 2.2: `slots` tiles have the chip full and
+// take `full` per K tile, up to `free` of them no longer than one, `one`; a tile's first loads and its results take as long as `lead` K tiles.  Of 34 products and 16
+// sets of them, M from 64 to 16384, K from 256 to 4096, run by each of the kernels, this chose the fastest or one 1 % to 2 % behind it; without `lead` 6 % were lost and up to 65 %.
 enum { MX4_FEW_16 = 0, MX4_FEW_32 = 1, MX4_TILES_32 = 2, MX4_TILES_64 = 3, MX4_TILES_128 = 4, MX4_TILES_128_TWO = 5, MX4_TILES_256 = 6, MX4_KERNELS = 7 };
 struct Mx4Kernel {
     int bm, bn, slots, free;        // of 256 CUs
-    double one, full;
+    double one, full, lead;
 };
 TI8_HD Mx4Kernel mx4_kernel(int kernel) {
     switch (kernel) {
-        case MX4_TILES_32: return {32, 64, 512, 256, 0.29, 0.50};
-        case MX4_TILES_64: return {64, 64, 512, 256, 0.31, 0.56};
-        case MX4_TILES_128: return {128, 128, 256, 256, 0.61, 0.68};
-        case MX4_TILES_128_TWO: return {128, 128, 512, 256, 0.75, 1.22};
-        default: return {256, 256, 256, 64, 1.25, 2.10};
+        case MX4_TILES_32: return {32, 64, 512, 256, 0.29, 0.50, 5.0};
+        case MX4_TILES_64: return {64, 64, 512, 256, 0.31, 0.56, 5.0};
+        case MX4_TILES_128: return {128, 128, 256, 256, 0.61, 0.68, 5.0};
+        case MX4_TILES_128_TWO: return {128, 128, 512, 256, 0.75, 1.22, 3.5};
+        default: return {256, 256, 256, 64, 1.25, 2.10, 3.5};
     }
 }
 TI8_HD int64_t mx4_blocks(int64_t M, int64_t N, const Mx4Kernel& k) { return ((M + k.bm - 1) / k.bm) * ((N + k.bn - 1) / k.bn); }
@@ -806,14 +807,14 @@ TI8_HD bool mx4_few(int64_t M, int64_t strips, int cus) { return M <= 32 && stri
 TI8_HD Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t nk, int64_t batch, int cus) {
     // one round of 16 rows of the weight to a CU; us, this kernel / tiles of 32 rows: 1 x 4096 x 4096 3.8 / 6.5, 32 x 4096 x 4096 5.4 / 6.8, 32 x 4096 x 14336 12.9 / 16,
     // and beyond one round 1 x 14336 x 4096 7.4 / 6.5, 32 x 14336 x 4096 14.7 / 6.7
-    if (mx4_few(M, (N + 15) / 16 * batch, cus)) return {M <= 16 ? MX4_FEW_16 : MX4_FEW_32, 1, 1.5 + 0.1 * (double)nk};
+    if (mx4_few(M, (N + 15) / 16 * batch, cus)) return {M <= 16 ? MX4_FEW_16 : MX4_FEW_32, 1, 1.0 + 0.1 * (double)nk};
     Mx4Plan best{MX4_TILES_256, 1, 1e30};
     for (int kernel = M <= 64 ? MX4_TILES_32 : MX4_TILES_64; kernel < MX4_KERNELS; ++kernel) {
         const Mx4Kernel k = mx4_kernel(kernel);
         const int64_t tiles = mx4_blocks(M, N, k) * batch;
         // a part's sums are written and read again, by another launch
         for (int parts = 1; parts <= 8 && (parts == 1 || (nk >= 4 * parts && tiles * parts <= cus)); parts *= 2) {
-            double us = (double)((nk + parts - 1) / parts) * mx4_rounds(tiles * parts, k, cus);
+            double us = ((double)((nk + parts - 1) / parts) + k.lead) * mx4_rounds(tiles * parts, k, cus);
             if (parts > 1) us += 2.5 + (double)(batch * M * N) * (8.0 * parts + 2.0) / 4e6;
             if (us < best.us) best = {kernel, parts, us};
         }
@@ -823,7 +824,7 @@ TI8_HD Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t nk, int64_t batch, int cus
 // Products in one launch: the kernel of all of them, or -1 where launches of their own take no longer.  sizes: M, N, nk of each.  A CU takes the next tile, of
 // whichever product, when it has done one: what counts is all of the work, or the longest tile.
 TI8_HD int mx4_plan_together(const int64_t (*sizes)[3], int count, int cus) {
-    double apart = 2.5 * (count - 1), least = 1e30;
+    double apart = 2.2 * (count - 1), least = 1e30;
     int64_t strips = 0, most_m = 0;
     for (int i = 0; i < count; ++i) {
         apart += mx4_plan(sizes[i][0], sizes[i][1], sizes[i][2], 1, cus).us;
@@ -839,10 +840,10 @@ TI8_HD int mx4_plan_together(const int64_t (*sizes)[3], int count, int cus) {
         for (int i = 0; i < count; ++i) {
             const int64_t n = mx4_blocks(sizes[i][0], sizes[i][1], k);
             tiles += n;
-            work += (double)(n * sizes[i][2]);
+            work += (double)n * ((double)sizes[i][2] + k.lead);
             if (sizes[i][2] > longest) longest = sizes[i][2];
         }
-        const double even = work / (double)tiles * mx4_rounds(tiles, k, cus), alone = (double)longest * k.one, us = even > alone ? even : alone;
+        const double even = work / (double)tiles * mx4_rounds(tiles, k, cus), alone = ((double)longest + k.lead) * k.one, us = even > alone ? even : alone;
         if (us < least) {
             least = us;
             best = kernel;
