@@ -756,7 +756,8 @@ TI8_HD int64_t xcd_range(int64_t block, int64_t blocks) {
 
 // quantiser by rows: 256 threads, a tile of 32 rows x 256 columns; thread t has octet t % 32 of rows t / 32 + 8 i, i < 4
 constexpr int MX4_ROW_BLOCK = 32;
-// quantiser by columns: waves of 32 rows x 256 columns; lane l has octet l % 32 of rows 16 (l / 32) .. + 15
+// quantiser by columns: a column's 16 NW bytes of codes from NW waves of 32 rows each; the waves' pieces lie in another order in every octet of columns, so that eight
+// columns side by side do not write into the same banks
 TI8_HD int mx4_col_chunk(int wave, int octet, int waves) { return wave ^ (octet & (waves - 1)); }     // where 16 bytes of a column lie in its LDS line
 
 // product: rows of an operand that a workgroup's loads go to stay within it
