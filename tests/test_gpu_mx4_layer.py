@@ -252,6 +252,24 @@ def test_captured_norm_and_products(T, dev):
             assert all(bits_equal(u, v) for u, v in zip(got, want))
 
 
+# (the first launch in two parts along the contraction, with a workspace; the second for all products)
+@pytest.mark.parametrize("sizes", [((5, 40, 16384), (300, 100, 600)), ((20, 300, 1000), (20, 70, 1000), (20, 900, 1000))])
+def test_captured_products_together(T, dev, sizes):
+    gen = make_gen(1)
+    inputs = [[t for m, n, k in sizes for t in (*T.mx4.quant_row(randn_bf16(gen, m, k).to(dev)), *T.mx4.quant_row(randn_bf16(gen, n, k, std=0.1).to(dev)))] for _ in range(2)]
+
+    def run(*t):
+        return tuple(T.mx4.gemm_nt_multi([t[i:i + 4] for i in range(0, len(t), 4)]))
+    want = [[t.clone() for t in run(*i)] for i in inputs]
+    steps = [T.GraphedStep(run, *inputs[0]) for _ in range(2)]
+    for turn in range(4):
+        for step in steps:
+            got = step(*inputs[turn % 2])
+            torch.cuda.synchronize()
+            assert all(bits_equal(a, b) for a, b in zip(got, want[turn % 2]))
+            run(*inputs[(turn + 1) % 2])
+
+
 def test_on_other_streams(T, dev):
     """Calls on two streams at once, each behind what made its inputs there."""
     gen = torch.Generator(device=dev).manual_seed(3)
@@ -279,6 +297,7 @@ def test_both_ways_from_python(T, dev, native, monkeypatch):
         q, s = T.mx4.quant_row(x)
         out = [q, s, *T.mx4.quant_row(x.view(5, 10, 256)), *T.mx4.quant_col_t(x), *T.mx4.quant_row_col_t(x), T.mx4.dequant(q, s, 256), *T.mx4.linear_fwd_bwd(x, w, dy)]
         out += [T.mx4.gemm_nt(q, s, *T.mx4.quant_row(w), out_dtype=d) for d in (torch.bfloat16, torch.float32)]
+        out += [y for n in (1, 2, 3) for y in T.mx4.gemm_nt_multi([(q, s, *T.mx4.quant_row(w)), (q, s, q, s), (q[3:], s[:, 3:], q, s)][:n])]
         for kw in (dict(), dict(residual=r), dict(to="int8"), dict(to="int8", group=128, residual=r, inv_mode=1)):
             out += T.ops.rmsnorm_quant(x, nw, 1e-5, **kw)
         out += [T.ops.dequant_row(*T.ops.rmsnorm_quant(x, nw, 1e-5, to="int8", group=g)[:2]) for g in (0, 128)]

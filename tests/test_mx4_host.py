@@ -205,7 +205,7 @@ def test_python_refusals(recorded):
         M.linear_fwd_bwd(bf(5, 300), bf(7, 300), bf(6, 7))
     with pytest.raises(ValueError, match="positive"):
         M.Mx4Linear(0, 4)
-    for problems, msg in (([], "between 1 and 3"), ([(q, s, q, s)] * 4, "between 1 and 3"), ([(q, s, q, s), (q, s, q1, s1)], "as many tiles"), ([(q3, s3, q, s)], "matrices")):
+    for problems, msg in (([], "between 1 and 3"), ([(q, s, q, s)] * 4, "between 1 and 3"), ([(q, s, q, s), (q, s, q1, s1)], "as many tiles"), ([(q, s, q), (s, q, s, q, s)], "a product is"), ([(q3, s3, q, s)], "matrices")):
         with pytest.raises(ValueError, match=msg):
             M.gemm_nt_multi(problems)
 
