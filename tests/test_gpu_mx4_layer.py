@@ -318,6 +318,9 @@ def test_inference_mode(T, dev):
     with torch.inference_mode():
         y = m(x)
         assert y.is_inference() and bits_equal(y.clone(), want)
+        w = torch.ones(256, dtype=torch.bfloat16, device=dev)
+        assert all(t.is_inference() for t in (*T.ops.rmsnorm_quant(x, w, 1e-5, residual=x), *T.mx4.quant_row_col_t(x)))
+    assert not any(t.is_inference() for t in (*T.ops.rmsnorm_quant(x, w.clone(), 1e-5, residual=x), *T.mx4.quant_row_col_t(x)))
     assert not m(x.requires_grad_()).is_inference()
 
 

@@ -78,6 +78,21 @@ def test_many_rows(T, dev, rows):
     check(T, dev, *inputs(rows, 384), to="int8", group=128)
 
 
+@pytest.mark.parametrize("rows", [1, 7, 60, 61, 62, 63, 64, 300])       # (around 1 MB in all, up to which they share a block)
+def test_results_lie_apart(T, dev, rows):
+    x, w, r = (t.to(dev) for t in inputs(rows, 4096))
+    for results in (T.ops.rmsnorm_quant(x, w, EPS, residual=r), T.ops.rmsnorm_quant(x, w, EPS, residual=r, to="int8", group=128), T.ops.rmsnorm_quant(x, w, EPS),
+                    T.mx4.quant_row_col_t(x[:, :1000])):
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in results)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])) and all(a % 16 == 0 for a, _ in spans)
+        for t in results:
+            assert t.is_contiguous() and t.untyped_storage().nbytes() >= (t.storage_offset() + t.numel()) * t.element_size()
+        kept = [t.clone() for t in results]
+        for i, t in enumerate(results):
+            t.zero_()
+            assert all(torch.equal(a, b) for a, b in zip(results[i + 1:], kept[i + 1:]))
+
+
 @pytest.mark.parametrize("eps", [0.0, 1e-12, 1.0])
 def test_eps(T, dev, eps):
     x, w, r = inputs(3, 512)

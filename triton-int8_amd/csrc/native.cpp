@@ -361,17 +361,40 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
     return at::detail::empty_generic(sizes, at::detail::getCUDAHooks().getCUDADeviceAllocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, c10::nullopt);
 }
 
+// Room for the results of one call that die together.  Up to 1 MB in all they share a block of memory: asking for one and giving it back takes 0.4 us of a call
+// that takes 5.
+class Room {
+  public:
+    explicit Room(int64_t bytes = INT64_MAX) {
+        if (bytes <= 1 << 20) block_ = fresh({bytes}, at::kByte);
+    }
+    static int64_t of(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+    static int64_t of_mx4(int64_t rows, int64_t cols) { return of(rows * ((cols + 255) / 256) * 128) + of(rows * ((cols + 255) / 256) * 8); }
+    at::Tensor operator()(at::IntArrayRef sizes, at::ScalarType type) {
+        if (!block_.defined()) return fresh(sizes, type);
+        at::Tensor t = at::detail::make_tensor<at::TensorImpl>(c10::Storage(block_.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(at_ / (int64_t)c10::elementSize(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        at_ += of(t.numel() * (int64_t)c10::elementSize(type));
+        return t;
+    }
+
+  private:
+    at::Tensor block_;
+    int64_t at_ = 0;
+};
+
 // room for a tensor in 4 bits
 struct Mx4Out {
     at::Tensor codes, scales;
     ti8_mx4 mx = {};
     Mx4Out() = default;
-    Mx4Out(at::IntArrayRef lead, int64_t rows, int64_t cols) {
+    Mx4Out(Room& room, at::IntArrayRef lead, int64_t rows, int64_t cols) {
         const int64_t tiles = (cols + 255) / 256;
         c10::SmallVector<int64_t, 4> sizes(lead.begin(), lead.end());
         sizes.push_back(tiles * 128);
-        codes = fresh(sizes, at::kByte);
-        scales = fresh({tiles, rows, 8}, at::kByte);
+        codes = room(sizes, at::kByte);
+        scales = room({tiles, rows, 8}, at::kByte);
         mx = ti8_mx4{codes.data_ptr(), scales.data_ptr(), tiles * 128, rows * 8};
     }
 };
@@ -408,8 +431,10 @@ PyObject* mx4_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int status;
     {
         const GilReleased released;
-        if (by_rows) rows = Mx4Out(x.sizes().slice(0, x.dim() - 1), R, C);
-        if (by_columns) cols = Mx4Out({C}, C, R);
+        // (one view alone may be a weight's, kept and saved: two tensors of their own)
+        Room room = by_rows && by_columns ? Room(Room::of_mx4(R, C) + Room::of_mx4(C, R)) : Room();
+        if (by_rows) rows = Mx4Out(room, x.sizes().slice(0, x.dim() - 1), R, C);
+        if (by_columns) cols = Mx4Out(room, {C}, C, R);
         const ti8_mx4_operand o = {x.data_ptr(), ldx, R, C, rows.mx, cols.mx};
         status = mx4_quant_entry(&o, 1, stream_of(stream));
     }
@@ -555,18 +580,19 @@ PyObject* rmsnorm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
         ti8_rmsnorm_quant_args a = {};
         Mx4Out out;
-        rstd = fresh(lead, at::kFloat);
-        if (r.defined()) h = fresh(x.sizes(), at::kBFloat16);
+        Room room(Room::of(rows * 4) + (r.defined() ? Room::of(rows * dim * 2) : 0) + (mx ? Room::of_mx4(rows, dim) : Room::of(rows * dim) + Room::of(group ? rows * (dim / 128) * 4 : rows * 4)));
+        rstd = room(lead, at::kFloat);
+        if (r.defined()) h = room(x.sizes(), at::kBFloat16);
         if (mx) {
-            out = Mx4Out(lead, rows, dim);
+            out = Mx4Out(room, lead, rows, dim);
             q = out.codes;
             s = out.scales;
             a.mx4 = out.mx;
         } else {
-            q = fresh(x.sizes(), at::kChar);
+            q = room(x.sizes(), at::kChar);
             c10::SmallVector<int64_t, 4> sizes(lead.begin(), lead.end());
             if (group) sizes.push_back(dim / 128);
-            s = fresh(sizes, at::kFloat);
+            s = room(sizes, at::kFloat);
             a.q = static_cast<int8_t*>(q.data_ptr());
             a.ldq = dim;
             a.s = static_cast<float*>(s.data_ptr());
