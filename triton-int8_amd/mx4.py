@@ -261,7 +261,9 @@ class Mx4LinearFunction(torch.autograd.Function):
             if tokens == 0:
                 dx, dws[i] = dys[i].new_empty((0, K)), dys[i].new_zeros((ctx.features[i], K)) if wants[i] else None
                 continue
-            rows, cols = _quant(dys[i].reshape(tokens, ctx.features[i]), wants_x, wants[i])
+            d = dys[i].reshape(tokens, ctx.features[i])
+            made = _natively("mx4_quant", d, int(wants_x), int(wants[i]))
+            rows, cols = _quant(d, wants_x, wants[i]) if made is None else (made[:2], made[-2:])
             made = gemm_nt_multi(([(*rows, *of_weights[2 * i:2 * i + 2])] if wants_x else []) + ([(*cols, *x)] if wants[i] else []))
             if wants_x:
                 dx = made[0] if dx is None else dx.add_(made[0])
