@@ -778,9 +778,10 @@ TI8_HD Mx4Part mx4_part(int p, int parts, int nk) {
 }
 
 // Which kernel multiplies [M][K] and [N][K], K in nk tiles, and in how many parts along K.  In us, behind the launch's own 2.2: `slots` tiles have the chip full and
-// take `full` per K tile, up to `free` of them no longer than one, `one`; a tile's first loads and its results take as long as `lead` K tiles.  Of 34 products and 16
-// sets of them, M from 64 to 16384, K from 256 to 4096, run by each of the kernels, this chose the fastest or one 1 % to 2 % behind it; without `lead` 6 % were lost and up to 65 %.
-enum { MX4_FEW_16 = 0, MX4_FEW_32 = 1, MX4_TILES_32 = 2, MX4_TILES_64 = 3, MX4_TILES_128 = 4, MX4_TILES_128_TWO = 5, MX4_TILES_256 = 6, MX4_KERNELS = 7 };
+// take `full` per K tile, up to `free` of them no longer than one, `one`; a tile's first loads and its results take as long as `lead` K tiles.  Of 52 products and 26
+// sets of them, M from 64 to 16384, K from 256 to 4096, run by each of the kernels, this chose the fastest of them or one behind it, by 7 % at most and 0.2 % on
+// average; without `lead` 6 % on average and up to 65 %.
+enum { MX4_FEW_16 = 0, MX4_FEW_32 = 1, MX4_TILES_32 = 2, MX4_TILES_64 = 3, MX4_TILES_128 = 4, MX4_TILES_128_TWO = 5, MX4_TILES_256 = 6, MX4_TILES_64_128 = 7, MX4_KERNELS = 8 };
 struct Mx4Kernel {
     int bm, bn, slots, free;        // of 256 CUs
     double one, full, lead;
@@ -788,7 +789,8 @@ struct Mx4Kernel {
 TI8_HD Mx4Kernel mx4_kernel(int kernel) {
     switch (kernel) {
         case MX4_TILES_32: return {32, 64, 512, 256, 0.29, 0.50, 5.0};
-        case MX4_TILES_64: return {64, 64, 512, 256, 0.31, 0.56, 5.0};
+        case MX4_TILES_64: return {64, 64, 512, 256, 0.30, 0.50, 5.5};
+        case MX4_TILES_64_128: return {64, 128, 256, 256, 0.36, 0.42, 6.5};
         case MX4_TILES_128: return {128, 128, 256, 256, 0.61, 0.68, 5.0};
         case MX4_TILES_128_TWO: return {128, 128, 512, 256, 0.75, 1.22, 3.5};
         default: return {256, 256, 256, 64, 1.25, 2.10, 3.5};
@@ -806,8 +808,8 @@ struct Mx4Plan {
 };
 TI8_HD bool mx4_few(int64_t M, int64_t strips, int cus) { return M <= 32 && strips <= cus; }
 TI8_HD Mx4Plan mx4_plan(int64_t M, int64_t N, int64_t nk, int64_t batch, int cus) {
-    // one round of 16 rows of the weight to a CU; us, this kernel / tiles of 32 rows: 1 x 4096 x 4096 3.8 / 6.5, 32 x 4096 x 4096 5.4 / 6.8, 32 x 4096 x 14336 12.9 / 16,
-    // and beyond one round 1 x 14336 x 4096 7.4 / 6.5, 32 x 14336 x 4096 14.7 / 6.7
+    // one round of 16 rows of the weight to a CU; us with weights from memory, this kernel / tiles of 32 rows: 1 x 4096 x 4096 4.6 / 6.7, 32 x 4096 x 4096 6.4 / 7.0,
+    // 1 x 4096 x 14336 8.7 / 17.0, 32 x 4096 x 14336 14.5 / 17.8, and beyond one round 1 x 8192 x 4096 6.5 / 7.1, 32 x 8192 x 4096 9.5 / 7.4, 16 x 14336 x 4096 11.4 / 7.9
     if (mx4_few(M, (N + 15) / 16 * batch, cus)) return {M <= 16 ? MX4_FEW_16 : MX4_FEW_32, 1, 1.0 + 0.1 * (double)nk};
     Mx4Plan best{MX4_TILES_256, 1, 1e30};
     for (int kernel = M <= 64 ? MX4_TILES_32 : MX4_TILES_64; kernel < MX4_KERNELS; ++kernel) {

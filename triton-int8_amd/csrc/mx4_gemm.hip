@@ -73,6 +73,14 @@ __device__ __forceinline__ void interleave() {
 #endif
 }
 
+// What of n pieces of work goes beside matrix instruction q of `count`: f(i) for its share
+template <class F>
+__device__ __forceinline__ void beside(int q, int count, int n, const F& f) {
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+        if (i >= q * n / count && i < (q + 1) * n / count) f(i);
+}
+
 // One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS
 constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
 constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
@@ -88,7 +96,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int A_INSTR = BM / 8 / NW, B_INSTR = BN / 8 / NW, A_BYTES = BM * 128, B_BYTES = BN * 128;
     constexpr int SA_INSTR = (BM / 32 + NW - 1) / NW, SB_INSTR = (BN / 32 + NW - 1) / NW, S_BYTES = (BM + BN) * 8, RING = scale_stages(STAGES);
-    constexpr bool WHOLE = TM * TN <= 2;
+    constexpr bool WHOLE = TM * TN <= 4;
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     uint8_t* const ldsA = smem;
     uint8_t* const ldsB = smem + STAGES * A_BYTES;
@@ -134,21 +142,17 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products
     for (int i = 0; i < SA_INSTR; ++i) soff_a[i] = idx::mx4_row((wave + i * NW) % (BM / 32) * 32 + (lane >> 1), rows_a) * 8 + (lane & 1) * 4;
 #pragma unroll
     for (int i = 0; i < SB_INSTR; ++i) soff_b[i] = idx::mx4_row((wave + i * NW) % (BN / 32) * 32 + (lane >> 1), rows_b) * 8 + (lane & 1) * 4;
+    constexpr int SCALE_LOADS = SA_INSTR + SB_INSTR;
+    const auto issue_scale = [&](int kt, int i) {
+        const bool of_a = i < SA_INSTR;
+        const uint8_t* const from = of_a ? scales_a + min(kt, last) * g.sla : scales_b + min(kt, last) * g.slb;
+        uint32_t o = of_a ? soff_a[of_a ? i : 0] : soff_b[of_a ? 0 : i - SA_INSTR];
+        asm volatile("" : "+v"(o));
+        __builtin_amdgcn_global_load_lds(from + o, ldsS + kt % RING * S_BYTES + (of_a ? (wave + i * NW) % (BM / 32) * 256 : BM * 8 + (wave + (i - SA_INSTR) * NW) % (BN / 32) * 256), 4, 0, 0);
+    };
     const auto issue_scales = [&](int kt) {
-        const uint8_t *a = scales_a + min(kt, last) * g.sla, *b = scales_b + min(kt, last) * g.slb;
-        uint8_t* const slot = ldsS + kt % RING * S_BYTES;
 #pragma unroll
-        for (int i = 0; i < SA_INSTR; ++i) {
-            uint32_t o = soff_a[i];
-            asm volatile("" : "+v"(o));
-            __builtin_amdgcn_global_load_lds(a + o, slot + (wave + i * NW) % (BM / 32) * 256, 4, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < SB_INSTR; ++i) {
-            uint32_t o = soff_b[i];
-            asm volatile("" : "+v"(o));
-            __builtin_amdgcn_global_load_lds(b + o, slot + BM * 8 + (wave + i * NW) % (BN / 32) * 256, 4, 0, 0);
-        }
+        for (int i = 0; i < SCALE_LOADS; ++i) issue_scale(kt, i);
     };
 
     // LDS -> registers
@@ -182,26 +186,23 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products
         for (int j = 0; j < TN; ++j) nb[j] = *reinterpret_cast<const int*>(scale_b + kt % RING * S_BYTES + j * 256);
     };
 
-    constexpr int SCALE_LOADS = SA_INSTR + SB_INSTR;
     if constexpr (WHOLE) {
-        // Few matrix instructions to a tile: all of the next tile's fragments are read beside them (a step at a time every step waits for LDS; 64 x 4096 x 4096
-        // 7.1 us).  Tile kt + STAGES is asked for once everybody has tile kt in registers.
+        // All of the next tile's fragments are read beside this one's matrix instructions, and tile kt + STAGES asked for (everybody has tile kt in registers), a piece
+        // of both behind each instruction and in this order: left to the compiler they come in bunches, and LDS and the matrix pipe take turns (512 x 4096 x 4096
+        // 12.4 us on 128 x 128, 10.8 on 64 x 64, so 11.2 and 10.1).  That 256 x 256 is no faster with it: it is bound by power.
         constexpr int BEHIND = (STAGES - 2) * (LOADS + SCALE_LOADS);
         static_assert((STAGES - 1) * (LOADS + SCALE_LOADS) < 64 && RING >= STAGES, "vmcnt has six bits");
         v4i wa[2][TM][4], wb[2][TN][4];
         int ws[2][TM], wt[2][TN];
-        const auto read = [&](int set, int stage, int kt) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) ws[set][i] = *reinterpret_cast<const int*>(scale_a + kt % RING * S_BYTES + i * 256);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) wt[set][j] = *reinterpret_cast<const int*>(scale_b + kt % RING * S_BYTES + j * 256);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-                for (int i = 0; i < TM; ++i) wa[set][i][ks] = *reinterpret_cast<const v4i*>(frag_a + stage * A_BYTES + i * 4096 + chunk[ks]);
-#pragma unroll
-                for (int j = 0; j < TN; ++j) wb[set][j][ks] = *reinterpret_cast<const v4i*>(frag_b + stage * B_BYTES + j * 4096 + chunk[ks]);
-            }
+        constexpr int FRAGS = 4 * (TM + TN), STEPS = 4 * TM * TN;
+        const auto read_scale = [&](int set, int kt, int i) {
+            if (i < TM) ws[set][i < TM ? i : 0] = *reinterpret_cast<const int*>(scale_a + kt % RING * S_BYTES + i * 256);
+            else wt[set][i < TM ? 0 : i - TM] = *reinterpret_cast<const int*>(scale_b + kt % RING * S_BYTES + (i - TM) * 256);
+        };
+        const auto read = [&](int set, int stage, int i) {
+            const int ks = i / (TM + TN), x = i % (TM + TN);
+            if (x < TM) wa[set][x < TM ? x : 0][ks] = *reinterpret_cast<const v4i*>(frag_a + stage * A_BYTES + x * 4096 + chunk[ks]);
+            else wb[set][x < TM ? 0 : x - TM][ks] = *reinterpret_cast<const v4i*>(frag_b + stage * B_BYTES + (x - TM) * 4096 + chunk[ks]);
         };
 #pragma unroll
         for (int t = 0; t < STAGES; ++t) {
@@ -211,22 +212,27 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products
         }
         __builtin_amdgcn_s_waitcnt(waitcnt((STAGES - 1) * (LOADS + SCALE_LOADS), 0x70));
         asm volatile("s_barrier" ::: "memory");
-        read(0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < TM + TN; ++i) read_scale(0, 0, i);
+#pragma unroll
+        for (int i = 0; i < FRAGS; ++i) read(0, 0, i);
         int cur = 0, kt = 0;
 #define TI8_STEP(KS, SET)                                                                                                     \
-    _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j) acc[i][j] =                 \
-        multiply<KS>(wb[SET][j][KS], wa[SET][i][KS], acc[i][j], wt[SET][j], ws[SET][i]);
+    _Pragma("unroll") for (int i = 0; i < TM; ++i) _Pragma("unroll") for (int j = 0; j < TN; ++j) {                           \
+        const int q = KS * TM * TN + i * TN + j;                                                                              \
+        acc[i][j] = multiply<KS>(wb[SET][j][KS], wa[SET][i][KS], acc[i][j], wt[SET][j], ws[SET][i]);                          \
+        beside(q, STEPS, FRAGS, [&](int x) { read(1 - SET, next, x); });                                                      \
+        if (q == 0) _Pragma("unroll") for (int x = 0; x < TM + TN; ++x) read_scale(1 - SET, kt + 1, x);                       \
+        beside(q, STEPS, LOADS, [&](int x) { issue(kt + STAGES, cur, x, x + 1); });                                           \
+        beside(q, STEPS, SCALE_LOADS, [&](int x) { issue_scale(kt + STAGES, x); });                                           \
+        __builtin_amdgcn_sched_barrier(0);                                                                                    \
+    }
 #define TI8_TILE(SET)                                                                                                         \
     {                                                                                                                         \
         const int next = cur + 1 == STAGES ? 0 : cur + 1;                                                                     \
         __builtin_amdgcn_s_waitcnt(waitcnt(BEHIND, 0x70));                                                                    \
         asm volatile("s_barrier" ::: "memory");                                                                               \
-        issue(kt + STAGES, cur, 0, LOADS);                                                                                    \
-        issue_scales(kt + STAGES);                                                                                            \
-        read(1 - SET, next, kt + 1);                                                                                          \
-        __builtin_amdgcn_sched_barrier(0);                                                                                    \
         TI8_STEP(0, SET) TI8_STEP(1, SET) TI8_STEP(2, SET) TI8_STEP(3, SET)                                                   \
-        __builtin_amdgcn_sched_barrier(0);                                                                                    \
         cur = next;                                                                                                           \
         ++kt;                                                                                                                 \
     }
@@ -546,6 +552,7 @@ int launch_plan(const char* fn, int kernel, const Gemms& all, int64_t batch, hip
         case idx::MX4_FEW_32: return launch_few<2, 1, 8>(fn, all, batch, st);
         case idx::MX4_TILES_32: return launch<32, 64, 1, 2, 4>(fn, all, batch, st);
         case idx::MX4_TILES_64: return launch<64, 64, 2, 2, 4>(fn, all, batch, st);
+        case idx::MX4_TILES_64_128: return launch<64, 128, 2, 2, 4>(fn, all, batch, st);
         case idx::MX4_TILES_128: return launch<128, 128, 2, 2, 3>(fn, all, batch, st);
         case idx::MX4_TILES_128_TWO: return launch<128, 128, 2, 2, 2>(fn, all, batch, st);
         default: return launch<256, 256, 2, 4, 2>(fn, all, batch, st);
