@@ -590,7 +590,7 @@ int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b, int64_t 
 /* bytes of workspace that the call above needs (0: none; -1 for sizes it does not take), 16-byte aligned, contents undefined before and after: few tiles over a
  * long K are shared among workgroups, whose parts are added up in order */
 int64_t ti8_mx4_gemm_nt_workspace(int64_t batch, int64_t M, int64_t N, int64_t K);
-/* Up to 3 such products (batch 1), in one launch where that is faster: the bits of separate calls but for the order in which long contractions are added up.  `problems` is a HOST
+/* Up to 3 such products (batch 1), in one launch where that is faster: the bits of separate calls but for the order in which contractions are added up.  `problems` is a HOST
  * array.  workspace: the bytes that ti8_mx4_gemm_nt_multi_workspace gives for these sizes (it reads nothing else), -1 for those that are not taken.  Outputs share no
  * memory with each other. */
 typedef struct {

@@ -213,3 +213,23 @@ def test_products_together(M, dev, sizes):
     for c, (a, b), (m, n, k) in zip(got, inputs, sizes):
         assert c.dtype == torch.bfloat16 and c.shape == (m, n)
         close(c, *oracle.gemm_nt(oracle.rounded(a), oracle.rounded(b)), k, (m, n, k))
+
+
+@pytest.mark.parametrize("sizes", [[(3, 64, 512), (3, 200, 512)], [(100, 333, 1000), (257, 100, 40), (40, 1000, 5000)], [(5, 40, 16384), (300, 100, 600)]], ids=str)
+def test_products_together_into_wider_rows(M, dev, sizes):
+    """From C: results in either type, rows apart; what lies between them is left as it was."""
+    gen = make_gen(3)
+    lib, problems, kept, outs = M._lib, (M._lib.Mx4GemmProblem * len(sizes))(), [], []
+    for i, (m, n, k) in enumerate(sizes):
+        a, b = tensor(gen, m, k), tensor(gen, n, k, spread=False)
+        da, db = M._operand(*M.quant_row(a.to(dev)), "a"), M._operand(*M.quant_row(b.to(dev)), "b")
+        c = torch.full((m, n + 5), 7.0, dtype=torch.bfloat16 if i % 2 else torch.float32, device=dev)
+        problems[i] = lib.Mx4GemmProblem(da[2], db[2], c.data_ptr(), n + 5, m, n, k, 1 - i % 2)
+        kept.append((da, db))
+        outs.append((c, a, b, n, k))
+    need = lib.lib().ti8_mx4_gemm_nt_multi_workspace(problems, len(sizes))
+    workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    lib.call("ti8_mx4_gemm_nt_multi", problems, len(sizes), workspace.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    for c, a, b, n, k in outs:
+        assert bool((c[:, n:] == 7.0).all())
+        close(c[:, :n], *oracle.gemm_nt(oracle.rounded(a), oracle.rounded(b)), k, n)

@@ -2,7 +2,7 @@
 // operands' scales and adds up in fp32; C is rounded once.
 //
 // A K tile is 256 elements: 128 bytes of codes per row, staged in LDS by direct loads (16-byte chunks XOR-swizzled by row, so that the 16 rows a quarter
-// of a wave reads at one chunk lie in distinct banks), double buffered, and 8 scales per row, which go straight into registers.  Lane l of an instruction
+// of a wave reads at one chunk lie in distinct banks), two to four tiles of them, and 8 scales per row, which go the same way (a ring of four or eight).  Lane l of an instruction
 // supplies row l % 32 of its operand and 32 elements of the 64 that it contracts.  Which 32 is free as long as both operands agree: step ks of a tile takes
 // chunk ks from lanes below 32 and chunk 4 + ks from the others, so that a lane's four scales of a tile are one word, and the step's number picks the byte.
 // The operands change places (the instruction's rows are C's columns), so that a lane holds four neighbouring elements of a row of C.
@@ -81,7 +81,10 @@ __device__ __forceinline__ void beside(int q, int count, int n, const F& f) {
         if (i >= q * n / count && i < (q + 1) * n / count) f(i);
 }
 
-// One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS
+// One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS.  256 x 256: per K tile a CU's matrix instructions take 2048 cycles, its LDS reads and writes
+// as many; 8192 x 14336 x 4096 235 us (4.1 PFLOP/s) at a clock of 1.75 GHz, on codes of zero 172: the chip's power bounds it (a loop of nothing but these instructions
+// reaches 6.6 PFLOP/s on random codes, 9.7 on zeros).  16 x 16 x 128 instructions, four waves of 128 x 128, workgroups that go on to the next tile: within 3 %.  Smaller
+// tiles where those do not fill the CUs: 700 x 4096 x 4096 10.5 us, 128 x 4096 x 4096 5.9, of which 2.2 are the launch and 1.5 to 3 a tile's first loads and results.
 constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
 constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
 constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14

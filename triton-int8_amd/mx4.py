@@ -148,7 +148,7 @@ def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
 
 def gemm_nt_multi(problems):
     """Up to three products ``(A, sA, B, sB)`` of matrices, in one launch where that is faster: a list of bf16 matrices.  What :func:`gemm_nt` gives, but for the order
-    in which long contractions may be added up."""
+    in which contractions are added up."""
     _need(1 <= len(problems) <= 3, f"between 1 and 3 products, got {len(problems)}")
     _need(all(len(p) == 4 for p in problems), "a product is (codes of A, scales of A, codes of B, scales of B)")
     made = _natively("mx4_gemm_nt_multi", *(t for p in problems for t in p))

@@ -688,8 +688,7 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
     multiple of 8 (with "int8" of 128) up to 16384.
 
-    Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean in 64 bits: no code depends on an order of
-    summation.  Quantised tensors have no gradients: x, weight and residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and,
+    Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean added up in 64 bits.  Quantised tensors have no gradients: x, weight and residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and,
     the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
     made = _natively("rmsnorm_quant", x, weight, residual, eps, int(to == "mx4"), group, inv_mode, Q_CLAMP) if to in ("mx4", "int8") else None
     if made is not None:
