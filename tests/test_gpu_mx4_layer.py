@@ -332,3 +332,44 @@ def test_weights_that_change_are_quantised_again(T, dev):
         first = m(x)
         m.weight.data.mul_(2.0)
         assert bits_equal(m(x), first * 2)
+
+
+def test_packed_layers_are_saved_and_loaded(T, dev):
+    """Into a layer that is packed too."""
+    for bias in (False, True):
+        (m,) = layers_of(T, dev, 520, (96,))
+        m = T.Mx4Linear(520, 96, bias=bias, device=dev).pack()
+        x = randn_bf16(make_gen(1), 7, 520).to(dev)
+        other = T.Mx4Linear(520, 96, bias=bias, device=dev).pack()
+        with torch.no_grad():
+            assert not bits_equal(m(x), other(x))
+            other.load_state_dict({k: v.clone() for k, v in m.state_dict().items()})
+            assert bits_equal(m(x), other(x)) and set(m.state_dict()) == {"codes", "scales"} | ({"bias"} if bias else set())
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_products_of_column_slices(T, dev, native, monkeypatch):
+    """Slices of columns that begin at a tile, in place, by the call from C++ and by the one from Python."""
+    if not native:
+        monkeypatch.setattr(T._lib, "native", lambda: None)
+    gen = make_gen(4)
+    a, b = randn_bf16(gen, 40, 1300), randn_bf16(gen, 70, 1300)
+    (qa, sa), (qb, sb) = T.mx4.quant_row(a.to(dev)), T.mx4.quant_row(b.to(dev))
+    want = T.mx4.gemm_nt(*T.mx4.quant_row(a[:, 512:1024].to(dev)), *T.mx4.quant_row(b[:, 512:1024].to(dev)))
+    part = slice(256, 512)
+    assert bits_equal(T.mx4.gemm_nt(qa[:, part], sa[2:4], qb[:, part], sb[2:4]), want)
+    assert bits_equal(T.mx4.dequant(qa[:, part], sa[2:4], 512), T.mx4.dequant(*T.mx4.quant_row(a[:, 512:1024].to(dev)), 512))
+
+
+def test_tangents_and_traces_are_refused(T, dev):
+    from torch.autograd import forward_ad
+    x, w = randn_bf16(make_gen(1), 7, 256).to(dev), torch.ones(256, dtype=torch.bfloat16, device=dev)
+    layer = T.Mx4Linear(256, 96, device=dev).requires_grad_(False)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        for call in (lambda: layer(d), lambda: T.ops.rmsnorm_quant(d, w, 1e-5)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+    for call in (layer, T.mx4.quant_row, lambda t: T.ops.rmsnorm_quant(t, w, 1e-5)[0]):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)

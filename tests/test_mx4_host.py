@@ -304,3 +304,31 @@ def test_gradients_that_are_not_wanted_are_not_computed(recorded):
     calls.clear()
     z.sum().backward()
     assert a.grad is None and b.grad.shape == (8, 40) and names() == ["ti8_mx4_quant", "ti8_mx4_gemm_nt_multi"]
+
+
+def test_tracing_is_refused(recorded):
+    """A trace would hold nothing of what a call launches."""
+    T, calls = recorded
+    x, w, layer = torch.ones(4, 256, dtype=torch.bfloat16), torch.ones(256, dtype=torch.bfloat16), T.Mx4Linear(256, 8).requires_grad_(False)
+    q, s = torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(1, 4, 8, dtype=torch.uint8)
+    for call in (layer, T.mx4.quant_row, T.mx4.quant_row_col_t, lambda t: T.mx4.linear_fwd_bwd(t, t, t[:, :4]), lambda t: T.ops.rmsnorm_quant(t, w, 1e-5)[0],
+                 lambda t: T.mx4.gemm_nt(q, s, q, s) + t[:, :4], lambda t: T.mx4.dequant(q, s, 256) + t, lambda t: T.mx4.gemm_nt_multi([(q, s, q, s)])[0] + t[:, :4],
+                 lambda t: T.ops.dequant_row(t.to(torch.int8), torch.ones(4))):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+    assert not calls
+
+
+def test_tangents_are_refused(recorded):
+    T, calls = recorded
+    from torch.autograd import forward_ad
+    x, w = torch.ones(4, 256, dtype=torch.bfloat16), torch.ones(256, dtype=torch.bfloat16)
+    layer = T.Mx4Linear(256, 8, bias=True).requires_grad_(False)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        for call in (lambda: layer(d), lambda: T.mx4.linears(d, (layer, layer)), lambda: T.ops.rmsnorm_quant(d, w, 1e-5), lambda: T.ops.rmsnorm_quant(x, w, 1e-5, residual=d)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        assert not calls
+        layer(x)        # (no tangent of its own)
+    assert [c[0] for c in calls] == ["ti8_mx4_quant", "ti8_mx4_quant", "ti8_mx4_gemm_nt_multi"]

@@ -8,6 +8,7 @@ The functions take bf16 tensors on the current GPU, enqueue on torch's current s
 :class:`Mx4Linear` does, with every product of forward and backward in 4 bits.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -28,7 +29,13 @@ def _here(t):
     return ops._on_gpu(t) and t.get_device() == torch._C._cuda_getDevice()
 
 
+def _recorded():
+    """Refuses calls under a tracer: what they launch would not be recorded."""
+    _need(torch._C._get_tracing_state() is None, "calls in 4 bits cannot be traced: what they launch would not be recorded")
+
+
 def _bf16(x, name, dim=None):
+    _recorded()
     _need(isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and _here(x), f"{name} must be a bfloat16 tensor on the current GPU")
     _need(x.dim() >= 1 and x.numel() > 0 and dim in (None, x.dim()), f"{name} must be a non-empty tensor" + ("" if dim is None else f" of {dim} dimensions"))
 
@@ -92,6 +99,7 @@ def quant_row_col_t(x):
 
 def _operand(codes, scales, name):
     """Codes [rows, bytes] or [batch, rows, bytes] with their scales as the kernels read them: (codes, scales, C description)."""
+    _recorded()
     _need(isinstance(codes, torch.Tensor) and codes.dtype == torch.uint8 and codes.dim() in (2, 3) and codes.numel() > 0 and codes.shape[-1] % 128 == 0 and _here(codes),
           f"codes of {name} must be a uint8 tensor [rows, tiles * 128] or [batch, rows, tiles * 128] on the current GPU")
     tiles, rows = codes.shape[-1] // 128, codes.shape[:-1].numel()
@@ -299,6 +307,9 @@ def linears(x, layers):
     """The outputs of several :class:`Mx4Linear` for the same x, which is quantised once, three products to a launch."""
     for m in layers:
         _need(x.shape[-1] == m.in_features, f"expected {m.in_features} input features, got {x.shape[-1]}")
+    if forward_ad._current_level >= 0:
+        for t in (x, *(t for m in layers for t in (m.weight, m.bias) if t is not None)):
+            _need(forward_ad.unpack_dual(t).tangent is None, "a tensor with a tangent, which a layer in 4 bits does not carry on")
     if torch.is_grad_enabled() and (x.requires_grad or any(not m.packed and m.weight.requires_grad for m in layers)):
         _need(not any(m.packed for m in layers), "a packed layer serves the forward only: call it under torch.no_grad()")
         ys = Mx4LinearFunction.apply(x, *(m.weight for m in layers))

@@ -11,6 +11,7 @@ import functools
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (COMBINE_DIV_PROD, COMBINE_MUL_MUL, COMBINE_MUL_PROD, GEMM_LARGE_TILES, GEMM_ONE_TILE, GEMM_SKINNY, GEMM_STRICT, GEMM_TILED, GEMM_TOGETHER, INV_AMAX_DIV_127,
@@ -699,6 +700,8 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
         _check_bf16(t, name)
         _need(t.get_device() == torch._C._cuda_getDevice(), f"{name} must be on the current GPU")
         _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a quantised tensor does not give: call this under torch.no_grad()")
+        _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent, which a quantised tensor does not carry on")
+    _need(torch._C._get_tracing_state() is None, "rmsnorm_quant cannot be traced: what it launches would not be recorded")
     dim = x.shape[-1] if x.dim() else 0
     _need(x.numel() > 0 and dim % (8 if to == "mx4" else 128) == 0 and dim <= 16384,
           f"x must be non-empty and its last dim a multiple of {8 if to == 'mx4' else 128} up to 16384, got {tuple(x.shape)}")
@@ -732,6 +735,7 @@ def dequant_row(q, s):
     y = _natively("dequant_row", q, s)
     if y is not None:
         return y
+    _need(torch._C._get_tracing_state() is None, "dequant_row cannot be traced: what it launches would not be recorded")
     _need(isinstance(q, torch.Tensor) and isinstance(s, torch.Tensor) and _on_gpu(q) and _on_gpu(s) and q.get_device() == s.get_device() == torch._C._cuda_getDevice(),
           "q and s must be tensors on the current GPU")
     _need(q.dtype == torch.int8 and s.dtype == torch.float32 and q.dim() >= 1 and q.numel() > 0 and q.shape[-1] % 8 == 0,
