@@ -373,3 +373,59 @@ def test_tangents_and_traces_are_refused(T, dev):
     for call in (layer, T.mx4.quant_row, lambda t: T.ops.rmsnorm_quant(t, w, 1e-5)[0]):
         with pytest.raises(ValueError, match="traced"):
             torch.jit.trace(call, (x,), check_trace=False)
+
+
+def test_broadcast_inputs_and_gradients(T, dev):
+    """An input that is one row expanded, and a gradient that is one number expanded: what copies of them give; the row's gradient is the sum of the copies'."""
+    (m,) = layers_of(T, dev, 256, (96,))
+    row = randn_bf16(make_gen(1), 256).to(dev)
+    grads = []
+    for expanded in (True, False):
+        leaf = (row.clone() if expanded else row.expand(5, 256).clone()).requires_grad_()
+        m.weight.grad = None
+        y = m(leaf.expand(5, 256) if expanded else leaf)
+        (y.sum() if expanded else (y * torch.ones_like(y)).sum()).backward()
+        grads.append((y.detach(), m.weight.grad, leaf.grad if expanded else leaf.grad.sum(0)))
+    assert all(bits_equal(a, b) for a, b in zip(*grads))
+
+
+def test_the_same_weight_twice(T, dev):
+    """Its gradient is the sum of both uses'."""
+    (m,) = layers_of(T, dev, 256, (96,))
+    x, dy = randn_bf16(make_gen(1), 7, 256).to(dev), [randn_bf16(make_gen(s), 7, 96).to(dev) for s in (2, 3)]
+    single = []
+    for d in dy:
+        m.weight.grad = None
+        m(x).backward(d)
+        single.append(m.weight.grad)
+    m.weight.grad = None
+    a, b = T.mx4.linears(x, (m, m))
+    assert bits_equal(a, b)
+    torch.autograd.backward((a, b), dy)
+    assert bits_equal(m.weight.grad, single[0] + single[1]) or bits_equal(m.weight.grad, single[1] + single[0])
+
+
+def test_threads(T, dev):
+    """Calls from several threads at once, each on a stream of its own."""
+    import threading
+    work = []
+    for n, k, tokens in ((96, 256, 50), (640, 512, 300), (64, 1000, 7)):
+        gen = make_gen(n)
+        x, w, dy = (randn_bf16(gen, *s).to(dev) for s in ((tokens, k), (n, k), (tokens, n)))
+        work.append(((x, w, dy), [t.clone() for t in T.mx4.linear_fwd_bwd(x, w, dy)]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(inputs, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = T.mx4.linear_fwd_bwd(*inputs)
+                torch.cuda.current_stream().synchronize()
+                if not all(bits_equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(inputs[0].shape)
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -321,11 +321,14 @@ def linears(x, layers):
 
 def _as_written(modules, cls, call):
     """Whether calls of these modules do just what their class does: no hooks, nothing replaced."""
+    for m in modules:
+        if type(m) is not cls:
+            return False
     if torch.nn.modules.module._has_any_global_hook() or (cls.forward, cls.__call__, cls._call_impl) != call:
         return False
     for m in modules:
         own = m.__dict__
-        if type(m) is not cls or "forward" in own or "_call_impl" in own or m._compiled_call_impl is not None:
+        if "forward" in own or "_call_impl" in own or m._compiled_call_impl is not None:
             return False
         if m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks:
             return False
