@@ -132,10 +132,12 @@ def dequant(codes, scales, cols):
 def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
     """``A B^T`` of tensors in 4 bits: A [M, ..] or [batch, M, ..], B [N, ..] (that all batches share) or [batch, N, ..]; bf16 or float32, [M, N] or [batch, M, N].
     Added up in fp32 in a fixed order and rounded once."""
+    wide = out_dtype is torch.float32
+    if wide or out_dtype is torch.bfloat16:
+        out = _natively("mx4_gemm_nt", A, sA, B, sB, 1 if wide else 0)
+        if out is not None:
+            return out
     _need(out_dtype in (torch.bfloat16, torch.float32), f"out_dtype must be bfloat16 or float32, got {out_dtype}")
-    out = _natively("mx4_gemm_nt", A, sA, B, sB, int(out_dtype == torch.float32))
-    if out is not None:
-        return out
     A, sA, a = _operand(A, sA, "A")
     B, sB, b = _operand(B, sB, "B")
     _need(A.shape[-1] == B.shape[-1], f"A has {A.shape[-1] // 128} tiles along the contraction, B {B.shape[-1] // 128}")
@@ -149,7 +151,7 @@ def gemm_nt(A, sA, B, sB, out_dtype=torch.bfloat16):
     _need(batch <= 65535 and M <= MOST_ROWS, f"a product takes up to 65535 batches and 2^28 rows, got {batch} and {M}")
     need = _lib.lib().ti8_mx4_gemm_nt_workspace(batch, M, N, K)
     workspace = torch.empty((need,), dtype=torch.uint8, device=A.device) if need > 0 else None
-    _lib.call("ti8_mx4_gemm_nt", a, rows_a if batch > 1 else 0, b, rows_b if batch > 1 else 0, out.data_ptr(), N, M * N, batch, M, N, K, int(out_dtype == torch.float32),
+    _lib.call("ti8_mx4_gemm_nt", a, rows_a if batch > 1 else 0, b, rows_b if batch > 1 else 0, out.data_ptr(), N, M * N, batch, M, N, K, int(wide),
               None if workspace is None else workspace.data_ptr(), need, _stream())
     return out
 

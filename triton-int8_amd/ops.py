@@ -678,7 +678,9 @@ def rmsnorm(x, weight, eps):
 def _natively(name, *args):
     """A call with its checks, allocations and launch made from C++, or None where it takes the Python way, which says what is wrong."""
     native = _lib.native()
-    out = None if native is None else getattr(native, name)(*args, _stream())
+    if native is None:
+        return None
+    out = getattr(native, name)(*args, _stream())
     if type(out) is tuple:
         raise _lib.failed(*out)
     return out
@@ -689,11 +691,12 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
     multiple of 8 (with "int8" of 128) up to 16384.
 
-    Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean added up in 64 bits.  Quantised tensors have no gradients: x, weight and residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and,
-    the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
-    made = _natively("rmsnorm_quant", x, weight, residual, eps, int(to == "mx4"), group, inv_mode, Q_CLAMP) if to in ("mx4", "int8") else None
-    if made is not None:
-        return tuple(made)
+    Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean added up in 64 bits.  Quantised tensors have no gradients: x, weight and
+    residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and, the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
+    if to == "mx4" or to == "int8":
+        made = _natively("rmsnorm_quant", x, weight, residual, eps, 1 if to == "mx4" else 0, group, inv_mode, Q_CLAMP)
+        if made is not None:
+            return tuple(made)
     _need(to in ("mx4", "int8"), f"`to` must be 'mx4' or 'int8', got {to!r}")
     _need(group in (0, 128) and (group == 0 or to == "int8"), f"group must be 0 or, with 'int8', 128, got {group}")
     for t, name in ((x, "x"), (weight, "weight")) + (() if residual is None else ((residual, "residual"),)):
