@@ -534,25 +534,33 @@ PyObject* mx4_gemm_nt_multi(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     END_HANDLE_TH_ERRORS
 }
 
-// mx4_linear_fwd_bwd(X, W, dY, stream) -> [Y, dX, dW]
+// mx4_linear_fwd_bwd(X [.., K], W, dY [.., N], stream) -> [Y, dX, dW]
 PyObject* mx4_linear_fwd_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     at::Tensor X, W, dY, Y, dX, dW;
     at::Tensor* const tensors[] = {&X, &W, &dY};
     int64_t stream;
     if (nargs != 4 || !tensors_of(args, tensors, 3) || !number(args[3], &stream)) Py_RETURN_NONE;
-    for (const at::Tensor* t : tensors)
-        if (!on(*t, at::kBFloat16, current_device()) || t->dim() != 2 || t->stride(1) != 1 || t->stride(0) < t->size(1)) Py_RETURN_NONE;
-    const int64_t T = X.size(0), K = X.size(1), N = W.size(0), need = mx4_step_workspace(T, K, N);
-    if (W.size(1) != K || dY.size(0) != T || dY.size(1) != N || need < 0) Py_RETURN_NONE;
+    // rows apart, or in a tensor of other dimensions dense
+    int64_t ld[3];
+    for (int i = 0; i < 3; ++i) {
+        const at::Tensor& t = *tensors[i];
+        if (!on(t, at::kBFloat16, current_device()) || t.dim() < 1 || (t.dim() == 2 ? t.stride(1) != 1 || t.stride(0) < t.size(1) : !t.is_contiguous())) Py_RETURN_NONE;
+        ld[i] = t.dim() == 2 ? t.stride(0) : t.size(-1);
+    }
+    if (W.dim() != 2 || dY.dim() != X.dim() || dY.sizes().slice(0, dY.dim() - 1) != X.sizes().slice(0, X.dim() - 1)) Py_RETURN_NONE;
+    const int64_t K = X.size(-1), T = X.numel() / K, N = W.size(0);
+    if (W.size(1) != K || dY.size(-1) != N) Py_RETURN_NONE;
+    const int64_t need = mx4_step_workspace(T, K, N);
+    if (need < 0) Py_RETURN_NONE;
     int status;
     {
         const GilReleased released;
-        Y = fresh({T, N}, at::kBFloat16);
-        dX = fresh({T, K}, at::kBFloat16);
+        Y = fresh(dY.sizes(), at::kBFloat16);
+        dX = fresh(X.sizes(), at::kBFloat16);
         dW = fresh({N, K}, at::kBFloat16);
         const Workspace workspace(need, X.device(), at::TensorOptions().dtype(at::kByte).device(X.device()));
-        status = mx4_step_entry(X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), dY.data_ptr(), dY.stride(0), Y.data_ptr(), dX.data_ptr(), dW.data_ptr(), T, K, N,
+        status = mx4_step_entry(X.data_ptr(), ld[0], W.data_ptr(), ld[1], dY.data_ptr(), ld[2], Y.data_ptr(), dX.data_ptr(), dW.data_ptr(), T, K, N,
                                 workspace.p, need, stream_of(stream));
     }
     if (status != TI8_OK) return Py_BuildValue("(si)", "ti8_mx4_linear_fwd_bwd", status);

@@ -160,8 +160,9 @@ def gemm_nt_multi(problems):
     """Up to three products ``(A, sA, B, sB)`` of matrices, in one launch where that is faster: a list of bf16 matrices.  What :func:`gemm_nt` gives, but for the order
     in which contractions are added up."""
     _need(1 <= len(problems) <= 3, f"between 1 and 3 products, got {len(problems)}")
-    _need(all(len(p) == 4 for p in problems), "a product is (codes of A, scales of A, codes of B, scales of B)")
-    made = _natively("mx4_gemm_nt_multi", *(t for p in problems for t in p))
+    for p in problems:
+        _need(len(p) == 4, "a product is (codes of A, scales of A, codes of B, scales of B)")
+    made = _natively("mx4_gemm_nt_multi", *[t for p in problems for t in p])
     if made is not None:
         return made
     descs, outs, keep = (_lib.Mx4GemmProblem * len(problems))(), [], []
@@ -193,24 +194,24 @@ def _dense_rows(x):
 def linear_fwd_bwd(X, W, dY):
     """One forward and backward of a layer, every product in 4 bits: ``(Y, dX, dW)`` for X bf16 [.., K], W bf16 [N, K] and dY bf16 [.., N].  The operands of
     dX = dY W are in 4 bits along N, those of dW = dY^T X along the tokens."""
+    made = _natively("mx4_linear_fwd_bwd", X, W, dY)
+    if made is not None:
+        return tuple(made)
     K, N = X.shape[-1], W.shape[0]
     X2, dY2 = X.reshape(-1, K), dY.reshape(-1, N)
     _fit(X2, W, dY2)
     if X2.shape[0] == 0:    # nothing to multiply: empty Y and dX, a zero weight gradient (as torch.nn.functional.linear gives)
         return X.new_empty((*X.shape[:-1], N)), torch.empty_like(X), torch.zeros_like(W)
-    made = _natively("mx4_linear_fwd_bwd", X2, W, dY2)
-    if made is None:
-        for t, name in ((X2, "X"), (W, "W"), (dY2, "dY")):
-            _bf16(t, name)
-        X2, W, dY2 = (_dense_rows(t) for t in (X2, W, dY2))
-        T, dev = X2.shape[0], X2.device
-        need = _lib.lib().ti8_mx4_linear_fwd_bwd_workspace(T, K, N)
-        _need(need >= 0, f"a step takes up to 2^22 tokens and features, got {T}, {K} and {N}")
-        made = [torch.empty(shape, dtype=torch.bfloat16, device=dev) for shape in ((T, N), (T, K), (N, K))]
-        workspace = ops._workspace(need, dev)
-        _lib.call("ti8_mx4_linear_fwd_bwd", X2.data_ptr(), X2.stride(0), W.data_ptr(), W.stride(0), dY2.data_ptr(), dY2.stride(0), *(t.data_ptr() for t in made), T, K, N,
-                  workspace.data_ptr(), need, _stream())
-    Y, dX, dW = made
+    for t, name in ((X2, "X"), (W, "W"), (dY2, "dY")):
+        _bf16(t, name)
+    X2, W, dY2 = (_dense_rows(t) for t in (X2, W, dY2))
+    T, dev = X2.shape[0], X2.device
+    need = _lib.lib().ti8_mx4_linear_fwd_bwd_workspace(T, K, N)
+    _need(need >= 0, f"a step takes up to 2^22 tokens and features, got {T}, {K} and {N}")
+    Y, dX, dW = (torch.empty(shape, dtype=torch.bfloat16, device=dev) for shape in ((T, N), (T, K), (N, K)))
+    workspace = ops._workspace(need, dev)
+    _lib.call("ti8_mx4_linear_fwd_bwd", X2.data_ptr(), X2.stride(0), W.data_ptr(), W.stride(0), dY2.data_ptr(), dY2.stride(0), Y.data_ptr(), dX.data_ptr(), dW.data_ptr(), T, K, N,
+              workspace.data_ptr(), need, _stream())
     return Y.view(*X.shape[:-1], N), dX.view(X.shape), dW
 
 
@@ -223,7 +224,7 @@ def _column_sum(x):
 def _products(codes, scales, views, shape):
     """Outputs [*shape, features] for an input in 4 bits and the forward's views of several weights: three to a launch."""
     ys = [y for i in range(0, len(views), 3) for y in gemm_nt_multi([(codes, scales, *v) for v in views[i:i + 3]])]
-    return tuple(y.view(*shape, y.shape[1]) for y in ys)
+    return tuple(ys) if len(shape) == 1 else tuple(y.view(*shape, y.shape[1]) for y in ys)
 
 
 class Mx4LinearFunction(torch.autograd.Function):
@@ -302,7 +303,8 @@ class _BiasFunction(torch.autograd.Function):
 def _served(codes, scales, shape, layers):
     """Outputs [*shape, out_features] of layers whose input is already in 4 bits."""
     ys = _products(codes, scales, [m.quantised() for m in layers], shape)
-    return tuple(y if m.bias is None else y + m.bias for y, m in zip(ys, layers))
+    biases = [m.bias for m in layers]       # (a module's attributes take a while)
+    return tuple(y if b is None else y + b for y, b in zip(ys, biases))
 
 
 def linears(x, layers):
@@ -318,7 +320,7 @@ def linears(x, layers):
         return tuple(y if m.bias is None else _BiasFunction.apply(y, m.bias) for y, m in zip(ys, layers))
     if x.numel() == 0:
         return tuple(x.new_empty((*x.shape[:-1], m.out_features)) for m in layers)
-    return _served(*quant_row(x.reshape(-1, x.shape[-1])), x.shape[:-1], layers)
+    return _served(*quant_row(x if x.dim() == 2 else x.reshape(-1, x.shape[-1])), x.shape[:-1], layers)
 
 
 def _as_written(modules, cls, call):
@@ -366,7 +368,8 @@ class Mx4Linear(torch.nn.Module):
 
     def quantised(self):
         """The forward's view of the weight, ``(codes, scales)``: the packed one, or one made now."""
-        return (self.codes, self.scales) if self.packed else quant_row(self.weight.detach())
+        codes = self.codes
+        return quant_row(self.weight.detach()) if codes is None else (codes, self.scales)
 
     def forward(self, x):
         return linears(x, (self,))[0]
