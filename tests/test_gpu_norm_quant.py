@@ -78,7 +78,7 @@ def test_many_rows(T, dev, rows):
     check(T, dev, *inputs(rows, 384), to="int8", group=128)
 
 
-@pytest.mark.parametrize("rows", [1, 7, 60, 61, 62, 63, 64, 300])       # (around 1 MB in all, up to which they share a block)
+@pytest.mark.parametrize("rows", [1, 7, 300, 400, 401, 402, 403, 404, 405, 900])       # (around 4 MB in all, up to which they share a block)
 def test_results_lie_apart(T, dev, rows):
     x, w, r = (t.to(dev) for t in inputs(rows, 4096))
     for results in (T.ops.rmsnorm_quant(x, w, EPS, residual=r), T.ops.rmsnorm_quant(x, w, EPS, residual=r, to="int8", group=128), T.ops.rmsnorm_quant(x, w, EPS),

@@ -355,11 +355,11 @@ extern "C" int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_str
         return check_launch(fn);
     }
     if (!mx4::grid_ok(elements / (64 * 64))) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    // Up to four workgroups of 64 x 64 elements per CU: small ones, whose code is a quarter as long (it is read from memory too); behind that 128 or 256 rows of a
-    // column to a workgroup, whose codes are written in longer pieces.  us, both ways, small / large: 200 x 300 4.3 / 5.8, 1001 x 1016 4.6 / 5.1, 1000 x 2560 5.3 / 5.6,
-    // 2048 x 4096 9.4 / 8.5, 14336 x 4096 44 / 37 (4.9 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
+    // Small tensors: workgroups of 128 x 64 elements (by columns alone 64 x 64), whose code is a quarter as long (it is read from memory too); behind that twice as many
+    // columns to a workgroup, whose rows' codes are written in longer pieces.  us, both ways, small / large, tensors from memory: 200 x 300 4.1 / 5.5, 1001 x 1016 4.9 / 5.3,
+    // 1500 x 1500 6.3 / 8.3, 2048 x 2048 7.4 / 6.9, 4096 x 4096 17 / 16, 14336 x 4096 50 / 41 (4.4 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
     const bool small = elements < (int64_t)16384 * device_cu_count(), rows = operands[0].by_rows.codes;
-    if (small) rows ? mx4::launch_cols<2, 8, true>(g, st) : mx4::launch_cols<2, 8, false>(g, st);
+    if (small) rows ? mx4::launch_cols<4, 8, true>(g, st) : mx4::launch_cols<2, 8, false>(g, st);
     else rows ? mx4::launch_cols<4, 4, true>(g, st) : mx4::launch_cols<8, 4, false>(g, st);
     return check_launch(fn);
 }

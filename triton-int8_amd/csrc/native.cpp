@@ -361,12 +361,12 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
     return at::detail::empty_generic(sizes, at::detail::getCUDAHooks().getCUDADeviceAllocator(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, c10::nullopt);
 }
 
-// Room for the results of one call that die together.  Up to 1 MB in all they share a block of memory: asking for one and giving it back takes 0.4 us of a call
-// that takes 5.
+// Room for the results of one call that die together.  Up to 4 MB in all they share a block of memory: asking for one and giving it back takes 0.4 us of a call
+// that takes 5, and up to about there the kernel takes no longer than that.
 class Room {
   public:
     explicit Room(int64_t bytes = INT64_MAX) {
-        if (bytes <= 1 << 20) block_ = fresh({bytes}, at::kByte);
+        if (bytes <= 4 << 20) block_ = fresh({bytes}, at::kByte);
     }
     static int64_t of(int64_t bytes) { return (bytes + 255) / 256 * 256; }
     static int64_t of_mx4(int64_t rows, int64_t cols) { return of(rows * ((cols + 255) / 256) * 128) + of(rows * ((cols + 255) / 256) * 8); }
