@@ -135,7 +135,7 @@ def test_products(M, dev, m, n, k, out_dtype):
     products(M, dev, tensor(gen, m, k), tensor(gen, n, k, spread=False), out_dtype)
 
 
-@pytest.mark.parametrize("batch,m,n,k", [(2, 3, 5, 300), (5, 40, 33, 256), (3, 150, 70, 520), (9, 1, 17, 1000)])
+@pytest.mark.parametrize("batch,m,n,k", [(2, 3, 5, 300), (5, 40, 33, 256), (3, 150, 70, 520), (9, 1, 17, 1000), (3, 40, 30, 9000)])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_batches(M, dev, batch, m, n, k, out_dtype):
     gen = make_gen(batch)

@@ -42,6 +42,7 @@ extern "C" int ti8_init(void) {
     if (int e = init_attention_kernels()) return e;
     if (int e = cache4::init()) return e;
     if (int e = cache4::init_attention()) return e;
+    if (int e = mx4::init()) return e;
     if (int e = init_quant_scratch()) return e;
     // last: a device that refuses the persistent kernel's 160 KiB of LDS is not an error (the one-tile kernel serves
     // its shapes), but the message says so

@@ -493,22 +493,30 @@ int launch_few(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES>
-int launch(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
+int prepare(const char* fn, bool many) {
     constexpr int LDS = gemm_lds(BM, BN, STAGES);
     static_assert(LDS <= 160 * 1024, "LDS of a CU");
+    static OncePerDevice once[2];
+    const void* const kernel = many ? reinterpret_cast<const void*>(gemm_kernel<BM, BN, WM, WN, STAGES, Gemms>) : reinterpret_cast<const void*>(gemm_kernel<BM, BN, WM, WN, STAGES, Gemm>);
+    if (LDS > 65536 && raise_lds_limit(once[many], kernel, LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
+    return TI8_OK;
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES>
+int launch(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     const int64_t tiles = share_out(all, [](Gemm& g) {
         g.tiles_m = (g.M + BM - 1) / BM;
         g.tiles_n = (g.N + BN - 1) / BN;
         return (int64_t)g.tiles_m * g.tiles_n;
     });
     if (tiles < 0 || tiles > 0x3fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
-    const auto run = [&](auto kernel, OncePerDevice& once, const auto& products) {
-        if (LDS > 65536 && raise_lds_limit(once, reinterpret_cast<const void*>(kernel), LDS) != hipSuccess) return fail(TI8_ERR_HIP, "%s: %d bytes of LDS refused", fn, LDS);
-        kernel<<<dim3((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), dim3(64 * WM * WN), LDS, st>>>(products);
-        return check_launch(fn);
-    };
-    static OncePerDevice one, many;
-    return all.count > 1 ? run(gemm_kernel<BM, BN, WM, WN, STAGES, Gemms>, many, all) : run(gemm_kernel<BM, BN, WM, WN, STAGES, Gemm>, one, all.g[0]);
+    if (int e = prepare<BM, BN, WM, WN, STAGES>(fn, all.count > 1)) return e;
+    const dim3 grid((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), block(64 * WM * WN);
+    if (all.count > 1)
+        gemm_kernel<BM, BN, WM, WN, STAGES, Gemms><<<grid, block, gemm_lds(BM, BN, STAGES), st>>>(all);
+    else
+        gemm_kernel<BM, BN, WM, WN, STAGES, Gemm><<<grid, block, gemm_lds(BM, BN, STAGES), st>>>(all.g[0]);
+    return check_launch(fn);
 }
 
 // The parts of a contraction added up in order: [parts][batch][M][N] in fp32 -> C
@@ -582,6 +590,20 @@ int describe(const char* fn, const ti8_mx4* a, int64_t rows_a, const ti8_mx4* b,
     return TI8_OK;
 }
 }  // namespace
+
+int init() {
+    const char* const fn = "ti8_init";
+    for (const bool many : {false, true}) {
+        int e = prepare<32, 64, 1, 2, 4>(fn, many);
+        if (!e) e = prepare<64, 64, 2, 2, 4>(fn, many);
+        if (!e) e = prepare<64, 128, 2, 2, 4>(fn, many);
+        if (!e) e = prepare<128, 128, 2, 2, 3>(fn, many);
+        if (!e) e = prepare<128, 128, 2, 2, 2>(fn, many);
+        if (!e) e = prepare<256, 256, 2, 4, 2>(fn, many);
+        if (e) return e;
+    }
+    return TI8_OK;
+}
 }  // namespace mx4
 }  // namespace ti8
 

@@ -66,6 +66,9 @@ namespace cache4 {
 int init();
 int init_attention();
 }
+namespace mx4 {
+int init();
+}
 
 // ---- pieces of quant.hip and fwht.hip that the layer calls (step.hip) use ----------
 // `valid_rows` (of R, the rest counts as zeros and is not read): an activation whose token count is no multiple of the tile
