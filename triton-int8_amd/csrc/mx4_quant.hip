@@ -211,6 +211,7 @@ struct NormArgs {
     int64_t ldq;
     float* s;
     QMode mode;
+    int once;       // whether what is read goes past the caches
 };
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -220,8 +221,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 }
 
 // h = bf16(x + residual), r = 1 / sqrt(mean(h^2) + eps), y = bf16(bf16(h r) w), quantised: a row in the registers of T threads (64: four rows to a workgroup),
-// NV octets each.  The squares are added up in 64 bits (they are exact in it) and r is rounded to 32 once, so that an order of summation moves it by parts in 2^53 before that.  With a residual, 4 bits: 1 x 4096 3.3 us,
-// 16384 x 4096 93 (4.7 TB/s); int8 by groups 2047 x 4096 15.7 (3.7 TB/s: all rows are loaded at once, then all stored).
+// NV octets each.  The squares are added up in 64 bits (they are exact in it) and r is rounded to 32 once, so that an order of summation moves it by parts in 2^53 before that.  With a residual, 4 bits, tensors from memory: 1 x 4096 3.4
+// us, 2047 x 4096 16.9, 16384 x 4096 84 (5.2 TB/s; a load at a time in front of a store 90); int8 by groups 2047 x 4096 17.9, 16384 x 4096 84 (5.6 TB/s).
 template <int T, int NV, int TO>
 __global__ __launch_bounds__(THREADS) void rmsnorm_quant_kernel(NormArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -232,19 +233,26 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_quant_kernel(NormArgs g) {
     const int t = threadIdx.x % T, octets = g.dim >> 3;
     uint4 v[NV];
     double sum = 0.0;
+    // all loads in front of the first store, which they might overlap for all that the compiler knows
+    const auto load_row = [&](auto load) {
+        uint4 b[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int o = t + i * T;
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (o < octets) {
-            v[i] = load16(g.x + row * g.ldx + o * 8);
-            if (g.residual) {
-                const uint4 b = load16(g.residual + row * g.ldr + o * 8);
-                v[i] = make_uint4(add_bf16x2(v[i].x, b.x), add_bf16x2(v[i].y, b.y), add_bf16x2(v[i].z, b.z), add_bf16x2(v[i].w, b.w));
-                *reinterpret_cast<uint4*>(g.h + row * g.ldh + o * 8) = v[i];
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int o = t + i * T;
+            v[i] = o < octets ? load(g.x + row * g.ldx + o * 8) : make_uint4(0, 0, 0, 0);
+            if (g.residual && o < octets) b[i] = load(g.residual + row * g.ldr + o * 8);
         }
-    }
+        if (!g.residual) return;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int o = t + i * T;
+            if (o >= octets) continue;
+            v[i] = make_uint4(add_bf16x2(v[i].x, b[i].x), add_bf16x2(v[i].y, b[i].y), add_bf16x2(v[i].z, b[i].z), add_bf16x2(v[i].w, b[i].w));
+            *reinterpret_cast<uint4*>(g.h + row * g.ldh + o * 8) = v[i];
+        }
+    };
+    if (g.once) load_row([](const uint16_t* p) { return load16_once(p); });
+    else load_row([](const uint16_t* p) { return load16(p); });
     const auto word = [&](int i, int j) { return j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w; };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -306,8 +314,14 @@ __global__ __launch_bounds__(THREADS) void rmsnorm_quant_kernel(NormArgs g) {
 
 constexpr int NORM_MAX_DIM = THREADS * 8 * 8;
 
+// Tensors that the last-level cache does not hold beside what is written are read past the caches; smaller ones, which whoever made them has left there, are not.  us, x
+// just written by another kernel, a load at a time, past them / not: 1024 x 4096 9.4 / 8.6, 2047 x 4096 17.2 / 15.6, 4096 x 4096 26.3 / 26.1, 8192 x 4096 43.7 / 48.3,
+// 16384 x 4096 83.5 / 87.7.
+constexpr int64_t NORM_ONCE = (int64_t)24 << 20;
+
 template <int TO>
-void launch_norm(const NormArgs& g, hipStream_t st) {
+void launch_norm(NormArgs g, hipStream_t st) {
+    g.once = g.rows * g.dim > NORM_ONCE;
     const auto go = [&](auto kernel, int rows_per_group) { kernel<<<dim3((unsigned)((g.rows + rows_per_group - 1) / rows_per_group)), dim3(THREADS), 0, st>>>(g); };
     if (g.dim <= 512) go(rmsnorm_quant_kernel<64, 1, TO>, 4);
     else if (g.dim <= 1024) go(rmsnorm_quant_kernel<64, 2, TO>, 4);
@@ -406,7 +420,7 @@ extern "C" int ti8_rmsnorm_quant(const ti8_rmsnorm_quant_args* a, ti8_stream_t s
         (reinterpret_cast<uintptr_t>(a->rstd) & 3))
         return fail(TI8_ERR_ALIGN, "%s: rows of x, residual and h and the weight must be 16-byte aligned", fn);
     mx4::NormArgs g{static_cast<const uint16_t*>(a->x), static_cast<const uint16_t*>(a->residual), static_cast<const uint16_t*>(a->w), a->ldx, a->ldr, a->ldh, rows,
-                    static_cast<uint16_t*>(a->h), a->rstd, (int)dim, a->eps, {}, a->q, a->ldq, a->s, {}};
+                    static_cast<uint16_t*>(a->h), a->rstd, (int)dim, a->eps, {}, a->q, a->ldq, a->s, {}, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->mx4.codes) {
         if (int e = mx4::check(fn, "mx4", &a->mx4, rows, dim, g.mx)) return e;
