@@ -82,9 +82,9 @@ __device__ __forceinline__ void beside(int q, int count, int n, const F& f) {
 }
 
 // One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS.  256 x 256: per K tile a CU's matrix instructions take 2048 cycles, its LDS reads and writes
-// as many; 8192 x 14336 x 4096 235 us (4.1 PFLOP/s) at a clock of 1.75 GHz, on codes of zero 172: the chip's power bounds it (a loop of nothing but these instructions
+// as many; 8192 x 14336 x 4096 225 to 235 us (4.1 to 4.3 PFLOP/s) at a clock of 1.7 GHz, on codes of zero 172: the chip's power bounds it (a loop of nothing but these instructions
 // reaches 6.6 PFLOP/s on random codes, 9.7 on zeros).  16 x 16 x 128 instructions, four waves of 128 x 128, workgroups that go on to the next tile: within 3 %.  Smaller
-// tiles where those do not fill the CUs: 700 x 4096 x 4096 10.5 us, 128 x 4096 x 4096 5.9, of which 2.2 are the launch and 1.5 to 3 a tile's first loads and results.
+// tiles where those do not fill the CUs: 700 x 4096 x 4096 10.3 to 11.5 us, 128 x 4096 x 4096 5.9, of which 2.2 are the launch and 1.5 to 3 a tile's first loads and results.
 constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
 constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
 constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14

@@ -23,7 +23,7 @@ struct QuantArgs {
 };
 
 // By rows: 32 rows x 256 columns per workgroup; a row's 512 bytes are read by half a wave, a group's maximum is over four lanes.
-// 14336 x 4096: 24 us (6.1 TB/s).
+// 14336 x 4096: 24 to 26 us (5.6 to 6.1 TB/s).
 __global__ __launch_bounds__(THREADS) void quant_row_kernel(QuantOperand g) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const int64_t tiles = idx::mx4_tiles(g.C), tile = blockIdx.x % tiles, first = (int64_t)(blockIdx.x / tiles) * idx::MX4_ROW_BLOCK, row0 = first + (threadIdx.x >> 5);
@@ -371,7 +371,7 @@ extern "C" int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_str
     if (!mx4::grid_ok(elements / (64 * 64))) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     // Small tensors: workgroups of 128 x 64 elements (by columns alone 64 x 64), whose code is a quarter as long (it is read from memory too); behind that twice as many
     // columns to a workgroup, whose rows' codes are written in longer pieces.  us, both ways, small / large, tensors from memory: 200 x 300 4.1 / 5.5, 1001 x 1016 4.9 / 5.3,
-    // 1500 x 1500 6.3 / 8.3, 2048 x 2048 7.4 / 6.9, 4096 x 4096 17 / 16, 14336 x 4096 50 / 41 (4.4 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
+    // 1500 x 1500 6.3 / 8.3, 2048 x 2048 7.4 / 6.9, 4096 x 4096 17 / 16, 14336 x 4096 50 / 41 (37 since x is read past the caches: 4.9 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
     const bool small = elements < (int64_t)16384 * device_cu_count(), rows = operands[0].by_rows.codes;
     if (small) rows ? mx4::launch_cols<4, 8, true>(g, st) : mx4::launch_cols<2, 8, false>(g, st);
     else rows ? mx4::launch_cols<4, 4, true>(g, st) : mx4::launch_cols<8, 4, false>(g, st);
