@@ -255,9 +255,15 @@ class DecoderLayer(torch.nn.Module):
         return mx4._served(q.view(-1, q.shape[-1]), s, x.shape[:-1], layers), h[0] if h else x
 
     def copy_weights_from(self, other):
-        """Share initial values with another layer (int8 layer <-> bf16 twin)."""
+        """Share initial values with another layer (int8 layer <-> bf16 twin) of the same sizes, also one inside a wrapper.  Packed layers copy their codes, from packed ones alone."""
+        mine, theirs = (sorted([*m.named_parameters(), *((n, b) for n, b in m.named_buffers() if n.endswith((".codes", ".scales")))]) for m in (self, other))
+        if len(mine) != len(theirs) or not all(b == a or b.endswith("." + a) for (a, _), (b, _) in zip(mine, theirs)):
+            raise ValueError(f"the layers do not hold the same weights (is one of them packed?): {sorted({n for n, _ in mine} ^ {n for n, _ in theirs})}")
+        for (name, p), (_, q) in zip(mine, theirs):
+            if p.shape != q.shape:
+                raise ValueError(f"{name} has the shape {tuple(p.shape)} here, {tuple(q.shape)} there")
         with torch.no_grad():
-            for (_, p), (_, q) in zip(sorted(self.named_parameters()), sorted(other.named_parameters())):
+            for (_, p), (_, q) in zip(mine, theirs):
                 p.copy_(q)
 
     def forward(self, x):
