@@ -84,7 +84,7 @@ struct Workspace {
 
 // Whether a tracer, a dispatch mode or a function transform looks at the operators of this thread
 bool followed() {
-    return at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled() ||
+    return at::tracer::impl::is_dispatch_enabled() || c10::impl::dispatch_mode_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
 }
 

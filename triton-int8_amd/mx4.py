@@ -12,7 +12,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .ops import _natively, _need, _stream
+from .ops import _natively, _need, _stream, _unrecorded
 
 __all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "gemm_nt_multi", "linear_fwd_bwd", "linears", "quant_col_t", "quant_row", "quant_row_col_t"]
 
@@ -29,13 +29,8 @@ def _here(t):
     return ops._on_gpu(t) and t.get_device() == torch._C._cuda_getDevice()
 
 
-def _recorded():
-    """Refuses calls under a tracer: what they launch would not be recorded."""
-    _need(torch._C._get_tracing_state() is None, "calls in 4 bits cannot be traced: what they launch would not be recorded")
-
-
 def _bf16(x, name, dim=None):
-    _recorded()
+    _unrecorded("a call in 4 bits")
     _need(isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and _here(x), f"{name} must be a bfloat16 tensor on the current GPU")
     _need(x.dim() >= 1 and x.numel() > 0 and dim in (None, x.dim()), f"{name} must be a non-empty tensor" + ("" if dim is None else f" of {dim} dimensions"))
 
@@ -99,7 +94,7 @@ def quant_row_col_t(x):
 
 def _operand(codes, scales, name):
     """Codes [rows, bytes] or [batch, rows, bytes] with their scales as the kernels read them: (codes, scales, C description)."""
-    _recorded()
+    _unrecorded("a call in 4 bits")
     _need(isinstance(codes, torch.Tensor) and codes.dtype == torch.uint8 and codes.dim() in (2, 3) and codes.numel() > 0 and codes.shape[-1] % 128 == 0 and _here(codes),
           f"codes of {name} must be a uint8 tensor [rows, tiles * 128] or [batch, rows, tiles * 128] on the current GPU")
     tiles, rows = codes.shape[-1] // 128, codes.shape[:-1].numel()
@@ -119,6 +114,7 @@ def dequant(codes, scales, cols):
     y = _natively("mx4_dequant", codes, scales, cols)
     if y is not None:
         return y
+    _unrecorded("a call in 4 bits")
     _need(isinstance(codes, torch.Tensor) and codes.dim() >= 1 and codes.numel() > 0, "codes must be a non-empty uint8 tensor [.., tiles * 128]")
     _need(isinstance(cols, int) and cols > 0 and codes.shape[-1] == _tiles(cols) * 128, f"{cols} columns have {_tiles(cols) * 128 if isinstance(cols, int) else '?'} bytes of codes, got {codes.shape[-1]}")
     flat = codes.reshape(-1, codes.shape[-1])

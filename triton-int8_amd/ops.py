@@ -686,6 +686,20 @@ def _natively(name, *args):
     return out
 
 
+_MODES_THAT_RECORD = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
+
+
+def _unrecorded(what):
+    """Refuses calls under a tracer (torch.jit.trace, make_fx, tensors without memory, functionalize): it would record the outputs' memory and nothing that fills it.
+    Modes that only watch are none, nor is vmap, whose mapped tensors have no address to call with."""
+    if torch.compiler.is_dynamo_compiling():     # (torch.compile leaves such calls out of its graphs and makes them)
+        return
+    level = torch._C._functorch.peek_interpreter_stack()
+    _need(torch._C._get_tracing_state() is None and not torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch)
+          and (torch._C._len_torch_dispatch_stack() == 0 or all(torch._C._get_dispatch_mode(k) is None for k in _MODES_THAT_RECORD))
+          and (level is None or level.key() == torch._C._functorch.TransformType.Vmap), f"{what} cannot be traced: what is launched would not be recorded")
+
+
 def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV_RCP_OF_SCALE):
     """``h = x + residual`` (bf16), ``y = bf16(h * rstd) * weight`` over the last dim and y quantised, in one pass: the step from a linear's output to the next one's operand.
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
@@ -697,6 +711,7 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
         made = _natively("rmsnorm_quant", x, weight, residual, eps, 1 if to == "mx4" else 0, group, inv_mode, Q_CLAMP)
         if made is not None:
             return tuple(made)
+    _unrecorded("rmsnorm_quant")
     _need(to in ("mx4", "int8"), f"`to` must be 'mx4' or 'int8', got {to!r}")
     _need(group in (0, 128) and (group == 0 or to == "int8"), f"group must be 0 or, with 'int8', 128, got {group}")
     for t, name in ((x, "x"), (weight, "weight")) + (() if residual is None else ((residual, "residual"),)):
@@ -704,7 +719,6 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
         _need(t.get_device() == torch._C._cuda_getDevice(), f"{name} must be on the current GPU")
         _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a quantised tensor does not give: call this under torch.no_grad()")
         _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent, which a quantised tensor does not carry on")
-    _need(torch._C._get_tracing_state() is None, "rmsnorm_quant cannot be traced: what it launches would not be recorded")
     dim = x.shape[-1] if x.dim() else 0
     _need(x.numel() > 0 and dim % (8 if to == "mx4" else 128) == 0 and dim <= 16384,
           f"x must be non-empty and its last dim a multiple of {8 if to == 'mx4' else 128} up to 16384, got {tuple(x.shape)}")
@@ -738,7 +752,7 @@ def dequant_row(q, s):
     y = _natively("dequant_row", q, s)
     if y is not None:
         return y
-    _need(torch._C._get_tracing_state() is None, "dequant_row cannot be traced: what it launches would not be recorded")
+    _unrecorded("dequant_row")
     _need(isinstance(q, torch.Tensor) and isinstance(s, torch.Tensor) and _on_gpu(q) and _on_gpu(s) and q.get_device() == s.get_device() == torch._C._cuda_getDevice(),
           "q and s must be tensors on the current GPU")
     _need(q.dtype == torch.int8 and s.dtype == torch.float32 and q.dim() >= 1 and q.numel() > 0 and q.shape[-1] % 8 == 0,
