@@ -82,7 +82,8 @@ def _natively(name, *args):
     out = None if native is None else getattr(native, name)(*args, _stream())
     if type(out) is tuple:
         raise _lib.failed(*out)
-    _need(out is not None or torch._C._get_tracing_state() is None, "calls on a cache cannot be traced: what they launch would not be recorded")
+    if out is None:
+        ops._unrecorded("a call on a cache")
     return out
 
 
