@@ -351,8 +351,9 @@ PyObject* cache4_evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 constexpr int64_t MX4_ROWS = 1 << 28, MX4_CONTRACTED = 1 << 22;
 
+// (codes carry no tangent on)
 bool on(const at::Tensor& t, at::ScalarType type, c10::DeviceIndex device) {
-    return t.defined() && t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.numel() > 0;
+    return t.defined() && t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.numel() > 0 && !t._fw_grad(0).defined();
 }
 bool at_multiple(const at::Tensor& t, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }
 

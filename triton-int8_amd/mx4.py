@@ -12,7 +12,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .ops import _natively, _need, _stream, _unrecorded
+from .ops import _natively, _need, _no_tangent, _stream, _unrecorded
 
 __all__ = ["Mx4Linear", "Mx4LinearFunction", "dequant", "gemm_nt", "gemm_nt_multi", "linear_fwd_bwd", "linears", "quant_col_t", "quant_row", "quant_row_col_t"]
 
@@ -33,6 +33,7 @@ def _bf16(x, name, dim=None):
     _unrecorded("a call in 4 bits")
     _need(isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16 and _here(x), f"{name} must be a bfloat16 tensor on the current GPU")
     _need(x.dim() >= 1 and x.numel() > 0 and dim in (None, x.dim()), f"{name} must be a non-empty tensor" + ("" if dim is None else f" of {dim} dimensions"))
+    _no_tangent(x, name)
 
 
 def _empty(rows, cols, device, lead=None):
@@ -268,6 +269,7 @@ class Mx4LinearFunction(torch.autograd.Function):
             if tokens == 0:
                 dx, dws[i] = dys[i].new_empty((0, K)), dys[i].new_zeros((ctx.features[i], K)) if wants[i] else None
                 continue
+            _no_tangent(dys[i], "a gradient")
             d = dys[i].reshape(tokens, ctx.features[i])
             made = _natively("mx4_quant", d, int(wants_x), int(wants[i]))
             rows, cols = _quant(d, wants_x, wants[i]) if made is None else (made[:2], made[-2:])
@@ -292,6 +294,7 @@ class _BiasFunction(torch.autograd.Function):
         d2 = d.reshape(-1, d.shape[-1])
         db = None
         if ctx.needs_input_grad[1]:
+            _no_tangent(d, "a gradient")
             db = _column_sum(d2) if d2.shape[0] else d2.new_zeros(d2.shape[1:])
         return d, db
 

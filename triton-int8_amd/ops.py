@@ -700,6 +700,11 @@ def _unrecorded(what):
           and (level is None or level.key() == torch._C._functorch.TransformType.Vmap), f"{what} cannot be traced: what is launched would not be recorded")
 
 
+def _no_tangent(t, name):
+    """Refuses a tensor with a forward-mode tangent, which codes do not carry on."""
+    _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent, which a quantised tensor does not carry on")
+
+
 def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV_RCP_OF_SCALE):
     """``h = x + residual`` (bf16), ``y = bf16(h * rstd) * weight`` over the last dim and y quantised, in one pass: the step from a linear's output to the next one's operand.
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
@@ -718,7 +723,7 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
         _check_bf16(t, name)
         _need(t.get_device() == torch._C._cuda_getDevice(), f"{name} must be on the current GPU")
         _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which a quantised tensor does not give: call this under torch.no_grad()")
-        _need(forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None, f"{name} has a tangent, which a quantised tensor does not carry on")
+        _no_tangent(t, name)
     dim = x.shape[-1] if x.dim() else 0
     _need(x.numel() > 0 and dim % (8 if to == "mx4" else 128) == 0 and dim <= 16384,
           f"x must be non-empty and its last dim a multiple of {8 if to == 'mx4' else 128} up to 16384, got {tuple(x.shape)}")
@@ -757,6 +762,7 @@ def dequant_row(q, s):
           "q and s must be tensors on the current GPU")
     _need(q.dtype == torch.int8 and s.dtype == torch.float32 and q.dim() >= 1 and q.numel() > 0 and q.shape[-1] % 8 == 0,
           f"q must be a non-empty int8 tensor whose last dim is a multiple of 8, s float32; got {tuple(q.shape)} {q.dtype}, {s.dtype}")
+    _no_tangent(s, "s")
     cols, lead = q.shape[-1], tuple(q.shape[:-1])
     by_group = tuple(s.shape) != lead
     _need(not by_group or (cols % 128 == 0 and tuple(s.shape) == (*lead, cols // 128)), f"scales {tuple(s.shape)} do not fit codes {tuple(q.shape)}")
