@@ -573,14 +573,14 @@ typedef struct {
     int64_t ld, scale_ld;
 } ti8_mx4;
 /* x bf16 [rows][cols] (ldx, any alignment) quantised by its rows (by_rows: [rows][cols]), by its columns (by_columns: the transposed tensor [cols][rows]), or
- * both from one read: what has no codes (NULL) is not made.  `operands` is a HOST array; 2 or 3 of them, each both ways, go in one launch, with the same bits. */
+ * both from one read: what has no codes (NULL) is not made.  rows and cols up to 2^28, with whole tiles fewer than 2^37 elements.  `operands` is a HOST array; 2 or 3 of them, each both ways, go in one launch, with the same bits. */
 typedef struct {
     const void* x; int64_t ldx;
     int64_t rows, cols;
     ti8_mx4 by_rows, by_columns;
 } ti8_mx4_operand;
 int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_stream_t stream);
-/* y bf16 [rows][cols] (ldy): the values that the codes stand for, exactly */
+/* y bf16 [rows][cols] (ldy): the values that the codes stand for, exactly; sizes as above */
 int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, void* y, int64_t ldy, ti8_stream_t stream);
 /* C[b] = A[b] B[b]^T, A [M][K] and B [N][K]: batch b of A is the rows from b * rows_a on of `a` (0: all batches share A), of B likewise; C bf16 (wide: float)
  * [M][N], rows ldc and batches bsc elements apart.  Products and sums in fp32, rounded once.  K up to 2^22; behind K both operands hold zeros up to
@@ -611,7 +611,7 @@ int ti8_mx4_linear_fwd_bwd(const void* X, int64_t ldx, const void* W, int64_t ld
 /* A decoder layer's step from one linear's output to the next one's operand: h = bf16(x + residual) (residual and h NULL: h is x), rstd = 1 / sqrt(mean(h^2) + eps)
  * (float [rows]; the mean in 64 bits), y = bf16(bf16(h * rstd) * w), and y quantised: into 4 bits (mx4.codes not NULL), or into int8 codes q [rows][dim] with the
  * arithmetic of ti8_quant_row (s, group 0 or 128, qflags and inv_mode as there).  h may be the memory of x or residual.
- * dim a multiple of 8 up to 16384 (of 128 with q); x, residual, h and w 16-byte aligned, leading dimensions multiples of 8. */
+ * dim a multiple of 8 up to 16384 (of 128 with q); rows up to 2^26 - 4, with dim > 1024 up to 2^24 - 1; x, residual, h and w 16-byte aligned, leading dimensions multiples of 8. */
 typedef struct {
     const void* x; int64_t ldx;
     const void* residual; int64_t ldr;
@@ -626,7 +626,8 @@ typedef struct {
     int group, qflags, inv_mode;
 } ti8_rmsnorm_quant_args;
 int ti8_rmsnorm_quant(const ti8_rmsnorm_quant_args* a, ti8_stream_t stream);
-/* y bf16 [rows][cols] (ldy) = q * s: what the codes of ti8_quant_row stand for, s [rows] (group 0) or [rows][cols / 128] (group 128); cols % 8 == 0 */
+/* y bf16 [rows][cols] (ldy) = q * s: what the codes of ti8_quant_row stand for, s [rows] (group 0) or [rows][cols / 128] (group 128); cols % 8 == 0, fewer than
+ * 2^35 elements */
 int ti8_dequant_row(const int8_t* q, int64_t ldq, const float* s, int64_t rows, int64_t cols, int group, void* y, int64_t ldy, ti8_stream_t stream);
 
 /* ---------------------------------------------------------------------------------

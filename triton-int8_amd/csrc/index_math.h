@@ -754,6 +754,11 @@ TI8_HD int64_t xcd_range(int64_t block, int64_t blocks) {
     return xcd * (blocks >> 3) + (xcd < rest ? xcd : rest) + (block >> 3);
 }
 
+// A launch counts its work-items in 32 bits
+TI8_HD bool grid_fits(int64_t blocks, int threads) { return blocks > 0 && blocks < ((int64_t)1 << 32) / threads; }
+// norm that quantises: rows to a workgroup of 256 threads
+constexpr int mx4_norm_rows(int64_t dim) { return dim <= 1024 ? 4 : 1; }
+
 // quantiser by rows: 256 threads, a tile of 32 rows x 256 columns; thread t has octet t % 32 of rows t / 32 + 8 i, i < 4
 constexpr int MX4_ROW_BLOCK = 32;
 // quantiser by columns: a column's 16 NW bytes of codes from NW waves of 32 rows each; the waves' pieces lie in another order in every octet of columns, so that eight

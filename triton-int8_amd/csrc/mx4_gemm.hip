@@ -489,7 +489,7 @@ int launch_few(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
     int most = 0;
     for (int i = 0; i < all.count; ++i) most = all.g[i].M > most ? all.g[i].M : most;
     const int64_t strips = share_out(all, [](const Gemm& g) { return (int64_t)(g.N + 16 * NB - 1) / (16 * NB); });
-    if (strips < 0) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (!idx::grid_fits(strips, 64 * NW)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     const dim3 grid((unsigned)strips, (unsigned)((most + 16 * MB - 1) / (16 * MB)), (unsigned)batch), block(64 * NW);
     if (all.count > 1)
         few_rows_kernel<MB, NB, NW, Gemms><<<grid, block, LDS, st>>>(all);
@@ -515,7 +515,7 @@ int launch(const char* fn, Gemms all, int64_t batch, hipStream_t st) {
         g.tiles_n = (g.N + BN - 1) / BN;
         return (int64_t)g.tiles_m * g.tiles_n;
     });
-    if (tiles < 0 || tiles > 0x3fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (!idx::grid_fits(tiles, 64 * WM * WN)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     if (int e = prepare<BM, BN, WM, WN, STAGES>(fn, all.count > 1)) return e;
     const dim3 grid((unsigned)tiles, (unsigned)all.g[0].parts, (unsigned)batch), block(64 * WM * WN);
     if (all.count > 1)
@@ -640,7 +640,7 @@ extern "C" int ti8_mx4_gemm_nt(const ti8_mx4* a, int64_t rows_a, const ti8_mx4* 
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t blocks = need ? (batch * M * ((N + 3) / 4) + 255) / 256 : 0;
-    if (blocks > 0x7fffffff) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (need && !idx::grid_fits(blocks, 256)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     if (int e = mx4::launch_plan(fn, plan.kernel, all, batch, st)) return e;
     if (!need) return TI8_OK;
     mx4::join_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(static_cast<const float*>(workspace), plan.parts, g.part, batch * M, (int)M, (int)N, c, ldc, bsc, wide ? 1 : 0);

@@ -131,9 +131,11 @@ __global__ __launch_bounds__(64 * NW, 4) void quant_cols_kernel(QuantArgs args) 
 #endif
 }
 
+int too_many(const char* fn) { return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn); }
+
 // Workgroups over all of x^T's tiles (those behind its last rows make the zeros up to the end of a tile) and, with them, over all columns of x
 template <int NW, int RB, bool ROWS>
-void launch_cols(QuantArgs g, hipStream_t st) {
+int launch_cols(const char* fn, QuantArgs g, hipStream_t st) {
     constexpr int COLS = 512 / RB;
     int64_t blocks = 0;
     for (int i = 0; i < g.count; ++i) {
@@ -142,7 +144,9 @@ void launch_cols(QuantArgs g, hipStream_t st) {
         o.strips = (int)(ROWS ? idx::mx4_tiles(o.C) * (idx::MX4_TILE / COLS) : (o.C + COLS - 1) / COLS);
         blocks += o.strips * idx::mx4_tiles(o.R) * (8 / NW);
     }
+    if (!idx::grid_fits(blocks, 64 * NW)) return too_many(fn);
     quant_cols_kernel<NW, RB, ROWS><<<dim3((unsigned)blocks), dim3(64 * NW), 0, st>>>(g);
+    return check_launch(fn);
 }
 
 // The values back, exact in bf16
@@ -319,19 +323,21 @@ constexpr int NORM_MAX_DIM = THREADS * 8 * 8;
 // 16384 x 4096 83.5 / 87.7.
 constexpr int64_t NORM_ONCE = (int64_t)24 << 20;
 
+int64_t norm_blocks(int64_t rows, int64_t dim) { return (rows + idx::mx4_norm_rows(dim) - 1) / idx::mx4_norm_rows(dim); }
+
 template <int TO>
 void launch_norm(NormArgs g, hipStream_t st) {
     g.once = g.rows * g.dim > NORM_ONCE;
-    const auto go = [&](auto kernel, int rows_per_group) { kernel<<<dim3((unsigned)((g.rows + rows_per_group - 1) / rows_per_group)), dim3(THREADS), 0, st>>>(g); };
-    if (g.dim <= 512) go(rmsnorm_quant_kernel<64, 1, TO>, 4);
-    else if (g.dim <= 1024) go(rmsnorm_quant_kernel<64, 2, TO>, 4);
-    else if (g.dim <= 2048) go(rmsnorm_quant_kernel<THREADS, 1, TO>, 1);
-    else if (g.dim <= 4096) go(rmsnorm_quant_kernel<THREADS, 2, TO>, 1);
-    else if (g.dim <= 8192) go(rmsnorm_quant_kernel<THREADS, 4, TO>, 1);
-    else go(rmsnorm_quant_kernel<THREADS, 8, TO>, 1);
+    const int64_t blocks = norm_blocks(g.rows, g.dim);
+    const auto go = [&](auto kernel) { kernel<<<dim3((unsigned)blocks), dim3(THREADS), 0, st>>>(g); };
+    static_assert(idx::mx4_norm_rows(1024) == THREADS / 64 && idx::mx4_norm_rows(1025) == 1, "a row to a wave, or to a workgroup");
+    if (g.dim <= 512) go(rmsnorm_quant_kernel<64, 1, TO>);
+    else if (g.dim <= 1024) go(rmsnorm_quant_kernel<64, 2, TO>);
+    else if (g.dim <= 2048) go(rmsnorm_quant_kernel<THREADS, 1, TO>);
+    else if (g.dim <= 4096) go(rmsnorm_quant_kernel<THREADS, 2, TO>);
+    else if (g.dim <= 8192) go(rmsnorm_quant_kernel<THREADS, 4, TO>);
+    else go(rmsnorm_quant_kernel<THREADS, 8, TO>);
 }
-
-bool grid_ok(int64_t blocks) { return blocks > 0 && blocks <= 0x7fffffff; }
 
 }  // namespace
 }  // namespace mx4
@@ -350,8 +356,8 @@ extern "C" int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_str
         const ti8_mx4_operand& o = operands[i];
         if (!o.x || (!o.by_rows.codes && !o.by_columns.codes)) return fail(TI8_ERR_NULL, "%s: x and one of by_rows and by_columns are required", fn);
         if (count > 1 && (!o.by_rows.codes || !o.by_columns.codes)) return fail(TI8_ERR_NULL, "%s: several operands are quantised by rows and by columns", fn);
-        if (o.rows <= 0 || o.cols <= 0 || o.rows > (1 << 28) || o.cols > (1 << 28) || (o.rows > 1 && o.ldx < o.cols) || o.rows * o.cols > (1ll << 40))
-            return fail(TI8_ERR_SHAPE, "%s: need rows, cols in 1 .. 2^28, up to 2^40 elements and ldx >= cols; got rows=%lld cols=%lld ldx=%lld", fn, (long long)o.rows,
+        if (o.rows <= 0 || o.cols <= 0 || o.rows > (1 << 28) || o.cols > (1 << 28) || (o.rows > 1 && o.ldx < o.cols) || o.rows * o.cols > (1ll << 37))
+            return fail(TI8_ERR_SHAPE, "%s: need rows, cols in 1 .. 2^28, up to 2^37 elements and ldx >= cols; got rows=%lld cols=%lld ldx=%lld", fn, (long long)o.rows,
                         (long long)o.cols, (long long)o.ldx);
         if (reinterpret_cast<uintptr_t>(o.x) & 1) return fail(TI8_ERR_ALIGN, "%s: x must be 2-byte aligned", fn);
         g.o[i] = {static_cast<const uint16_t*>(o.x), o.ldx, o.rows, o.cols, {}, {}, 0, 0};
@@ -364,18 +370,16 @@ extern "C" int ti8_mx4_quant(const ti8_mx4_operand* operands, int count, ti8_str
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (!operands[0].by_columns.codes) {
         const int64_t blocks = idx::mx4_tiles(g.o[0].C) * ((g.o[0].R + idx::MX4_ROW_BLOCK - 1) / idx::MX4_ROW_BLOCK);
-        if (!mx4::grid_ok(blocks)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+        if (!idx::grid_fits(blocks, mx4::THREADS)) return mx4::too_many(fn);
         mx4::quant_row_kernel<<<dim3((unsigned)blocks), dim3(mx4::THREADS), 0, st>>>(g.o[0]);
         return check_launch(fn);
     }
-    if (!mx4::grid_ok(elements / (64 * 64))) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
     // Small tensors: workgroups of 128 x 64 elements (by columns alone 64 x 64), whose code is a quarter as long (it is read from memory too); behind that twice as many
     // columns to a workgroup, whose rows' codes are written in longer pieces.  us, both ways, small / large, tensors from memory: 200 x 300 4.1 / 5.5, 1001 x 1016 4.9 / 5.3,
     // 1500 x 1500 6.3 / 8.3, 2048 x 2048 7.4 / 6.9, 4096 x 4096 17 / 16, 14336 x 4096 50 / 41 (37 since x is read past the caches: 4.9 TB/s).  By columns alone 14336 x 4096 29 (5.2 TB/s).
     const bool small = elements < (int64_t)16384 * device_cu_count(), rows = operands[0].by_rows.codes;
-    if (small) rows ? mx4::launch_cols<4, 8, true>(g, st) : mx4::launch_cols<2, 8, false>(g, st);
-    else rows ? mx4::launch_cols<4, 4, true>(g, st) : mx4::launch_cols<8, 4, false>(g, st);
-    return check_launch(fn);
+    if (small) return rows ? mx4::launch_cols<4, 8, true>(fn, g, st) : mx4::launch_cols<2, 8, false>(fn, g, st);
+    return rows ? mx4::launch_cols<4, 4, true>(fn, g, st) : mx4::launch_cols<8, 4, false>(fn, g, st);
 }
 
 extern "C" int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, void* y, int64_t ldy, ti8_stream_t stream) {
@@ -387,7 +391,7 @@ extern "C" int ti8_mx4_dequant(const ti8_mx4* q, int64_t rows, int64_t cols, voi
     mx4::Tensor t;
     if (int e = mx4::check(fn, "q", q, rows, cols, t)) return e;
     const int64_t blocks = idx::mx4_tiles(cols) * ((rows + idx::MX4_ROW_BLOCK - 1) / idx::MX4_ROW_BLOCK);
-    if (!mx4::grid_ok(blocks)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (!idx::grid_fits(blocks, mx4::THREADS)) return mx4::too_many(fn);
     mx4::dequant_kernel<<<dim3((unsigned)blocks), dim3(mx4::THREADS), 0, static_cast<hipStream_t>(stream)>>>(t, rows, cols, static_cast<uint16_t*>(y), ldy);
     return check_launch(fn);
 }
@@ -402,7 +406,7 @@ extern "C" int ti8_dequant_row(const int8_t* q, int64_t ldq, const float* s, int
     if ((reinterpret_cast<uintptr_t>(q) & 7) || ldq % 8 || !aligned16(y) || ldy % 8 || (reinterpret_cast<uintptr_t>(s) & 3))
         return fail(TI8_ERR_ALIGN, "%s: rows of q must be 8-byte aligned, those of y 16-byte, s 4-byte", fn);
     const int64_t blocks = (rows * (cols >> 3) + mx4::THREADS - 1) / mx4::THREADS;
-    if (!mx4::grid_ok(blocks)) return fail(TI8_ERR_SHAPE, "%s: too many elements for one call", fn);
+    if (!idx::grid_fits(blocks, mx4::THREADS)) return mx4::too_many(fn);
     mx4::dequant_row_kernel<<<dim3((unsigned)blocks), dim3(mx4::THREADS), 0, static_cast<hipStream_t>(stream)>>>(q, ldq, s, rows, cols, group ? 1 : 0, static_cast<uint16_t*>(y), ldy);
     return check_launch(fn);
 }
@@ -413,9 +417,11 @@ extern "C" int ti8_rmsnorm_quant(const ti8_rmsnorm_quant_args* a, ti8_stream_t s
     if (!a->residual != !a->h) return fail(TI8_ERR_NULL, "%s: residual and h go together", fn);
     if (!a->mx4.codes == !a->q) return fail(TI8_ERR_NULL, "%s: one of mx4 and q is required", fn);
     const int64_t rows = a->rows, dim = a->dim;
-    if (rows <= 0 || rows > (1 << 28) || dim <= 0 || dim % 8 || dim > mx4::NORM_MAX_DIM || a->ldx < dim || (a->residual && (a->ldr < dim || a->ldh < dim)))
-        return fail(TI8_ERR_SHAPE, "%s: need rows in 1 .. 2^28, dim a multiple of 8 up to %d and leading dimensions of at least dim; got rows=%lld dim=%lld", fn, mx4::NORM_MAX_DIM,
+    if (rows <= 0 || dim <= 0 || dim % 8 || dim > mx4::NORM_MAX_DIM || a->ldx < dim || (a->residual && (a->ldr < dim || a->ldh < dim)))
+        return fail(TI8_ERR_SHAPE, "%s: need rows, dim a multiple of 8 up to %d and leading dimensions of at least dim; got rows=%lld dim=%lld", fn, mx4::NORM_MAX_DIM,
                     (long long)rows, (long long)dim);
+    if (rows > (1 << 28) || !idx::grid_fits(mx4::norm_blocks(rows, dim), mx4::THREADS))
+        return fail(TI8_ERR_SHAPE, "%s: up to 2^26 - 4 rows, of more than 1024 elements up to 2^24 - 1; got rows=%lld dim=%lld", fn, (long long)rows, (long long)dim);
     if (!aligned16(a->x) || !aligned16(a->w) || !aligned16(a->residual) || !aligned16(a->h) || a->ldx % 8 || (a->residual && (a->ldr % 8 || a->ldh % 8)) ||
         (reinterpret_cast<uintptr_t>(a->rstd) & 3))
         return fail(TI8_ERR_ALIGN, "%s: rows of x, residual and h and the weight must be 16-byte aligned", fn);

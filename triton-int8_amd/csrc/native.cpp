@@ -582,7 +582,7 @@ PyObject* rmsnorm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const auto dense = [&](const at::Tensor& t) { return on(t, at::kBFloat16, device) && t.is_contiguous() && at_multiple(t, 16) && !derived(t); };
     if (!dense(x) || !dense(w) || (r.defined() && (!dense(r) || r.sizes() != x.sizes())) || x.dim() < 1 || w.dim() != 1) Py_RETURN_NONE;
     const int64_t dim = x.size(-1), rows = x.numel() / dim;
-    if (w.size(0) != dim || dim % (mx ? 8 : 128) || dim > 16384 || rows > MX4_ROWS || (group != 0 && (group != 128 || mx))) Py_RETURN_NONE;
+    if (w.size(0) != dim || dim % (mx ? 8 : 128) || dim > 16384 || rows > (dim > 1024 ? (1 << 24) - 1 : (1 << 26) - 4) || (group != 0 && (group != 128 || mx))) Py_RETURN_NONE;
     int status;
     {
         const GilReleased released;

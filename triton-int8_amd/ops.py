@@ -708,7 +708,7 @@ def _no_tangent(t, name):
 def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV_RCP_OF_SCALE):
     """``h = x + residual`` (bf16), ``y = bf16(h * rstd) * weight`` over the last dim and y quantised, in one pass: the step from a linear's output to the next one's operand.
     ``to`` "mx4": codes and scales as ``mx4.quant_row(y)`` gives them; "int8": as ``quant_row(y, group=group, inv_mode=inv_mode)``.  x and residual bf16 [.., dim], dim a
-    multiple of 8 (with "int8" of 128) up to 16384.
+    multiple of 8 (with "int8" of 128) up to 16384; up to 2^26 - 4 rows, of more than 1024 elements up to 2^24 - 1.
 
     Returns ``(q, s, rstd)``, and h behind them where there is a residual.  rstd float32 [..] = 1 / sqrt(mean(h^2) + eps), the mean added up in 64 bits.  Quantised tensors have no gradients: x, weight and
     residual that require one are refused while gradients are recorded.  A gradient of y goes back to h (and, the sum's, to x and residual alike) by ``rmsnorm_backward(dy, h, weight, rstd)``."""
@@ -729,12 +729,11 @@ def rmsnorm_quant(x, weight, eps, residual=None, to="mx4", group=0, inv_mode=INV
           f"x must be non-empty and its last dim a multiple of {8 if to == 'mx4' else 128} up to 16384, got {tuple(x.shape)}")
     _need(tuple(weight.shape) == (dim,) and (residual is None or residual.shape == x.shape),
           f"shapes do not fit: x {tuple(x.shape)}, weight {tuple(weight.shape)}" + ("" if residual is None else f", residual {tuple(residual.shape)}"))
-    lead = x.shape[:-1]
+    lead, rows, dev = x.shape[:-1], x.numel() // dim, x.device
+    _need(rows < (1 << 24 if dim > 1024 else (1 << 26) - 3), f"up to 2^26 - 4 rows, of more than 1024 elements up to 2^24 - 1, got {rows} of {dim}")
     x2, r2 = rows16(x.reshape(-1, dim)), None if residual is None else rows16(residual.reshape(-1, dim))
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
-    rows, dev = x2.shape[0], x.device
-    _need(rows <= 1 << 28, f"up to 2^28 rows, got {rows}")
     rstd = torch.empty(lead, dtype=torch.float32, device=dev)
     h = None if residual is None else torch.empty((*lead, dim), dtype=torch.bfloat16, device=dev)
     a = _lib.RmsnormQuantArgs(x=x2.data_ptr(), ldx=dim if rows == 1 else x2.stride(0), w=weight.data_ptr(), rstd=rstd.data_ptr(), rows=rows, dim=dim, eps=eps, group=group, inv_mode=inv_mode)
