@@ -295,7 +295,8 @@ class _BiasFunction(torch.autograd.Function):
         db = None
         if ctx.needs_input_grad[1]:
             _no_tangent(d, "a gradient")
-            db = _column_sum(d2) if d2.shape[0] else d2.new_zeros(d2.shape[1:])
+            # (a sum with a bias of another type has that type: not for the kernel)
+            db = d2.new_zeros(d2.shape[1:]) if d2.shape[0] == 0 else _column_sum(d2) if d2.dtype == torch.bfloat16 else d2.sum(0)
         return d, db
 
 
