@@ -300,11 +300,16 @@ class _BiasFunction(torch.autograd.Function):
         return d, db
 
 
+def _with_bias(y, bias):
+    """y + bias, also where the bias alone has a gradient."""
+    return y if bias is None else _BiasFunction.apply(y, bias) if bias.requires_grad and torch.is_grad_enabled() else y + bias
+
+
 def _served(codes, scales, shape, layers):
     """Outputs [*shape, out_features] of layers whose input is already in 4 bits."""
     ys = _products(codes, scales, [m.quantised() for m in layers], shape)
     biases = [m.bias for m in layers]       # (a module's attributes take a while)
-    return tuple(y if b is None else y + b for y, b in zip(ys, biases))
+    return tuple(map(_with_bias, ys, biases))
 
 
 def linears(x, layers):
@@ -319,7 +324,7 @@ def linears(x, layers):
         ys = Mx4LinearFunction.apply(x, *(m.weight for m in layers))
         return tuple(y if m.bias is None else _BiasFunction.apply(y, m.bias) for y, m in zip(ys, layers))
     if x.numel() == 0:
-        return tuple(x.new_empty((*x.shape[:-1], m.out_features)) for m in layers)
+        return tuple(_with_bias(x.new_empty((*x.shape[:-1], m.out_features)), m.bias) for m in layers)
     return _served(*quant_row(x if x.dim() == 2 else x.reshape(-1, x.shape[-1])), x.shape[:-1], layers)
 
 
