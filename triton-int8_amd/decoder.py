@@ -246,7 +246,8 @@ class DecoderLayer(torch.nn.Module):
 
     def _norm_quantises(self, x):
         """Whether norms and what quantises their results for the projections behind them may be one kernel each (ops.rmsnorm_quant)."""
-        return (mx4.all_as_written(self._linears()) and mx4._as_written((self.input_norm, self.post_norm), RMSNorm, _NORM_CALL)
+        # (one look for layers of other schemes: all seven take 5 us of their serving)
+        return (type(self.q_proj) is mx4.Mx4Linear and mx4.all_as_written(self._linears()) and mx4._as_written((self.input_norm, self.post_norm), RMSNorm, _NORM_CALL)
                 and self.hidden % 8 == 0 and self.hidden <= 16384 and _kernels_take(x, self.input_norm.weight, self.post_norm.weight))
 
     def _normed(self, x, norm, layers, residual=None):
