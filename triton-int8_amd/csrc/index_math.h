@@ -785,7 +785,8 @@ TI8_HD Mx4Part mx4_part(int p, int parts, int nk) {
 // Which kernel multiplies [M][K] and [N][K], K in nk tiles, and in how many parts along K.  In us, behind the launch's own 2.2: `slots` tiles have the chip full and
 // take `full` per K tile, up to `free` of them no longer than one, `one`; a tile's first loads and its results take as long as `lead` K tiles.  Of 52 products and 26
 // sets of them, M from 64 to 16384, K from 256 to 4096, run by each of the kernels, this chose the fastest of them or one behind it, by 7 % at most and 0.2 % on
-// average; without `lead` 6 % on average and up to 65 %.
+// average (measured again on another card: 0.6 % on average, 17 % and 16 % at 2048 and 4096 x 4096 with K of 1024 and 512, 3.4 % at most elsewhere); without `lead` 6 % on
+// average and up to 65 %.  No bytes are counted: one row through 128256 x 4096 takes 50.9 us, 48.6 with the best kernel, 32 rows 55.9 and 55.3.
 enum { MX4_FEW_16 = 0, MX4_FEW_32 = 1, MX4_TILES_32 = 2, MX4_TILES_64 = 3, MX4_TILES_128 = 4, MX4_TILES_128_TWO = 5, MX4_TILES_256 = 6, MX4_TILES_64_128 = 7, MX4_KERNELS = 8 };
 struct Mx4Kernel {
     int bm, bn, slots, free;        // of 256 CUs

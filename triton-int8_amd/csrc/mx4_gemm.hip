@@ -81,10 +81,12 @@ __device__ __forceinline__ void beside(int q, int count, int n, const F& f) {
         if (i >= q * n / count && i < (q + 1) * n / count) f(i);
 }
 
-// One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS.  256 x 256: per K tile a CU's matrix instructions take 2048 cycles, its LDS reads and writes
-// as many; 8192 x 14336 x 4096 225 to 235 us (4.1 to 4.3 PFLOP/s) at a clock of 1.7 GHz, on codes of zero 172: the chip's power bounds it (a loop of nothing but these instructions
-// reaches 6.6 PFLOP/s on random codes, 9.7 on zeros).  16 x 16 x 128 instructions, four waves of 128 x 128, workgroups that go on to the next tile: within 3 %.  Smaller
-// tiles where those do not fill the CUs: 700 x 4096 x 4096 10.3 to 11.5 us, 128 x 4096 x 4096 5.9, of which 2.2 are the launch and 1.5 to 3 a tile's first loads and results.
+// One BM x BN tile of C on WM x WN waves, with STAGES tiles of codes in LDS.  256 x 256, 8192 x 14336 x 4096: 220 to 235 us (4.1 to 4.4 PFLOP/s).  A K tile takes 3520
+// cycles of a CU in all, of which the matrix pipe has 2048 (0.58) and LDS 1180 (0.17 of them conflicts); 4 to 5 us of each round of tiles are first loads and results,
+// the rest is the one barrier per tile, behind which all eight waves read at once.  On codes of zero the cycles are the same, at 2.16 GHz instead of 1.76: power sets the
+// clock (a loop of nothing but these instructions reaches 6.5 PFLOP/s on random codes, 9.8 on zeros), not the cycles without the pipe.  16 x 16 x 128 instructions (their
+// loop: 7.2 and 9.7), four waves of 128 x 128, workgroups that go on to the next tile: within 3 %.  Smaller tiles where those do not fill the CUs: 700 x 4096 x 4096 10.3
+// to 11.5 us, 128 x 4096 x 4096 5.9, of which 2.2 are the launch and 1.5 to 3 a tile's first loads and results.
 constexpr int scale_stages(int stages) { return stages == 2 ? 4 : 8; }
 constexpr int gemm_lds(int bm, int bn, int stages) { return (bm + bn) * (128 * stages + 8 * scale_stages(stages)); }
 constexpr int waitcnt(int vm, int other) { return ((vm >> 4) << 14) | (vm & 15) | other; }      // vmcnt[3:0] | expcnt << 4 | lgkmcnt << 8 | vmcnt[5:4] << 14
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_kernel(Products products
     if constexpr (WHOLE) {
         // All of the next tile's fragments are read beside this one's matrix instructions, and tile kt + STAGES asked for (everybody has tile kt in registers), a piece
         // of both behind each instruction and in this order: left to the compiler they come in bunches, and LDS and the matrix pipe take turns (512 x 4096 x 4096
-        // 12.4 us on 128 x 128, 10.8 on 64 x 64, so 11.2 and 10.1).  That 256 x 256 is no faster with it: it is bound by power.
+        // 12.4 us on 128 x 128, 10.8 on 64 x 64, so 11.2 and 10.1).  (256 x 256 is no faster with it.)
         constexpr int BEHIND = (STAGES - 2) * (LOADS + SCALE_LOADS);
         static_assert((STAGES - 1) * (LOADS + SCALE_LOADS) < 64 && RING >= STAGES, "vmcnt has six bits");
         v4i wa[2][TM][4], wb[2][TN][4];
